@@ -510,6 +510,138 @@ trellis_status trellis_sparse_hip_conv_add(trellis_sparse_backend * backend, con
                                            trellis_sparse_buffer * out, int64_t n, int ci, int co);
 
 /* ------------------------------------------------------------------------ */
+/* Memory and stream of the caller (no counterpart in the reference): for    */
+/* programs that keep rows on the device themselves, such as the models     */
+/* whose latents this backend decodes.                                       */
+/* ------------------------------------------------------------------------ */
+
+/* A buffer over `count` elements of the caller's device memory, in the
+ * backend's compute_dtype (_f32) or int32 (_i32).  The memory stays the caller's
+ * and outlives the buffer and the work queued on it; free_buffer releases only the
+ * handle.  INVALID_ARGUMENT unless it is 16-byte aligned, on the backend's device
+ * and within one allocation. */
+trellis_status trellis_sparse_hip_wrap_f32(trellis_sparse_backend * backend, void * device_ptr, size_t count,
+                                           trellis_sparse_buffer ** out);
+trellis_status trellis_sparse_hip_wrap_i32(trellis_sparse_backend * backend, void * device_ptr, size_t count,
+                                           trellis_sparse_buffer ** out);
+
+/* From this call on the backend queues its work on `stream` (a hipStream_t of
+ * the backend's device; NULL is the default stream), behind what it has queued
+ * before; own_stream goes back to the stream it was created with.  The stream
+ * outlives its use here: go back, or destroy the backend, before destroying it.
+ * While the stream is captured into a graph, calls that need no memory can be
+ * captured: buffers exist before, weights are on the device from an earlier
+ * call, and all stay until the last replay; a call that would allocate returns
+ * TRELLIS_STATUS_ERROR. */
+trellis_status trellis_sparse_hip_set_stream(trellis_sparse_backend * backend, void * stream);
+trellis_status trellis_sparse_hip_own_stream(trellis_sparse_backend * backend);
+
+/* ------------------------------------------------------------------------ */
+/* Transformer blocks over voxel rows (no vtable counterpart).  The          */
+/* structured latents that the decoders take come from transformers over the */
+/* same voxels (src/architectures/dit_flow/dit_flow.c:258-375), which the     */
+/* reference runs on its dense layers (include/trellis_ggml_layers.h:10-274). */
+/* Rows are [n][channels] in the backend's compute_dtype, sums, norms and      */
+/* softmax statistics are fp32, and each output is rounded once.  An output    */
+/* may be the very rows of an input only where a call says so; rows that        */
+/* overlap otherwise -> INVALID_ARGUMENT.                                         */
+/* ------------------------------------------------------------------------ */
+
+/* 8-bit rows: n rows of c channels as e4m3 values, each 32 channels with one scale
+ * 2^e, e >= -126 the least for which the largest magnitude is at most 448 * 2^e
+ * (1 for 32 zeros).  32 channels with an infinity or a NaN among them become
+ * NaN.  A buffer for free_buffer; the slots, uploads and downloads do not take it. */
+trellis_status trellis_sparse_hip_alloc_rows8(trellis_sparse_backend * backend, int64_t n, int c,
+                                              trellis_sparse_buffer ** out);
+/* rows8 = x, rounded to nearest even; y = the values of rows8 (exact in
+ * bf16 and fp32 but for 2^128, the code nearest fp32's largest). */
+trellis_status trellis_sparse_hip_pack_rows8(trellis_sparse_backend * backend, const trellis_sparse_buffer * x,
+                                             trellis_sparse_buffer * rows8, int64_t n, int c);
+trellis_status trellis_sparse_hip_expand_rows8(trellis_sparse_backend * backend, const trellis_sparse_buffer * rows8,
+                                               trellis_sparse_buffer * y, int64_t n, int c);
+
+/* s = x + residual; total = s; y = s / sqrt(mean(s^2) + eps) * gamma, the mean
+ * over a row's c channels and s unrounded in y.  residual, gamma (fp32 [c]) and
+ * total may be NULL; y is rows of the compute_dtype or 8-bit rows (n, c).  y and
+ * total may each be x or residual.  eps > 0. */
+trellis_status trellis_sparse_hip_rms_norm(trellis_sparse_backend * backend, const trellis_sparse_buffer * x,
+                                           const trellis_sparse_buffer * residual, const float * gamma,
+                                           trellis_sparse_buffer * total, trellis_sparse_buffer * y, int64_t n, int c,
+                                           float eps);
+
+typedef enum trellis_sparse_hip_act {
+    TRELLIS_SPARSE_HIP_ACT_NONE = 0,
+    TRELLIS_SPARSE_HIP_ACT_SILU = 1,     /* v / (1 + exp(-v)) */
+    TRELLIS_SPARSE_HIP_ACT_GELU = 2,     /* v (1 + erf(v / sqrt(2))) / 2 */
+    TRELLIS_SPARSE_HIP_ACT_GELU_TANH = 3 /* v (1 + tanh(sqrt(2 / pi) (v + 0.044715 v^3))) / 2 */
+} trellis_sparse_hip_act;
+
+/* y = act(x W^T + bias) + residual: weight fp32 [co][ci], bias fp32 [co] and
+ * residual [n][co] may be NULL, y may be residual.  x is rows of the
+ * compute_dtype, with the weights rounded to it, or 8-bit rows (n, ci), with the
+ * weights in the same 8-bit format; sums are fp32.  (Of 8-bit rows the matrix unit
+ * first adds eight neighbouring products, each cut at 2^-13 of the largest: some
+ * 2e-5 of an output's size.)  Always this library's kernels, whatever linear_algo
+ * says.  ci up to 1,048,576. */
+trellis_status trellis_sparse_hip_linear_act(trellis_sparse_backend * backend, const trellis_sparse_buffer * x,
+                                             const float * weight, const float * bias, int act,
+                                             const trellis_sparse_buffer * residual, trellis_sparse_buffer * y,
+                                             int64_t n, int ci, int co);
+
+/* Rotary positions with three axes.  Each head's head_dim channels are
+ * head_dim / 2 pairs; the first pairs[0] belong to x, the next pairs[1] to y,
+ * the next pairs[2] to z, the rest pass unturned.  Pair j of an axis turns by
+ * the row's coordinate * base^(-j / pairs[axis]): (a, b) -> (a cos - b sin, a sin
+ * + b cos).  Offsets and strides are in elements. */
+typedef struct trellis_sparse_hip_rotary_desc {
+    uint32_t struct_size;  /* sizeof(trellis_sparse_hip_rotary_desc) */
+    int32_t heads;
+    int32_t head_dim;      /* up to 256 */
+    int32_t pairs[3];
+    int32_t split;         /* 0: pair p is channels (2p, 2p + 1); 1: (p, p + head_dim / 2) */
+    float eps;             /* > 0: each head is divided by sqrt(mean(h^2) + eps) first; 0: no norm */
+    double base;
+    const float * gamma;   /* fp32 [heads][head_dim] for the norm, or NULL */
+    int64_t x_offset, x_stride;  /* row i's first head at x_offset + i * x_stride; stride 0: heads * head_dim */
+    int64_t y_offset, y_stride;
+} trellis_sparse_hip_rotary_desc;
+/* coords: an int32 buffer [n][4] (b, x, y, z), or a device map's coordinates
+ * (coords_map wins).  y may be the rows of x, or other columns of their buffer.
+ * NOT_IMPLEMENTED unless head_dim, offsets and strides are multiples of 8. */
+trellis_status trellis_sparse_hip_rotary(trellis_sparse_backend * backend, const trellis_sparse_buffer * x,
+                                         const trellis_sparse_buffer * coords,
+                                         const trellis_sparse_c2s_device_map * coords_map, trellis_sparse_buffer * y,
+                                         int64_t n, const trellis_sparse_hip_rotary_desc * desc);
+
+/* Attention: for every query row i and head h, y = sum over the keys j of its
+ * sequence of softmax_j(scale q_i . k_j) v_j; heads h of q share kv head
+ * h / (heads / kv_heads).  Offsets and strides are in elements. */
+typedef struct trellis_sparse_hip_attention_desc {
+    uint32_t struct_size;  /* sizeof(trellis_sparse_hip_attention_desc) */
+    int32_t heads;
+    int32_t kv_heads;      /* divides heads */
+    int32_t head_dim;      /* up to 192 */
+    float scale;           /* 0: 1 / sqrt(head_dim) */
+    int64_t q_offset, q_stride;  /* row i's first head at q_offset + i * q_stride; stride 0: packed */
+    int64_t k_offset, k_stride;
+    int64_t v_offset, v_stride;
+    int64_t y_offset, y_stride;
+} trellis_sparse_hip_attention_desc;
+/* q, y [nq] rows of heads * head_dim, k, v [nkv] rows of kv_heads * head_dim.
+ * q_offsets, kv_offsets: int32 buffers [n_seqs + 1], sequence s has query rows
+ * q_offsets[s] .. q_offsets[s + 1] - 1 and keys likewise; both NULL: one
+ * sequence of all rows (n_seqs 1).  They are read on the device, where they are
+ * clamped to the rows that there are; ascending offsets are the caller's to give
+ * (of others every access stays within the buffers).  A sequence without keys
+ * gives zeros; rows of y in no sequence are left as they were.  y may be the rows of q. */
+trellis_status trellis_sparse_hip_attention(trellis_sparse_backend * backend, const trellis_sparse_buffer * q,
+                                            const trellis_sparse_buffer * k, const trellis_sparse_buffer * v,
+                                            trellis_sparse_buffer * y, int64_t nq, int64_t nkv,
+                                            const trellis_sparse_buffer * q_offsets,
+                                            const trellis_sparse_buffer * kv_offsets, int n_seqs,
+                                            const trellis_sparse_hip_attention_desc * desc);
+
+/* ------------------------------------------------------------------------ */
 /* Stage timing with HIP events recorded on the backend's own stream.        */
 /* ------------------------------------------------------------------------ */
 typedef enum trellis_sparse_hip_stage {

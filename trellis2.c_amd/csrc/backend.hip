@@ -15,6 +15,7 @@
 
 #include <algorithm>
 #include <chrono>
+#include <cmath>
 #include <cstdio>
 #include <cstdlib>
 #include <cstring>
@@ -60,7 +61,9 @@ enum WeightLayout : int {
     kLayoutMlp0 = 7,             // as kLayoutLinearMfma, the fused MLP's first GEMM grouping
     kLayoutMlp2 = 8,             // as kLayoutLinearMfma, the fused MLP's second GEMM grouping
     kLayoutLinear16 = 9,         // storage type [co][ci] (narrow MFMA linear)
-    kLayoutGemm = 10             // as kLayoutLinearMfma, groups of 128 columns, 8 adjacent channels per lane
+    kLayoutGemm = 10,            // as kLayoutLinearMfma, groups of 128 columns, 8 adjacent channels per lane
+    kLayoutAct = 11,             // storage type [linear_act_rows(co)][ci to whole 128 bytes], zeros beyond co and ci
+    kLayoutAct8 = 12             // 8-bit rows [linear_act_rows(co)] of ci channels
 };
 
 struct StageMark {
@@ -74,7 +77,9 @@ struct Backend {
     trellis_sparse_backend base;
     int device = 0;
     int cus = 0;  // compute units of the device
-    hipStream_t stream = nullptr;
+    hipStream_t stream = nullptr;      // where calls enqueue: own_stream, or the caller's (set_stream)
+    hipStream_t own_stream = nullptr;
+    hipEvent_t stream_left = nullptr;  // orders a new stream behind the one left (created on first use)
     trellis_sparse_hip_policy policy{};
     std::string last_error;
     // Pool: size class -> free device blocks.
@@ -211,10 +216,26 @@ hipError_t device_malloc(Backend * be, void ** p, size_t bytes) {
     return hipMalloc(p, bytes);
 }
 
+// Whether the caller's stream (set_stream) is being captured into a graph: no
+// memory is handed out then.  A fresh allocation cannot be captured, and a pool
+// block would go back to the pool while the graph still writes to it.
+bool capturing(const Backend * be) {
+    if (be->stream == be->own_stream) return false;
+    hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+    if (hipStreamIsCapturing(be->stream, &status) != hipSuccess) {
+        (void) hipGetLastError();
+        return true;
+    }
+    return status != hipStreamCaptureStatusNone;
+}
+
 trellis_status dev_alloc(Backend * be, size_t bytes, DevMem * out) {
     out->ptr = nullptr;
     out->bytes = 0;
     if (bytes == 0) return TRELLIS_STATUS_OK;
+    if (capturing(be)) {
+        return fail(be, TRELLIS_STATUS_ERROR, "no memory is allocated while the stream is captured: run the call once before");
+    }
     const size_t cls = size_class(bytes);
     auto it = be->free_blocks.find(cls);
     if (it != be->free_blocks.end() && !it->second.empty()) {
@@ -416,6 +437,50 @@ trellis_status upload_bytes(Backend * be, const void * src, size_t bytes, DevMem
 }
 
 // ---- weight / vector cache ---------------------------------------------------
+
+// e4m3 code of v, |v| <= 448, to nearest even: steps of 2^-3 of the value's
+// power of two, of 2^-9 below 2^-6.
+uint8_t e4m3_code(float v) {
+    const uint8_t sign = std::signbit(v) ? 0x80 : 0;
+    const float a = std::fabs(v);
+    int e = a > 0.0f ? std::ilogb(a) : -6;
+    if (e < -6) e = -6;
+    const int m = (int) std::nearbyint(std::ldexp(a, 3 - e));  // 0 .. 16 steps
+    // Subnormal codes are 0 .. 7; 8 .. 15 carry the implicit bit, and 16 moves on to the next power of two.
+    return sign | (uint8_t) (m < 8 ? m : ((e + 6) << 3) + m);
+}
+
+// One row of 8-bit rows on the host (weights), as the device packs features:
+// per 32 channels the least scale 2^e, e >= -126, with max|v| <= 448 * 2^e.
+void pack8_row(const float * v, int c, uint8_t * codes, uint8_t * scales) {
+    const int cp = rows8_width(c);
+    memset(codes, 0, (size_t) cp);
+    for (int b = 0; b < cp / 32; ++b) {
+        const int end = std::min(c, 32 * b + 32);
+        float most = 0.0f;
+        bool finite = true;
+        for (int i = 32 * b; i < end; ++i) {
+            finite = finite && std::isfinite(v[i]);
+            most = std::max(most, std::fabs(v[i]));
+        }
+        int e = 0;
+        if (!finite) {
+            scales[b] = 255;
+            for (int i = 32 * b; i < end; ++i) codes[i] = 0x7f;
+            continue;
+        }
+        if (most > 0.0f) {
+            int power;
+            const float m = std::frexp(most, &power);
+            e = std::max(-126, power - (m <= 0.875f ? 9 : 8));
+        }
+        scales[b] = (uint8_t) (127 + e);
+        for (int i = 32 * b; i < end; ++i) codes[i] = e4m3_code(std::ldexp(v[i], -e));
+    }
+}
+
+int linear_act_bytes(int dt, int ci) { return (int) (((size_t) ci * dtype_bytes(dt) + 127) / 128 * 128); }
+
 trellis_status get_weight(Backend * be, const float * host, size_t count, int layout, int ci, int co,
                           const void ** dev_out, bool * finite_out = nullptr) {
     *dev_out = nullptr;
@@ -519,6 +584,30 @@ trellis_status get_weight(Backend * be, const float * host, size_t count, int la
             float * w = (float *) staged.data();
             for (int o = 0; o < co; ++o)
                 for (int c = 0; c < ci; ++c) w[(size_t) c * co + o] = host[(size_t) o * ci + c];
+            break;
+        }
+        case kLayoutAct: {
+            const size_t elem = dtype_bytes(dt), pitch = linear_act_bytes(dt, ci);
+            staged.resize((size_t) linear_act_rows(co) * pitch);
+            for (int o = 0; o < co; ++o) {
+                unsigned char * row = staged.data() + (size_t) o * pitch;
+                const float * h = host + (size_t) o * ci;
+                if (dt == kF32) {
+                    memcpy(row, h, ci * elem);
+                } else if (dt == kBF16) {
+                    for (int c = 0; c < ci; ++c) ((uint16_t *) row)[c] = f32_to_bf16(h[c]);
+                } else {
+                    for (int c = 0; c < ci; ++c) ((_Float16 *) row)[c] = (_Float16) h[c];
+                }
+            }
+            break;
+        }
+        case kLayoutAct8: {
+            const int rows = linear_act_rows(co), cp = rows8_width(ci);
+            staged.resize(rows8_bytes(rows, ci));
+            for (int o = 0; o < co; ++o)
+                pack8_row(host + (size_t) o * ci, ci, staged.data() + (size_t) o * cp,
+                          staged.data() + rows8_scales(rows, ci) + (size_t) o * (cp / 32));
             break;
         }
         case kLayoutVector: {
@@ -627,7 +716,7 @@ trellis_status op_upload_i32(trellis_sparse_backend * backend, const int32_t * s
 
 trellis_status op_download_f32(trellis_sparse_backend * backend, const trellis_sparse_buffer * src, float * dst,
                                size_t count) {
-    if (backend == nullptr || src == nullptr || dst == nullptr || count > src->count) {
+    if (backend == nullptr || src == nullptr || dst == nullptr || count > src->count || src->dtype == kRows8) {
         return TRELLIS_STATUS_INVALID_ARGUMENT;
     }
     Backend * be = as_backend(backend);
@@ -652,7 +741,7 @@ void op_free_buffer(trellis_sparse_backend * backend, trellis_sparse_buffer * bu
     if (backend == nullptr || buffer == nullptr) return;
     Backend * be = as_backend(backend);
     DevMem m{buffer->ptr, buffer->cap};
-    dev_release(be, &m);
+    if (buffer->cap != 0) dev_release(be, &m);  // a wrapped buffer's memory is the caller's
     free(buffer);
 }
 
@@ -1937,6 +2026,403 @@ trellis_status fdg_mesh_impl(trellis_sparse_backend * backend, const int32_t * c
     return TRELLIS_STATUS_OK;
 }
 
+// ---- transformer blocks over voxel rows --------------------------------------------
+
+// The calling thread's device is left as it was.
+struct DeviceScope {
+    Backend * be;
+    int before = -1;
+    explicit DeviceScope(Backend * b) : be(b) {
+        if (hipGetDevice(&before) != hipSuccess) before = -1;
+        if (before != b->device) select_device(b);
+    }
+    ~DeviceScope() {
+        end_call(be);
+        if (before >= 0 && before != be->device) (void) hipSetDevice(before);
+    }
+};
+
+// Rows of `width` bytes, `pitch` bytes apart.
+struct Span {
+    const char * at;
+    int64_t rows, width, pitch;
+    const char * end() const { return at + (rows - 1) * pitch + width; }
+};
+
+// Whether writing `a` touches bytes of `b`.  Rows of the same pitch may lie
+// beside each other (columns of one buffer); `same` says whether the very same
+// place is fine (each element read before it is written).
+bool spans_clash(const Span & a, const Span & b, bool same) {
+    if (a.at == nullptr || b.at == nullptr || a.rows <= 0 || b.rows <= 0) return false;
+    if (a.at == b.at && a.rows == b.rows && a.width == b.width && a.pitch == b.pitch) return !same;
+    if (a.end() <= b.at || b.end() <= a.at) return false;
+    if (a.pitch != b.pitch) return true;
+    int64_t d = (b.at - a.at) % a.pitch;
+    if (d < 0) d += a.pitch;
+    return d < a.width || a.pitch - d < b.width;
+}
+
+Span packed(const trellis_sparse_buffer * b, int64_t n, int64_t c) {
+    if (b == nullptr) return Span{nullptr, 0, 0, 0};
+    const int64_t w = c * (int64_t) dtype_bytes(b->dtype);
+    return Span{(const char *) b->ptr, n, w, w};
+}
+
+bool rows8_ok(const trellis_sparse_buffer * b, int64_t n, int c) {
+    return b != nullptr && b->dtype == kRows8 && b->rows == n && b->width == c;
+}
+
+uint8_t * rows8_codes(const trellis_sparse_buffer * b) { return (uint8_t *) b->ptr; }
+uint8_t * rows8_scale_bytes(const trellis_sparse_buffer * b) {
+    return (uint8_t *) b->ptr + rows8_scales(b->rows, b->width);
+}
+
+// n rows of c channels, with sizes that every address computation holds.
+bool rows_ok(int64_t n, int64_t c) { return n > 0 && c > 0 && n <= INT64_MAX / 64 / c; }
+
+// Runs a call; a failed host allocation (packed weights, the weight table) is a
+// status, not an exception that leaves a C entry point.
+template <class F> trellis_status no_throw(trellis_sparse_backend * backend, F && call) {
+    try {
+        return call();
+    } catch (...) {
+        return fail(as_backend(backend), TRELLIS_STATUS_OUT_OF_MEMORY, "host allocation");
+    }
+}
+
+trellis_status alloc_rows8_impl(trellis_sparse_backend * backend, int64_t n, int c, trellis_sparse_buffer ** out) {
+    if (backend == nullptr || out == nullptr) return TRELLIS_STATUS_INVALID_ARGUMENT;
+    *out = nullptr;
+    Backend * be = as_backend(backend);
+    if (c <= 0 || c > INT32_MAX - 128 || !rows_ok(n, c)) {
+        return fail(be, TRELLIS_STATUS_INVALID_ARGUMENT, "alloc_rows8: bad argument");
+    }
+    DeviceScope scope(be);
+    auto * b = (trellis_sparse_buffer *) calloc(1, sizeof(trellis_sparse_buffer));
+    if (b == nullptr) return fail(be, TRELLIS_STATUS_OUT_OF_MEMORY, "host allocation");
+    DevMem m;
+    const trellis_status st = dev_alloc(be, rows8_bytes(n, c), &m);
+    if (st != TRELLIS_STATUS_OK) {
+        free(b);
+        return st;
+    }
+    b->ptr = m.ptr;
+    b->count = (size_t) n * c;
+    b->bytes = rows8_bytes(n, c);
+    b->cap = m.bytes;
+    b->dtype = kRows8;
+    b->rows = n;
+    b->width = c;
+    *out = b;
+    return TRELLIS_STATUS_OK;
+}
+
+trellis_status rms_norm_impl(trellis_sparse_backend * backend, const trellis_sparse_buffer * x,
+                             const trellis_sparse_buffer * residual, const float * gamma,
+                             trellis_sparse_buffer * total, trellis_sparse_buffer * y, int64_t n, int c, float eps) {
+    if (backend == nullptr) return TRELLIS_STATUS_INVALID_ARGUMENT;
+    Backend * be = as_backend(backend);
+    const int dt = be->policy.compute_dtype;
+    const bool to8 = y != nullptr && y->dtype == kRows8;
+    if (c <= 0 || !rows_ok(n, c) || !(eps > 0.0f) || !std::isfinite(eps) || !float_buffer_ok(be, x, (size_t) n * c) ||
+        (residual != nullptr && !float_buffer_ok(be, residual, (size_t) n * c)) ||
+        (total != nullptr && !float_buffer_ok(be, total, (size_t) n * c)) ||
+        !(to8 ? rows8_ok(y, n, c) : float_buffer_ok(be, y, (size_t) n * c))) {
+        return fail(be, TRELLIS_STATUS_INVALID_ARGUMENT, "rms_norm: bad argument");
+    }
+    const Span sx = packed(x, n, c), sr = packed(residual, n, c), st_ = packed(total, n, c);
+    const Span sy = to8 ? Span{nullptr, 0, 0, 0} : packed(y, n, c);
+    if (spans_clash(sy, sx, true) || spans_clash(sy, sr, true) || spans_clash(st_, sx, true) ||
+        spans_clash(st_, sr, true) || spans_clash(sy, st_, false)) {
+        return fail(be, TRELLIS_STATUS_INVALID_ARGUMENT, "rms_norm: overlapping rows");
+    }
+    DeviceScope scope(be);
+    const void * g = nullptr;
+    const trellis_status st = get_weight(be, gamma, (size_t) c, kLayoutVector, 0, c, &g);
+    if (st != TRELLIS_STATUS_OK) return st;
+    stage_begin(be, TRELLIS_SPARSE_HIP_STAGE_ELEMENTWISE);
+    const void * r = residual != nullptr ? residual->ptr : nullptr;
+    void * t = total != nullptr ? total->ptr : nullptr;
+    const hipError_t err =
+        to8 ? launch_rms_norm8(dt, x->ptr, r, (const float *) g, t, rows8_codes(y), rows8_scale_bytes(y), n, c, eps,
+                               be->cus, be->stream)
+            : launch_rms_norm(dt, x->ptr, r, (const float *) g, t, y->ptr, n, c, eps, be->cus, be->stream);
+    stage_end(be, TRELLIS_SPARSE_HIP_STAGE_ELEMENTWISE);
+    return hip_status(be, err, "rms_norm");
+}
+
+trellis_status pack_rows8_impl(trellis_sparse_backend * backend, const trellis_sparse_buffer * x,
+                               trellis_sparse_buffer * rows8, int64_t n, int c) {
+    if (backend == nullptr) return TRELLIS_STATUS_INVALID_ARGUMENT;
+    Backend * be = as_backend(backend);
+    if (c <= 0 || !rows_ok(n, c) || !float_buffer_ok(be, x, (size_t) n * c) || !rows8_ok(rows8, n, c)) {
+        return fail(be, TRELLIS_STATUS_INVALID_ARGUMENT, "pack_rows8: bad argument");
+    }
+    DeviceScope scope(be);
+    stage_begin(be, TRELLIS_SPARSE_HIP_STAGE_ELEMENTWISE);
+    const hipError_t err = launch_pack8(be->policy.compute_dtype, x->ptr, rows8_codes(rows8),
+                                        rows8_scale_bytes(rows8), n, c, be->cus, be->stream);
+    stage_end(be, TRELLIS_SPARSE_HIP_STAGE_ELEMENTWISE);
+    return hip_status(be, err, "pack_rows8");
+}
+
+trellis_status expand_rows8_impl(trellis_sparse_backend * backend, const trellis_sparse_buffer * rows8,
+                                 trellis_sparse_buffer * y, int64_t n, int c) {
+    if (backend == nullptr) return TRELLIS_STATUS_INVALID_ARGUMENT;
+    Backend * be = as_backend(backend);
+    if (c <= 0 || !rows_ok(n, c) || !float_buffer_ok(be, y, (size_t) n * c) || !rows8_ok(rows8, n, c)) {
+        return fail(be, TRELLIS_STATUS_INVALID_ARGUMENT, "expand_rows8: bad argument");
+    }
+    DeviceScope scope(be);
+    stage_begin(be, TRELLIS_SPARSE_HIP_STAGE_ELEMENTWISE);
+    const hipError_t err = launch_expand8(be->policy.compute_dtype, rows8_codes(rows8), rows8_scale_bytes(rows8),
+                                          y->ptr, n, c, be->stream);
+    stage_end(be, TRELLIS_SPARSE_HIP_STAGE_ELEMENTWISE);
+    return hip_status(be, err, "expand_rows8");
+}
+
+trellis_status linear_act_impl(trellis_sparse_backend * backend, const trellis_sparse_buffer * x, const float * weight,
+                               const float * bias, int act, const trellis_sparse_buffer * residual,
+                               trellis_sparse_buffer * y, int64_t n, int ci, int co) {
+    if (backend == nullptr) return TRELLIS_STATUS_INVALID_ARGUMENT;
+    Backend * be = as_backend(backend);
+    const int dt = be->policy.compute_dtype;
+    const bool from8 = x != nullptr && x->dtype == kRows8;
+    if (weight == nullptr || ci <= 0 || co <= 0 || !rows_ok(n, ci) || !rows_ok(n, co) ||
+        act < TRELLIS_SPARSE_HIP_ACT_NONE || act > TRELLIS_SPARSE_HIP_ACT_GELU_TANH ||
+        !(from8 ? rows8_ok(x, n, ci) : float_buffer_ok(be, x, (size_t) n * ci)) ||
+        (residual != nullptr && !float_buffer_ok(be, residual, (size_t) n * co)) ||
+        !float_buffer_ok(be, y, (size_t) n * co)) {
+        return fail(be, TRELLIS_STATUS_INVALID_ARGUMENT, "linear_act: bad argument");
+    }
+    if ((int64_t) ci * 4 > kLinearActMaxBytes || co > INT32_MAX - 256) {
+        return fail(be, TRELLIS_STATUS_INVALID_ARGUMENT, "linear_act: rows too wide");
+    }
+    if ((!from8 && spans_clash(packed(y, n, co), packed(x, n, ci), false)) ||
+        spans_clash(packed(y, n, co), packed(residual, n, co), true)) {
+        return fail(be, TRELLIS_STATUS_INVALID_ARGUMENT, "linear_act: overlapping rows");
+    }
+    DeviceScope scope(be);
+    LinearAct p{};
+    const void *w = nullptr, *b = nullptr;
+    trellis_status st =
+        get_weight(be, weight, (size_t) ci * co, from8 ? kLayoutAct8 : kLayoutAct, ci, co, &w);
+    if (st == TRELLIS_STATUS_OK) st = get_weight(be, bias, (size_t) co, kLayoutVector, 0, co, &b);
+    if (st != TRELLIS_STATUS_OK) return st;
+    p.x = x->ptr;
+    p.w = w;
+    if (from8) {
+        p.x_scales = rows8_scale_bytes(x);
+        p.w_scales = (const uint8_t *) w + rows8_scales(linear_act_rows(co), ci);
+        p.row_bytes = p.w_bytes = rows8_width(ci);
+    } else {
+        p.row_bytes = (int) (ci * dtype_bytes(dt));
+        p.w_bytes = linear_act_bytes(dt, ci);
+    }
+    p.bias = (const float *) b;
+    p.residual = residual != nullptr ? residual->ptr : nullptr;
+    p.y = y->ptr;
+    p.n = n;
+    p.ci = ci;
+    p.co = co;
+    stage_begin(be, TRELLIS_SPARSE_HIP_STAGE_ELEMENTWISE);
+    const hipError_t err = launch_linear_act(dt, from8 ? kRows8 : dt, p, act, be->cus, be->stream);
+    stage_end(be, TRELLIS_SPARSE_HIP_STAGE_ELEMENTWISE);
+    return hip_status(be, err, "linear_act");
+}
+
+// Rows of `width` elements at `offset`, `stride` apart (0: packed), within a
+// float buffer; 16-byte aligned when `aligned`.
+bool strided_ok(const Backend * be, const trellis_sparse_buffer * b, int64_t n, int64_t width, int64_t offset,
+                int64_t * stride) {
+    if (offset < 0 || *stride < 0 || (*stride != 0 && *stride < width)) return false;
+    if (*stride == 0) *stride = width;
+    if (*stride > INT64_MAX / 64 / n || offset > INT64_MAX / 64) return false;
+    return float_buffer_ok(be, b, (size_t) (offset + (n - 1) * *stride + width));
+}
+
+Span strided(const Backend * be, const trellis_sparse_buffer * b, int64_t n, int64_t width, int64_t offset,
+             int64_t stride) {
+    const int64_t e = (int64_t) dtype_bytes(be->policy.compute_dtype);
+    return Span{(const char *) b->ptr + offset * e, n, width * e, stride * e};
+}
+
+trellis_status rotary_impl(trellis_sparse_backend * backend, const trellis_sparse_buffer * x,
+                           const trellis_sparse_buffer * coords, const trellis_sparse_c2s_device_map * coords_map,
+                           trellis_sparse_buffer * y, int64_t n, const trellis_sparse_hip_rotary_desc * desc) {
+    if (backend == nullptr) return TRELLIS_STATUS_INVALID_ARGUMENT;
+    Backend * be = as_backend(backend);
+    if (desc == nullptr || desc->struct_size != sizeof(*desc)) {
+        return fail(be, TRELLIS_STATUS_INVALID_ARGUMENT, "rotary: bad desc");
+    }
+    const trellis_sparse_hip_rotary_desc & d = *desc;
+    if (n <= 0 || n > INT32_MAX || d.heads <= 0 || d.heads > 65536 || d.head_dim <= 0 ||
+        d.head_dim > kRotaryMaxDim || d.pairs[0] < 0 || d.pairs[1] < 0 || d.pairs[2] < 0 ||
+        (int64_t) d.pairs[0] + d.pairs[1] + d.pairs[2] > d.head_dim / 2 || !(d.base > 0.0) || !std::isfinite(d.base) ||
+        !(d.eps >= 0.0f) || !std::isfinite(d.eps) || (d.gamma != nullptr && !(d.eps > 0.0f)) ||
+        (d.split != 0 && d.split != 1)) {
+        return fail(be, TRELLIS_STATUS_INVALID_ARGUMENT, "rotary: bad argument");
+    }
+    if (d.head_dim % 8 != 0 || d.x_offset % 8 != 0 || d.x_stride % 8 != 0 || d.y_offset % 8 != 0 ||
+        d.y_stride % 8 != 0) {
+        return fail(be, TRELLIS_STATUS_NOT_IMPLEMENTED,
+                    "rotary: head_dim, offsets and strides are multiples of 8 elements");
+    }
+    const int64_t width = (int64_t) d.heads * d.head_dim;
+    int64_t xs = d.x_stride, ys = d.y_stride;
+    if (!strided_ok(be, x, n, width, d.x_offset, &xs) || !strided_ok(be, y, n, width, d.y_offset, &ys)) {
+        return fail(be, TRELLIS_STATUS_INVALID_ARGUMENT, "rotary: rows outside their buffer");
+    }
+    const int32_t * at = nullptr;
+    if (coords_map != nullptr) {
+        if (coords_map->n >= n) at = (const int32_t *) coords_map->coords.ptr;
+    } else if (coords != nullptr && coords->dtype < 0 && coords->count >= (size_t) n * 4) {
+        at = (const int32_t *) coords->ptr;
+    }
+    if (at == nullptr) return fail(be, TRELLIS_STATUS_INVALID_ARGUMENT, "rotary: coordinates are int32 [n][4]");
+    const Span sx = strided(be, x, n, width, d.x_offset, xs), sy = strided(be, y, n, width, d.y_offset, ys);
+    if (spans_clash(sy, sx, true) || spans_clash(sy, Span{(const char *) at, n, 16, 16}, false)) {
+        return fail(be, TRELLIS_STATUS_INVALID_ARGUMENT, "rotary: overlapping rows");
+    }
+    DeviceScope scope(be);
+    const void * g = nullptr;
+    const trellis_status st = get_weight(be, d.gamma, (size_t) width, kLayoutVector, 0, (int) width, &g);
+    if (st != TRELLIS_STATUS_OK) return st;
+    RotaryPlan plan{};
+    plan.n = n;
+    plan.x_stride = xs;
+    plan.y_stride = ys;
+    plan.heads = d.heads;
+    plan.dim = d.head_dim;
+    plan.split = d.split;
+    for (int a = 0; a < 3; ++a) plan.pairs[a] = d.pairs[a];
+    plan.base = d.base;
+    plan.norm = d.eps > 0.0f;
+    plan.eps = d.eps;
+    stage_begin(be, TRELLIS_SPARSE_HIP_STAGE_ELEMENTWISE);
+    const hipError_t err = launch_rotary(be->policy.compute_dtype, sx.at, at, (const float *) g, (void *) sy.at, plan,
+                                         be->cus, be->stream);
+    stage_end(be, TRELLIS_SPARSE_HIP_STAGE_ELEMENTWISE);
+    return hip_status(be, err, "rotary");
+}
+
+trellis_status attention_impl(trellis_sparse_backend * backend, const trellis_sparse_buffer * q,
+                              const trellis_sparse_buffer * k, const trellis_sparse_buffer * v,
+                              trellis_sparse_buffer * y, int64_t nq, int64_t nkv,
+                              const trellis_sparse_buffer * q_offsets, const trellis_sparse_buffer * kv_offsets,
+                              int n_seqs, const trellis_sparse_hip_attention_desc * desc) {
+    if (backend == nullptr) return TRELLIS_STATUS_INVALID_ARGUMENT;
+    Backend * be = as_backend(backend);
+    if (desc == nullptr || desc->struct_size != sizeof(*desc)) {
+        return fail(be, TRELLIS_STATUS_INVALID_ARGUMENT, "attention: bad desc");
+    }
+    const trellis_sparse_hip_attention_desc & d = *desc;
+    if (nq <= 0 || nq > INT32_MAX || nkv < 0 || nkv > INT32_MAX || d.heads <= 0 || d.heads > 65536 ||
+        d.kv_heads <= 0 || d.heads % d.kv_heads != 0 || d.head_dim <= 0 || !std::isfinite(d.scale) ||
+        (q_offsets == nullptr) != (kv_offsets == nullptr) || n_seqs <= 0 || (q_offsets == nullptr && n_seqs != 1)) {
+        return fail(be, TRELLIS_STATUS_INVALID_ARGUMENT, "attention: bad argument");
+    }
+    if (d.head_dim > kAttentionMaxDim) {
+        return fail(be, TRELLIS_STATUS_NOT_IMPLEMENTED, "attention: head_dim up to 192");
+    }
+    for (const trellis_sparse_buffer * b : {q_offsets, kv_offsets}) {
+        if (b != nullptr && (b->dtype >= 0 || b->count < (size_t) n_seqs + 1)) {
+            return fail(be, TRELLIS_STATUS_INVALID_ARGUMENT, "attention: offsets are int32 [n_seqs + 1]");
+        }
+    }
+    const int64_t qw = (int64_t) d.heads * d.head_dim, kw = (int64_t) d.kv_heads * d.head_dim;
+    const int64_t nk = nkv > 0 ? nkv : 1;
+    int64_t qs = d.q_stride, ks = d.k_stride, vs = d.v_stride, ys = d.y_stride;
+    if (!strided_ok(be, q, nq, qw, d.q_offset, &qs) || !strided_ok(be, y, nq, qw, d.y_offset, &ys) ||
+        (nkv > 0 && (!strided_ok(be, k, nk, kw, d.k_offset, &ks) || !strided_ok(be, v, nk, kw, d.v_offset, &vs)))) {
+        return fail(be, TRELLIS_STATUS_INVALID_ARGUMENT, "attention: rows outside their buffer");
+    }
+    const Span sq = strided(be, q, nq, qw, d.q_offset, qs), sy = strided(be, y, nq, qw, d.y_offset, ys);
+    Span sk{nullptr, 0, 0, 0}, sv{nullptr, 0, 0, 0};
+    if (nkv > 0) {
+        sk = strided(be, k, nkv, kw, d.k_offset, ks);
+        sv = strided(be, v, nkv, kw, d.v_offset, vs);
+    }
+    // Other blocks still read keys and values where one has written its queries' rows; q itself may be y.
+    if (spans_clash(sy, sq, true) || spans_clash(sy, sk, false) || spans_clash(sy, sv, false)) {
+        return fail(be, TRELLIS_STATUS_INVALID_ARGUMENT, "attention: overlapping rows");
+    }
+    DeviceScope scope(be);
+    Attention p{};
+    p.q = sq.at;
+    p.k = sk.at;
+    p.v = sv.at;
+    p.y = (void *) sy.at;
+    p.q_at = q_offsets != nullptr ? (const int32_t *) q_offsets->ptr : nullptr;
+    p.k_at = kv_offsets != nullptr ? (const int32_t *) kv_offsets->ptr : nullptr;
+    p.nq = nq;
+    p.nk = nkv;
+    p.q_stride = qs;
+    p.k_stride = ks;
+    p.v_stride = vs;
+    p.y_stride = ys;
+    p.seqs = n_seqs;
+    p.heads = d.heads;
+    p.kv_heads = d.kv_heads;
+    p.dim = d.head_dim;
+    const double scale = d.scale == 0.0f ? 1.0 / std::sqrt((double) d.head_dim) : (double) d.scale;
+    p.scale = (float) (scale * 1.4426950408889634);
+    stage_begin(be, TRELLIS_SPARSE_HIP_STAGE_ELEMENTWISE);
+    const hipError_t err = launch_attention(be->policy.compute_dtype, p, be->stream);
+    stage_end(be, TRELLIS_SPARSE_HIP_STAGE_ELEMENTWISE);
+    return hip_status(be, err, "attention");
+}
+
+// ---- the caller's memory and stream ---------------------------------------------------
+
+trellis_status wrap_impl(trellis_sparse_backend * backend, void * ptr, size_t count, int dtype,
+                         trellis_sparse_buffer ** out) {
+    if (backend == nullptr || out == nullptr) return TRELLIS_STATUS_INVALID_ARGUMENT;
+    *out = nullptr;
+    Backend * be = as_backend(backend);
+    const size_t elem = dtype < 0 ? 4 : dtype_bytes(dtype);
+    if (ptr == nullptr || count == 0 || count > SIZE_MAX / elem || (uintptr_t) ptr % 16 != 0) {
+        return fail(be, TRELLIS_STATUS_INVALID_ARGUMENT, "wrap: 16-byte aligned device memory");
+    }
+    DeviceScope scope(be);
+    hipPointerAttribute_t attr{};
+    hipDeviceptr_t base = nullptr;
+    size_t size = 0;
+    if (hipPointerGetAttributes(&attr, ptr) != hipSuccess || attr.type != hipMemoryTypeDevice ||
+        attr.device != be->device || hipMemGetAddressRange(&base, &size, (hipDeviceptr_t) ptr) != hipSuccess) {
+        (void) hipGetLastError();
+        return fail(be, TRELLIS_STATUS_INVALID_ARGUMENT, "wrap: not memory of this backend's device");
+    }
+    if ((size_t) ((char *) ptr - (char *) base) > size || count * elem > size - (size_t) ((char *) ptr - (char *) base)) {
+        return fail(be, TRELLIS_STATUS_INVALID_ARGUMENT, "wrap: beyond the end of its allocation");
+    }
+    auto * b = (trellis_sparse_buffer *) calloc(1, sizeof(trellis_sparse_buffer));
+    if (b == nullptr) return fail(be, TRELLIS_STATUS_OUT_OF_MEMORY, "host allocation");
+    b->ptr = ptr;
+    b->count = count;
+    b->bytes = count * elem;
+    b->cap = 0;
+    b->dtype = dtype;
+    *out = b;
+    return TRELLIS_STATUS_OK;
+}
+
+trellis_status set_stream_impl(trellis_sparse_backend * backend, hipStream_t stream) {
+    if (backend == nullptr) return TRELLIS_STATUS_INVALID_ARGUMENT;
+    Backend * be = as_backend(backend);
+    if (stream == be->stream) return TRELLIS_STATUS_OK;
+    DeviceScope scope(be);
+    if (be->stream_left == nullptr) {
+        TSH_TRY(be, hipEventCreateWithFlags(&be->stream_left, hipEventDisableTiming));
+    }
+    // Pool blocks and weights in use by the old stream's work come to the new
+    // one without further waits.
+    TSH_TRY(be, hipEventRecord(be->stream_left, be->stream));
+    TSH_TRY(be, hipStreamWaitEvent(stream, be->stream_left, 0));
+    be->stream = stream;
+    return TRELLIS_STATUS_OK;
+}
+
 trellis_status op_trim(trellis_sparse_backend * backend, unsigned flags, size_t * released_bytes) {
     if (released_bytes != nullptr) *released_bytes = 0;
     if (backend == nullptr || (flags & ~(unsigned) TRELLIS_SPARSE_TRIM_ALL) != 0) {
@@ -2038,7 +2524,8 @@ void op_destroy(trellis_sparse_backend * backend) {
     if (be->words_ready != nullptr) (void) hipEventDestroy(be->words_ready);
     if (be->copy_from != nullptr) (void) hipEventDestroy(be->copy_from);
     if (be->copy_stream != nullptr) (void) hipStreamDestroy(be->copy_stream);
-    (void) hipStreamDestroy(be->stream);
+    if (be->stream_left != nullptr) (void) hipEventDestroy(be->stream_left);
+    (void) hipStreamDestroy(be->own_stream);
     delete be;
 }
 
@@ -2098,11 +2585,12 @@ trellis_status trellis_sparse_hip_backend_create_ex(int device, const trellis_sp
     auto * be = new (std::nothrow) Backend();
     if (be == nullptr) return TRELLIS_STATUS_OUT_OF_MEMORY;
     be->cus = cus;
-    if (hipStreamCreateWithFlags(&be->stream, hipStreamNonBlocking) != hipSuccess) {
+    if (hipStreamCreateWithFlags(&be->own_stream, hipStreamNonBlocking) != hipSuccess) {
         (void) hipGetLastError();
         delete be;
         return TRELLIS_STATUS_CUDA_UNAVAILABLE;
     }
+    be->stream = be->own_stream;
     // Small reads fall back to pageable copies and a stream synchronisation
     // when either of these is missing.
     if (hipHostMalloc((void **) &be->host_words, tsh::kHostWords * 4, hipHostMallocDefault) != hipSuccess) {
@@ -2281,7 +2769,7 @@ trellis_status trellis_sparse_hip_upload_raw(trellis_sparse_backend * backend, c
 
 trellis_status trellis_sparse_hip_download_raw(trellis_sparse_backend * backend, const trellis_sparse_buffer * src,
                                                void * dst, size_t count) {
-    if (backend == nullptr || src == nullptr || dst == nullptr || count > src->count) {
+    if (backend == nullptr || src == nullptr || dst == nullptr || count > src->count || src->dtype == tsh::kRows8) {
         return TRELLIS_STATUS_INVALID_ARGUMENT;
     }
     Backend * be = tsh::as_backend(backend);
@@ -2439,6 +2927,84 @@ trellis_status trellis_sparse_hip_conv_add(trellis_sparse_backend * backend, con
                                            const float * bias, const trellis_sparse_buffer * residual,
                                            trellis_sparse_buffer * out, int64_t n, int ci, int co) {
     return tsh::conv_add_impl(backend, rulebook, feats, weight, bias, residual, out, n, ci, co);
+}
+
+trellis_status trellis_sparse_hip_wrap_f32(trellis_sparse_backend * backend, void * device_ptr, size_t count,
+                                           trellis_sparse_buffer ** out) {
+    return tsh::wrap_impl(backend, device_ptr, count,
+                          backend != nullptr ? tsh::as_backend(backend)->policy.compute_dtype : 0, out);
+}
+
+trellis_status trellis_sparse_hip_wrap_i32(trellis_sparse_backend * backend, void * device_ptr, size_t count,
+                                           trellis_sparse_buffer ** out) {
+    return tsh::wrap_impl(backend, device_ptr, count, -1, out);
+}
+
+trellis_status trellis_sparse_hip_set_stream(trellis_sparse_backend * backend, void * stream) {
+    return tsh::set_stream_impl(backend, (hipStream_t) stream);
+}
+
+trellis_status trellis_sparse_hip_own_stream(trellis_sparse_backend * backend) {
+    return tsh::set_stream_impl(backend, backend != nullptr ? tsh::as_backend(backend)->own_stream : nullptr);
+}
+
+trellis_status trellis_sparse_hip_alloc_rows8(trellis_sparse_backend * backend, int64_t n, int c,
+                                              trellis_sparse_buffer ** out) {
+    return tsh::no_throw(backend, [&] {
+        return tsh::alloc_rows8_impl(backend, n, c, out);
+    });
+}
+
+trellis_status trellis_sparse_hip_pack_rows8(trellis_sparse_backend * backend, const trellis_sparse_buffer * x,
+                                             trellis_sparse_buffer * rows8, int64_t n, int c) {
+    return tsh::no_throw(backend, [&] {
+        return tsh::pack_rows8_impl(backend, x, rows8, n, c);
+    });
+}
+
+trellis_status trellis_sparse_hip_expand_rows8(trellis_sparse_backend * backend, const trellis_sparse_buffer * rows8,
+                                               trellis_sparse_buffer * y, int64_t n, int c) {
+    return tsh::no_throw(backend, [&] {
+        return tsh::expand_rows8_impl(backend, rows8, y, n, c);
+    });
+}
+
+trellis_status trellis_sparse_hip_rms_norm(trellis_sparse_backend * backend, const trellis_sparse_buffer * x,
+                                           const trellis_sparse_buffer * residual, const float * gamma,
+                                           trellis_sparse_buffer * total, trellis_sparse_buffer * y, int64_t n, int c,
+                                           float eps) {
+    return tsh::no_throw(backend, [&] {
+        return tsh::rms_norm_impl(backend, x, residual, gamma, total, y, n, c, eps);
+    });
+}
+
+trellis_status trellis_sparse_hip_linear_act(trellis_sparse_backend * backend, const trellis_sparse_buffer * x,
+                                             const float * weight, const float * bias, int act,
+                                             const trellis_sparse_buffer * residual, trellis_sparse_buffer * y,
+                                             int64_t n, int ci, int co) {
+    return tsh::no_throw(backend, [&] {
+        return tsh::linear_act_impl(backend, x, weight, bias, act, residual, y, n, ci, co);
+    });
+}
+
+trellis_status trellis_sparse_hip_rotary(trellis_sparse_backend * backend, const trellis_sparse_buffer * x,
+                                         const trellis_sparse_buffer * coords,
+                                         const trellis_sparse_c2s_device_map * coords_map, trellis_sparse_buffer * y,
+                                         int64_t n, const trellis_sparse_hip_rotary_desc * desc) {
+    return tsh::no_throw(backend, [&] {
+        return tsh::rotary_impl(backend, x, coords, coords_map, y, n, desc);
+    });
+}
+
+trellis_status trellis_sparse_hip_attention(trellis_sparse_backend * backend, const trellis_sparse_buffer * q,
+                                            const trellis_sparse_buffer * k, const trellis_sparse_buffer * v,
+                                            trellis_sparse_buffer * y, int64_t nq, int64_t nkv,
+                                            const trellis_sparse_buffer * q_offsets,
+                                            const trellis_sparse_buffer * kv_offsets, int n_seqs,
+                                            const trellis_sparse_hip_attention_desc * desc) {
+    return tsh::no_throw(backend, [&] {
+        return tsh::attention_impl(backend, q, k, v, y, nq, nkv, q_offsets, kv_offsets, n_seqs, desc);
+    });
 }
 
 trellis_status trellis_sparse_hip_profile_enable(trellis_sparse_backend * backend, int enable) {

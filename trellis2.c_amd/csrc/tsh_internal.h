@@ -66,6 +66,15 @@ template <> struct Store<kBF16> {
     }
 };
 
+// 8-bit rows (a buffer's dtype beside the storage types): [n][rows8_width(c)]
+// e4m3 codes, zeros beyond c, then, from rows8_scales on, one scale byte (a
+// power of two, 127 + exponent; 255 = NaN) per 32 channels, [n][width / 32].
+// Rows are whole 128-byte steps of the scaled MFMA.
+constexpr int kRows8 = 3;
+__host__ __device__ inline int rows8_width(int c) { return (c + 127) / 128 * 128; }
+inline size_t rows8_scales(int64_t n, int c) { return ((size_t) n * rows8_width(c) + 255) / 256 * 256; }
+inline size_t rows8_bytes(int64_t n, int c) { return rows8_scales(n, c) + (size_t) n * (rows8_width(c) / 32); }
+
 // A 16-byte chunk of 16-bit storage values (8 of them) to fp32 and back,
 // with round-to-nearest-even on the way back.
 template <int DT> __device__ inline void unpack_chunk(const int4 & c, float * v) {
@@ -134,8 +143,10 @@ struct trellis_sparse_buffer {
     void * ptr;
     size_t count;   // elements
     size_t bytes;   // count * element size
-    size_t cap;     // bytes actually reserved (pool size class)
-    int dtype;      // tsh::Dtype of the storage, or -1 for raw int32
+    size_t cap;     // bytes actually reserved (pool size class); 0: the caller's own memory
+    int dtype;      // tsh::Dtype of the storage, -1 for raw int32, tsh::kRows8
+    int64_t rows;   // 8-bit rows: their count
+    int width;      // 8-bit rows: channels
 };
 
 struct trellis_sparse_rulebook {
@@ -341,6 +352,62 @@ hipError_t launch_s2c_pack(int dtype, const void * x, const int32_t * child, voi
                            hipStream_t s);
 hipError_t launch_s2c_skip_mean(int dtype, const void * x, const int32_t * child, void * y, int64_t m, int ci,
                                 int co, hipStream_t s);
+
+// Row operators of transformer blocks (kernels_rows.hip).  residual, gamma and
+// total may be null; total and y may be x or residual themselves.
+hipError_t launch_rms_norm(int dtype, const void * x, const void * residual, const float * gamma, void * total,
+                           void * y, int64_t n, int c, float eps, int cus, hipStream_t s);
+hipError_t launch_rms_norm8(int dtype, const void * x, const void * residual, const float * gamma, void * total,
+                            uint8_t * codes, uint8_t * scales, int64_t n, int c, float eps, int cus, hipStream_t s);
+hipError_t launch_pack8(int dtype, const void * x, uint8_t * codes, uint8_t * scales, int64_t n, int c, int cus,
+                        hipStream_t s);
+hipError_t launch_expand8(int dtype, const uint8_t * codes, const uint8_t * scales, void * y, int64_t n, int c,
+                          hipStream_t s);
+constexpr int kRotaryMaxDim = 256;
+struct RotaryPlan {
+    int64_t n, x_stride, y_stride;
+    int heads, dim, split, pairs[3];
+    double base;
+    bool norm;
+    float eps;
+};
+hipError_t launch_rotary(int dtype, const void * x, const int32_t * coords, const float * gamma, void * y,
+                         const RotaryPlan & plan, int cus, hipStream_t s);
+// Linear with activation and residual (kernels_act.hip).  w: rows of w_bytes (a
+// multiple of 128, zeros beyond ci), linear_act_rows(co) of them, in the
+// storage type or, for x_type kRows8, as 8-bit rows.
+struct LinearAct {
+    const void * x;
+    const uint8_t * x_scales;
+    const void * w;
+    const uint8_t * w_scales;
+    const float * bias;      // [co] or null
+    const void * residual;   // [n][co] or null; may be y
+    void * y;
+    int64_t n;
+    int ci, co;
+    int row_bytes, w_bytes;  // of a row of x and of w
+    int64_t row_tiles;       // set by the launcher
+    int col_tiles;
+};
+inline int linear_act_rows(int co) { return (co + 255) / 256 * 256; }
+// Widest row: a block's 256 rows stay below 2 GiB.
+constexpr int kLinearActMaxBytes = 1 << 22;
+hipError_t launch_linear_act(int dtype, int x_type, const LinearAct & p, int act, int cus, hipStream_t s);
+// Attention within sequences of rows (kernels_attn.hip).
+struct Attention {
+    const void * q;
+    const void * k;
+    const void * v;
+    void * y;
+    const int32_t * q_at;    // [seqs + 1] or null: one sequence of all rows
+    const int32_t * k_at;
+    int64_t nq, nk, q_stride, k_stride, v_stride, y_stride;
+    int seqs, heads, kv_heads, dim;
+    float scale;             // times log2(e)
+};
+constexpr int kAttentionMaxDim = 192;
+hipError_t launch_attention(int dtype, const Attention & p, hipStream_t s);
 
 // Narrow MFMA linear (bf16/fp16, Co <= 16, Ci a power of two in 32..1024):
 // weights [co][ci] in the storage type.

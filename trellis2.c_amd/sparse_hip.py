@@ -32,6 +32,7 @@ TRIM_FREE_BUFFERS, TRIM_WEIGHTS = 1, 2
 F32, F16, BF16 = 0, 1, 2
 CONV_AUTO, CONV_GENERIC, CONV_MASKED, CONV_COMPACT = 0, 1, 2, 3
 LINEAR_AUTO, LINEAR_KERNEL = 0, 1
+ACTS = {"none": 0, "silu": 1, "gelu": 2, "gelu_tanh": 3}
 STAGES = ["hash", "map", "conv", "subdivide", "broadcast", "elementwise"]
 
 _p = c_void_p  # opaque pointers (buffer, rulebook, device map, backend)
@@ -95,6 +96,19 @@ class Mesh(Structure):
                 ("n_vertices", c_int64), ("n_faces", c_int64)]
 
 
+class RotaryDesc(Structure):
+    _fields_ = [("struct_size", c_uint32), ("heads", c_int32), ("head_dim", c_int32), ("pairs", c_int32 * 3),
+                ("split", c_int32), ("eps", c_float), ("base", c_double), ("gamma", _f32p), ("x_offset", c_int64),
+                ("x_stride", c_int64), ("y_offset", c_int64), ("y_stride", c_int64)]
+
+
+class AttentionDesc(Structure):
+    _fields_ = [("struct_size", c_uint32), ("heads", c_int32), ("kv_heads", c_int32), ("head_dim", c_int32),
+                ("scale", c_float), ("q_offset", c_int64), ("q_stride", c_int64), ("k_offset", c_int64),
+                ("k_stride", c_int64), ("v_offset", c_int64), ("v_stride", c_int64), ("y_offset", c_int64),
+                ("y_stride", c_int64)]
+
+
 # The C ABI of include/trellis_sparse_hip.h: name -> (restype, argtypes).
 ABI = {
     "trellis_sparse_hip_policy_init": (None, [POINTER(Policy)]),
@@ -136,6 +150,18 @@ ABI = {
     "trellis_sparse_hip_conv_norm": (c_int, [_p, _p, _p, _f32p, _f32p, _f32p, _f32p, c_float, c_int, _p, c_int64,
                                              c_int, c_int]),
     "trellis_sparse_hip_conv_add": (c_int, [_p, _p, _p, _f32p, _f32p, _p, _p, c_int64, c_int, c_int]),
+    "trellis_sparse_hip_wrap_f32": (c_int, [_p, c_void_p, c_size_t, POINTER(_p)]),
+    "trellis_sparse_hip_wrap_i32": (c_int, [_p, c_void_p, c_size_t, POINTER(_p)]),
+    "trellis_sparse_hip_set_stream": (c_int, [_p, c_void_p]),
+    "trellis_sparse_hip_own_stream": (c_int, [_p]),
+    "trellis_sparse_hip_alloc_rows8": (c_int, [_p, c_int64, c_int, POINTER(_p)]),
+    "trellis_sparse_hip_pack_rows8": (c_int, [_p, _p, _p, c_int64, c_int]),
+    "trellis_sparse_hip_expand_rows8": (c_int, [_p, _p, _p, c_int64, c_int]),
+    "trellis_sparse_hip_rms_norm": (c_int, [_p, _p, _p, _f32p, _p, _p, c_int64, c_int, c_float]),
+    "trellis_sparse_hip_linear_act": (c_int, [_p, _p, _f32p, _f32p, c_int, _p, _p, c_int64, c_int, c_int]),
+    "trellis_sparse_hip_rotary": (c_int, [_p, _p, _p, _p, _p, c_int64, POINTER(RotaryDesc)]),
+    "trellis_sparse_hip_attention": (c_int, [_p, _p, _p, _p, _p, c_int64, c_int64, _p, _p, c_int,
+                                             POINTER(AttentionDesc)]),
 }
 
 
@@ -411,6 +437,81 @@ class Backend:
         out = np.empty(count, dtype=np.float32 if self.dtype == F32 else np.uint16)
         self._check(LIB.trellis_sparse_hip_download_raw(self.ptr, buf.handle, out.ctypes.data, count), "download_raw")
         return out
+
+    # -- the caller's memory and stream ---------------------------------------------
+    def wrap(self, tensor) -> Buffer:
+        """A buffer over a contiguous device tensor's memory (anything with torch's data_ptr(), numel() and dtype): of
+        the backend's dtype, or int32.  The buffer keeps the tensor.  A process that uses torch imports it before this
+        module, so that both use the HIP runtime that torch brings."""
+        name = str(tensor.dtype).rpartition(".")[2]
+        if name != "int32" and name != ("float32", "float16", "bfloat16")[self.dtype]:
+            raise TypeError(f"wrap: {name} rows on a backend of dtype {self.dtype}")
+        if not tensor.is_contiguous():
+            raise ValueError("wrap: the tensor is not contiguous")
+        fn = LIB.trellis_sparse_hip_wrap_i32 if name == "int32" else LIB.trellis_sparse_hip_wrap_f32
+        h = c_void_p()
+        count = tensor.numel()
+        self._check(fn(self.ptr, tensor.data_ptr(), count, ctypes.byref(h)), "wrap")
+        buf = Buffer(self, h, count)
+        buf.tensor = tensor
+        return buf
+
+    def set_stream(self, stream: int | None):
+        """Queue on a hipStream_t (0: the default stream; None: the backend's own)."""
+        st = (LIB.trellis_sparse_hip_own_stream(self.ptr) if stream is None else
+              LIB.trellis_sparse_hip_set_stream(self.ptr, stream))
+        self._check(st, "set_stream")
+
+    # -- transformer blocks over voxel rows -----------------------------------------
+    def alloc_rows8(self, n: int, c: int) -> Buffer:
+        """8-bit rows: e4m3 values with one power-of-two scale per 32 channels."""
+        h = c_void_p()
+        self._check(LIB.trellis_sparse_hip_alloc_rows8(self.ptr, n, c, ctypes.byref(h)), "alloc_rows8")
+        return Buffer(self, h, n * c)
+
+    def pack_rows8(self, x: Buffer, rows8: Buffer, n: int, c: int):
+        self._check(LIB.trellis_sparse_hip_pack_rows8(self.ptr, x.handle, rows8.handle, n, c), "pack_rows8")
+
+    def expand_rows8(self, rows8: Buffer, y: Buffer, n: int, c: int):
+        self._check(LIB.trellis_sparse_hip_expand_rows8(self.ptr, rows8.handle, y.handle, n, c), "expand_rows8")
+
+    def rms_norm(self, x: Buffer, gamma, y: Buffer, n: int, c: int, eps: float, residual: Buffer | None = None,
+                 total: Buffer | None = None):
+        """total = x + residual; y (rows or 8-bit rows) = total / sqrt(mean(total^2) + eps) * gamma."""
+        g = None if gamma is None else self.keep(_f32(gamma))
+        self._check(LIB.trellis_sparse_hip_rms_norm(self.ptr, x.handle, residual and residual.handle, _ptr(g, _f32p),
+                                                    total and total.handle, y.handle, n, c, eps), "rms_norm")
+
+    def linear_act(self, x: Buffer, weight, bias, y: Buffer, n: int, ci: int, co: int, act: str = "none",
+                   residual: Buffer | None = None):
+        """y = act(x W^T + bias) + residual, x rows or 8-bit rows; act one of ACTS."""
+        w = self.keep(_f32(weight))
+        b = None if bias is None else self.keep(_f32(bias))
+        self._check(LIB.trellis_sparse_hip_linear_act(self.ptr, x.handle, _ptr(w, _f32p), _ptr(b, _f32p), ACTS[act],
+                                                      residual and residual.handle, y.handle, n, ci, co), "linear_act")
+
+    def rotary(self, x: Buffer, coords, y: Buffer, n: int, heads: int, head_dim: int, pairs, base: float = 10000.0,
+               split: bool = False, gamma=None, eps: float | None = None, x_offset: int = 0, x_stride: int = 0,
+               y_offset: int = 0, y_stride: int = 0):
+        """Rotary positions with three axes; coords an int32 buffer [n][4] or a DeviceMap; eps: RMS norm per head first."""
+        g = None if gamma is None else self.keep(_f32(gamma))
+        d = RotaryDesc(ctypes.sizeof(RotaryDesc), heads, head_dim, (c_int32 * 3)(*pairs), int(split),
+                       0.0 if eps is None else eps, base, _ptr(g, _f32p), x_offset, x_stride, y_offset, y_stride)
+        at, dmap = (None, coords.handle) if isinstance(coords, DeviceMap) else (coords.handle, None)
+        self._check(LIB.trellis_sparse_hip_rotary(self.ptr, x.handle, at, dmap, y.handle, n, ctypes.byref(d)), "rotary")
+
+    def attention(self, q: Buffer, k: Buffer | None, v: Buffer | None, y: Buffer, nq: int, nkv: int, heads: int,
+                  kv_heads: int, head_dim: int, scale: float = 0.0, q_offsets: Buffer | None = None,
+                  kv_offsets: Buffer | None = None, q_offset: int = 0, q_stride: int = 0, k_offset: int = 0,
+                  k_stride: int = 0, v_offset: int = 0, v_stride: int = 0, y_offset: int = 0, y_stride: int = 0):
+        """Attention within sequences: q_offsets and kv_offsets int32 [sequences + 1], or neither for one sequence."""
+        d = AttentionDesc(ctypes.sizeof(AttentionDesc), heads, kv_heads, head_dim, scale, q_offset, q_stride, k_offset,
+                          k_stride, v_offset, v_stride, y_offset, y_stride)
+        seqs = 1 if q_offsets is None else q_offsets.count - 1
+        self._check(LIB.trellis_sparse_hip_attention(self.ptr, q.handle, k and k.handle, v and v.handle, y.handle, nq,
+                                                     nkv, q_offsets and q_offsets.handle,
+                                                     kv_offsets and kv_offsets.handle, seqs, ctypes.byref(d)),
+                    "attention")
 
     # -- rulebook / conv --------------------------------------------------------
     def build_rulebook(self, coords) -> Rulebook:
