@@ -2367,9 +2367,16 @@ trellis_status attention_impl(trellis_sparse_backend * backend, const trellis_sp
     p.dim = d.head_dim;
     const double scale = d.scale == 0.0f ? 1.0 / std::sqrt((double) d.head_dim) : (double) d.scale;
     p.scale = (float) (scale * 1.4426950408889634);
+    // Scratch for split keys is the pool's; where none is to be had (also under
+    // capture, where two graphs could share it) one block takes all of a
+    // query's keys.
+    const AttentionShape shape = attention_shape(be->policy.compute_dtype, p, be->cus);
+    DevMem scratch;
+    if (shape.scratch > 0 && dev_alloc(be, shape.scratch, &scratch) != TRELLIS_STATUS_OK) be->last_error.clear();
     stage_begin(be, TRELLIS_SPARSE_HIP_STAGE_ELEMENTWISE);
-    const hipError_t err = launch_attention(be->policy.compute_dtype, p, be->stream);
+    const hipError_t err = launch_attention(be->policy.compute_dtype, p, shape, scratch.ptr, be->stream);
     stage_end(be, TRELLIS_SPARSE_HIP_STAGE_ELEMENTWISE);
+    dev_release(be, &scratch);
     return hip_status(be, err, "attention");
 }
 

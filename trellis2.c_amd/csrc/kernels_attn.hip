@@ -4,11 +4,17 @@
 namespace tsh {
 namespace {
 
-// A block's place: rows [q0, q0 + nq) of one sequence's queries, keys [k0, k0 + nk).
+// A block's place: nq queries from `first` of a sequence whose rows begin at q0, its keys [k0, k0 + nk).
 struct Place {
-    int64_t q0, k0;
+    int64_t q0, first, k0;
     int nq, nk;
 };
+
+// The same value in every lane, in scalar registers.
+__device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
+__device__ __forceinline__ int64_t uniform(int64_t v) {
+    return (int64_t) (((uint64_t) (uint32_t) uniform((int) (v >> 32)) << 32) | (uint32_t) uniform((int) v));
+}
 
 __device__ __forceinline__ int64_t offset_of(const int32_t * at, int i, int64_t n) {
     const int64_t v = at[i];
@@ -16,14 +22,15 @@ __device__ __forceinline__ int64_t offset_of(const int32_t * at, int i, int64_t 
 }
 
 // Tile `tile` of TQ queries among all sequences' tiles, in order; nq = 0 past
-// the last.  Offsets are read on the device, so a grid has an upper bound of
-// tiles; they are clamped to the rows that there are, and a sequence whose
-// offsets fall is empty.
-template <int TQ> __device__ Place find_place(const Attention & p, int64_t tile) {
-    Place r{0, 0, 0, 0};
+// the last.  A query is a row and one of the `group` heads that share a kv head:
+// query i of a sequence is its row i / group, head i % group of them.  Offsets
+// are read on the device, so a grid has an upper bound of tiles; they are
+// clamped to the rows that there are, and a sequence whose offsets fall is empty.
+template <int TQ> __device__ Place find_place(const Attention & p, int64_t tile, int group) {
+    Place r{0, 0, 0, 0, 0};
     if (p.q_at == nullptr) {
-        r.q0 = tile * TQ;
-        r.nq = (int) max((int64_t) 0, min((int64_t) TQ, p.nq - r.q0));
+        r.first = tile * TQ;
+        r.nq = (int) max((int64_t) 0, min((int64_t) TQ, p.nq * group - r.first));
         r.nk = (int) p.nk;
         return r;
     }
@@ -34,26 +41,25 @@ template <int TQ> __device__ Place find_place(const Attention & p, int64_t tile)
         int64_t lo = 0, len = 0;
         if (i < p.seqs) {
             lo = offset_of(p.q_at, i, p.nq);
-            len = max((int64_t) 0, offset_of(p.q_at, i + 1, p.nq) - lo);
+            len = max((int64_t) 0, offset_of(p.q_at, i + 1, p.nq) - lo) * group;
         }
-        int64_t sum = (len + TQ - 1) / TQ;
+        const int64_t tiles = (len + TQ - 1) / TQ;
+        int64_t sum = tiles;
         for (int d = 1; d < 64; d <<= 1) {
             const int64_t o = __shfl_up(sum, d);
             if (lane >= d) sum += o;
         }
         const unsigned long long past = __ballot(sum > tile);
         if (past != 0) {
-            const int at = __ffsll(past) - 1;
-            const int64_t tiles = (len + TQ - 1) / TQ;
-            const int64_t in = tile - __shfl(sum - tiles, at);
-            const int seq = s0 + at;
-            r.q0 = __shfl(lo, at) + in * TQ;
-            r.nq = (int) min((int64_t) TQ, __shfl(len, at) - in * TQ);
-            r.k0 = offset_of(p.k_at, seq, p.nk);
-            r.nk = (int) max((int64_t) 0, offset_of(p.k_at, seq + 1, p.nk) - r.k0);
+            const int at = __ffsll(past) - 1, seq = s0 + at;
+            r.q0 = uniform((int64_t) __shfl(lo, at));
+            r.first = uniform((tile - __shfl(sum - tiles, at)) * TQ);
+            r.nq = uniform((int) min((int64_t) TQ, __shfl(len, at) - r.first));
+            r.k0 = uniform(offset_of(p.k_at, seq, p.nk));
+            r.nk = uniform((int) max((int64_t) 0, offset_of(p.k_at, seq + 1, p.nk) - r.k0));
             return r;
         }
-        tile -= __shfl(sum, 63);
+        tile -= uniform((int64_t) __shfl(sum, 63));
     }
     return r;
 }
@@ -71,7 +77,7 @@ template <int DT> __global__ void __launch_bounds__(256) k_attention_any(Attenti
     float * s_v = s_k + TK * pitch;      // [TK][pitch]
     float * s_p = s_v + TK * pitch;      // [TQ][TK + 1]
     const int head = blockIdx.x % p.heads;
-    const Place at = find_place<TQ>(p, blockIdx.x / p.heads);
+    const Place at = find_place<TQ>(p, blockIdx.x / p.heads, 1);
     if (at.nq <= 0) return;
     const int kv = head / (p.heads / p.kv_heads);
     const T * q = (const T *) p.q + (int64_t) head * p.dim;
@@ -80,7 +86,7 @@ template <int DT> __global__ void __launch_bounds__(256) k_attention_any(Attenti
     const int t = threadIdx.x, row = t / 16, l = t % 16;
     for (int i = t; i < TQ * p.dim; i += 256) {
         const int r = i / p.dim, c = i % p.dim;
-        s_q[r * pitch + c] = r < at.nq ? Store<DT>::ld(q, (at.q0 + r) * p.q_stride + c) : 0.0f;
+        s_q[r * pitch + c] = r < at.nq ? Store<DT>::ld(q, (at.q0 + at.first + r) * p.q_stride + c) : 0.0f;
     }
     float most = -__builtin_inff(), sum = 0.0f;
     float acc[kAttentionMaxDim / 16];
@@ -129,7 +135,7 @@ template <int DT> __global__ void __launch_bounds__(256) k_attention_any(Attenti
     if (row < at.nq) {
         // No keys (or none above -inf): zeros.
         const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-        T * y = (T *) p.y + (at.q0 + row) * p.y_stride + (int64_t) head * p.dim;
+        T * y = (T *) p.y + (at.q0 + at.first + row) * p.y_stride + (int64_t) head * p.dim;
 #pragma unroll
         for (int u = 0; u < kAttentionMaxDim / 16; ++u) {
             const int c = u * 16 + l;
@@ -148,14 +154,381 @@ template <int DT> hipError_t launch_any(const Attention & p, hipStream_t s) {
     return hipGetLastError();
 }
 
+// ---- MFMA ---------------------------------------------------------------------------------------
+
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef short s16x8 __attribute__((ext_vector_type(8)));
+
+template <int DT> __device__ __forceinline__ f32x16 mac32(s16x8 a, s16x8 b, f32x16 c) {
+    using V = typename Mfma<DT>::V;
+    if constexpr (DT == kBF16) {
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(V, a), __builtin_bit_cast(V, b), c, 0, 0, 0);
+    } else {
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(V, a), __builtin_bit_cast(V, b), c, 0, 0, 0);
+    }
+}
+
+// A lane's value and that of the lane 32 further on, in both lanes the same
+// way round: v_permlane32_swap exchanges the upper half of a with the lower half
+// of b.  In assembly because the builtin's two results come out as one; the
+// waits are those that the instruction needs after a vector write.
+__device__ __forceinline__ void both_halves(float v, float & a, float & b) {
+    a = b = v;
+    asm("s_nop 1\n\tv_permlane32_swap_b32 %0, %1\n\ts_nop 1" : "+v"(a), "+v"(b));
+}
+__device__ __forceinline__ float max_halves(float v) {
+    float a, b;
+    both_halves(v, a, b);
+    return fmaxf(a, b);
+}
+__device__ __forceinline__ float sum_halves(float v) {
+    float a, b;
+    both_halves(v, a, b);
+    return a + b;
+}
+
+// Where the keys are split over blocks: each split's running maximum, sum and
+// unnormalised output of every query (row * heads + head), joined by k_join.
+struct Partial {
+    float * out;   // [splits][nq * heads][dim]
+    float2 * stat; // [splits][nq * heads]: maximum (log2 units), sum
+    int splits;
+};
+
+// NW wavefronts of 32 queries each, keys in tiles of 64 straight into LDS, two
+// tiles deep.  Scores are computed transposed (keys x queries, K as the A
+// operand): a lane then holds 32 of one query's 64 scores, its softmax needs
+// one exchange with the lane 32 further on, and the weights are, rounded to the
+// storage type, the B operand of V^T x weights as they stand: rows 8 i + 4 h + j
+// of a 32 x 32 result (h the lane's half) are K values 8 h + .. of the next
+// product if V^T's columns are read in the same order, which the transposing
+// LDS read gives (16 lanes read four rows of 16 values and get a column each).
+//
+// Weights are 2^(score - reference), in [0, 2^8]: the reference is a running
+// maximum that moves only when some query's scores exceed it by 8, so most
+// tiles leave the output unscaled.
+//
+// LDS: rows of 64 or 128 values, chunk c of row r at c ^ f(r): the 16 lanes of
+// a K read (16 rows, one chunk) and the 32 of a V read (4 rows x 4 chunks, two of
+// them) touch different banks.
+template <int DT, int DC, int NW>
+__global__ void __launch_bounds__(64 * NW, 2) k_attention(Attention p, Partial part, int tiles) {
+    using T = typename Store<DT>::T;
+    constexpr int TQ = 32 * NW, TK = 64;
+    constexpr int LP = DC <= 64 ? 64 : 128;      // values per LDS row
+    constexpr int ROW = LP * 2, CH = LP / 8;     // its bytes and chunks
+    constexpr int KS = DC / 16, DT32 = DC / 32;  // K steps of the scores, 32-row tiles of the output
+    constexpr int TILE = TK * ROW;
+    constexpr int RPL = 64 / CH;                 // rows per load of 1 KB
+    constexpr int LOADS = TILE / 1024;
+    constexpr int PER = LOADS / NW;              // of K, and of V, per wavefront
+    static_assert(LOADS % NW == 0, "whole loads");
+    __shared__ __attribute__((aligned(1024))) unsigned char s_tile[4 * TILE];  // K, V of two tiles
+
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int l32 = lane & 31, half = lane >> 5;
+    const int group = p.heads / p.kv_heads;
+
+    // Neighbouring blocks share a kv head; each XCD takes a contiguous range.
+    const int64_t unit = xcd_remap(blockIdx.x, gridDim.x);
+    const int split = (int) (unit % part.splits);
+    const int kv = (int) (unit / part.splits / tiles);
+    const Place at = find_place<TQ>(p, unit / part.splits % tiles, group);
+    if (at.nq <= 0) return;
+    const int all = (at.nk + TK - 1) / TK;
+    const int t0 = (int) ((int64_t) all * split / part.splits), t1 = (int) ((int64_t) all * (split + 1) / part.splits);
+
+    // This lane's query.
+    const int qi = wave * 32 + l32;
+    const int64_t vq = at.first + qi;
+    const int64_t row = at.q0 + vq / group;
+    const int head = kv * group + (int) (vq % group);
+    const bool live = qi < at.nq;
+    s16x8 q[KS];
+    {
+        const T * qr = (const T *) p.q + row * p.q_stride + (int64_t) head * p.dim;
+        const int flip = p.scale < 0.0f ? (int) 0x80008000u : 0;  // the reference follows the largest score
+#pragma unroll
+        for (int k = 0; k < KS; ++k) {
+            const int c = (2 * k + half) * 8;
+            int4 v{0, 0, 0, 0};
+            if (live && c < p.dim) v = *(const int4 *) (qr + c);
+            q[k] = __builtin_bit_cast(s16x8, int4{v.x ^ flip, v.y ^ flip, v.z ^ flip, v.w ^ flip});
+        }
+    }
+    const float scale = fabsf(p.scale);
+
+    const auto swizzle = [](int r) {
+        if constexpr (LP == 128) return ((r & 3) << 2) | ((r >> 2) & 3);
+        return (((r >> 1) & 1) << 2) | (((r >> 2) & 1) << 1) | ((r >> 3) & 1);
+    };
+    // Loads: row lane / CH of RPL, the chunk that lands at place lane % CH.
+    // Rows of one load and the next differ in bits that swizzle sees, so each
+    // load has its own chunk.
+    const char * kb = (const char *) ((const T *) p.k + at.k0 * p.k_stride + (int64_t) kv * p.dim);
+    const char * vb = (const char *) ((const T *) p.v + at.k0 * p.v_stride + (int64_t) kv * p.dim);
+    const int ks = (int) p.k_stride * 2, vs = (int) p.v_stride * 2;
+    constexpr uint32_t kOutside = 0x80000000u;
+    uint32_t k_off[PER], v_off[PER];
+#pragma unroll
+    for (int j = 0; j < PER; ++j) {
+        const int r = (wave * PER + j) * RPL + lane / CH;
+        const int c = (lane % CH) ^ swizzle(r);
+        const bool in = c * 8 < p.dim;
+        k_off[j] = in ? (uint32_t) (r * ks + c * 16) : kOutside;
+        v_off[j] = in ? (uint32_t) (r * vs + c * 16) : kOutside;
+    }
+    const uint32_t lds0 = (uint32_t) (uintptr_t) (__attribute__((address_space(3))) unsigned char *) s_tile;
+    const auto load = [&](int t) {
+        const int left = at.nk - t * TK;
+        const int rows = left < TK ? left : TK;
+        const __amdgpu_buffer_rsrc_t kr = __builtin_amdgcn_make_buffer_rsrc((void *) (kb + (int64_t) t * TK * ks), 0,
+                                                                            (rows - 1) * ks + p.dim * 2, 0x00020000);
+        const __amdgpu_buffer_rsrc_t vr = __builtin_amdgcn_make_buffer_rsrc((void *) (vb + (int64_t) t * TK * vs), 0,
+                                                                            (rows - 1) * vs + p.dim * 2, 0x00020000);
+        const uint32_t to = lds0 + (uint32_t) ((t & 1) * 2 * TILE + wave * PER * 1024);
+#pragma unroll
+        for (int j = 0; j < PER; ++j) {
+            // Rows past the end are zeros.
+            const bool in = (wave * PER + j) * RPL + lane / CH < rows;
+            dma_b128(kr, to + j * 1024u, in ? k_off[j] : kOutside, 0);
+            dma_b128(vr, to + TILE + j * 1024u, in ? v_off[j] : kOutside, 0);
+        }
+    };
+
+    // Reads: K row l32 (+ 32), chunk 2 k + half; V rows 4 half + (lane % 16) / 4
+    // (+ 8, + 16 g), 16-value column block (lane / 16) % 2 of each 32.
+    uint32_t k_read[KS];
+#pragma unroll
+    for (int k = 0; k < KS; ++k) k_read[k] = (uint32_t) (l32 * ROW + (((2 * k + half) ^ swizzle(l32)) * 16));
+    uint32_t v_read[DT32][2];
+#pragma unroll
+    for (int d = 0; d < DT32; ++d)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            const int r = 8 * e + 4 * half + ((lane & 15) >> 2);
+            const int c = 4 * d + 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
+            v_read[d][e] = (uint32_t) (r * ROW + ((c ^ swizzle(r)) * 16) + (lane & 1) * 8);
+        }
+
+    f32x16 out[DT32];
+#pragma unroll
+    for (int d = 0; d < DT32; ++d)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) out[d][i] = 0.0f;
+    float ref = -__builtin_inff(), sum = 0.0f;
+
+    if (t0 < t1) load(t0);
+    for (int t = t0; t < t1; ++t) {
+        wait_vmcnt<0>();
+        lds_barrier();
+        if (t + 1 < t1) load(t + 1);
+        const unsigned char * sk = s_tile + (t & 1) * 2 * TILE;
+        f32x16 s[2];
+#pragma unroll
+        for (int n = 0; n < 2; ++n) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) s[n][i] = 0.0f;
+#pragma unroll
+            for (int k = 0; k < KS; ++k)
+                s[n] = mac32<DT>(*(const s16x8 *) (sk + n * 32 * ROW + k_read[k]), q[k], s[n]);
+        }
+        const int left = at.nk - t * TK;
+        if (left < TK) {
+#pragma unroll
+            for (int n = 0; n < 2; ++n)
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+                    if (n * 32 + 8 * (i / 4) + 4 * half + i % 4 >= left) s[n][i] = -__builtin_inff();
+        }
+        float m = s[0][0];
+#pragma unroll
+        for (int n = 0; n < 2; ++n)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) m = fmaxf(m, s[n][i]);
+        m = max_halves(m) * scale;
+        if (__any(m > ref + 8.0f)) {
+            const float next = fmaxf(ref, m);
+            const float keep = next == -__builtin_inff() ? 1.0f : __builtin_amdgcn_exp2f(ref - next);
+            ref = next;
+            sum *= keep;
+#pragma unroll
+            for (int d = 0; d < DT32; ++d)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) out[d][i] *= keep;
+        }
+        const float base = ref == -__builtin_inff() ? 0.0f : ref;
+#pragma unroll
+        for (int n = 0; n < 2; ++n)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                s[n][i] = __builtin_amdgcn_exp2f(fmaf(s[n][i], scale, -base));
+                sum += s[n][i];
+            }
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            union {
+                T h[8];
+                s16x8 v;
+            } w;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) w.h[i] = round_to_store<DT>(s[g / 2][8 * (g % 2) + i]);
+#pragma unroll
+            for (int d = 0; d < DT32; ++d) {
+                union {
+                    s16x4 h[2];
+                    s16x8 v;
+                } a;
+#pragma unroll
+                for (int e = 0; e < 2; ++e)
+                    a.h[e] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                        (__attribute__((address_space(3))) s16x4 *) (sk + TILE + g * 16 * ROW + v_read[d][e]));
+                out[d] = mac32<DT>(a.v, w.v, out[d]);
+            }
+        }
+    }
+
+    sum = sum_halves(sum);
+    if (!live) return;
+    if (part.splits > 1) {
+        const int64_t at_q = ((int64_t) split * p.nq + row) * p.heads + head;
+        if (half == 0) part.stat[at_q] = float2{ref, sum};
+        if (t0 < t1) {
+            float * o = part.out + at_q * p.dim;
+#pragma unroll
+            for (int d = 0; d < DT32; ++d)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int c = d * 32 + i * 8 + half * 4;
+                    if (c < p.dim)
+                        *(float4 *) (o + c) =
+                            float4{out[d][4 * i], out[d][4 * i + 1], out[d][4 * i + 2], out[d][4 * i + 3]};
+                }
+        }
+        return;
+    }
+    // No keys (or none above -inf): zeros.
+    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+    T * y = (T *) p.y + row * p.y_stride + (int64_t) head * p.dim;
+#pragma unroll
+    for (int d = 0; d < DT32; ++d)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int c = d * 32 + i * 8 + half * 4;
+            union {
+                T h[4];
+                int2 v;
+            } w;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) w.h[j] = round_to_store<DT>(out[d][4 * i + j] * inv);
+            if (c < p.dim) *(int2 *) (y + c) = w.v;
+        }
+}
+
+// Joins the splits: 4 channels a thread, queries found as k_attention<.., NW> does.
+template <int DT, int TQ>
+__global__ void __launch_bounds__(256) k_join(Attention p, Partial part, int tiles) {
+    using T = typename Store<DT>::T;
+    const int group = p.heads / p.kv_heads, kv = blockIdx.x / tiles;
+    const Place at = find_place<TQ>(p, blockIdx.x % tiles, group);
+    const int quads = p.dim / 4;
+    for (int i = threadIdx.x; i < at.nq * quads; i += 256) {
+        const int64_t vq = at.first + i / quads;
+        const int64_t row = at.q0 + vq / group;
+        const int head = kv * group + (int) (vq % group), c = i % quads * 4;
+        const int64_t q = row * p.heads + head, step = p.nq * p.heads;
+        float most = -__builtin_inff();
+        for (int s = 0; s < part.splits; ++s) most = fmaxf(most, part.stat[s * step + q].x);
+        const float base = most == -__builtin_inff() ? 0.0f : most;
+        float sum = 0.0f, v[4] = {0.f, 0.f, 0.f, 0.f};
+        for (int s = 0; s < part.splits; ++s) {
+            const float2 st = part.stat[s * step + q];
+            if (st.x == -__builtin_inff() && st.y == 0.0f) continue;  // no keys: nothing was written
+            const float w = exp2f(st.x - base);
+            const float4 o = *(const float4 *) (part.out + (s * step + q) * p.dim + c);
+            sum += w * st.y;
+            v[0] += w * o.x;
+            v[1] += w * o.y;
+            v[2] += w * o.z;
+            v[3] += w * o.w;
+        }
+        const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+        T * y = (T *) p.y + row * p.y_stride + (int64_t) head * p.dim + c;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) Store<DT>::st(y, j, v[j] * inv);
+    }
+}
+
+template <int DT, int DC, int NW>
+hipError_t launch_nw(const Attention & p, const Partial & part, int64_t tiles, hipStream_t s) {
+    const int64_t grid = tiles * p.kv_heads * part.splits;
+    if (grid > 0x7fffffffLL) return hipErrorInvalidValue;
+    k_attention<DT, DC, NW><<<(unsigned) grid, 64 * NW, 0, s>>>(p, part, (int) tiles);
+    hipError_t err = hipGetLastError();
+    if (err == hipSuccess && part.splits > 1) {
+        k_join<DT, 32 * NW><<<(unsigned) (tiles * p.kv_heads), 256, 0, s>>>(p, part, (int) tiles);
+        err = hipGetLastError();
+    }
+    return err;
+}
+
+template <int DT, int DC>
+hipError_t launch_dc(const Attention & p, const Partial & part, const AttentionShape & sh, hipStream_t s) {
+    return sh.waves == 1 ? launch_nw<DT, DC, 1>(p, part, sh.tiles, s) : launch_nw<DT, DC, 4>(p, part, sh.tiles, s);
+}
+
+template <int DT>
+hipError_t launch_mfma(const Attention & p, const Partial & part, const AttentionShape & sh, hipStream_t s) {
+    if (p.dim <= 32) return launch_dc<DT, 32>(p, part, sh, s);
+    if (p.dim <= 64) return launch_dc<DT, 64>(p, part, sh, s);
+    if (p.dim <= 96) return launch_dc<DT, 96>(p, part, sh, s);
+    return launch_dc<DT, 128>(p, part, sh, s);
+}
+
 }  // namespace
 
-hipError_t launch_attention(int dtype, const Attention & p, hipStream_t s) {
-    switch (dtype) {
-        case kF32: return launch_any<kF32>(p, s);
-        case kF16: return launch_any<kF16>(p, s);
-        default: return launch_any<kBF16>(p, s);
+AttentionShape attention_shape(int dtype, const Attention & p, int cus) {
+    AttentionShape sh{0, 0, 1, 0};
+    const auto aligned = [](const void * ptr, int64_t stride) { return (uintptr_t) ptr % 16 == 0 && stride % 8 == 0; };
+    // A tile's 64 rows stay within a buffer's 2 GiB of offsets.
+    constexpr int64_t kMaxStride = 1 << 23;
+    if (dtype == kF32 || p.dim % 8 != 0 || p.dim > 128 || !aligned(p.q, p.q_stride) || !aligned(p.k, p.k_stride) ||
+        !aligned(p.v, p.v_stride) || !aligned(p.y, p.y_stride) || p.k_stride > kMaxStride || p.v_stride > kMaxStride) {
+        return sh;
     }
+    const int group = p.heads / p.kv_heads;
+    const int64_t queries = p.nq * group, seqs = p.q_at != nullptr ? p.seqs : 1;
+    // Sequences of up to 32 queries: one wavefront a block, as the others would only help to load.
+    sh.waves = queries <= 32 * seqs ? 1 : 4;
+    const int tq = 32 * sh.waves;
+    sh.tiles = queries / tq + seqs;  // every sequence may add one partly filled tile
+    const int64_t blocks = (queries + tq - 1) / tq * p.kv_heads;
+    const int64_t want = (int64_t) cus * 8 / sh.waves;  // two wavefronts per SIMD
+    // Few queries: the keys split over more blocks, at least four tiles of 64 each.
+    const int64_t key_tiles = (p.nk / seqs + 63) / 64;
+    if (blocks < want) sh.splits = (int) std::max<int64_t>(1, std::min(want / std::max<int64_t>(blocks, 1), key_tiles / 4));
+    if (sh.splits > 1) sh.scratch = (size_t) sh.splits * p.nq * p.heads * (p.dim + 2) * sizeof(float);
+    return sh;
+}
+
+hipError_t launch_attention(int dtype, const Attention & p, const AttentionShape & sh, void * scratch, hipStream_t s) {
+    if (sh.waves == 0) {
+        switch (dtype) {
+            case kF32: return launch_any<kF32>(p, s);
+            case kF16: return launch_any<kF16>(p, s);
+            default: return launch_any<kBF16>(p, s);
+        }
+    }
+    Partial part{nullptr, nullptr, 1};
+    if (scratch != nullptr && sh.splits > 1) {
+        part.splits = sh.splits;
+        part.out = (float *) scratch;
+        part.stat = (float2 *) (part.out + (size_t) sh.splits * p.nq * p.heads * p.dim);
+    }
+    if (sh.tiles > 0x7fffffffLL) return hipErrorInvalidValue;
+    return dtype == kBF16 ? launch_mfma<kBF16>(p, part, sh, s) : launch_mfma<kF16>(p, part, sh, s);
 }
 
 }  // namespace tsh

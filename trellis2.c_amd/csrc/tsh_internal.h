@@ -407,7 +407,18 @@ struct Attention {
     float scale;             // times log2(e)
 };
 constexpr int kAttentionMaxDim = 192;
-hipError_t launch_attention(int dtype, const Attention & p, hipStream_t s);
+// How attention is run: wavefronts per block of the MFMA kernel (0: the general
+// kernel), blocks of queries, parts of the keys and the scratch memory to join
+// them (without it they are not split).
+struct AttentionShape {
+    int waves;
+    int64_t tiles;
+    int splits;
+    size_t scratch;
+};
+AttentionShape attention_shape(int dtype, const Attention & p, int cus);
+hipError_t launch_attention(int dtype, const Attention & p, const AttentionShape & shape, void * scratch,
+                            hipStream_t s);
 
 // Narrow MFMA linear (bf16/fp16, Co <= 16, Ci a power of two in 32..1024):
 // weights [co][ci] in the storage type.
