@@ -2195,7 +2195,7 @@ trellis_status linear_act_impl(trellis_sparse_backend * backend, const trellis_s
         !float_buffer_ok(be, y, (size_t) n * co)) {
         return fail(be, TRELLIS_STATUS_INVALID_ARGUMENT, "linear_act: bad argument");
     }
-    if ((int64_t) ci * 4 > kLinearActMaxBytes || co > INT32_MAX - 256) {
+    if ((int64_t) ci * 4 > kLinearActMaxBytes || (int64_t) co * 4 > kLinearActMaxBytes) {
         return fail(be, TRELLIS_STATUS_INVALID_ARGUMENT, "linear_act: rows too wide");
     }
     if ((!from8 && spans_clash(packed(y, n, co), packed(x, n, ci), false)) ||
@@ -2225,8 +2225,9 @@ trellis_status linear_act_impl(trellis_sparse_backend * backend, const trellis_s
     p.n = n;
     p.ci = ci;
     p.co = co;
+    p.act = act;
     stage_begin(be, TRELLIS_SPARSE_HIP_STAGE_ELEMENTWISE);
-    const hipError_t err = launch_linear_act(dt, from8 ? kRows8 : dt, p, act, be->cus, be->stream);
+    const hipError_t err = launch_linear_act(dt, from8 ? kRows8 : dt, p, be->cus, be->stream);
     stage_end(be, TRELLIS_SPARSE_HIP_STAGE_ELEMENTWISE);
     return hip_status(be, err, "linear_act");
 }

@@ -1,4 +1,7 @@
 // kernels_act.hip - linear with activation and residual in its epilogue, from rows of the storage type or 8-bit rows.
+#include <cstdlib>
+#include <type_traits>
+
 #include "mfma_common.h"
 
 namespace tsh {
@@ -7,40 +10,93 @@ namespace {
 // ---- activations --------------------------------------------------------------------------------
 
 // For 16-bit outputs the hardware exponential and reciprocal (about 2^-21
-// relative) and an erf of 1.5e-7 (Abramowitz and Stegun 7.1.26) stay far below the
-// output's rounding; fp32 outputs take the accurate functions.
+// relative) stay far below the output's rounding; fp32 outputs take the accurate
+// functions.  All are v times a logistic function of v: SiLU of v itself, GELU with
+// tanh of 2 sqrt(2 / pi) (v + 0.044715 v^3), and the normal distribution function
+// of GELU of v R(v^2), R a minimax polynomial of its logit (in log2 units) on
+// [0, 6]: 1.5e-6 off, and six operations less than a rational erf, which count:
+// a 256 x 256 block's GELU takes as long as 1,000 K values of its products.
+constexpr float kG0 = 2.30216527f, kG1 = 0.105008416f, kG2 = -2.55234947e-4f, kG3 = -1.0548038e-4f, kG4 = 4.0871505e-6f;
 template <int DT, int ACT> __device__ __forceinline__ float activate(float v) {
     if constexpr (ACT == TRELLIS_SPARSE_HIP_ACT_SILU) {
         if constexpr (DT == kF32) return v / (1.0f + expf(-v));
-        return v * __builtin_amdgcn_rcpf(1.0f + __expf(-v));
+        return v * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-1.4426950408889634f * v));
     } else if constexpr (ACT == TRELLIS_SPARSE_HIP_ACT_GELU) {
         if constexpr (DT == kF32) return 0.5f * v * (1.0f + erff(v * 0.70710678118654752f));
-        // erf(|z|) = 1 - t (a1 + t (a2 + ...)) exp(-z^2), t = 1 / (1 + 0.3275911 |z|).
-        const float z = fabsf(v) * 0.70710678118654752f;
-        const float t = __builtin_amdgcn_rcpf(1.0f + 0.3275911f * z);
-        const float poly =
-            t * (0.254829592f + t * (-0.284496736f + t * (1.421413741f + t * (-1.453152027f + t * 1.061405429f))));
-        const float tail = 0.5f * poly * __expf(-z * z);  // (1 - erf(z)) / 2
-        return v * (v < 0.0f ? tail : 1.0f - tail);
+        const float t = v * v;
+        const float r = kG0 + t * (kG1 + t * (kG2 + t * (kG3 + t * kG4)));
+        return v * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-v * r));
     } else if constexpr (ACT == TRELLIS_SPARSE_HIP_ACT_GELU_TANH) {
         // (1 + tanh(u)) / 2 = 1 / (1 + exp(-2u))
-        const float u2 = 1.5957691216057308f * (v + 0.044715f * v * v * v);
-        if constexpr (DT == kF32) return v / (1.0f + expf(-u2));
-        return v * __builtin_amdgcn_rcpf(1.0f + __expf(-u2));
+        const float r = 1.5957691216057308f + 0.0713548162726f * v * v;
+        if constexpr (DT == kF32) return v / (1.0f + expf(-v * r));
+        return v * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-1.4426950408889634f * v * r));
     } else {
         return v;
     }
 }
 
+// f(the activation as a constant).
+template <class F> __device__ __forceinline__ void by_act(int act, F && f) {
+    switch (act) {
+        case TRELLIS_SPARSE_HIP_ACT_SILU: f(std::integral_constant<int, TRELLIS_SPARSE_HIP_ACT_SILU>()); break;
+        case TRELLIS_SPARSE_HIP_ACT_GELU: f(std::integral_constant<int, TRELLIS_SPARSE_HIP_ACT_GELU>()); break;
+        case TRELLIS_SPARSE_HIP_ACT_GELU_TANH: f(std::integral_constant<int, TRELLIS_SPARSE_HIP_ACT_GELU_TANH>()); break;
+        default: f(std::integral_constant<int, TRELLIS_SPARSE_HIP_ACT_NONE>()); break;
+    }
+}
+
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+
+// N (1, 2 or 4) adjacent values at byte voff + soff of a buffer, whole and
+// aligned; beyond the buffer loads give zeros and stores nothing.
+template <int DT, int N>
+__device__ __forceinline__ void load_adjacent(__amdgpu_buffer_rsrc_t rsrc, uint32_t voff, uint32_t soff, float * v) {
+    using T = typename Store<DT>::T;
+    constexpr int B = N * sizeof(T);
+    union {
+        T h[N];
+        uint16_t b2;
+        uint32_t b4;
+        u32x2 b8;
+        u32x4 b16;
+    } w;
+    if constexpr (B == 2) w.b2 = __builtin_amdgcn_raw_buffer_load_b16(rsrc, (int) voff, (int) soff, 0);
+    if constexpr (B == 4) w.b4 = __builtin_amdgcn_raw_buffer_load_b32(rsrc, (int) voff, (int) soff, 0);
+    if constexpr (B == 8) w.b8 = __builtin_amdgcn_raw_buffer_load_b64(rsrc, (int) voff, (int) soff, 0);
+    if constexpr (B == 16) w.b16 = __builtin_amdgcn_raw_buffer_load_b128(rsrc, (int) voff, (int) soff, 0);
+#pragma unroll
+    for (int u = 0; u < N; ++u) v[u] = Store<DT>::ld(w.h, u);
+}
+template <int DT, int N>
+__device__ __forceinline__ void store_adjacent(__amdgpu_buffer_rsrc_t rsrc, uint32_t voff, uint32_t soff, const float * v) {
+    using T = typename Store<DT>::T;
+    constexpr int B = N * sizeof(T);
+    union {
+        T h[N];
+        uint16_t b2;
+        uint32_t b4;
+        u32x2 b8;
+        u32x4 b16;
+    } w;
+#pragma unroll
+    for (int u = 0; u < N; ++u) w.h[u] = round_to_store<DT>(v[u]);
+    if constexpr (B == 2) __builtin_amdgcn_raw_buffer_store_b16(w.b2, rsrc, (int) voff, (int) soff, 0);
+    if constexpr (B == 4) __builtin_amdgcn_raw_buffer_store_b32(w.b4, rsrc, (int) voff, (int) soff, 0);
+    if constexpr (B == 8) __builtin_amdgcn_raw_buffer_store_b64(w.b8, rsrc, (int) voff, (int) soff, 0);
+    if constexpr (B == 16) __builtin_amdgcn_raw_buffer_store_b128(w.b16, rsrc, (int) voff, (int) soff, 0);
+}
+
 // ---- MFMA GEMM ----------------------------------------------------------------------------------
 
 typedef int i32x8 __attribute__((ext_vector_type(8)));
-typedef float f32x4v __attribute__((ext_vector_type(4)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
 
-// A fragment is two 16-byte chunks, g and g + 4 for lane group g = lane / 16, of
-// row lane % 16 (of x or of W) in a step of 128 bytes: 32, 64 or 128 K values in
-// fp32, 16 or 8 bits.  The scaled MFMA takes the chunks as K values 16 g .. and
-// 64 + 16 g .., and from lane group g the scale of K values 32 g .. 32 g + 31.  It
+// A fragment is two 16-byte chunks, h and h + 2 for lane half h = lane / 32, of
+// row lane % 32 (of x or of W) in a step of 64 bytes: 16, 32 or 64 K values in
+// fp32, 16 or 8 bits.  The scaled MFMA takes the chunks as K values 16 h .. and
+// 32 + 16 h .., and from lane half h the scale of K values 32 h .. 32 h + 31.  It
 // adds eight neighbouring products at a time on the scale of the largest, cutting
 // each at 2^-13 of it (measured: 2^-13 stays, 2^-14 goes), before the fp32 sums: an
 // error near 2e-5 of a sum's size, a hundredth of a bf16 rounding, for twice the
@@ -49,22 +105,31 @@ struct Frag {
     int4 c[2];
 };
 
-template <int MT> __device__ __forceinline__ f32x4 mac(const Frag & a, const Frag & b, f32x4 c, int sa, int sb) {
+// SEL: which of a scale register's bytes counts (0 or 2).
+template <int MT, int SEL> __device__ __forceinline__ f32x16 mac(const Frag & a, const Frag & b, f32x16 c, int sa, int sb) {
     if constexpr (MT == kF32) {
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const f32x4v x = __builtin_bit_cast(f32x4v, a.c[h]), w = __builtin_bit_cast(f32x4v, b.c[h]);
+        for (int e = 0; e < 2; ++e) {
+            const f32x4 x = __builtin_bit_cast(f32x4, a.c[e]), w = __builtin_bit_cast(f32x4, b.c[e]);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) c = __builtin_amdgcn_mfma_f32_16x16x4f32(x[j], w[j], c, 0, 0, 0);
+            for (int j = 0; j < 4; ++j) c = __builtin_amdgcn_mfma_f32_32x32x2f32(x[j], w[j], c, 0, 0, 0);
         }
         return c;
     } else if constexpr (MT == kRows8) {
-        return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(__builtin_bit_cast(i32x8, a), __builtin_bit_cast(i32x8, b),
-                                                                c, 0, 0, 0, sa, 0, sb);
+        return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(__builtin_bit_cast(i32x8, a), __builtin_bit_cast(i32x8, b),
+                                                               c, 0, 0, SEL, sa, SEL, sb);
     } else {
         using V = typename Mfma<MT>::V;
-        c = Mfma<MT>::mac(__builtin_bit_cast(V, a.c[0]), __builtin_bit_cast(V, b.c[0]), c);
-        return Mfma<MT>::mac(__builtin_bit_cast(V, a.c[1]), __builtin_bit_cast(V, b.c[1]), c);
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            const V x = __builtin_bit_cast(V, a.c[e]), w = __builtin_bit_cast(V, b.c[e]);
+            if constexpr (MT == kBF16) {
+                c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x, w, c, 0, 0, 0);
+            } else {
+                c = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, w, c, 0, 0, 0);
+            }
+        }
+        return c;
     }
 }
 
@@ -84,31 +149,39 @@ __device__ __forceinline__ void dma_b32(__amdgpu_buffer_rsrc_t rsrc, uint32_t ld
 
 constexpr uint32_t kOutside = 0x80000000u;  // beyond every buffer here: loads fetch zeros
 
-// A block multiplies BM rows of x by BN rows of W (output channels), RW x CW
-// wavefronts of BM / RW rows and 128 channels each, 128 bytes of both a step.
+// A block of RW x CW wavefronts multiplies BM rows of x by BN rows of W (output
+// channels), a wavefront RB blocks of 32 rows by NT tiles of 32 channels, in
+// steps of 128 bytes of K (whole cache lines: with 64 bytes a step each line
+// comes twice from the L2 and the loads bound the kernel, 16,384 x 4096 -> 4096
+// bf16 474 us).  Two steps are in LDS or on their way there.  A step is two
+// halves of 64 bytes: while the first half's products run, the second half's fragments
+// are read; then comes the one barrier, after which the step's slot is free for
+// the loads of the step after next, and the next step, whose loads were issued
+// a step ago, has landed for the reads under the second half's products.
 //
-// LDS: a step's slot holds 16-row blocks of 2 KB, row i at (i % 8) * 256 + (i / 8)
-// * 128, its chunk c at ((c ^ i) % 8) * 16: the 16 lanes that read one chunk of
-// 16 rows touch each of the 64 banks once, and eight lanes of a load fetch one
-// row's 128 contiguous bytes.  Tile t's lane i multiplies channel 8 i + t of a
-// wavefront's 128, so that a lane ends with eight adjacent channels and a row
-// leaves in 16-byte pieces.
-template <int MT, int DT, int ACT, int BM, int BN, int RW, int CW>
-__global__ void __launch_bounds__(64 * RW * CW, 1) k_linear_act(LinearAct p) {
+// LDS: a slot holds the rows of x and of W, 128 bytes each, chunk c of row r at c ^ f(r),
+// f(r) the bits 1, 2, 3 of r in reverse: the 16 lanes that ds_read_b128 serves at
+// once (0-3, 12-15, 20-23 and 24-27 of each 32, and the others) touch each of
+// the 64 banks once, and eight lanes of a load fetch one row's 128 bytes.
+// Of 32 NT channels, tile t's lane i has channel NT i + t: a lane ends with NT
+// adjacent ones, and a row leaves in pieces of 32 NT adjacent channels.
+// 8-bit rows: a step's scales are 4 bytes a row.
+template <int MT, int DT, int RW, int CW, int RB, int NT, int PER_CU>
+__global__ void __launch_bounds__(64 * RW * CW, RW * CW * PER_CU / 4) k_linear_act(LinearAct p) {
     using T = typename Store<DT>::T;
-    constexpr int NW = RW * CW, NT = 8, QB = BM / RW / 16;
-    static_assert(BN == CW * 128 && BM % (RW * 16) == 0, "128 channels per wavefront");
+    constexpr int NW = RW * CW, BM = RW * RB * 32, BN = CW * NT * 32;
     constexpr bool kScaled = MT == kRows8;
-    constexpr int kBytes = (BM + BN) * 128, kSlot = kBytes + (kScaled ? (BM + BN) * 4 : 0);
-    constexpr int kLoads = (BM + BN) / 8, kPer = kLoads / NW;  // 1 KB each
-    static_assert(kLoads % NW == 0, "as many loads for every wavefront");
-    constexpr int kScaleLoads = (BM + BN) / 64;
+    constexpr int kRows = BM + BN, kBytes = kRows * 128, kSlot = kBytes + (kScaled ? kRows * 4 : 0);
+    // Loads of 1 KB (8 rows) per step and wavefront, of x and of W.
+    constexpr int NA = BM / 8 / NW, NB = BN / 8 / NW, kPer = NA + NB;
+    static_assert(BM % (8 * NW) == 0 && BN % (8 * NW) == 0, "as many loads for every wavefront");
+    static_assert(!kScaled || (BM % 64 == 0 && kRows / 64 <= NW), "one load of scales per wavefront, all of x or of W");
     __shared__ __attribute__((aligned(1024))) unsigned char s_slot[2 * kSlot];
 
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int rw = wave % RW, cw = wave / RW;
-    const int l16 = lane & 15, lg = lane >> 4;
+    const int l32 = lane & 31, half = lane >> 5;
 
     // Blocks b, b + 8, ... run on one XCD, which multiplies a row block by
     // every channel block in turn: the rows stay in its L2.
@@ -123,145 +196,192 @@ __global__ void __launch_bounds__(64 * RW * CW, 1) k_linear_act(LinearAct p) {
         (void *) ((const char *) p.x + row0 * p.row_bytes), 0, (int) (rows * p.row_bytes), 0x00020000);
     const __amdgpu_buffer_rsrc_t wres = __builtin_amdgcn_make_buffer_rsrc(
         (void *) ((const char *) p.w + (int64_t) col0 * p.w_bytes), 0, (int) (BN * p.w_bytes), 0x00020000);
-    const uint32_t slot0 = (uint32_t) (uintptr_t) (__attribute__((address_space(3))) unsigned char *) s_slot;
+    const uint32_t slots = (uint32_t) (uintptr_t) (__attribute__((address_space(3))) unsigned char *) s_slot;
 
-    // This lane's piece of load j of this wavefront: 8 lines of 128 bytes.
-    const auto of_x = [&](int j) { return wave * kPer + j < BM / 8; };
-    uint32_t at[kPer];
-    int chunk[kPer];
+    // The channel of a row of W in LDS.
+    const auto channel_of = [](int r) { return r / (32 * NT) * (32 * NT) + r % 32 * NT + r % (32 * NT) / 32; };
+    const auto swizzle = [](int r) { return (((r >> 1) & 1) << 2) | (((r >> 2) & 1) << 1) | ((r >> 3) & 1); };
+    // This lane's piece of a load: 8 lines of 128 bytes.
+    uint32_t x_at[NA], w_at[NB];
+    int x_chunk[NA];
 #pragma unroll
-    for (int j = 0; j < kPer; ++j) {
-        const int q = wave * kPer + j - (of_x(j) ? 0 : BM / 8);  // KB of x's or W's part
-        const int line = (q & 1) * 4 + (lane >> 4), i = line + ((lane >> 3) & 1) * 8;
-        chunk[j] = (lane ^ i) & 7;
-        const int row = q / 2 * 16 + i;  // of x's rows or W's LDS rows
-        if (of_x(j)) {
-            at[j] = row < rows ? (uint32_t) (row * p.row_bytes) + chunk[j] * 16u : kOutside;
-        } else {
-            const int ch = row / 128 * 128 + row % 16 * 8 + row % 128 / 16;
-            at[j] = (uint32_t) (ch * p.w_bytes) + chunk[j] * 16u;
-        }
+    for (int j = 0; j < NA; ++j) {
+        const int row = (wave * NA + j) * 8 + (lane >> 3);
+        x_chunk[j] = (lane & 7) ^ swizzle(row);
+        x_at[j] = row < rows ? (uint32_t) (row * p.row_bytes) + x_chunk[j] * 16u : kOutside;
     }
-    // Scales: 64 rows of 4 bytes a load, one wavefront each.
+#pragma unroll
+    for (int j = 0; j < NB; ++j) {
+        const int row = (wave * NB + j) * 8 + (lane >> 3);
+        w_at[j] = (uint32_t) (channel_of(row) * p.w_bytes) + ((lane & 7) ^ swizzle(row)) * 16u;
+    }
+    // Scales: 64 rows a wavefront (the last ones again for wavefronts beyond them).
+    const int scale_load = min(wave, kRows / 64 - 1);
     uint32_t scale_at = kOutside;
     __amdgpu_buffer_rsrc_t sres = xres;
     if constexpr (kScaled) {
-        static_assert(kScaleLoads <= NW, "one load per wavefront");
-        const int row = wave * 64 + lane;
-        const int xs = p.row_bytes / 32, ws = p.w_bytes / 32;
-        if (wave * 64 < BM) {
-            sres = __builtin_amdgcn_make_buffer_rsrc((void *) (p.x_scales + row0 * xs), 0, rows * xs, 0x00020000);
-            if (row < rows) scale_at = (uint32_t) (row * xs);
-        } else {
-            sres = __builtin_amdgcn_make_buffer_rsrc((void *) (p.w_scales + (int64_t) col0 * ws), 0, BN * ws, 0x00020000);
-            const int r = row - BM;
-            scale_at = (uint32_t) ((r / 128 * 128 + r % 16 * 8 + r % 128 / 16) * ws);
+        const bool of_x = scale_load * 64 < BM;
+        const int pitch = (of_x ? p.row_bytes : p.w_bytes) / 32;
+        const uint8_t * base = of_x ? p.x_scales + row0 * pitch : p.w_scales + (int64_t) col0 * pitch;
+        const int row = scale_load * 64 + lane;
+        if (!of_x) {
+            scale_at = (uint32_t) (channel_of(row - BM) * pitch);
+        } else if (row < rows) {
+            scale_at = (uint32_t) (row * pitch);
         }
+        sres = __builtin_amdgcn_make_buffer_rsrc((void *) base, 0, (of_x ? rows : BN) * pitch, 0x00020000);
     }
+
     const int steps = p.w_bytes / 128;
-    const auto load = [&](int s) {
-        const uint32_t to = slot0 + (s & 1) * kSlot + (uint32_t) (wave * kPer) * 1024u;
-        const bool end = (s + 1) * 128 > p.row_bytes;  // what follows a row of x is the next one
-#pragma unroll
-        for (int j = 0; j < kPer; ++j) {
-            if (of_x(j)) {
-                dma_b128(xres, to + j * 1024u, end && s * 128 + chunk[j] * 16 >= p.row_bytes ? kOutside : at[j],
-                         s * 128u);
-            } else {
-                dma_b128(wres, to + j * 1024u, at[j], s * 128u);
-            }
+    // Past the last step loads fetch zeros; what follows a row of x is the next one.
+    const auto load = [&](int s, uint32_t slot, int j) {
+        if (j < NA) {
+            dma_b128(xres, slot + (wave * NA + j) * 1024u, s * 128 + x_chunk[j] * 16 < p.row_bytes ? x_at[j] : kOutside,
+                     s * 128u);
+        } else {
+            dma_b128(wres, slot + BM * 128 + (wave * NB + j - NA) * 1024u, s < steps ? w_at[j - NA] : kOutside, s * 128u);
         }
+    };
+    const auto load_scales = [&](int s, uint32_t slot) {
+        if constexpr (kScaled) dma_b32(sres, slot + kBytes + scale_load * 256u, s < steps ? scale_at : kOutside, s * 4u);
+    };
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+        load_scales(s, slots + s * kSlot);
+#pragma unroll
+        for (int j = 0; j < kPer; ++j) load(s, slots + s * kSlot, j);
+    }
+
+    const int ch = col0 + (cw * 32 + l32) * NT;  // the lane's first channel
+    f32x16 acc[RB][NT];
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+        const float bias = p.bias != nullptr && ch + t < p.co ? p.bias[ch + t] : 0.0f;
+#pragma unroll
+        for (int q = 0; q < RB; ++q)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) acc[q][t][i] = bias;
+    }
+
+    Frag fa[2][RB], fb[2][NT];
+    int sa[RB], sb[NT];
+    const uint32_t c0 = (uint32_t) (l32 * 128 + ((half ^ swizzle(l32)) * 16));  // chunk c: c0 ^ 16 c for even c
+    const auto read_a = [&](int h, uint32_t slot, int q) {
+        const unsigned char * r = s_slot + slot + (rw * RB + q) * 4096;
+        fa[h][q].c[0] = *(const int4 *) (r + (c0 ^ (h * 64)));
+        fa[h][q].c[1] = *(const int4 *) (r + (c0 ^ (h * 64 + 32)));
+    };
+    const auto read_b = [&](int h, uint32_t slot, int t) {
+        const unsigned char * r = s_slot + slot + BM * 128 + (cw * NT + t) * 4096;
+        fb[h][t].c[0] = *(const int4 *) (r + (c0 ^ (h * 64)));
+        fb[h][t].c[1] = *(const int4 *) (r + (c0 ^ (h * 64 + 32)));
+    };
+    // Byte 2 h + half of a row's four scales, moved down by the half.
+    const auto read_scales = [&](uint32_t slot) {
         if constexpr (kScaled) {
-            if (wave < kScaleLoads) dma_b32(sres, slot0 + (s & 1) * kSlot + kBytes + wave * 256u, scale_at, s * 4u);
+            const unsigned char * r = s_slot + slot + kBytes;
+#pragma unroll
+            for (int q = 0; q < RB; ++q)
+                sa[q] = (int) (*(const uint32_t *) (r + ((rw * RB + q) * 32 + l32) * 4) >> (8 * half));
+#pragma unroll
+            for (int t = 0; t < NT; ++t)
+                sb[t] = (int) (*(const uint32_t *) (r + (BM + (cw * NT + t) * 32 + l32) * 4) >> (8 * half));
+        }
+    };
+    // The products of half h; between one tile and the next a fragment of the
+    // other half is read from `from`, and in the second half a load is issued.
+    const auto products = [&](auto h_c, uint32_t from, int s, uint32_t to) {
+        constexpr int H = decltype(h_c)::value, READS = RB + NT, TILES = RB * NT;
+#pragma unroll
+        for (int k = 0; k < TILES; ++k) {
+#pragma unroll
+            for (int i = READS * k / TILES; i < READS * (k + 1) / TILES; ++i) {
+                if (i < RB) {
+                    read_a(H ^ 1, from, i);
+                } else {
+                    read_b(H ^ 1, from, i - RB);
+                }
+            }
+            if constexpr (H == 1) {
+                if (k == 0) load_scales(s, slots + to);
+#pragma unroll
+                for (int j = kPer * k / TILES; j < kPer * (k + 1) / TILES; ++j) load(s, slots + to, j);
+            }
+            const int q = k / NT, t = k % NT;
+            acc[q][t] = mac<MT, 2 * H>(fa[H][q], fb[H][t], acc[q][t], kScaled ? sa[q] : 0, kScaled ? sb[t] : 0);
+            __builtin_amdgcn_sched_barrier(0);
         }
     };
 
-    f32x4 acc[QB][NT];
+    wait_vmcnt<0>();
+    lds_barrier();
+    read_scales(0);
 #pragma unroll
-    for (int q = 0; q < QB; ++q)
+    for (int q = 0; q < RB; ++q) read_a(0, 0, q);
 #pragma unroll
-        for (int t = 0; t < NT; ++t) acc[q][t] = f32x4{0.f, 0.f, 0.f, 0.f};
-    const int line = (l16 & 7) * 256 + (l16 >> 3) * 128;
-    const int c0 = line + ((lg ^ l16) & 7) * 16;
-    const int c1 = line + (((lg + 4) ^ l16) & 7) * 16;
-    load(0);
+    for (int t = 0; t < NT; ++t) read_b(0, 0, t);
+    uint32_t here = 0, there = kSlot;
+    using std::integral_constant;
     for (int s = 0; s < steps; ++s) {
+        products(integral_constant<int, 0>(), here, 0, 0);
+        // Step s + 1 has landed, and every wavefront has read all of step s.
         wait_vmcnt<0>();
         lds_barrier();
-        if (s + 1 < steps) load(s + 1);
-        const unsigned char * sx = s_slot + (s & 1) * kSlot + rw * QB * 2048;
-        const unsigned char * sw = s_slot + (s & 1) * kSlot + BM * 128 + cw * NT * 2048;
-        const unsigned char * ss = s_slot + (s & 1) * kSlot + kBytes;
-        Frag a[QB], b[NT];
-        int sa[QB], sb[NT];
-#pragma unroll
-        for (int q = 0; q < QB; ++q) {
-            a[q].c[0] = *(const int4 *) (sx + q * 2048 + c0);
-            a[q].c[1] = *(const int4 *) (sx + q * 2048 + c1);
-            sa[q] = kScaled ? ss[((rw * QB + q) * 16 + l16) * 4 + lg] : 0;
-        }
-#pragma unroll
-        for (int t = 0; t < NT; ++t) {
-            b[t].c[0] = *(const int4 *) (sw + t * 2048 + c0);
-            b[t].c[1] = *(const int4 *) (sw + t * 2048 + c1);
-            sb[t] = kScaled ? ss[(BM + (cw * NT + t) * 16 + l16) * 4 + lg] : 0;
-        }
-#pragma unroll
-        for (int t = 0; t < NT; ++t)
-#pragma unroll
-            for (int q = 0; q < QB; ++q) acc[q][t] = mac<MT>(a[q], b[t], acc[q][t], sa[q], sb[t]);
+        __builtin_amdgcn_sched_barrier(0);
+        products(integral_constant<int, 1>(), there, s + 2, here);
+        read_scales(there);
+        const uint32_t swap = here;
+        here = there;
+        there = swap;
     }
+    wait_vmcnt<0>();
 
-    // Lane (l16, lg) holds rows 4 lg + i of each row block, channels 8 l16 .. 8 l16 + 7 of the wavefront's 128.
-    const int ch = col0 + cw * 128 + l16 * 8;
-    float bias[8];
+    // Lane (l32, half) holds rows 8 (i / 4) + 4 half + i % 4 of each row block.
+    // Buffer offsets: the lane's place, and the row's in a scalar; rows past
+    // the last and channels past co (a multiple of NT) fall outside.
+    const int pitch = p.co * (int) sizeof(T);
+    const __amdgpu_buffer_rsrc_t yres =
+        __builtin_amdgcn_make_buffer_rsrc((char *) p.y + row0 * pitch, 0, rows * pitch, 0x00020000);
+    const __amdgpu_buffer_rsrc_t rres = __builtin_amdgcn_make_buffer_rsrc(
+        (char *) (p.residual != nullptr ? p.residual : p.y) + row0 * pitch, 0, rows * pitch, 0x00020000);
+    const uint32_t at =
+        ch < p.co ? (uint32_t) ((rw * RB * 32 + 4 * half) * pitch + ch * (int) sizeof(T)) : kOutside;
+    const auto finish = [&](auto act_c, auto res_c) {
 #pragma unroll
-    for (int u = 0; u < 8; ++u) bias[u] = p.bias != nullptr && ch + u < p.co ? p.bias[ch + u] : 0.0f;
-    const bool whole = p.co % 8 == 0 && ch < p.co;  // all eight channels, 16-byte aligned
-    const T * residual = (const T *) p.residual;
-    T * y = (T *) p.y;
+        for (int q = 0; q < RB; ++q)
 #pragma unroll
-    for (int q = 0; q < QB; ++q) {
+            for (int g = 0; g < 4; ++g) {
+                float r[4][NT];
+                if constexpr (decltype(res_c)::value) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int64_t row = row0 + rw * (BM / RW) + q * 16 + lg * 4 + i;
-            if (row >= p.n) continue;
-            float v[8];
+                    for (int i = 0; i < 4; ++i)
+                        load_adjacent<DT, NT>(rres, at, (uint32_t) ((q * 32 + g * 8 + i) * pitch), r[i]);
+                }
 #pragma unroll
-            for (int u = 0; u < 8; ++u) v[u] = activate<DT, ACT>(acc[q][u][i] + bias[u]);
-            const int64_t e = row * p.co + ch;
-            if (whole) {
-                if (residual != nullptr) {
-                    float r[8];
-                    if constexpr (DT == kF32) {
+                for (int i = 0; i < 4; ++i) {
+                    float v[NT];
 #pragma unroll
-                        for (int u = 0; u < 8; ++u) r[u] = residual[e + u];
-                    } else {
-                        unpack_chunk<DT>(*(const int4 *) (residual + e), r);
+                    for (int t = 0; t < NT; ++t) {
+                        v[t] = activate<DT, decltype(act_c)::value>(acc[q][t][4 * g + i]);
+                        if constexpr (decltype(res_c)::value) v[t] += r[i][t];
                     }
-#pragma unroll
-                    for (int u = 0; u < 8; ++u) v[u] += r[u];
+                    store_adjacent<DT, NT>(yres, at, (uint32_t) ((q * 32 + g * 8 + i) * pitch), v);
                 }
-                if constexpr (DT == kF32) {
-                    *(float4 *) (y + e) = float4{v[0], v[1], v[2], v[3]};
-                    *(float4 *) (y + e + 4) = float4{v[4], v[5], v[6], v[7]};
-                } else {
-                    *(int4 *) (y + e) = pack_chunk<DT>(v);
-                }
-            } else {
-#pragma unroll
-                for (int u = 0; u < 8; ++u) {
-                    if (ch + u >= p.co) break;
-                    Store<DT>::st(y, e + u, residual != nullptr ? v[u] + Store<DT>::ld(residual, e + u) : v[u]);
-                }
+                __builtin_amdgcn_sched_barrier(0);
             }
+    };
+    by_act(p.act, [&](auto act_c) {
+        if (p.residual != nullptr) {
+            finish(act_c, std::true_type());
+        } else {
+            finish(act_c, std::false_type());
         }
-    }
+    });
 }
 
 // Rows that are no whole number of 16-byte chunks: 64 x 64 outputs a block
 // from fp32 copies in LDS, four by four a thread.
-template <int DT, int ACT> __global__ void __launch_bounds__(256) k_linear_act_any(LinearAct p) {
+template <int DT> __global__ void __launch_bounds__(256) k_linear_act_any(LinearAct p) {
     using T = typename Store<DT>::T;
     constexpr int K = 16;
     __shared__ float s_x[K][68], s_w[K][68];
@@ -296,69 +416,74 @@ template <int DT, int ACT> __global__ void __launch_bounds__(256) k_linear_act_a
         }
     }
     const T * residual = (const T *) p.residual;
+    by_act(p.act, [&](auto act_c) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const int64_t row = row0 + tr * 4 + i;
+        for (int i = 0; i < 4; ++i) {
+            const int64_t row = row0 + tr * 4 + i;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const int ch = col0 + tc * 4 + j;
-            if (row >= p.n || ch >= p.co) continue;
-            const int64_t e = row * p.co + ch;
-            float v = activate<DT, ACT>(acc[i][j] + (p.bias != nullptr ? p.bias[ch] : 0.0f));
-            if (residual != nullptr) v += Store<DT>::ld(residual, e);
-            Store<DT>::st((T *) p.y, e, v);
+            for (int j = 0; j < 4; ++j) {
+                const int ch = col0 + tc * 4 + j;
+                if (row >= p.n || ch >= p.co) continue;
+                const int64_t e = row * p.co + ch;
+                float v = activate<DT, decltype(act_c)::value>(acc[i][j] + (p.bias != nullptr ? p.bias[ch] : 0.0f));
+                if (residual != nullptr) v += Store<DT>::ld(residual, e);
+                Store<DT>::st((T *) p.y, e, v);
+            }
         }
-    }
+    });
 }
 
-template <int MT, int DT, int ACT, int BM, int BN, int RW, int CW>
+template <int MT, int DT, int RW, int CW, int RB, int NT, int PER_CU>
 hipError_t launch_gemm_t(LinearAct p, hipStream_t s) {
+    constexpr int BM = RW * RB * 32, BN = CW * NT * 32;
     p.row_tiles = (p.n + BM - 1) / BM;
     p.col_tiles = (p.co + BN - 1) / BN;
     const int64_t grid = (p.row_tiles + 7) / 8 * 8 * p.col_tiles;
     if (grid > 0x7fffffffLL) return hipErrorInvalidValue;
-    k_linear_act<MT, DT, ACT, BM, BN, RW, CW><<<(unsigned) grid, 64 * RW * CW, 0, s>>>(p);
+    k_linear_act<MT, DT, RW, CW, RB, NT, PER_CU><<<(unsigned) grid, 64 * RW * CW, 0, s>>>(p);
     return hipGetLastError();
 }
 
-template <int MT, int DT, int ACT> hipError_t launch_act_t(const LinearAct & p, int cus, hipStream_t s) {
+template <int MT, int DT> hipError_t launch_gemm(const LinearAct & p, int cus, hipStream_t s) {
     const auto blocks = [&](int bm, int bn) { return (p.n + bm - 1) / bm * ((p.co + bn - 1) / bn); };
-    if (blocks(256, 256) >= 2 * (int64_t) cus) return launch_gemm_t<MT, DT, ACT, 256, 256, 4, 2>(p, s);
-    if (blocks(128, 128) >= cus) return launch_gemm_t<MT, DT, ACT, 128, 128, 4, 1>(p, s);
-    return launch_gemm_t<MT, DT, ACT, 64, 128, 4, 1>(p, s);
+    static const int force = getenv("TSH_FORCE") ? atoi(getenv("TSH_FORCE")) : -1;
+    switch (force) {
+        case 0: return launch_gemm_t<MT, DT, 4, 2, 2, 4, 1>(p, s);  // 256 x 256
+        case 1: return launch_gemm_t<MT, DT, 2, 4, 3, 2, 1>(p, s);  // 192 x 256
+        case 2: return launch_gemm_t<MT, DT, 2, 4, 2, 2, 1>(p, s);  // 128 x 256, 8 waves
+        case 3: return launch_gemm_t<MT, DT, 2, 2, 2, 2, 2>(p, s);  // 128 x 128, two per CU
+        case 4: return launch_gemm_t<MT, DT, 2, 2, 1, 2, 3>(p, s);  // 64 x 128
+        case 5: return launch_gemm_t<MT, DT, 2, 4, 2, 1, 2>(p, s);  // 128 x 128, 8 waves, two per CU
+        case 6: return launch_gemm_t<MT, DT, 4, 2, 1, 2, 2>(p, s);  // 128 x 128, 8 waves, two per CU
+        default: break;
+    }
+    if (p.co % 2 != 0) return launch_gemm_t<MT, DT, 2, 4, 2, 1, 2>(p, s);
+    if (p.co % 4 == 0 && blocks(256, 256) >= 2 * (int64_t) cus) return launch_gemm_t<MT, DT, 4, 2, 2, 4, 1>(p, s);
+    if (blocks(128, 128) >= cus) return launch_gemm_t<MT, DT, 2, 2, 2, 2, 2>(p, s);
+    return launch_gemm_t<MT, DT, 2, 2, 1, 2, 3>(p, s);
 }
 
-template <int DT, int ACT> hipError_t launch_any_t(LinearAct p, hipStream_t s) {
+template <int DT> hipError_t launch_any(LinearAct p, hipStream_t s) {
     p.col_tiles = (p.co + 63) / 64;
     const int64_t grid = (p.n + 63) / 64 * p.col_tiles;
     if (grid > 0x7fffffffLL) return hipErrorInvalidValue;
-    k_linear_act_any<DT, ACT><<<(unsigned) grid, 256, 0, s>>>(p);
+    k_linear_act_any<DT><<<(unsigned) grid, 256, 0, s>>>(p);
     return hipGetLastError();
 }
 
-template <int DT, int ACT> hipError_t launch_dt(const LinearAct & p, int x_type, int cus, hipStream_t s) {
-    if (x_type == kRows8) return launch_act_t<kRows8, DT, ACT>(p, cus, s);
-    if (p.row_bytes % 16 == 0) return launch_act_t<DT, DT, ACT>(p, cus, s);
-    return launch_any_t<DT, ACT>(p, s);
-}
-
-template <int DT> hipError_t launch_act(const LinearAct & p, int x_type, int act, int cus, hipStream_t s) {
-    switch (act) {
-        case TRELLIS_SPARSE_HIP_ACT_SILU: return launch_dt<DT, TRELLIS_SPARSE_HIP_ACT_SILU>(p, x_type, cus, s);
-        case TRELLIS_SPARSE_HIP_ACT_GELU: return launch_dt<DT, TRELLIS_SPARSE_HIP_ACT_GELU>(p, x_type, cus, s);
-        case TRELLIS_SPARSE_HIP_ACT_GELU_TANH:
-            return launch_dt<DT, TRELLIS_SPARSE_HIP_ACT_GELU_TANH>(p, x_type, cus, s);
-        default: return launch_dt<DT, TRELLIS_SPARSE_HIP_ACT_NONE>(p, x_type, cus, s);
-    }
+template <int DT> hipError_t launch_dt(const LinearAct & p, int x_type, int cus, hipStream_t s) {
+    if (x_type == kRows8) return launch_gemm<kRows8, DT>(p, cus, s);
+    if (p.row_bytes % 16 == 0) return launch_gemm<DT, DT>(p, cus, s);
+    return launch_any<DT>(p, s);
 }
 
 }  // namespace
 
-hipError_t launch_linear_act(int dtype, int x_type, const LinearAct & p, int act, int cus, hipStream_t s) {
+hipError_t launch_linear_act(int dtype, int x_type, const LinearAct & p, int cus, hipStream_t s) {
     switch (dtype) {
-        case kF32: return launch_act<kF32>(p, x_type, act, cus, s);
-        case kF16: return launch_act<kF16>(p, x_type, act, cus, s);
-        default: return launch_act<kBF16>(p, x_type, act, cus, s);
+        case kF32: return launch_dt<kF32>(p, x_type, cus, s);
+        case kF16: return launch_dt<kF16>(p, x_type, cus, s);
+        default: return launch_dt<kBF16>(p, x_type, cus, s);
     }
 }
 

@@ -385,7 +385,7 @@ struct LinearAct {
     const void * residual;   // [n][co] or null; may be y
     void * y;
     int64_t n;
-    int ci, co;
+    int ci, co, act;
     int row_bytes, w_bytes;  // of a row of x and of w
     int64_t row_tiles;       // set by the launcher
     int col_tiles;
@@ -393,7 +393,7 @@ struct LinearAct {
 inline int linear_act_rows(int co) { return (co + 255) / 256 * 256; }
 // Widest row: a block's 256 rows stay below 2 GiB.
 constexpr int kLinearActMaxBytes = 1 << 22;
-hipError_t launch_linear_act(int dtype, int x_type, const LinearAct & p, int act, int cus, hipStream_t s);
+hipError_t launch_linear_act(int dtype, int x_type, const LinearAct & p, int cus, hipStream_t s);
 // Attention within sequences of rows (kernels_attn.hip).
 struct Attention {
     const void * q;
