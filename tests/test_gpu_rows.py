@@ -343,7 +343,7 @@ def test_refusals(backends, dtype):
     refused(bad, be.linear_act, q, w, None, y, 64, 32, 64)       # 8-bit rows of another width
     refused(bad, be.linear_act, x, w, None, x, 64, 64, 64)       # y over x
     refused(bad, be.linear_act, x, w, None, y, 64, 1 << 21, 64)
-    st = sh.LIB.trellis_sparse_hip_linear_act(be.ptr, x.handle, w.ctypes.data_as(sh._f32p), None, 4, None, y.handle, 64, 64, 64)
+    st = sh.LIB.trellis_sparse_hip_linear_act(be.ptr, x.handle, w.ctypes.data, None, 4, None, y.handle, 64, 64, 64)
     assert st == bad
     st = sh.LIB.trellis_sparse_hip_linear_act(be.ptr, x.handle, None, None, 0, None, y.handle, 64, 64, 64)
     assert st == bad

@@ -169,14 +169,6 @@ template <int DT> __device__ __forceinline__ f32x16 mac32(s16x8 a, s16x8 b, f32x
     }
 }
 
-// A lane's value and that of the lane 32 further on, in both lanes the same
-// way round: v_permlane32_swap exchanges the upper half of a with the lower half
-// of b.  In assembly because the builtin's two results come out as one; the
-// waits are those that the instruction needs after a vector write.
-__device__ __forceinline__ void both_halves(float v, float & a, float & b) {
-    a = b = v;
-    asm("s_nop 1\n\tv_permlane32_swap_b32 %0, %1\n\ts_nop 1" : "+v"(a), "+v"(b));
-}
 __device__ __forceinline__ float max_halves(float v) {
     float a, b;
     both_halves(v, a, b);
@@ -427,33 +419,49 @@ __global__ void __launch_bounds__(64 * NW, 2) k_attention(Attention p, Partial p
         }
 }
 
-// Joins the splits: 4 channels a thread, queries found as k_attention<.., NW> does.
+// Joins the splits, a query a wavefront: QP lanes (a power of two) have four
+// channels each, 64 / QP groups of them every so many splits.  Queries are found
+// as k_attention<.., NW> does, TQ / 4 blocks for each of its tiles.
 template <int DT, int TQ>
-__global__ void __launch_bounds__(256) k_join(Attention p, Partial part, int tiles) {
+__global__ void __launch_bounds__(256) k_join(Attention p, Partial part, int tiles, int qp) {
     using T = typename Store<DT>::T;
-    const int group = p.heads / p.kv_heads, kv = blockIdx.x / tiles;
-    const Place at = find_place<TQ>(p, blockIdx.x % tiles, group);
-    const int quads = p.dim / 4;
-    for (int i = threadIdx.x; i < at.nq * quads; i += 256) {
-        const int64_t vq = at.first + i / quads;
-        const int64_t row = at.q0 + vq / group;
-        const int head = kv * group + (int) (vq % group), c = i % quads * 4;
-        const int64_t q = row * p.heads + head, step = p.nq * p.heads;
-        float most = -__builtin_inff();
-        for (int s = 0; s < part.splits; ++s) most = fmaxf(most, part.stat[s * step + q].x);
-        const float base = most == -__builtin_inff() ? 0.0f : most;
-        float sum = 0.0f, v[4] = {0.f, 0.f, 0.f, 0.f};
-        for (int s = 0; s < part.splits; ++s) {
+    constexpr int PER = TQ / 4;
+    const int group = p.heads / p.kv_heads, kv = blockIdx.x / PER / tiles;
+    const Place at = find_place<TQ>(p, blockIdx.x / PER % tiles, group);
+    const int i = blockIdx.x % PER * 4 + (int) (threadIdx.x >> 6), lane = threadIdx.x & 63;
+    if (i >= at.nq) return;
+    const int64_t vq = at.first + i;
+    const int64_t row = at.q0 + vq / group;
+    const int head = kv * group + (int) (vq % group);
+    const int64_t q = row * p.heads + head, step = p.nq * p.heads;
+    float most = -__builtin_inff();
+    for (int s = lane; s < part.splits; s += 64) most = fmaxf(most, part.stat[s * step + q].x);
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) most = fmaxf(most, __shfl_xor(most, d));
+    const float base = most == -__builtin_inff() ? 0.0f : most;
+    const int c = lane % qp * 4;
+    float sum = 0.0f, v[4] = {0.f, 0.f, 0.f, 0.f};
+    if (c < p.dim) {
+#pragma unroll 4
+        for (int s = lane / qp; s < part.splits; s += 64 / qp) {
             const float2 st = part.stat[s * step + q];
-            if (st.x == -__builtin_inff() && st.y == 0.0f) continue;  // no keys: nothing was written
-            const float w = exp2f(st.x - base);
-            const float4 o = *(const float4 *) (part.out + (s * step + q) * p.dim + c);
+            // No keys: nothing was written.
+            const bool some = st.x != -__builtin_inff() || st.y != 0.0f;
+            const float w = some ? exp2f(st.x - base) : 0.0f;
+            const float4 o = some ? *(const float4 *) (part.out + (s * step + q) * p.dim + c) : float4{0.f, 0.f, 0.f, 0.f};
             sum += w * st.y;
             v[0] += w * o.x;
             v[1] += w * o.y;
             v[2] += w * o.z;
             v[3] += w * o.w;
         }
+    }
+    for (int d = qp; d < 64; d <<= 1) {
+        sum += __shfl_xor(sum, d);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[j] += __shfl_xor(v[j], d);
+    }
+    if (lane < qp && c < p.dim) {
         const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
         T * y = (T *) p.y + row * p.y_stride + (int64_t) head * p.dim + c;
 #pragma unroll
@@ -468,7 +476,11 @@ hipError_t launch_nw(const Attention & p, const Partial & part, int64_t tiles, h
     k_attention<DT, DC, NW><<<(unsigned) grid, 64 * NW, 0, s>>>(p, part, (int) tiles);
     hipError_t err = hipGetLastError();
     if (err == hipSuccess && part.splits > 1) {
-        k_join<DT, 32 * NW><<<(unsigned) (tiles * p.kv_heads), 256, 0, s>>>(p, part, (int) tiles);
+        int qp = 1;
+        while (qp * 4 < p.dim) qp *= 2;
+        const int64_t joins = tiles * p.kv_heads * (8 * NW);
+        if (joins > 0x7fffffffLL) return hipErrorInvalidValue;
+        k_join<DT, 32 * NW><<<(unsigned) joins, 256, 0, s>>>(p, part, (int) tiles, qp);
         err = hipGetLastError();
     }
     return err;

@@ -1,5 +1,7 @@
 // kernels_rows.hip - row operators of transformer blocks over voxel rows: RMS norm, 8-bit rows, rotary positions.
-#include "tsh_internal.h"
+#include <type_traits>
+
+#include "mfma_common.h"
 
 namespace tsh {
 namespace {
@@ -9,15 +11,14 @@ namespace {
 // Values per 16-byte chunk.
 template <int DT> constexpr int kChunk = DT == kF32 ? 4 : 8;
 
-template <int DT> __device__ __forceinline__ void load_chunk(const typename Store<DT>::T * p, float * v) {
+template <int DT> __device__ __forceinline__ void unpack_chunk_of(const int4 & c, float * v) {
     if constexpr (DT == kF32) {
-        const float4 c = *(const float4 *) p;
-        v[0] = c.x;
-        v[1] = c.y;
-        v[2] = c.z;
-        v[3] = c.w;
+        v[0] = __builtin_bit_cast(float, c.x);
+        v[1] = __builtin_bit_cast(float, c.y);
+        v[2] = __builtin_bit_cast(float, c.z);
+        v[3] = __builtin_bit_cast(float, c.w);
     } else {
-        unpack_chunk<DT>(*(const int4 *) p, v);
+        unpack_chunk<DT>(c, v);
     }
 }
 
@@ -27,13 +28,6 @@ template <int DT> __device__ __forceinline__ void store_chunk(typename Store<DT>
     } else {
         *(int4 *) p = pack_chunk<DT>(v);
     }
-}
-
-// Sum over groups of G lanes (G a power of two, groups aligned), left in each of them.
-template <int G> __device__ __forceinline__ float group_sum(float v) {
-#pragma unroll
-    for (int d = 1; d < G; d <<= 1) v += __shfl_xor(v, d);
-    return v;
 }
 
 __device__ __forceinline__ float wave_sum(float v) { return group_sum<64>(v); }
@@ -71,15 +65,6 @@ __device__ __forceinline__ uint32_t codes4(const float * v, float inv, uint32_t 
 
 __device__ __forceinline__ uint32_t abs_bits(float v) { return __builtin_bit_cast(uint32_t, v) & 0x7fffffffu; }
 
-template <int G> __device__ __forceinline__ uint32_t group_max(uint32_t v) {
-#pragma unroll
-    for (int d = 1; d < G; d <<= 1) {
-        const uint32_t o = (uint32_t) __shfl_xor((int) v, d);
-        v = o > v ? o : v;
-    }
-    return v;
-}
-
 // Where the norm's rows go.
 struct NormOut {
     void * y;          // storage type [n][c], or null
@@ -108,31 +93,36 @@ __global__ void __launch_bounds__(256) k_norm_vec(const typename Store<DT>::T * 
             const int at = (i * LPR + l) * V + u;
             g[i][u] = NORM && gamma != nullptr && at < c ? gamma[at] : 1.0f;
         }
-    for (int64_t row = (int64_t) blockIdx.x * RPB + threadIdx.x / LPR; row < n; row += (int64_t) gridDim.x * RPB) {
+    // The next row's loads run under this one's sums and stores.
+    int4 xc[CPL], rc[CPL];
+    const auto fetch = [&](int64_t row) {
+#pragma unroll
+        for (int i = 0; i < CPL; ++i) {
+            const int at = (i * LPR + l) * V;
+            xc[i] = rc[i] = int4{0, 0, 0, 0};
+            if (at < c) {
+                xc[i] = *(const int4 *) (x + row * c + at);
+                if (residual != nullptr) rc[i] = *(const int4 *) (residual + row * c + at);
+            }
+        }
+    };
+    int64_t row = (int64_t) blockIdx.x * RPB + threadIdx.x / LPR;
+    const int64_t stride = (int64_t) gridDim.x * RPB;
+    if (row < n) fetch(row);
+    for (; row < n; row += stride) {
         float v[CPL][V];
         float sum = 0.0f;
 #pragma unroll
         for (int i = 0; i < CPL; ++i) {
-            const int at = (i * LPR + l) * V;
-            if (at < c) {
-                load_chunk<DT>(x + row * c + at, v[i]);
-            } else {
+            unpack_chunk_of<DT>(xc[i], v[i]);
+            if (residual != nullptr) {
+                float r[V];
+                unpack_chunk_of<DT>(rc[i], r);
 #pragma unroll
-                for (int u = 0; u < V; ++u) v[i][u] = 0.0f;
+                for (int u = 0; u < V; ++u) v[i][u] += r[u];
             }
         }
-        if (residual != nullptr) {
-#pragma unroll
-            for (int i = 0; i < CPL; ++i) {
-                const int at = (i * LPR + l) * V;
-                if (at < c) {
-                    float r[V];
-                    load_chunk<DT>(residual + row * c + at, r);
-#pragma unroll
-                    for (int u = 0; u < V; ++u) v[i][u] += r[u];
-                }
-            }
-        }
+        if (row + stride < n) fetch(row + stride);
         if (total != nullptr) {
 #pragma unroll
             for (int i = 0; i < CPL; ++i) {
@@ -225,23 +215,40 @@ __global__ void __launch_bounds__(256) k_norm_any(const typename Store<DT>::T * 
     }
 }
 
-// The values that 8-bit rows stand for, 4 per thread (cp is a multiple of 128).
-template <int DT>
+// The values that 8-bit rows stand for: 16 codes a thread, rows found once (whole
+// 16-byte chunks of y where a row is a whole number of them).
+template <int DT, bool WHOLE>
 __global__ void __launch_bounds__(256) k_expand8(const uint8_t * __restrict__ codes, const uint8_t * __restrict__ scales,
                                                  typename Store<DT>::T * __restrict__ y, int64_t n, int c, int cp) {
-    const int quads = (c + 3) / 4;
+    constexpr int V = kChunk<DT>;
+    const int pieces = (c + 15) / 16;
     const int64_t i = (int64_t) blockIdx.x * 256 + threadIdx.x;
-    if (i >= n * quads) return;
-    const int64_t row = i / quads;
-    const int at = (int) (i % quads) * 4;
-    const int w = *(const int *) (codes + row * cp + at);
+    if (i >= n * pieces) return;
+    const int64_t row = n * pieces <= INT32_MAX ? (int64_t) ((uint32_t) i / (uint32_t) pieces) : i / pieces;
+    const int at = (int) (i - row * pieces) * 16;
+    const int4 w = *(const int4 *) (codes + row * cp + at);
     const uint32_t byte = scales[row * (cp / 32) + at / 32];
     const float scale = byte == 255 ? __builtin_nanf("") : __builtin_bit_cast(float, byte << 23);
-    const auto lo = __builtin_amdgcn_cvt_pk_f32_fp8(w, false), hi = __builtin_amdgcn_cvt_pk_f32_fp8(w, true);
-    const float v[4] = {lo[0] * scale, lo[1] * scale, hi[0] * scale, hi[1] * scale};
+    const int quad[4] = {w.x, w.y, w.z, w.w};
+    float v[16];
 #pragma unroll
-    for (int u = 0; u < 4; ++u)
-        if (at + u < c) Store<DT>::st(y, row * c + at + u, v[u]);
+    for (int k = 0; k < 4; ++k) {
+        const auto lo = __builtin_amdgcn_cvt_pk_f32_fp8(quad[k], false), hi = __builtin_amdgcn_cvt_pk_f32_fp8(quad[k], true);
+        v[4 * k] = lo[0] * scale;
+        v[4 * k + 1] = lo[1] * scale;
+        v[4 * k + 2] = hi[0] * scale;
+        v[4 * k + 3] = hi[1] * scale;
+    }
+    typename Store<DT>::T * yr = y + row * c + at;
+    if constexpr (WHOLE) {
+#pragma unroll
+        for (int u = 0; u < 16; u += V)
+            if (at + u < c) store_chunk<DT>(yr + u, v + u);
+    } else {
+#pragma unroll
+        for (int u = 0; u < 16; ++u)
+            if (at + u < c) Store<DT>::st(yr, u, v[u]);
+    }
 }
 
 template <int DT, bool Q8, bool NORM>
@@ -261,7 +268,7 @@ hipError_t norm_dt(const void * x, const void * residual, const float * gamma, v
     const auto launch = [&](auto lpr, auto cpl) {
         constexpr int LPR = decltype(lpr)::value, CPL = decltype(cpl)::value;
         constexpr int RPB = 256 / LPR;
-        const int64_t g = std::min<int64_t>((n + RPB - 1) / RPB, (int64_t) cus * 8);
+        const int64_t g = std::min<int64_t>((n + RPB - 1) / RPB, (int64_t) cus * 4);
         k_norm_vec<DT, LPR, CPL, Q8, NORM><<<(unsigned) g, 256, 0, s>>>((const T *) x, (const T *) residual, gamma,
                                                                         (T *) total, out, n, c, eps);
         return hipGetLastError();
@@ -292,7 +299,7 @@ hipError_t norm_dt(const void * x, const void * residual, const float * gamma, v
 // each over all rows, gamma in registers.
 struct RotaryShape {
     int64_t n, x_stride, y_stride;
-    int heads, dim, split, total;  // total: turned pairs
+    int heads, dim, total;  // total: turned pairs
     int axis1, axis2;              // first pair of the y and z axes
     float eps;
     int rows;                      // rows per block
@@ -301,7 +308,7 @@ struct RotaryFreq {
     double turns[kRotaryMaxDim / 2];  // freq / 2 pi per pair
 };
 
-template <int DT, int GP, bool NORM>
+template <int DT, int GP, bool NORM, bool SPLIT>
 __global__ void __launch_bounds__(256) k_rotary(const typename Store<DT>::T * x, const int32_t * __restrict__ coords,
                                                 const float * __restrict__ gamma, typename Store<DT>::T * y,
                                                 RotaryShape p, RotaryFreq f) {
@@ -310,6 +317,32 @@ __global__ void __launch_bounds__(256) k_rotary(const typename Store<DT>::T * x,
     const int64_t row0 = (int64_t) blockIdx.x * p.rows;
     const int rows = (int) min((int64_t) p.rows, p.n - row0);
     const int half = p.dim / 2;
+
+    constexpr int GROUPS = 256 / GP;  // (row, head) items at a time
+    const int lanes = p.dim / 8;      // lanes with channels in a group of GP
+    const int l = threadIdx.x % GP, item = threadIdx.x / GP;
+    const int heads = min(p.heads, GROUPS);
+    const int step = GROUPS / heads;  // rows at a time
+    const int hi = item % heads, ri = item / heads;
+    const bool on = l < lanes && ri < step;
+    // A lane's two runs of four channels, and its first pair.
+    const int a_at = SPLIT ? 4 * l : 8 * l, b_at = SPLIT ? half + 4 * l : 8 * l + 4, pair = 4 * l;
+    // Two runs as they are in memory; the next item's are on their way while one is turned.
+    using Run = typename std::conditional<DT == kF32, int4, int2>::type;
+    Run na{}, nb{};
+    const auto fetch = [&](int h, int r) {
+        if (!on || h >= p.heads || r >= rows) return;
+        const T * xr = x + (row0 + r) * p.x_stride + (int64_t) h * p.dim;
+        if constexpr (DT != kF32 && !SPLIT) {
+            const int4 c = *(const int4 *) (xr + a_at);
+            na = int2{c.x, c.y};
+            nb = int2{c.z, c.w};
+        } else {
+            na = *(const Run *) (xr + a_at);
+            nb = *(const Run *) (xr + b_at);
+        }
+    };
+    fetch(hi, ri);
     for (int i = threadIdx.x; i < rows * half; i += 256) {
         const int r = i / half, j = i % half;
         float sn = 0.0f, cs = 1.0f;
@@ -321,17 +354,7 @@ __global__ void __launch_bounds__(256) k_rotary(const typename Store<DT>::T * x,
         s_turn[i] = float2{cs, sn};
     }
     __syncthreads();
-
-    constexpr int GROUPS = 256 / GP;  // (row, head) items at a time
-    const int lanes = p.dim / 8;      // lanes with channels in a group of GP
-    const int l = threadIdx.x % GP, item = threadIdx.x / GP;
-    const int heads = min(p.heads, GROUPS);
-    const int step = GROUPS / heads;  // rows at a time
-    const int hi = item % heads, ri = item / heads;
     if (ri >= step) return;
-    const bool on = l < lanes;
-    // A lane's two runs of four channels, and its first pair.
-    const int a_at = p.split ? 4 * l : 8 * l, b_at = p.split ? half + 4 * l : 8 * l + 4, pair = 4 * l;
     for (int h = hi; h < p.heads; h += heads) {
         float g[8];
         if constexpr (NORM) {
@@ -341,17 +364,18 @@ __global__ void __launch_bounds__(256) k_rotary(const typename Store<DT>::T * x,
         }
         for (int r = ri; r < rows; r += step) {
             float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-            const T * xr = x + (row0 + r) * p.x_stride + (int64_t) h * p.dim;
             if (on) {
                 if constexpr (DT == kF32) {
-                    load_chunk<DT>(xr + a_at, v);
-                    load_chunk<DT>(xr + b_at, v + 4);
-                } else if (p.split) {
-                    const int2 a = *(const int2 *) (xr + a_at), b = *(const int2 *) (xr + b_at);
-                    unpack_chunk<DT>(int4{a.x, a.y, b.x, b.y}, v);
+                    unpack_chunk_of<DT>(na, v);
+                    unpack_chunk_of<DT>(nb, v + 4);
                 } else {
-                    load_chunk<DT>(xr + a_at, v);
+                    unpack_chunk<DT>(int4{na.x, na.y, nb.x, nb.y}, v);
                 }
+            }
+            if (r + step < rows) {
+                fetch(h, r + step);
+            } else {
+                fetch(h + heads, ri);
             }
             if constexpr (NORM) {
                 float sum = 0.0f;
@@ -366,15 +390,10 @@ __global__ void __launch_bounds__(256) k_rotary(const typename Store<DT>::T * x,
 #pragma unroll
                 for (int u = 0; u < 4; ++u) {
                     const float2 t = s_turn[r * half + pair + u];
-                    const float a = p.split ? v[u] : v[2 * u], b = p.split ? v[u + 4] : v[2 * u + 1];
+                    const float a = v[SPLIT ? u : 2 * u], b = v[SPLIT ? u + 4 : 2 * u + 1];
                     const float oa = a * t.x - b * t.y, ob = a * t.y + b * t.x;
-                    if (p.split) {
-                        o[u] = oa;
-                        o[u + 4] = ob;
-                    } else {
-                        o[2 * u] = oa;
-                        o[2 * u + 1] = ob;
-                    }
+                    o[SPLIT ? u : 2 * u] = oa;
+                    o[SPLIT ? u + 4 : 2 * u + 1] = ob;
                 }
                 T * yr = y + (row0 + r) * p.y_stride + (int64_t) h * p.dim;
                 if constexpr (DT == kF32) {
@@ -382,7 +401,7 @@ __global__ void __launch_bounds__(256) k_rotary(const typename Store<DT>::T * x,
                     store_chunk<DT>(yr + b_at, o + 4);
                 } else {
                     const int4 c = pack_chunk<DT>(o);
-                    if (p.split) {
+                    if constexpr (SPLIT) {
                         *(int2 *) (yr + a_at) = int2{c.x, c.y};
                         *(int2 *) (yr + b_at) = int2{c.z, c.w};
                     } else {
@@ -396,21 +415,22 @@ __global__ void __launch_bounds__(256) k_rotary(const typename Store<DT>::T * x,
 
 template <int DT>
 hipError_t rotary_dt(const void * x, const int32_t * coords, const float * gamma, void * y, RotaryShape p,
-                     const RotaryFreq & f, bool norm, int cus, hipStream_t s) {
+                     const RotaryFreq & f, bool norm, bool split, int cus, hipStream_t s) {
     using T = typename Store<DT>::T;
     // Blocks of 16 rows share the sines' latency; with few rows smaller ones fill the CUs.
     p.rows = p.n >= (int64_t) cus * 64 ? 16 : 4;
     const int64_t g = (p.n + p.rows - 1) / p.rows;
     if (g > 0x7fffffffLL) return hipErrorInvalidValue;
     const size_t lds = (size_t) p.rows * (p.dim / 2) * sizeof(float2);
-    const auto launch = [&](auto gp) {
-        constexpr int GP = decltype(gp)::value;
-        if (norm) {
-            k_rotary<DT, GP, true><<<(unsigned) g, 256, lds, s>>>((const T *) x, coords, gamma, (T *) y, p, f);
-        } else {
-            k_rotary<DT, GP, false><<<(unsigned) g, 256, lds, s>>>((const T *) x, coords, gamma, (T *) y, p, f);
-        }
+    const auto launch_as = [&](auto gp, auto norm_c, auto split_c) {
+        k_rotary<DT, decltype(gp)::value, decltype(norm_c)::value, decltype(split_c)::value>
+            <<<(unsigned) g, 256, lds, s>>>((const T *) x, coords, gamma, (T *) y, p, f);
         return hipGetLastError();
+    };
+    const auto launch = [&](auto gp) {
+        using std::bool_constant;
+        if (norm) return split ? launch_as(gp, bool_constant<true>(), bool_constant<true>()) : launch_as(gp, bool_constant<true>(), bool_constant<false>());
+        return split ? launch_as(gp, bool_constant<false>(), bool_constant<true>()) : launch_as(gp, bool_constant<false>(), bool_constant<false>());
     };
     if (p.dim <= 32) return launch(std::integral_constant<int, 4>());
     if (p.dim <= 64) return launch(std::integral_constant<int, 8>());
@@ -452,15 +472,24 @@ hipError_t launch_pack8(int dtype, const void * x, uint8_t * codes, uint8_t * sc
 
 hipError_t launch_expand8(int dtype, const uint8_t * codes, const uint8_t * scales, void * y, int64_t n, int c,
                           hipStream_t s) {
-    const int64_t g = (n * ((c + 3) / 4) + 255) / 256;
+    const int64_t g = (n * ((c + 15) / 16) + 255) / 256;
     if (g > 0x7fffffffLL) return hipErrorInvalidValue;
     const int cp = rows8_width(c);
+    const auto launch = [&](auto dt) {
+        constexpr int DT = decltype(dt)::value;
+        using T = typename Store<DT>::T;
+        if (c % kChunk<DT> == 0) {
+            k_expand8<DT, true><<<(unsigned) g, 256, 0, s>>>(codes, scales, (T *) y, n, c, cp);
+        } else {
+            k_expand8<DT, false><<<(unsigned) g, 256, 0, s>>>(codes, scales, (T *) y, n, c, cp);
+        }
+        return hipGetLastError();
+    };
     switch (dtype) {
-        case kF32: k_expand8<kF32><<<(unsigned) g, 256, 0, s>>>(codes, scales, (float *) y, n, c, cp); break;
-        case kF16: k_expand8<kF16><<<(unsigned) g, 256, 0, s>>>(codes, scales, (_Float16 *) y, n, c, cp); break;
-        default: k_expand8<kBF16><<<(unsigned) g, 256, 0, s>>>(codes, scales, (uint16_t *) y, n, c, cp); break;
+        case kF32: return launch(std::integral_constant<int, kF32>());
+        case kF16: return launch(std::integral_constant<int, kF16>());
+        default: return launch(std::integral_constant<int, kBF16>());
     }
-    return hipGetLastError();
 }
 
 hipError_t launch_rotary(int dtype, const void * x, const int32_t * coords, const float * gamma, void * y,
@@ -471,7 +500,6 @@ hipError_t launch_rotary(int dtype, const void * x, const int32_t * coords, cons
     p.y_stride = plan.y_stride;
     p.heads = plan.heads;
     p.dim = plan.dim;
-    p.split = plan.split;
     p.axis1 = plan.pairs[0];
     p.axis2 = plan.pairs[0] + plan.pairs[1];
     p.total = p.axis2 + plan.pairs[2];
@@ -483,9 +511,9 @@ hipError_t launch_rotary(int dtype, const void * x, const int32_t * coords, cons
             f.turns[at++] = pow(plan.base, -(double) j / plan.pairs[a]) / (2.0 * M_PI);
     for (; at < kRotaryMaxDim / 2; ++at) f.turns[at] = 0.0;
     switch (dtype) {
-        case kF32: return rotary_dt<kF32>(x, coords, gamma, y, p, f, plan.norm, cus, s);
-        case kF16: return rotary_dt<kF16>(x, coords, gamma, y, p, f, plan.norm, cus, s);
-        default: return rotary_dt<kBF16>(x, coords, gamma, y, p, f, plan.norm, cus, s);
+        case kF32: return rotary_dt<kF32>(x, coords, gamma, y, p, f, plan.norm, plan.split != 0, cus, s);
+        case kF16: return rotary_dt<kF16>(x, coords, gamma, y, p, f, plan.norm, plan.split != 0, cus, s);
+        default: return rotary_dt<kBF16>(x, coords, gamma, y, p, f, plan.norm, plan.split != 0, cus, s);
     }
 }
 

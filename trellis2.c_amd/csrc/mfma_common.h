@@ -1,5 +1,7 @@
 // mfma_common.h - device helpers shared by the MFMA kernels (conv, linear).
 #pragma once
+#include <type_traits>
+
 #include "tsh_internal.h"
 
 namespace tsh {
@@ -94,6 +96,54 @@ __device__ __forceinline__ float row16_sum(float v) {
     v += __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, v), 0x122, 0xf, 0xf, false));
     v += __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, v), 0x121, 0xf, 0xf, false));
     return v;
+}
+
+// A lane's value and that of the lane 32 (16) further on, in both lanes the same
+// way round: v_permlane32_swap exchanges the upper half of a with the lower half
+// of b (v_permlane16_swap every odd row of 16 lanes of a with the even one before it
+// of b).  In assembly because the builtin's two results come out as one; the
+// waits are those that the instruction needs after a vector write.
+__device__ __forceinline__ void both_halves(float v, float & a, float & b) {
+    a = b = v;
+    asm("s_nop 1\n\tv_permlane32_swap_b32 %0, %1\n\ts_nop 1" : "+v"(a), "+v"(b));
+}
+__device__ __forceinline__ void both_rows(float v, float & a, float & b) {
+    a = b = v;
+    asm("s_nop 1\n\tv_permlane16_swap_b32 %0, %1\n\ts_nop 1" : "+v"(a), "+v"(b));
+}
+
+// op over aligned groups of G lanes (a power of two), left in each of them: the
+// neighbour and the next pair by DPP, then mirror images (a partial result is the
+// same in all lanes that it covers), then the exchanges above.
+template <int G, class Op> __device__ __forceinline__ float group_reduce(float v, Op op) {
+    const auto dpp = [&](auto ctrl) {
+        return __builtin_bit_cast(
+            float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, v), decltype(ctrl)::value, 0xf, 0xf, false));
+    };
+    if constexpr (G > 1) v = op(v, dpp(std::integral_constant<int, 0xB1>()));
+    if constexpr (G > 2) v = op(v, dpp(std::integral_constant<int, 0x4E>()));
+    if constexpr (G > 4) v = op(v, dpp(std::integral_constant<int, 0x141>()));
+    if constexpr (G > 8) v = op(v, dpp(std::integral_constant<int, 0x140>()));
+    float a, b;
+    if constexpr (G > 16) {
+        both_rows(v, a, b);
+        v = op(a, b);
+    }
+    if constexpr (G > 32) {
+        both_halves(v, a, b);
+        v = op(a, b);
+    }
+    return v;
+}
+template <int G> __device__ __forceinline__ float group_sum(float v) {
+    return group_reduce<G>(v, [](float a, float b) { return a + b; });
+}
+// The largest of non-negative values as bits (a NaN's are larger than any number's).
+template <int G> __device__ __forceinline__ uint32_t group_max(uint32_t v) {
+    return __builtin_bit_cast(uint32_t, group_reduce<G>(__builtin_bit_cast(float, v), [](float a, float b) {
+                                  const uint32_t x = __builtin_bit_cast(uint32_t, a), y = __builtin_bit_cast(uint32_t, b);
+                                  return __builtin_bit_cast(float, x > y ? x : y);
+                              }));
 }
 
 }  // namespace

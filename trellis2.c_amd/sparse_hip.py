@@ -15,7 +15,7 @@ from __future__ import annotations
 import ctypes
 import os
 from ctypes import (CFUNCTYPE, POINTER, Structure, c_char_p, c_double, c_float, c_int, c_int32, c_int64, c_size_t,
-                    c_uint, c_uint32, c_void_p)
+                    c_uint, c_uint32, c_void_p, byref)
 
 import numpy as np
 
@@ -157,8 +157,8 @@ ABI = {
     "trellis_sparse_hip_alloc_rows8": (c_int, [_p, c_int64, c_int, POINTER(_p)]),
     "trellis_sparse_hip_pack_rows8": (c_int, [_p, _p, _p, c_int64, c_int]),
     "trellis_sparse_hip_expand_rows8": (c_int, [_p, _p, _p, c_int64, c_int]),
-    "trellis_sparse_hip_rms_norm": (c_int, [_p, _p, _p, _f32p, _p, _p, c_int64, c_int, c_float]),
-    "trellis_sparse_hip_linear_act": (c_int, [_p, _p, _f32p, _f32p, c_int, _p, _p, c_int64, c_int, c_int]),
+    "trellis_sparse_hip_rms_norm": (c_int, [_p, _p, _p, c_void_p, _p, _p, c_int64, c_int, c_float]),
+    "trellis_sparse_hip_linear_act": (c_int, [_p, _p, c_void_p, c_void_p, c_int, _p, _p, c_int64, c_int, c_int]),
     "trellis_sparse_hip_rotary": (c_int, [_p, _p, _p, _p, _p, c_int64, POINTER(RotaryDesc)]),
     "trellis_sparse_hip_attention": (c_int, [_p, _p, _p, _p, _p, c_int64, c_int64, _p, _p, c_int,
                                              POINTER(AttentionDesc)]),
@@ -274,6 +274,10 @@ def _f32(a):
     return None if a is None else np.ascontiguousarray(a, dtype=np.float32)
 
 
+def _address(a):
+    return None if a is None else a.__array_interface__["data"][0]
+
+
 def _ptr(a, t):
     return None if a is None else a.ctypes.data_as(t)
 
@@ -288,7 +292,7 @@ class Buffer:
 
     def free(self):
         if self.handle:
-            self.backend.ops.free_buffer(self.backend.ptr, self.handle)
+            self.backend.free_buffer(self.backend.ptr, self.handle)
             self.handle = c_void_p()
 
     def __del__(self):
@@ -326,6 +330,18 @@ class DeviceMap:
         self.n = n
 
 
+_WRAP = {}  # (a tensor's dtype, a backend's) -> the entry point that takes it
+
+
+def _wrap_function(dtype, backend_dtype: int):
+    name = str(dtype).rpartition(".")[2]
+    if name != "int32" and name != ("float32", "float16", "bfloat16")[backend_dtype]:
+        raise TypeError(f"wrap: {name} rows on a backend of dtype {backend_dtype}")
+    fn = LIB.trellis_sparse_hip_wrap_i32 if name == "int32" else LIB.trellis_sparse_hip_wrap_f32
+    _WRAP[dtype, backend_dtype] = fn
+    return fn
+
+
 class Backend:
     """One sparse backend instance on one device."""
 
@@ -345,6 +361,7 @@ class Backend:
         self.ptr = out
         self.struct = ctypes.cast(out, POINTER(BackendStruct)).contents
         self.ops = self.struct.ops.contents
+        self.free_buffer = self.ops.free_buffer
         self.dtype = dtype
         self.linear_algo = linear_algo
         self.alive = True
@@ -443,15 +460,16 @@ class Backend:
         """A buffer over a contiguous device tensor's memory (anything with torch's data_ptr(), numel() and dtype): of
         the backend's dtype, or int32.  The buffer keeps the tensor.  A process that uses torch imports it before this
         module, so that both use the HIP runtime that torch brings."""
-        name = str(tensor.dtype).rpartition(".")[2]
-        if name != "int32" and name != ("float32", "float16", "bfloat16")[self.dtype]:
-            raise TypeError(f"wrap: {name} rows on a backend of dtype {self.dtype}")
+        fn = _WRAP.get((tensor.dtype, self.dtype))
+        if fn is None:
+            fn = _wrap_function(tensor.dtype, self.dtype)
         if not tensor.is_contiguous():
             raise ValueError("wrap: the tensor is not contiguous")
-        fn = LIB.trellis_sparse_hip_wrap_i32 if name == "int32" else LIB.trellis_sparse_hip_wrap_f32
         h = c_void_p()
         count = tensor.numel()
-        self._check(fn(self.ptr, tensor.data_ptr(), count, ctypes.byref(h)), "wrap")
+        st = fn(self.ptr, tensor.data_ptr(), count, byref(h))
+        if st != OK:
+            self._check(st, "wrap")
         buf = Buffer(self, h, count)
         buf.tensor = tensor
         return buf
@@ -479,7 +497,7 @@ class Backend:
                  total: Buffer | None = None):
         """total = x + residual; y (rows or 8-bit rows) = total / sqrt(mean(total^2) + eps) * gamma."""
         g = None if gamma is None else self.keep(_f32(gamma))
-        self._check(LIB.trellis_sparse_hip_rms_norm(self.ptr, x.handle, residual and residual.handle, _ptr(g, _f32p),
+        self._check(LIB.trellis_sparse_hip_rms_norm(self.ptr, x.handle, residual and residual.handle, _address(g),
                                                     total and total.handle, y.handle, n, c, eps), "rms_norm")
 
     def linear_act(self, x: Buffer, weight, bias, y: Buffer, n: int, ci: int, co: int, act: str = "none",
@@ -487,7 +505,7 @@ class Backend:
         """y = act(x W^T + bias) + residual, x rows or 8-bit rows; act one of ACTS."""
         w = self.keep(_f32(weight))
         b = None if bias is None else self.keep(_f32(bias))
-        self._check(LIB.trellis_sparse_hip_linear_act(self.ptr, x.handle, _ptr(w, _f32p), _ptr(b, _f32p), ACTS[act],
+        self._check(LIB.trellis_sparse_hip_linear_act(self.ptr, x.handle, _address(w), _address(b), ACTS[act],
                                                       residual and residual.handle, y.handle, n, ci, co), "linear_act")
 
     def rotary(self, x: Buffer, coords, y: Buffer, n: int, heads: int, head_dim: int, pairs, base: float = 10000.0,
