@@ -205,7 +205,7 @@ struct Partial {
 // a K read (16 rows, one chunk) and the 32 of a V read (4 rows x 4 chunks, two of
 // them) touch different banks.
 template <int DT, int DC, int NW>
-__global__ void __launch_bounds__(64 * NW, 2) k_attention(Attention p, Partial part, int tiles) {
+__global__ void __launch_bounds__(64 * NW, DC <= 64 ? 3 : 2) k_attention(Attention p, Partial part, int tiles) {
     using T = typename Store<DT>::T;
     constexpr int TQ = 32 * NW, TK = 64;
     constexpr int LP = DC <= 64 ? 64 : 128;      // values per LDS row
@@ -273,22 +273,20 @@ __global__ void __launch_bounds__(64 * NW, 2) k_attention(Attention p, Partial p
         v_off[j] = in ? (uint32_t) (r * vs + c * 16) : kOutside;
     }
     const uint32_t lds0 = (uint32_t) (uintptr_t) (__attribute__((address_space(3))) unsigned char *) s_tile;
-    const auto load = [&](int t) {
+    const auto load = [&](const char * base, int pitch, const uint32_t (&off)[PER], int t, uint32_t to) {
         const int left = at.nk - t * TK;
         const int rows = left < TK ? left : TK;
-        const __amdgpu_buffer_rsrc_t kr = __builtin_amdgcn_make_buffer_rsrc((void *) (kb + (int64_t) t * TK * ks), 0,
-                                                                            (rows - 1) * ks + p.dim * 2, 0x00020000);
-        const __amdgpu_buffer_rsrc_t vr = __builtin_amdgcn_make_buffer_rsrc((void *) (vb + (int64_t) t * TK * vs), 0,
-                                                                            (rows - 1) * vs + p.dim * 2, 0x00020000);
-        const uint32_t to = lds0 + (uint32_t) ((t & 1) * 2 * TILE + wave * PER * 1024);
+        const __amdgpu_buffer_rsrc_t res = __builtin_amdgcn_make_buffer_rsrc(
+            (void *) (base + (int64_t) t * TK * pitch), 0, (rows - 1) * pitch + p.dim * 2, 0x00020000);
+        // Rows past the end are zeros.
 #pragma unroll
-        for (int j = 0; j < PER; ++j) {
-            // Rows past the end are zeros.
-            const bool in = (wave * PER + j) * RPL + lane / CH < rows;
-            dma_b128(kr, to + j * 1024u, in ? k_off[j] : kOutside, 0);
-            dma_b128(vr, to + TILE + j * 1024u, in ? v_off[j] : kOutside, 0);
-        }
+        for (int j = 0; j < PER; ++j)
+            dma_b128(res, lds0 + to + (wave * PER + j) * 1024u,
+                     (wave * PER + j) * RPL + lane / CH < rows ? off[j] : kOutside, 0);
     };
+    // Keys of tile t in buffer (t - t0) % 2, its values in the same of two more.
+    const auto load_k = [&](int t) { load(kb, ks, k_off, t, (uint32_t) (((t - t0) & 1) * TILE)); };
+    const auto load_v = [&](int t) { load(vb, vs, v_off, t, (uint32_t) (((t - t0) & 1) * TILE + 2 * TILE)); };
 
     // Reads: K row l32 (+ 32), chunk 2 k + half; V rows 4 half + (lane % 16) / 4
     // (+ 8, + 16 g), 16-value column block (lane / 16) % 2 of each 32.
@@ -310,63 +308,85 @@ __global__ void __launch_bounds__(64 * NW, 2) k_attention(Attention p, Partial p
     for (int d = 0; d < DT32; ++d)
 #pragma unroll
         for (int i = 0; i < 16; ++i) out[d][i] = 0.0f;
-    float ref = -__builtin_inff(), sum = 0.0f;
+    float ref = -__builtin_inff(), sum0 = 0.0f, sum1 = 0.0f;
 
-    if (t0 < t1) load(t0);
-    for (int t = t0; t < t1; ++t) {
-        wait_vmcnt<0>();
-        lds_barrier();
-        if (t + 1 < t1) load(t + 1);
-        const unsigned char * sk = s_tile + (t & 1) * 2 * TILE;
-        f32x16 s[2];
+    // The scores' product k (of KS) of keys n (of 2).
+    const auto read_k = [&](const unsigned char * sk, int n, int k) {
+        return *(const s16x8 *) (sk + n * 32 * ROW + k_read[k]);
+    };
+    const auto zero = [](f32x16 & v) {
 #pragma unroll
-        for (int n = 0; n < 2; ++n) {
-#pragma unroll
-            for (int i = 0; i < 16; ++i) s[n][i] = 0.0f;
-#pragma unroll
-            for (int k = 0; k < KS; ++k)
-                s[n] = mac32<DT>(*(const s16x8 *) (sk + n * 32 * ROW + k_read[k]), q[k], s[n]);
-        }
+        for (int i = 0; i < 16; ++i) v[i] = 0.0f;
+    };
+    // One tile: softmax of `cur`, the scores of tile t, and their products with
+    // its values, and the scores of tile t + 1 into `nxt`.  Products and
+    // exponentials are written down in turns, in four steps of 16 keys:
+    //   step g: weights of group g; the values' products of group g - 1 beside the
+    //   first half of them, a quarter of the next scores beside the second.
+    // Fragments are read half a step before their products.
+    const auto tile = [&](int t, int j, f32x16 (&cur)[2], f32x16 (&nxt)[2]) {
         const int left = at.nk - t * TK;
         if (left < TK) {
 #pragma unroll
             for (int n = 0; n < 2; ++n)
 #pragma unroll
                 for (int i = 0; i < 16; ++i)
-                    if (n * 32 + 8 * (i / 4) + 4 * half + i % 4 >= left) s[n][i] = -__builtin_inff();
+                    if (n * 32 + 8 * (i / 4) + 4 * half + i % 4 >= left) cur[n][i] = -__builtin_inff();
         }
-        float m = s[0][0];
+        float m = cur[0][0];
 #pragma unroll
         for (int n = 0; n < 2; ++n)
 #pragma unroll
-            for (int i = 0; i < 16; ++i) m = fmaxf(m, s[n][i]);
+            for (int i = 0; i < 16; ++i) m = fmaxf(m, cur[n][i]);
         m = max_halves(m) * scale;
         if (__any(m > ref + 8.0f)) {
             const float next = fmaxf(ref, m);
             const float keep = next == -__builtin_inff() ? 1.0f : __builtin_amdgcn_exp2f(ref - next);
             ref = next;
-            sum *= keep;
+            sum0 *= keep;
+            sum1 *= keep;
 #pragma unroll
             for (int d = 0; d < DT32; ++d)
 #pragma unroll
                 for (int i = 0; i < 16; ++i) out[d][i] *= keep;
         }
         const float base = ref == -__builtin_inff() ? 0.0f : ref;
-#pragma unroll
-        for (int n = 0; n < 2; ++n)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                s[n][i] = __builtin_amdgcn_exp2f(fmaf(s[n][i], scale, -base));
-                sum += s[n][i];
-            }
+        // Keys of t + 1 and values of t have landed; every wavefront is done with
+        // the keys of t and the values of t - 1.
+        wait_vmcnt<0>();
+        lds_barrier();
+        if (t + 2 < t1) load_k(t + 2);
+        if (t + 1 < t1) load_v(t + 1);
+        // (Past the last tile these are old keys, and the scores are not used.)
+        const unsigned char * sk = s_tile + ((j & 1) ^ 1) * TILE;
+        const unsigned char * sv = s_tile + (j & 1) * TILE + 2 * TILE;
+        zero(nxt[0]);
+        zero(nxt[1]);
+        constexpr int QPS = KS / 2;  // products of the next scores per step
+        s16x8 kf[QPS], vf[DT32], w;
+        const auto values = [&](int d) { out[d] = mac32<DT>(vf[d], w, out[d]); };
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
-            union {
-                T h[8];
-                s16x8 v;
-            } w;
+            float e[8];
+            const auto weight = [&](int i) {
+                e[i] = __builtin_amdgcn_exp2f(fmaf(cur[g / 2][8 * (g % 2) + i], scale, -base));
+            };
 #pragma unroll
-            for (int i = 0; i < 8; ++i) w.h[i] = round_to_store<DT>(s[g / 2][8 * (g % 2) + i]);
+            for (int i = 0; i < QPS; ++i) kf[i] = read_k(sk, g / 2, g % 2 * QPS + i);
+            __builtin_amdgcn_sched_barrier(0);
+            if (g > 0) {
+#pragma unroll
+                for (int d = 0; d < DT32; ++d) {
+                    values(d);
+#pragma unroll
+                    for (int i = 4 * d / DT32; i < 4 * (d + 1) / DT32; ++i) weight(i);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) weight(i);
+                __builtin_amdgcn_sched_barrier(0);
+            }
 #pragma unroll
             for (int d = 0; d < DT32; ++d) {
                 union {
@@ -374,14 +394,59 @@ __global__ void __launch_bounds__(64 * NW, 2) k_attention(Attention p, Partial p
                     s16x8 v;
                 } a;
 #pragma unroll
-                for (int e = 0; e < 2; ++e)
-                    a.h[e] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                        (__attribute__((address_space(3))) s16x4 *) (sk + TILE + g * 16 * ROW + v_read[d][e]));
-                out[d] = mac32<DT>(a.v, w.v, out[d]);
+                for (int x = 0; x < 2; ++x)
+                    a.h[x] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                        (__attribute__((address_space(3))) s16x4 *) (sv + g * 16 * ROW + v_read[d][x]));
+                vf[d] = a.v;
             }
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int i = 0; i < QPS; ++i) {
+                nxt[g / 2] = mac32<DT>(kf[i], q[g % 2 * QPS + i], nxt[g / 2]);
+#pragma unroll
+                for (int x = 4 + 4 * i / QPS; x < 4 + 4 * (i + 1) / QPS; ++x) weight(x);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            union {
+                T h[8];
+                s16x8 v;
+            } r;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                r.h[i] = round_to_store<DT>(e[i]);
+                if (i % 2 == 0) {
+                    sum0 += e[i];
+                } else {
+                    sum1 += e[i];
+                }
+            }
+            w = r.v;
+        }
+#pragma unroll
+        for (int d = 0; d < DT32; ++d) values(d);
+    };
+
+    if (t0 < t1) {
+        load_k(t0);
+        load_v(t0);
+        if (t0 + 1 < t1) load_k(t0 + 1);
+        wait_vmcnt<0>();
+        lds_barrier();
+        f32x16 sa[2], sb[2];
+#pragma unroll
+        for (int n = 0; n < 2; ++n) {
+            zero(sa[n]);
+#pragma unroll
+            for (int k = 0; k < KS; ++k) sa[n] = mac32<DT>(read_k(s_tile, n, k), q[k], sa[n]);
+        }
+        for (int t = t0; t < t1; t += 2) {
+            tile(t, 0, sa, sb);
+            if (t + 1 >= t1) break;
+            tile(t + 1, 1, sb, sa);
         }
     }
 
+    float sum = sum0 + sum1;
     sum = sum_halves(sum);
     if (!live) return;
     if (part.splits > 1) {
