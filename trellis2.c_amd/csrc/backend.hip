@@ -2226,9 +2226,20 @@ trellis_status linear_act_impl(trellis_sparse_backend * backend, const trellis_s
     p.ci = ci;
     p.co = co;
     p.act = act;
+    // Scratch for split sums is the pool's; where none is to be had (also under
+    // capture, where two graphs could share it) a block takes all of K.
+    const int x_type = from8 ? kRows8 : dt;
+    LinearActPlan plan = linear_act_plan(dt, x_type, n, co, p.row_bytes, p.w_bytes, be->cus, !capturing(be));
+    DevMem scratch;
+    if (plan.scratch > 0 && dev_alloc(be, plan.scratch, &scratch) != TRELLIS_STATUS_OK) {
+        be->last_error.clear();
+        plan = linear_act_plan(dt, x_type, n, co, p.row_bytes, p.w_bytes, be->cus, false);
+    }
+    p.partial = (float *) scratch.ptr;
     stage_begin(be, TRELLIS_SPARSE_HIP_STAGE_ELEMENTWISE);
-    const hipError_t err = launch_linear_act(dt, from8 ? kRows8 : dt, p, be->cus, be->stream);
+    const hipError_t err = launch_linear_act(dt, x_type, p, plan, be->stream);
     stage_end(be, TRELLIS_SPARSE_HIP_STAGE_ELEMENTWISE);
+    dev_release(be, &scratch);
     return hip_status(be, err, "linear_act");
 }
 

@@ -1,5 +1,5 @@
 // kernels_act.hip - linear with activation and residual in its epilogue, from rows of the storage type or 8-bit rows.
-#include <cstdlib>
+#include <cmath>
 #include <type_traits>
 
 #include "mfma_common.h"
@@ -171,6 +171,7 @@ __global__ void __launch_bounds__(64 * RW * CW, RW * CW * PER_CU / 4) k_linear_a
     using T = typename Store<DT>::T;
     constexpr int NW = RW * CW, BM = RW * RB * 32, BN = CW * NT * 32;
     constexpr bool kScaled = MT == kRows8;
+    constexpr bool kMaySplit = BM * BN < 256 * 256;  // the largest blocks have no registers for it
     constexpr int kRows = BM + BN, kBytes = kRows * 128, kSlot = kBytes + (kScaled ? kRows * 4 : 0);
     // Loads of 1 KB (8 rows) per step and wavefront, of x and of W.
     constexpr int NA = BM / 8 / NW, NB = BN / 8 / NW, kPer = NA + NB;
@@ -183,13 +184,14 @@ __global__ void __launch_bounds__(64 * RW * CW, RW * CW * PER_CU / 4) k_linear_a
     const int rw = wave % RW, cw = wave / RW;
     const int l32 = lane & 31, half = lane >> 5;
 
-    // Blocks b, b + 8, ... run on one XCD, which multiplies a row block by
-    // every channel block in turn: the rows stay in its L2.
-    const int64_t in_xcd = blockIdx.x / 8;
-    const int64_t tile = in_xcd / p.col_tiles * 8 + blockIdx.x % 8;
-    if (tile >= p.row_tiles) return;
+    // An XCD (blocks b, b + 8, ...) takes a contiguous range of the tiles, row
+    // block by row block with every channel block in turn: the rows stay in its
+    // L2, and few tiles spread over all XCDs.
+    const int split = kMaySplit ? (int) (blockIdx.x / p.split_blocks) : 0;
+    const int64_t unit = xcd_remap(blockIdx.x - (int64_t) split * p.split_blocks, p.split_blocks);
+    const int64_t tile = unit / p.col_tiles;
     const int64_t row0 = tile * BM;
-    const int col0 = (int) (in_xcd % p.col_tiles) * BN;
+    const int col0 = (int) (unit % p.col_tiles) * BN;
     const int rows = (int) min((int64_t) BM, p.n - row0);
 
     const __amdgpu_buffer_rsrc_t xres = __builtin_amdgcn_make_buffer_rsrc(
@@ -232,12 +234,15 @@ __global__ void __launch_bounds__(64 * RW * CW, RW * CW * PER_CU / 4) k_linear_a
         sres = __builtin_amdgcn_make_buffer_rsrc((void *) base, 0, (of_x ? rows : BN) * pitch, 0x00020000);
     }
 
-    const int steps = p.w_bytes / 128;
+    // This split's steps.
+    const int all = p.w_bytes / 128;
+    const int first_step = kMaySplit ? (int) ((int64_t) all * split / p.splits) : 0;
+    const int steps = kMaySplit ? (int) ((int64_t) all * (split + 1) / p.splits) : all;
     // Past the last step loads fetch zeros; what follows a row of x is the next one.
     const auto load = [&](int s, uint32_t slot, int j) {
         if (j < NA) {
-            dma_b128(xres, slot + (wave * NA + j) * 1024u, s * 128 + x_chunk[j] * 16 < p.row_bytes ? x_at[j] : kOutside,
-                     s * 128u);
+            dma_b128(xres, slot + (wave * NA + j) * 1024u,
+                     (!kMaySplit || s < steps) && s * 128 + x_chunk[j] * 16 < p.row_bytes ? x_at[j] : kOutside, s * 128u);
         } else {
             dma_b128(wres, slot + BM * 128 + (wave * NB + j - NA) * 1024u, s < steps ? w_at[j - NA] : kOutside, s * 128u);
         }
@@ -247,16 +252,16 @@ __global__ void __launch_bounds__(64 * RW * CW, RW * CW * PER_CU / 4) k_linear_a
     };
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
-        load_scales(s, slots + s * kSlot);
+        load_scales(first_step + s, slots + s * kSlot);
 #pragma unroll
-        for (int j = 0; j < kPer; ++j) load(s, slots + s * kSlot, j);
+        for (int j = 0; j < kPer; ++j) load(first_step + s, slots + s * kSlot, j);
     }
 
     const int ch = col0 + (cw * 32 + l32) * NT;  // the lane's first channel
     f32x16 acc[RB][NT];
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
-        const float bias = p.bias != nullptr && ch + t < p.co ? p.bias[ch + t] : 0.0f;
+        const float bias = p.bias != nullptr && (!kMaySplit || p.splits == 1) && ch + t < p.co ? p.bias[ch + t] : 0.0f;
 #pragma unroll
         for (int q = 0; q < RB; ++q)
 #pragma unroll
@@ -322,7 +327,7 @@ __global__ void __launch_bounds__(64 * RW * CW, RW * CW * PER_CU / 4) k_linear_a
     for (int t = 0; t < NT; ++t) read_b(0, 0, t);
     uint32_t here = 0, there = kSlot;
     using std::integral_constant;
-    for (int s = 0; s < steps; ++s) {
+    for (int s = first_step; s < steps; ++s) {
         products(integral_constant<int, 0>(), here, 0, 0);
         // Step s + 1 has landed, and every wavefront has read all of step s.
         wait_vmcnt<0>();
@@ -370,6 +375,22 @@ __global__ void __launch_bounds__(64 * RW * CW, RW * CW * PER_CU / 4) k_linear_a
                 __builtin_amdgcn_sched_barrier(0);
             }
     };
+    if constexpr (kMaySplit) if (p.splits > 1) {
+        // The sums of this split, as they are.
+        const __amdgpu_buffer_rsrc_t pres = __builtin_amdgcn_make_buffer_rsrc(
+            p.partial + ((int64_t) split * p.n + row0) * p.co, 0, rows * p.co * 4, 0x00020000);
+        const uint32_t to = ch < p.co ? (uint32_t) (((rw * RB * 32 + 4 * half) * p.co + ch) * 4) : kOutside;
+#pragma unroll
+        for (int q = 0; q < RB; ++q)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                float v[NT];
+#pragma unroll
+                for (int t = 0; t < NT; ++t) v[t] = acc[q][t][i];
+                store_adjacent<kF32, NT>(pres, to, (uint32_t) ((q * 32 + i / 4 * 8 + i % 4) * p.co * 4), v);
+            }
+        return;
+    }
     by_act(p.act, [&](auto act_c) {
         if (p.residual != nullptr) {
             finish(act_c, std::true_type());
@@ -377,6 +398,52 @@ __global__ void __launch_bounds__(64 * RW * CW, RW * CW * PER_CU / 4) k_linear_a
             finish(act_c, std::false_type());
         }
     });
+}
+
+// Joins the splits' sums in their order, then bias, activation and residual: N
+// adjacent outputs a thread (N divides co).
+template <int DT, int N> __global__ void __launch_bounds__(256) k_linear_join(LinearAct p) {
+    using T = typename Store<DT>::T;
+    const int64_t e = ((int64_t) blockIdx.x * 256 + threadIdx.x) * N, count = p.n * p.co;
+    if (e >= count) return;
+    const int ch = (int) (e % p.co);
+    float v[N];
+#pragma unroll
+    for (int u = 0; u < N; ++u) v[u] = p.bias != nullptr ? p.bias[ch + u] : 0.0f;
+#pragma unroll 4
+    for (int s = 0; s < p.splits; ++s) {
+        const float * q = p.partial + s * count + e;
+        if constexpr (N == 4) {
+            const float4 c = *(const float4 *) q;
+            v[0] += c.x;
+            v[1] += c.y;
+            v[2] += c.z;
+            v[3] += c.w;
+        } else {
+#pragma unroll
+            for (int u = 0; u < N; ++u) v[u] += q[u];
+        }
+    }
+    const T * residual = (const T *) p.residual;
+    by_act(p.act, [&](auto act_c) {
+#pragma unroll
+        for (int u = 0; u < N; ++u) {
+            v[u] = activate<DT, decltype(act_c)::value>(v[u]);
+            if (residual != nullptr) v[u] += Store<DT>::ld(residual, e + u);
+        }
+    });
+    if constexpr (N == 4 && DT != kF32) {
+        union {
+            T h[4];
+            uint2 c;
+        } w;
+#pragma unroll
+        for (int u = 0; u < 4; ++u) w.h[u] = round_to_store<DT>(v[u]);
+        *(uint2 *) ((T *) p.y + e) = w.c;
+    } else {
+#pragma unroll
+        for (int u = 0; u < N; ++u) Store<DT>::st((T *) p.y, e + u, v[u]);
+    }
 }
 
 // Rows that are no whole number of 16-byte chunks: 64 x 64 outputs a block
@@ -433,34 +500,98 @@ template <int DT> __global__ void __launch_bounds__(256) k_linear_act_any(Linear
     });
 }
 
-template <int MT, int DT, int RW, int CW, int RB, int NT, int PER_CU>
-hipError_t launch_gemm_t(LinearAct p, hipStream_t s) {
-    constexpr int BM = RW * RB * 32, BN = CW * NT * 32;
-    p.row_tiles = (p.n + BM - 1) / BM;
-    p.col_tiles = (p.co + BN - 1) / BN;
-    const int64_t grid = (p.row_tiles + 7) / 8 * 8 * p.col_tiles;
-    if (grid > 0x7fffffffLL) return hipErrorInvalidValue;
-    k_linear_act<MT, DT, RW, CW, RB, NT, PER_CU><<<(unsigned) grid, 64 * RW * CW, 0, s>>>(p);
-    return hipGetLastError();
+// ---- which blocks, and how many splits --------------------------------------------------------------
+
+// Block shapes: rows, channels, adjacent channels per lane (which divide co),
+// blocks per CU, and what a step of 128 bytes and the rest of a block take with
+// all CUs busy, in us (measured on whole rounds of blocks, 1,024 channels, K of 4
+// and of 32 steps).
+struct Blocks {
+    int rows, channels, adjacent, per_cu;
+    float step16, step8, step32, rest, rest32;
+};
+constexpr Blocks kBlocks[] = {
+    {256, 256, 4, 1, 1.77f, 2.05f, 7.1f, 5.4f, 16.0f},
+    {192, 256, 2, 1, 1.50f, 1.80f, 5.4f, 3.7f, 12.5f},
+    {128, 128, 2, 2, 1.25f, 1.55f, 3.8f, 2.1f, 7.8f},
+    {64, 128, 2, 3, 1.15f, 1.53f, 3.0f, 2.0f, 5.4f},
+    {128, 128, 1, 2, 1.26f, 1.67f, 3.8f, 2.6f, 7.3f},
+    {64, 64, 1, 4, 0.80f, 1.26f, 2.2f, 2.5f, 4.4f},
+};
+constexpr int kShapes = sizeof(kBlocks) / sizeof(kBlocks[0]);
+
+inline float step_us(const Blocks & b, int mt) { return mt == kF32 ? b.step32 : (mt == kRows8 ? b.step8 : b.step16); }
+
+struct Choice {
+    int shape = -1, splits = 1;
+    float us = 0.0f;
+};
+
+// The shape and splits with the least estimated time for n rows.  Splits pay for
+// their sums' way to memory and back and for the join's launch.
+Choice choose(int mt, int64_t n, int co, int w_bytes, int cus, bool may_split) {
+    const int steps = w_bytes / 128;
+    Choice best;
+    for (int i = 0; i < kShapes; ++i) {
+        const Blocks & b = kBlocks[i];
+        if (co % b.adjacent != 0) continue;
+        const double blocks = (double) ((n + b.rows - 1) / b.rows) * ((co + b.channels - 1) / b.channels);
+        const double step = step_us(b, mt), rest = mt == kF32 ? b.rest32 : b.rest;
+        for (int s = 1; s <= (may_split ? 16 : 1); s *= 2) {
+            if (s > 1 && (s > steps / 2 || i == 0)) break;  // (the largest blocks do not split)
+            const double rounds = blocks * s / ((double) cus * b.per_cu), whole = std::floor(rounds);
+            // A last round of few blocks leaves each more of its CU where several share one.
+            const double last = rounds - whole;
+            const double tail = last == 0.0 ? 0.0 : (b.per_cu == 1 || whole > 0 ? 1.0 : 0.6 + 0.4 * last);
+            double us = (whole + tail) * ((steps + s - 1) / s * step + rest);
+            if (s > 1) us += 4.0 + (double) s * n * co * 8.0 / 4.5e6;
+            if (best.shape < 0 || us < best.us) {
+                best.shape = i;
+                best.splits = s;
+                best.us = (float) us;
+            }
+        }
+    }
+    return best;
 }
 
-template <int MT, int DT> hipError_t launch_gemm(const LinearAct & p, int cus, hipStream_t s) {
-    const auto blocks = [&](int bm, int bn) { return (p.n + bm - 1) / bm * ((p.co + bn - 1) / bn); };
-    static const int force = getenv("TSH_FORCE") ? atoi(getenv("TSH_FORCE")) : -1;
-    switch (force) {
-        case 0: return launch_gemm_t<MT, DT, 4, 2, 2, 4, 1>(p, s);  // 256 x 256
-        case 1: return launch_gemm_t<MT, DT, 2, 4, 3, 2, 1>(p, s);  // 192 x 256
-        case 2: return launch_gemm_t<MT, DT, 2, 4, 2, 2, 1>(p, s);  // 128 x 256, 8 waves
-        case 3: return launch_gemm_t<MT, DT, 2, 2, 2, 2, 2>(p, s);  // 128 x 128, two per CU
-        case 4: return launch_gemm_t<MT, DT, 2, 2, 1, 2, 3>(p, s);  // 64 x 128
-        case 5: return launch_gemm_t<MT, DT, 2, 4, 2, 1, 2>(p, s);  // 128 x 128, 8 waves, two per CU
-        case 6: return launch_gemm_t<MT, DT, 4, 2, 1, 2, 2>(p, s);  // 128 x 128, 8 waves, two per CU
-        default: break;
+template <int MT, int DT, int RW, int CW, int RB, int NT, int PER_CU>
+hipError_t launch_shape(LinearAct p, const Blocks & b, hipStream_t s) {
+    constexpr int BM = RW * RB * 32, BN = CW * NT * 32;
+    if (b.rows != BM || b.channels != BN || b.adjacent != NT || b.per_cu != PER_CU) return hipErrorInvalidValue;
+    p.row_tiles = (p.n + BM - 1) / BM;
+    p.col_tiles = (p.co + BN - 1) / BN;
+    const int64_t grid = p.row_tiles * p.col_tiles;
+    if (grid * p.splits > 0x7fffffffLL) return hipErrorInvalidValue;
+    p.split_blocks = (int) grid;
+    k_linear_act<MT, DT, RW, CW, RB, NT, PER_CU><<<(unsigned) (grid * p.splits), 64 * RW * CW, 0, s>>>(p);
+    hipError_t err = hipGetLastError();
+    if (err == hipSuccess && p.splits > 1) {
+        const bool four = p.co % 4 == 0;
+        const int64_t joins = (p.n * p.co + (four ? 1023 : 255)) / (four ? 1024 : 256);
+        if (joins > 0x7fffffffLL) return hipErrorInvalidValue;
+        if (four) {
+            k_linear_join<DT, 4><<<(unsigned) joins, 256, 0, s>>>(p);
+        } else {
+            k_linear_join<DT, 1><<<(unsigned) joins, 256, 0, s>>>(p);
+        }
+        err = hipGetLastError();
     }
-    if (p.co % 2 != 0) return launch_gemm_t<MT, DT, 2, 4, 2, 1, 2>(p, s);
-    if (p.co % 4 == 0 && blocks(256, 256) >= 2 * (int64_t) cus) return launch_gemm_t<MT, DT, 4, 2, 2, 4, 1>(p, s);
-    if (blocks(128, 128) >= cus) return launch_gemm_t<MT, DT, 2, 2, 2, 2, 2>(p, s);
-    return launch_gemm_t<MT, DT, 2, 2, 1, 2, 3>(p, s);
+    return err;
+}
+
+template <int MT, int DT> hipError_t launch_gemm(LinearAct p, int shape, int splits, hipStream_t s) {
+    p.splits = splits;
+    const Blocks & b = kBlocks[shape];
+    switch (shape) {
+        case 0: return launch_shape<MT, DT, 4, 2, 2, 4, 1>(p, b, s);
+        case 1: return launch_shape<MT, DT, 2, 4, 3, 2, 1>(p, b, s);
+        case 2: return launch_shape<MT, DT, 2, 2, 2, 2, 2>(p, b, s);
+        case 3: return launch_shape<MT, DT, 2, 2, 1, 2, 3>(p, b, s);
+        case 4: return launch_shape<MT, DT, 2, 4, 2, 1, 2>(p, b, s);
+        case 5: return launch_shape<MT, DT, 2, 2, 1, 1, 4>(p, b, s);
+        default: return hipErrorInvalidValue;
+    }
 }
 
 template <int DT> hipError_t launch_any(LinearAct p, hipStream_t s) {
@@ -471,19 +602,70 @@ template <int DT> hipError_t launch_any(LinearAct p, hipStream_t s) {
     return hipGetLastError();
 }
 
-template <int DT> hipError_t launch_dt(const LinearAct & p, int x_type, int cus, hipStream_t s) {
-    if (x_type == kRows8) return launch_gemm<kRows8, DT>(p, cus, s);
-    if (p.row_bytes % 16 == 0) return launch_gemm<DT, DT>(p, cus, s);
-    return launch_any<DT>(p, s);
+template <int DT> hipError_t launch_dt(const LinearAct & p, int x_type, const LinearActPlan & plan, hipStream_t s) {
+    if (plan.parts == 0) return launch_any<DT>(p, s);
+    int64_t row = 0;
+    for (int i = 0; i < plan.parts; ++i) {
+        const auto & part = plan.part[i];
+        LinearAct q = p;
+        const int64_t e = (int64_t) sizeof(typename Store<DT>::T);
+        q.x = (const char *) p.x + row * p.row_bytes;
+        if (p.x_scales != nullptr) q.x_scales = p.x_scales + row * (p.row_bytes / 32);
+        if (p.residual != nullptr) q.residual = (const char *) p.residual + row * p.co * e;
+        q.y = (char *) p.y + row * p.co * e;
+        q.n = part.rows;
+        const int splits = p.partial != nullptr ? part.splits : 1;
+        const hipError_t err = x_type == kRows8 ? launch_gemm<kRows8, DT>(q, part.shape, splits, s)
+                                                : launch_gemm<DT, DT>(q, part.shape, splits, s);
+        if (err != hipSuccess) return err;
+        row += part.rows;
+    }
+    return hipSuccess;
 }
 
 }  // namespace
 
-hipError_t launch_linear_act(int dtype, int x_type, const LinearAct & p, int cus, hipStream_t s) {
+// All rows in one launch, or whole rounds of large blocks in one and the rows that
+// are left in another, with blocks and splits of their own (18,216 x 4096 ->
+// 1024 bf16: 288 blocks of 256 x 256 are one round of 256 and one of 32).
+LinearActPlan linear_act_plan(int dtype, int x_type, int64_t n, int co, int row_bytes, int w_bytes, int cus,
+                              bool may_split) {
+    LinearActPlan plan{};
+    if (x_type != kRows8 && row_bytes % 16 != 0) return plan;
+    const int mt = x_type == kRows8 ? kRows8 : dtype;
+    const auto scratch = [&](const LinearActPart & part) {
+        return part.splits > 1 ? (size_t) part.splits * part.rows * co * sizeof(float) : 0;
+    };
+    const Choice one = choose(mt, n, co, w_bytes, cus, may_split);
+    plan.parts = 1;
+    plan.part[0] = {n, one.shape, one.splits};
+    plan.scratch = scratch(plan.part[0]);
+    float least = one.us;
+    for (int i = 0; i < 2; ++i) {
+        const Blocks & b = kBlocks[i];
+        if (co % b.adjacent != 0) continue;
+        const int64_t col_tiles = (co + b.channels - 1) / b.channels, row_tiles = n / b.rows;
+        const int64_t rounds = row_tiles * col_tiles / cus;
+        const int64_t rows = rounds * cus / col_tiles * b.rows;
+        if (rounds < 1 || rows <= 0 || rows >= n) continue;
+        const Choice rest = choose(mt, n - rows, co, w_bytes, cus, may_split);
+        const double block = w_bytes / 128 * step_us(b, mt) + (mt == kF32 ? b.rest32 : b.rest);
+        const float us = (float) (rounds * block) + rest.us + 3.0f;
+        if (us >= least) continue;
+        least = us;
+        plan.parts = 2;
+        plan.part[0] = {rows, i, 1};
+        plan.part[1] = {n - rows, rest.shape, rest.splits};
+        plan.scratch = scratch(plan.part[1]);
+    }
+    return plan;
+}
+
+hipError_t launch_linear_act(int dtype, int x_type, const LinearAct & p, const LinearActPlan & plan, hipStream_t s) {
     switch (dtype) {
-        case kF32: return launch_dt<kF32>(p, x_type, cus, s);
-        case kF16: return launch_dt<kF16>(p, x_type, cus, s);
-        default: return launch_dt<kBF16>(p, x_type, cus, s);
+        case kF32: return launch_dt<kF32>(p, x_type, plan, s);
+        case kF16: return launch_dt<kF16>(p, x_type, plan, s);
+        default: return launch_dt<kBF16>(p, x_type, plan, s);
     }
 }
 

@@ -387,13 +387,29 @@ struct LinearAct {
     int64_t n;
     int ci, co, act;
     int row_bytes, w_bytes;  // of a row of x and of w
-    int64_t row_tiles;       // set by the launcher
-    int col_tiles;
+    float * partial;         // [splits][rows][co] sums of a part's splits, or null
+    int splits;              // set by the launcher, as are:
+    int64_t row_tiles;
+    int col_tiles, split_blocks;
 };
+// How a linear is run: parts of its rows one after the other, each with a block
+// shape and its K in splits (for which the scratch memory is; without it they are
+// not split).  No parts: the general kernel.
+struct LinearActPart {
+    int64_t rows;
+    int shape, splits;
+};
+struct LinearActPlan {
+    int parts;
+    LinearActPart part[2];
+    size_t scratch;
+};
+LinearActPlan linear_act_plan(int dtype, int x_type, int64_t n, int co, int row_bytes, int w_bytes, int cus,
+                              bool may_split);
 inline int linear_act_rows(int co) { return (co + 255) / 256 * 256; }
 // Widest row: a block's 256 rows stay below 2 GiB.
 constexpr int kLinearActMaxBytes = 1 << 22;
-hipError_t launch_linear_act(int dtype, int x_type, const LinearAct & p, int cus, hipStream_t s);
+hipError_t launch_linear_act(int dtype, int x_type, const LinearAct & p, const LinearActPlan & plan, hipStream_t s);
 // Attention within sequences of rows (kernels_attn.hip).
 struct Attention {
     const void * q;
