@@ -273,20 +273,37 @@ __global__ void __launch_bounds__(64 * NW, DC <= 64 ? 3 : 2) k_attention(Attenti
         v_off[j] = in ? (uint32_t) (r * vs + c * 16) : kOutside;
     }
     const uint32_t lds0 = (uint32_t) (uintptr_t) (__attribute__((address_space(3))) unsigned char *) s_tile;
-    const auto load = [&](const char * base, int pitch, const uint32_t (&off)[PER], int t, uint32_t to) {
-        const int left = at.nk - t * TK;
-        const int rows = left < TK ? left : TK;
-        const __amdgpu_buffer_rsrc_t res = __builtin_amdgcn_make_buffer_rsrc(
-            (void *) (base + (int64_t) t * TK * pitch), 0, (rows - 1) * pitch + p.dim * 2, 0x00020000);
-        // Rows past the end are zeros.
+    const auto load = [&](const char * base, int pitch, const uint32_t (&off)[PER], int rows, uint32_t to) {
+        if (rows >= TK) {
+            const __amdgpu_buffer_rsrc_t res =
+                __builtin_amdgcn_make_buffer_rsrc((void *) base, 0, (TK - 1) * pitch + p.dim * 2, 0x00020000);
 #pragma unroll
-        for (int j = 0; j < PER; ++j)
-            dma_b128(res, lds0 + to + (wave * PER + j) * 1024u,
-                     (wave * PER + j) * RPL + lane / CH < rows ? off[j] : kOutside, 0);
+            for (int j = 0; j < PER; ++j) dma_b128_m0(res, lds0 + to + (wave * PER + j) * 1024u, off[j], 0);
+        } else {
+            // Rows past the end are zeros.
+            const __amdgpu_buffer_rsrc_t res =
+                __builtin_amdgcn_make_buffer_rsrc((void *) base, 0, (rows - 1) * pitch + p.dim * 2, 0x00020000);
+#pragma unroll
+            for (int j = 0; j < PER; ++j)
+                dma_b128_m0(res, lds0 + to + (wave * PER + j) * 1024u,
+                            (wave * PER + j) * RPL + lane / CH < rows ? off[j] : kOutside, 0);
+        }
     };
-    // Keys of tile t in buffer (t - t0) % 2, its values in the same of two more.
-    const auto load_k = [&](int t) { load(kb, ks, k_off, t, (uint32_t) (((t - t0) & 1) * TILE)); };
-    const auto load_v = [&](int t) { load(vb, vs, v_off, t, (uint32_t) (((t - t0) & 1) * TILE + 2 * TILE)); };
+    // Tile t's keys go to buffer (t - t0) % 2, its values to the same of two more;
+    // the next tile to load of each, and where it is.
+    int tk = t0, tv = t0;
+    const char * k_at = kb + (int64_t) t0 * TK * ks;
+    const char * v_at = vb + (int64_t) t0 * TK * vs;
+    const auto load_k = [&]() {
+        load(k_at, ks, k_off, at.nk - tk * TK, (uint32_t) (((tk - t0) & 1) * TILE));
+        ++tk;
+        k_at += (int64_t) TK * ks;
+    };
+    const auto load_v = [&]() {
+        load(v_at, vs, v_off, at.nk - tv * TK, (uint32_t) (((tv - t0) & 1) * TILE + 2 * TILE));
+        ++tv;
+        v_at += (int64_t) TK * vs;
+    };
 
     // Reads: K row l32 (+ 32), chunk 2 k + half; V rows 4 half + (lane % 16) / 4
     // (+ 8, + 16 g), 16-value column block (lane / 16) % 2 of each 32.
@@ -355,8 +372,8 @@ __global__ void __launch_bounds__(64 * NW, DC <= 64 ? 3 : 2) k_attention(Attenti
         // the keys of t and the values of t - 1.
         wait_vmcnt<0>();
         lds_barrier();
-        if (t + 2 < t1) load_k(t + 2);
-        if (t + 1 < t1) load_v(t + 1);
+        if (t + 2 < t1) load_k();
+        if (t + 1 < t1) load_v();
         // (Past the last tile these are old keys, and the scores are not used.)
         const unsigned char * sk = s_tile + ((j & 1) ^ 1) * TILE;
         const unsigned char * sv = s_tile + (j & 1) * TILE + 2 * TILE;
@@ -427,9 +444,9 @@ __global__ void __launch_bounds__(64 * NW, DC <= 64 ? 3 : 2) k_attention(Attenti
     };
 
     if (t0 < t1) {
-        load_k(t0);
-        load_v(t0);
-        if (t0 + 1 < t1) load_k(t0 + 1);
+        load_k();
+        load_v();
+        if (t0 + 1 < t1) load_k();
         wait_vmcnt<0>();
         lds_barrier();
         f32x16 sa[2], sb[2];
@@ -484,31 +501,34 @@ __global__ void __launch_bounds__(64 * NW, DC <= 64 ? 3 : 2) k_attention(Attenti
         }
 }
 
-// Joins the splits, a query a wavefront: QP lanes (a power of two) have four
-// channels each, 64 / QP groups of them every so many splits.  Queries are found
-// as k_attention<.., NW> does, TQ / 4 blocks for each of its tiles.
-template <int DT, int TQ>
+// Joins the splits, a query to WAVES wavefronts (one with few splits, four with
+// many): QP lanes (a power of two) have four channels each, and the 64 WAVES / QP
+// groups of them every so many splits.  Queries are found as k_attention<.., NW>
+// does, TQ blocks' worth for each of its tiles.
+template <int DT, int TQ, int WAVES>
 __global__ void __launch_bounds__(256) k_join(Attention p, Partial part, int tiles, int qp) {
     using T = typename Store<DT>::T;
-    constexpr int PER = TQ / 4;
+    constexpr int QUERIES = 4 / WAVES, PER = TQ / QUERIES;
+    __shared__ float s_sum[4][64][5];
     const int group = p.heads / p.kv_heads, kv = blockIdx.x / PER / tiles;
     const Place at = find_place<TQ>(p, blockIdx.x / PER % tiles, group);
-    const int i = blockIdx.x % PER * 4 + (int) (threadIdx.x >> 6), lane = threadIdx.x & 63;
-    if (i >= at.nq) return;
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    const int i = blockIdx.x % PER * QUERIES + wave / WAVES;
+    // With one wavefront a query no barrier follows.
+    if (WAVES == 1 ? i >= at.nq : (int) (blockIdx.x % PER) * QUERIES >= at.nq) return;
     const int64_t vq = at.first + i;
     const int64_t row = at.q0 + vq / group;
     const int head = kv * group + (int) (vq % group);
     const int64_t q = row * p.heads + head, step = p.nq * p.heads;
     float most = -__builtin_inff();
     for (int s = lane; s < part.splits; s += 64) most = fmaxf(most, part.stat[s * step + q].x);
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) most = fmaxf(most, __shfl_xor(most, d));
+    most = group_reduce<64>(most, [](float a, float b) { return fmaxf(a, b); });
     const float base = most == -__builtin_inff() ? 0.0f : most;
     const int c = lane % qp * 4;
     float sum = 0.0f, v[4] = {0.f, 0.f, 0.f, 0.f};
     if (c < p.dim) {
 #pragma unroll 4
-        for (int s = lane / qp; s < part.splits; s += 64 / qp) {
+        for (int s = (wave % WAVES * 64 + lane) / qp; s < part.splits; s += WAVES * 64 / qp) {
             const float2 st = part.stat[s * step + q];
             // No keys: nothing was written.
             const bool some = st.x != -__builtin_inff() || st.y != 0.0f;
@@ -525,6 +545,18 @@ __global__ void __launch_bounds__(256) k_join(Attention p, Partial part, int til
         sum += __shfl_xor(sum, d);
 #pragma unroll
         for (int j = 0; j < 4; ++j) v[j] += __shfl_xor(v[j], d);
+    }
+    if constexpr (WAVES > 1) {
+        s_sum[wave][lane][4] = sum;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) s_sum[wave][lane][j] = v[j];
+        __syncthreads();
+        if (wave > 0) return;
+        for (int w = 1; w < WAVES; ++w) {
+            sum += s_sum[w][lane][4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) v[j] += s_sum[w][lane][j];
+        }
     }
     if (lane < qp && c < p.dim) {
         const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
@@ -543,9 +575,15 @@ hipError_t launch_nw(const Attention & p, const Partial & part, int64_t tiles, h
     if (err == hipSuccess && part.splits > 1) {
         int qp = 1;
         while (qp * 4 < p.dim) qp *= 2;
-        const int64_t joins = tiles * p.kv_heads * (8 * NW);
+        // 77 splits of 64 channels: 12 us with a wavefront a query, 6.5 with four.
+        const bool wide = part.splits >= 32;
+        const int64_t joins = tiles * p.kv_heads * (wide ? 32 * NW : 8 * NW);
         if (joins > 0x7fffffffLL) return hipErrorInvalidValue;
-        k_join<DT, 32 * NW><<<(unsigned) joins, 256, 0, s>>>(p, part, (int) tiles, qp);
+        if (wide) {
+            k_join<DT, 32 * NW, 4><<<(unsigned) joins, 256, 0, s>>>(p, part, (int) tiles, qp);
+        } else {
+            k_join<DT, 32 * NW, 1><<<(unsigned) joins, 256, 0, s>>>(p, part, (int) tiles, qp);
+        }
         err = hipGetLastError();
     }
     return err;

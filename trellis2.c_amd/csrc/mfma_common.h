@@ -54,6 +54,17 @@ __device__ __forceinline__ void dma_b128(__amdgpu_buffer_rsrc_t rsrc, uint32_t l
         : "memory");
 }
 
+// The same without keeping M0, which nothing else here uses.
+__device__ __forceinline__ void dma_b128_m0(__amdgpu_buffer_rsrc_t rsrc, uint32_t lds, uint32_t voff, uint32_t soff) {
+    asm volatile(
+        "s_mov_b32 m0, %0\n\t"
+        "s_nop 0\n\t"
+        "buffer_load_dwordx4 %1, %2, %3 offen lds"
+        :
+        : "s"(lds), "v"(voff), "s"(rsrc), "s"(soff)
+        : "memory", "m0");
+}
+
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
