@@ -641,6 +641,51 @@ trellis_status trellis_sparse_hip_attention(trellis_sparse_backend * backend, co
                                             const trellis_sparse_buffer * kv_offsets, int n_seqs,
                                             const trellis_sparse_hip_attention_desc * desc);
 
+/* A whole block over voxel rows, c = heads * head_dim channels:
+ *   a   = attention over rotary(qkv(norm1(h))), q and k turned (and normed per
+ *         head where qk_eps > 0)
+ *   mid = h + a out_w^T + out_b
+ *   out = mid + act(norm2(mid) mlp0_w^T + mlp0_b) mlp2_w^T + mlp2_b
+ * from the calls above, bit for bit, through intermediates of the backend's
+ * pool (n x c, n x 3c, n x hidden).  rows8: each of the four linears reads
+ * 8-bit rows.  Weights fp32 on the host: qkv_w [3c][c], out_w [c][c], mlp0_w
+ * [hidden][c], mlp2_w [c][hidden]; gammas [c], qk_gamma [2 heads][head_dim] (q's
+ * heads, then k's); biases, gammas and qk_gamma may be NULL. */
+typedef struct trellis_sparse_hip_block_desc {
+    uint32_t struct_size;  /* sizeof(trellis_sparse_hip_block_desc) */
+    int32_t heads;
+    int32_t head_dim;      /* a multiple of 8, up to 192 */
+    int32_t hidden;
+    int32_t act;           /* trellis_sparse_hip_act */
+    int32_t rows8;         /* 0 or 1 */
+    int32_t pairs[3];      /* as in trellis_sparse_hip_rotary_desc */
+    int32_t split;
+    float eps;             /* of norm1 and norm2, > 0 */
+    float qk_eps;          /* 0: q and k are not normed */
+    double base;
+    const float * norm1_gamma;
+    const float * qkv_w;
+    const float * qkv_b;
+    const float * qk_gamma;
+    const float * out_w;
+    const float * out_b;
+    const float * norm2_gamma;
+    const float * mlp0_w;
+    const float * mlp0_b;
+    const float * mlp2_w;
+    const float * mlp2_b;
+} trellis_sparse_hip_block_desc;
+/* h, out [n][c] (out may be h); coords or coords_map as in rotary; offsets: an
+ * int32 buffer [n_seqs + 1] of the rows' sequences, or NULL for one (n_seqs 1);
+ * rows in no sequence have a = 0.  The calls' own refusals come through; out is
+ * then unspecified. */
+trellis_status trellis_sparse_hip_transformer_block(trellis_sparse_backend * backend, const trellis_sparse_buffer * h,
+                                                    const trellis_sparse_buffer * coords,
+                                                    const trellis_sparse_c2s_device_map * coords_map,
+                                                    const trellis_sparse_buffer * offsets, int n_seqs,
+                                                    const trellis_sparse_hip_block_desc * desc,
+                                                    trellis_sparse_buffer * out, int64_t n);
+
 /* ------------------------------------------------------------------------ */
 /* Stage timing with HIP events recorded on the backend's own stream.        */
 /* ------------------------------------------------------------------------ */

@@ -72,6 +72,105 @@ def test_block_stage_by_stage(dtype):
         be.destroy()
 
 
+def block_args(blk):
+    w = dict(norm1_gamma=blk.g1, qkv_w=blk.wqkv, qkv_b=blk.bqkv, qk_gamma=blk.gqk, out_w=blk.wo, out_b=blk.bo,
+             norm2_gamma=blk.g2, mlp0_w=blk.w1, mlp0_b=blk.b1, mlp2_w=blk.w2, mlp2_b=blk.b2)
+    return dict(heads=blk.heads, head_dim=blk.dim, hidden=blk.hidden, weights=w, pairs=(5, 5, 5), qk_eps=1e-6)
+
+
+@pytest.mark.parametrize("dtype", [sh.F32, sh.F16, sh.BF16])
+@pytest.mark.parametrize("rows8", [False, True])
+def test_block_in_one_call(dtype, rows8):
+    """transformer_block gives the very bits of the calls that it stands for, also over its own input, with one sequence
+    and with two, rows that are in none (no attention there), from an int32 buffer of coordinates and from a device map."""
+    be, rng, n = sh.Backend(0, dtype), np.random.default_rng(5), 270
+    try:
+        blk = rows_block.Block(dtype)
+        c, w, hid = blk.c, 3 * blk.c, blk.hidden
+        coords, at = rows_block.voxels(n, rng)
+        x = sh.storage_round(rng.standard_normal((n, c)).astype(np.float32), dtype)
+        xb, cb, dm, ab = be.upload(x), be.upload_i32(coords), be.upload_coords(coords), be.upload_i32(at)
+        short = be.upload_i32(np.array([0, 100, 230], np.int32))
+        for offsets in (None, ab, short):
+            rows = be.upload(np.zeros((n, c), np.float32))
+            qkv, mid, hidden, out = (be.alloc(n * m) for m in (w, c, hid, c))
+            dirt = be.upload(np.full((n, c), np.nan, np.float32))
+            dirt.free()  # what an intermediate's block held before shows nowhere
+            rows8b, hid8 = be.alloc_rows8(n, c), be.alloc_rows8(n, hid)
+            normed = rows8b if rows8 else be.alloc(n * c)
+            be.rms_norm(xb, blk.g1, normed, n, c, 1e-6)
+            be.linear_act(normed, blk.wqkv, blk.bqkv, qkv, n, c, w)
+            be.rotary(qkv, cb, qkv, n, 2 * blk.heads, blk.dim, (5, 5, 5), gamma=blk.gqk, eps=1e-6, x_stride=w, y_stride=w)
+            be.attention(qkv, qkv, qkv, rows, n, n, blk.heads, blk.heads, blk.dim, q_offsets=offsets, kv_offsets=offsets,
+                         q_stride=w, k_offset=c, k_stride=w, v_offset=2 * c, v_stride=w)
+            if rows8:
+                be.pack_rows8(rows, rows8b, n, c)
+            be.linear_act(rows8b if rows8 else rows, blk.wo, blk.bo, mid, n, c, c, residual=xb)
+            be.rms_norm(mid, blk.g2, normed, n, c, 1e-6)
+            be.linear_act(normed, blk.w1, blk.b1, hidden, n, c, hid, act="gelu_tanh")
+            if rows8:
+                be.pack_rows8(hidden, hid8, n, hid)
+            be.linear_act(hid8 if rows8 else hidden, blk.w2, blk.b2, out, n, hid, c, residual=mid)
+            exp = be.download(out)
+            assert np.isfinite(exp).all() and np.abs(exp - x.ravel()).max() > 0.1
+            got = be.alloc(n * c)
+            be.transformer_block(xb, cb, got, n, rows8=rows8, offsets=offsets, **block_args(blk))
+            assert np.array_equal(be.download(got), exp)
+            over = be.upload(x)
+            be.transformer_block(over, dm, over, n, rows8=rows8, offsets=offsets, **block_args(blk))
+            assert np.array_equal(be.download(over), exp)
+        be.free_map(dm)
+    finally:
+        be.destroy()
+
+
+def test_block_refusals():
+    be, n = sh.Backend(0, sh.BF16), 40
+    try:
+        blk = rows_block.Block(sh.BF16)
+        x, out, cb = be.alloc(n * blk.c), be.alloc(n * blk.c), be.upload_i32(np.zeros((n, 4), np.int32))
+        args = block_args(blk)
+
+        def refuse(status=sh.INVALID_ARGUMENT, **more):
+            a = {**args, **{k: v for k, v in more.items() if k in args}}
+            h, co, o, m = (more.get(k, v) for k, v in (("h", x), ("coords", cb), ("out", out), ("n", n)))
+            rest = {k: v for k, v in more.items() if k not in args and k not in ("h", "coords", "out", "n")}
+            with pytest.raises(sh.HipError) as e:
+                be.transformer_block(h, co, o, m, **a, **rest)
+            assert e.value.status == status, (more, e.value)
+
+        be.transformer_block(x, cb, out, n, **args)
+        refuse(n=0)
+        refuse(n=n + 1)
+        refuse(heads=0)
+        refuse(head_dim=0)
+        refuse(hidden=0)
+        refuse(eps=0.0)
+        refuse(pairs=(9, 9, 9))
+        refuse(weights={**args["weights"], "out_w": None})
+        refuse(coords=be.upload_i32(np.zeros((n - 1, 4), np.int32)))
+        refuse(offsets=x)
+        refuse(h=cb)
+        refuse(out=cb)
+        refuse(sh.NOT_IMPLEMENTED, heads=8, head_dim=12, pairs=(2, 2, 2), weights={**args["weights"], "qk_gamma": None})
+        with pytest.raises(TypeError):
+            be.transformer_block(x, cb, out, n, **{**args, "weights": {**args["weights"], "qkv": blk.wqkv}})
+        st = sh.LIB.trellis_sparse_hip_transformer_block(be.ptr, x.handle, cb.handle, None, None, 1,
+                                                         sh.ctypes.byref(sh.BlockDesc()), out.handle, n)
+        assert st == sh.INVALID_ARGUMENT
+        be.trim(sh.TRIM_FREE_BUFFERS)
+        for after in range(3):
+            be.fail_alloc(after)
+            try:
+                refuse(sh.OUT_OF_MEMORY)
+            finally:
+                be.fail_alloc(-1)
+            be.trim(sh.TRIM_FREE_BUFFERS)
+        be.transformer_block(x, cb, out, n, **args)
+    finally:
+        be.destroy()
+
+
 @pytest.fixture(scope="module")
 def torch_program():
     r = subprocess.run([sys.executable, "-u", os.path.join(HERE, "rows_with_torch.py")], capture_output=True, text=True,

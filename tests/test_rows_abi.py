@@ -23,12 +23,14 @@ def test_null_arguments():
     assert L.trellis_sparse_hip_rotary(None, None, None, None, None, 1, ctypes.byref(sh.RotaryDesc())) == bad
     assert L.trellis_sparse_hip_attention(None, None, None, None, None, 1, 1, None, None, 1,
                                           ctypes.byref(sh.AttentionDesc())) == bad
+    assert L.trellis_sparse_hip_transformer_block(None, None, None, None, None, 1, ctypes.byref(sh.BlockDesc()), None, 1) == bad
 
 
 def test_descriptors_match_the_header():
     text = open(os.path.join(ROOT, "include", "trellis_sparse_hip.h")).read()
     for cls, name, size in ((sh.RotaryDesc, "trellis_sparse_hip_rotary_desc", 80),
-                            (sh.AttentionDesc, "trellis_sparse_hip_attention_desc", 88)):
+                            (sh.AttentionDesc, "trellis_sparse_hip_attention_desc", 88),
+                            (sh.BlockDesc, "trellis_sparse_hip_block_desc", 144)):
         body = text[text.index(f"typedef struct {name} {{"):text.index(f"}} {name};")]
         body = re.sub(r"/\*.*?\*/", "", body.split("{", 1)[1], flags=re.S)
         fields = [re.sub(r"[\s*]|\[.*\]", "", f) for line in body.split(";") if line.strip()

@@ -2392,6 +2392,81 @@ trellis_status attention_impl(trellis_sparse_backend * backend, const trellis_sp
     return hip_status(be, err, "attention");
 }
 
+// A transformer block over voxel rows, from the calls above: each half is a norm,
+// its linears and the residual, added in the last linear's epilogue.
+trellis_status transformer_block_impl(trellis_sparse_backend * backend, const trellis_sparse_buffer * h,
+                                      const trellis_sparse_buffer * coords,
+                                      const trellis_sparse_c2s_device_map * coords_map,
+                                      const trellis_sparse_buffer * offsets, int n_seqs,
+                                      const trellis_sparse_hip_block_desc * desc, trellis_sparse_buffer * out,
+                                      int64_t n) {
+    if (backend == nullptr) return TRELLIS_STATUS_INVALID_ARGUMENT;
+    Backend * be = as_backend(backend);
+    if (desc == nullptr || desc->struct_size != sizeof(*desc)) {
+        return fail(be, TRELLIS_STATUS_INVALID_ARGUMENT, "transformer_block: bad desc");
+    }
+    const trellis_sparse_hip_block_desc & d = *desc;
+    const int64_t wide = (int64_t) d.heads * d.head_dim;
+    if (n <= 0 || n > INT32_MAX || d.heads <= 0 || d.heads > 32768 || d.head_dim <= 0 || d.hidden <= 0 ||
+        wide > (1 << 18) || d.hidden > (1 << 20) || d.qkv_w == nullptr || d.out_w == nullptr || d.mlp0_w == nullptr ||
+        d.mlp2_w == nullptr || (d.rows8 != 0 && d.rows8 != 1) || !float_buffer_ok(be, h, (size_t) (n * wide)) ||
+        !float_buffer_ok(be, out, (size_t) (n * wide)) || spans_clash(packed(out, n, wide), packed(h, n, wide), true)) {
+        return fail(be, TRELLIS_STATUS_INVALID_ARGUMENT, "transformer_block: bad argument");
+    }
+    const int c = (int) wide;
+    trellis_sparse_buffer *row = nullptr, *qkv = nullptr, *hid = nullptr, *row8 = nullptr, *hid8 = nullptr;
+    trellis_status st = op_alloc_f32(backend, (size_t) n * c, &row);
+    if (st == TRELLIS_STATUS_OK) st = op_alloc_f32(backend, (size_t) n * 3 * c, &qkv);
+    if (st == TRELLIS_STATUS_OK) st = op_alloc_f32(backend, (size_t) n * d.hidden, &hid);
+    if (st == TRELLIS_STATUS_OK && d.rows8) st = alloc_rows8_impl(backend, n, c, &row8);
+    if (st == TRELLIS_STATUS_OK && d.rows8) st = alloc_rows8_impl(backend, n, d.hidden, &hid8);
+    trellis_sparse_buffer * normed = d.rows8 ? row8 : row;
+
+    trellis_sparse_hip_rotary_desc rot{};
+    rot.struct_size = sizeof(rot);
+    rot.heads = 2 * d.heads;
+    rot.head_dim = d.head_dim;
+    for (int a = 0; a < 3; ++a) rot.pairs[a] = d.pairs[a];
+    rot.split = d.split;
+    rot.eps = d.qk_eps;
+    rot.base = d.base;
+    rot.gamma = d.qk_gamma;
+    rot.x_stride = rot.y_stride = 3 * wide;
+    trellis_sparse_hip_attention_desc att{};
+    att.struct_size = sizeof(att);
+    att.heads = att.kv_heads = d.heads;
+    att.head_dim = d.head_dim;
+    att.q_stride = att.k_stride = att.v_stride = 3 * wide;
+    att.k_offset = wide;
+    att.v_offset = 2 * wide;
+
+    const auto run = [&](auto && call) {
+        if (st == TRELLIS_STATUS_OK) st = call();
+    };
+    run([&] { return rms_norm_impl(backend, h, nullptr, d.norm1_gamma, nullptr, normed, n, c, d.eps); });
+    run([&] { return linear_act_impl(backend, normed, d.qkv_w, d.qkv_b, 0, nullptr, qkv, n, c, 3 * c); });
+    run([&] { return rotary_impl(backend, qkv, coords, coords_map, qkv, n, &rot); });
+    // Attention leaves rows in no sequence as they are: zeros.
+    if (offsets != nullptr) {
+        run([&] {
+            DeviceScope scope(be);
+            return hip_status(be, launch_fill_i32((int32_t *) row->ptr, (int64_t) (row->cap / 4), 0, be->stream), "fill");
+        });
+    }
+    run([&] { return attention_impl(backend, qkv, qkv, qkv, row, n, n, offsets, offsets, n_seqs, &att); });
+    if (d.rows8) run([&] { return pack_rows8_impl(backend, row, row8, n, c); });
+    run([&] { return linear_act_impl(backend, normed, d.out_w, d.out_b, 0, h, out, n, c, c); });
+    run([&] { return rms_norm_impl(backend, out, nullptr, d.norm2_gamma, nullptr, normed, n, c, d.eps); });
+    run([&] { return linear_act_impl(backend, normed, d.mlp0_w, d.mlp0_b, d.act, nullptr, hid, n, c, d.hidden); });
+    if (d.rows8) run([&] { return pack_rows8_impl(backend, hid, hid8, n, d.hidden); });
+    run([&] {
+        return linear_act_impl(backend, d.rows8 ? hid8 : hid, d.mlp2_w, d.mlp2_b, 0, out, out, n, d.hidden, c);
+    });
+    for (trellis_sparse_buffer * b : {hid8, row8, hid, qkv, row})
+        if (b != nullptr) op_free_buffer(backend, b);
+    return st;
+}
+
 // ---- the caller's memory and stream ---------------------------------------------------
 
 trellis_status wrap_impl(trellis_sparse_backend * backend, void * ptr, size_t count, int dtype,
@@ -3023,6 +3098,17 @@ trellis_status trellis_sparse_hip_attention(trellis_sparse_backend * backend, co
                                             const trellis_sparse_hip_attention_desc * desc) {
     return tsh::no_throw(backend, [&] {
         return tsh::attention_impl(backend, q, k, v, y, nq, nkv, q_offsets, kv_offsets, n_seqs, desc);
+    });
+}
+
+trellis_status trellis_sparse_hip_transformer_block(trellis_sparse_backend * backend, const trellis_sparse_buffer * h,
+                                                    const trellis_sparse_buffer * coords,
+                                                    const trellis_sparse_c2s_device_map * coords_map,
+                                                    const trellis_sparse_buffer * offsets, int n_seqs,
+                                                    const trellis_sparse_hip_block_desc * desc,
+                                                    trellis_sparse_buffer * out, int64_t n) {
+    return tsh::no_throw(backend, [&] {
+        return tsh::transformer_block_impl(backend, h, coords, coords_map, offsets, n_seqs, desc, out, n);
     });
 }
 

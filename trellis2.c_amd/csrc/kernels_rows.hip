@@ -65,6 +65,35 @@ __device__ __forceinline__ uint32_t codes4(const float * v, float inv, uint32_t 
 
 __device__ __forceinline__ uint32_t abs_bits(float v) { return __builtin_bit_cast(uint32_t, v) & 0x7fffffffu; }
 
+// 1 / sqrt(sum / c + eps), for 8-bit outputs as two floats from 64 bits: there a
+// value on the other side of a code's border is off by a whole code, so the last
+// bit of the norm counts (a value then carries two roundings less than in fp32,
+// at three more operations).
+struct Inverse {
+    float hi, lo;
+};
+template <bool FINE> __device__ __forceinline__ Inverse inverse_rms(float sum, int c, float eps) {
+    if constexpr (FINE) {
+        // The hardware's estimate and one Newton step in 64 bits (1e-13).
+        const double m = (double) sum / (double) c + (double) eps;
+        const double y = (double) __builtin_amdgcn_rsqf((float) m);
+        double d = fma(0.5 * y, fma(-m * y, y, 1.0), y);
+        if (!(m > 1e-30 && m < 1e38)) d = 1.0 / sqrt(m);
+        const float hi = (float) d;
+        return {hi, (float) (d - (double) hi)};
+    }
+    return {1.0f / sqrtf(sum / (float) c + eps), 0.0f};
+}
+// v * inv * g, rounded about once where FINE.
+template <bool FINE> __device__ __forceinline__ float scaled(float v, const Inverse & inv, float g) {
+    if constexpr (FINE) {
+        const float p = v * g;
+        const float low = fmaf(fmaf(v, g, -p), inv.hi, p * inv.lo);
+        return fmaf(p, inv.hi, low);
+    }
+    return v * inv.hi * g;
+}
+
 // Where the norm's rows go.
 struct NormOut {
     void * y;          // storage type [n][c], or null
@@ -132,14 +161,17 @@ __global__ void __launch_bounds__(256) k_norm_vec(const typename Store<DT>::T * 
         }
         if constexpr (NORM) {
 #pragma unroll
+            for (int i = 0; i < CPL; ++i) {
+                float part = 0.0f;
+#pragma unroll
+                for (int u = 0; u < V; ++u) part += v[i][u] * v[i][u];
+                sum += part;
+            }
+            const Inverse inv = inverse_rms<Q8>(group_sum<LPR>(sum), c, eps);
+#pragma unroll
             for (int i = 0; i < CPL; ++i)
 #pragma unroll
-                for (int u = 0; u < V; ++u) sum += v[i][u] * v[i][u];
-            const float inv = 1.0f / sqrtf(group_sum<LPR>(sum) / (float) c + eps);
-#pragma unroll
-            for (int i = 0; i < CPL; ++i)
-#pragma unroll
-                for (int u = 0; u < V; ++u) v[i][u] = v[i][u] * inv * g[i][u];
+                for (int u = 0; u < V; ++u) v[i][u] = scaled<Q8>(v[i][u], inv, g[i][u]);
         }
 #pragma unroll
         for (int i = 0; i < CPL; ++i) {
@@ -185,14 +217,14 @@ __global__ void __launch_bounds__(256) k_norm_any(const typename Store<DT>::T * 
         const float v = Store<DT>::ld(x, row * c + i);
         return residual != nullptr ? v + Store<DT>::ld(residual, row * c + i) : v;
     };
-    float inv = 1.0f;
+    Inverse inv{1.0f, 0.0f};
     if constexpr (NORM) {
         float sum = 0.0f;
         for (int i = lane; i < c; i += 64) {
             const float v = at(i);
             sum += v * v;
         }
-        inv = 1.0f / sqrtf(wave_sum(sum) / (float) c + eps);
+        inv = inverse_rms<Q8>(wave_sum(sum), c, eps);
     }
     const int end = Q8 ? out.cp : c;
     for (int i = lane; i < end; i += 64) {
@@ -202,7 +234,7 @@ __global__ void __launch_bounds__(256) k_norm_any(const typename Store<DT>::T * 
             // An element of total may be the same memory as that of x or residual: read first.
             if (total != nullptr) Store<DT>::st(total, row * c + i, s);
             v = s;
-            if constexpr (NORM) v = v * inv * (gamma != nullptr ? gamma[i] : 1.0f);
+            if constexpr (NORM) v = scaled<Q8>(v, inv, gamma != nullptr ? gamma[i] : 1.0f);
         }
         if constexpr (Q8) {
             const uint32_t scale = block_scale(group_max<32>(abs_bits(v)));

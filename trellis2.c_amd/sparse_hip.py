@@ -109,6 +109,13 @@ class AttentionDesc(Structure):
                 ("y_stride", c_int64)]
 
 
+class BlockDesc(Structure):
+    _fields_ = ([("struct_size", c_uint32)] + [(k, c_int32) for k in ("heads", "head_dim", "hidden", "act", "rows8")] +
+                [("pairs", c_int32 * 3), ("split", c_int32), ("eps", c_float), ("qk_eps", c_float), ("base", c_double)] +
+                [(k, c_void_p) for k in ("norm1_gamma", "qkv_w", "qkv_b", "qk_gamma", "out_w", "out_b", "norm2_gamma",
+                                         "mlp0_w", "mlp0_b", "mlp2_w", "mlp2_b")])
+
+
 # The C ABI of include/trellis_sparse_hip.h: name -> (restype, argtypes).
 ABI = {
     "trellis_sparse_hip_policy_init": (None, [POINTER(Policy)]),
@@ -162,6 +169,7 @@ ABI = {
     "trellis_sparse_hip_rotary": (c_int, [_p, _p, _p, _p, _p, c_int64, POINTER(RotaryDesc)]),
     "trellis_sparse_hip_attention": (c_int, [_p, _p, _p, _p, _p, c_int64, c_int64, _p, _p, c_int,
                                              POINTER(AttentionDesc)]),
+    "trellis_sparse_hip_transformer_block": (c_int, [_p, _p, _p, _p, _p, c_int, POINTER(BlockDesc), _p, c_int64]),
 }
 
 
@@ -530,6 +538,22 @@ class Backend:
                                                      nkv, q_offsets and q_offsets.handle,
                                                      kv_offsets and kv_offsets.handle, seqs, ctypes.byref(d)),
                     "attention")
+
+    def transformer_block(self, h: Buffer, coords, out: Buffer, n: int, heads: int, head_dim: int, hidden: int, weights: dict,
+                          pairs, act: str = "gelu_tanh", rows8: bool = False, split: bool = False, eps: float = 1e-6,
+                          qk_eps: float = 0.0, base: float = 10000.0, offsets: Buffer | None = None):
+        """A whole block over voxel rows; weights: the arrays of BlockDesc by name (qkv_w, out_w, mlp0_w and mlp2_w, the
+        others if there)."""
+        names = [f[0] for f in BlockDesc._fields_ if f[1] is c_void_p]
+        if set(weights) - set(names):
+            raise TypeError(f"transformer_block: unknown weights {sorted(set(weights) - set(names))}")
+        w = {k: None if weights.get(k) is None else self.keep(_f32(weights[k])) for k in names}
+        d = BlockDesc(ctypes.sizeof(BlockDesc), heads, head_dim, hidden, ACTS[act], int(rows8), (c_int32 * 3)(*pairs),
+                      int(split), eps, qk_eps, base, *(_address(w[k]) for k in names))
+        at, dmap = (None, coords.handle) if isinstance(coords, DeviceMap) else (coords.handle, None)
+        self._check(LIB.trellis_sparse_hip_transformer_block(self.ptr, h.handle, at, dmap, offsets and offsets.handle,
+                                                             1 if offsets is None else offsets.count - 1,
+                                                             ctypes.byref(d), out.handle, n), "transformer_block")
 
     # -- rulebook / conv --------------------------------------------------------
     def build_rulebook(self, coords) -> Rulebook:
