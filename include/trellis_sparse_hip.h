@@ -531,10 +531,22 @@ trellis_status trellis_sparse_hip_wrap_i32(trellis_sparse_backend * backend, voi
  * outlives its use here: go back, or destroy the backend, before destroying it.
  * While the stream is captured into a graph, calls that need no memory can be
  * captured: buffers exist before, weights are on the device from an earlier
- * call, and all stay until the last replay; a call that would allocate returns
- * TRELLIS_STATUS_ERROR. */
+ * call, and all stay until the last replay; a call that would allocate
+ * (transformer_block does) returns TRELLIS_STATUS_ERROR, and so does set_stream
+ * while either stream is captured. */
 trellis_status trellis_sparse_hip_set_stream(trellis_sparse_backend * backend, void * stream);
 trellis_status trellis_sparse_hip_own_stream(trellis_sparse_backend * backend);
+
+/* linear_act of few rows splits its sums, and attention of few queries its keys,
+ * over more blocks, through scratch of the backend's pool; a call that gets none
+ * (under capture, or out of memory) does without, in more time and with sums in
+ * another order.  With `scratch` set (NULL: the pool again) such calls use its
+ * memory where it is large enough, captured ones too: graphs, streams or backends
+ * that may run at the same time need scratch of their own.  It is the caller's, and
+ * free_buffer unsets it; rows in it -> INVALID_ARGUMENT.  scratch_bytes: the most
+ * that a call has asked for so far. */
+trellis_status trellis_sparse_hip_set_scratch(trellis_sparse_backend * backend, const trellis_sparse_buffer * scratch);
+size_t trellis_sparse_hip_scratch_bytes(const trellis_sparse_backend * backend);
 
 /* ------------------------------------------------------------------------ */
 /* Transformer blocks over voxel rows (no vtable counterpart).  The          */

@@ -104,6 +104,138 @@ def graphs(program):
     be.set_stream(None)
 
 
+def split_graphs(program):
+    """Calls that split through scratch, captured into two graphs with scratch of their own: every replay is the eager call's
+    result, bit for bit, with eager calls through the pool's scratch between; without scratch they are captured unsplit.
+    While a stream is captured no other can be set, and stage times are not recorded."""
+    be = program[0]
+    stream, other = torch.cuda.Stream(), torch.cuda.Stream()
+    be.set_stream(stream.cuda_stream)
+    be.profile(True)
+    gen = torch.Generator().manual_seed(5)
+    rows = lambda *shape: torch.randn(shape, generator=gen).to(torch.bfloat16).cuda()  # noqa: E731
+    w = np.random.default_rng(1).standard_normal((512, 4096)).astype(np.float32) / 64
+    k, v = rows(20000, 128), rows(20000, 128)
+    xs = [(rows(2, 4096), rows(3, 128)) for _ in range(3)]
+    kb, vb = be.wrap(k), be.wrap(v)
+
+    def run(x, q, y, o):
+        be.linear_act(x, w, None, y, 2, 4096, 512, act="gelu")
+        be.attention(q, kb, vb, o, 3, 20000, 2, 2, 64)
+
+    def outputs():
+        t = torch.empty((2, 512), dtype=torch.bfloat16, device="cuda"), torch.empty((3, 128), dtype=torch.bfloat16, device="cuda")
+        return t, [be.wrap(a) for a in t]
+
+    torch.cuda.synchronize()
+    exp = []
+    for x, q in xs:
+        t, b = outputs()
+        run(be.wrap(x), be.wrap(q), *b)
+        torch.cuda.synchronize()
+        exp.append([a.float().cpu().numpy() for a in t])
+    made = []
+    for with_scratch in (True, True, False):
+        x, q = (a.clone() for a in xs[0])
+        t, b = outputs()
+        scratch = torch.empty(be.scratch_bytes // 4, dtype=torch.int32, device="cuda")
+        xb, qb, sb = be.wrap(x), be.wrap(q), be.wrap(scratch)
+        torch.cuda.synchronize()
+        be.set_scratch(sb if with_scratch else None)
+        with torch.cuda.stream(stream):
+            g = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(g, stream=stream):
+                run(xb, qb, *b)
+                for back in (other.cuda_stream, 0, None):
+                    with raises(sh.HipError) as e:
+                        be.set_stream(back)
+                    assert e.value.status == sh.ERROR
+        be.set_scratch(None)
+        made.append((g, x, q, t, (b, scratch, xb, qb, sb)))
+    for step in range(9):
+        g, x, q, t, _ = made[step % 3]
+        i = step // 3
+        with torch.cuda.stream(stream):
+            x.copy_(xs[i][0])
+            q.copy_(xs[i][1])
+            for a in t:
+                a.zero_()
+            g.replay()
+            eager, b = outputs()
+            run(be.wrap(xs[(i + 1) % 3][0]), be.wrap(xs[(i + 1) % 3][1]), *b)
+        stream.synchronize()
+        for got, e in zip(t, exp[i]):
+            got = got.float().cpu().numpy()
+            # Unsplit sums: another order, within a few roundings of bf16.
+            assert np.array_equal(got, e) if step % 3 < 2 else np.allclose(got, e, rtol=2 ** -6, atol=2 ** -8), step
+        for got, e in zip(eager, exp[(i + 1) % 3]):
+            assert np.array_equal(got.float().cpu().numpy(), e), step
+    be.profile(False)
+    be.set_stream(None)
+
+
+def beyond_32_bits(program):
+    """Rows that lie more than 2^31 elements behind their buffer's start: keys and values far apart (both kernels), a norm,
+    8-bit rows, a linear and a rotary over 1.2 M rows of 2,048; the last rows are what the same rows give alone."""
+    be, dev = program[0], torch.device("cuda", 0)
+    bf = torch.bfloat16
+    gen = torch.Generator().manual_seed(9)
+    rows = lambda *shape: torch.randn(shape, generator=gen).to(bf).cuda()  # noqa: E731
+    for heads, dim, stride, n in ((2, 64, 1 << 22, 700), (1, 24, 1 << 24, 170)):
+        w = heads * dim
+        far = torch.zeros((n - 1) * stride + 2 * w, dtype=bf, device=dev)
+        kv = far.as_strided((n, 2 * w), (stride, 1))
+        kv.copy_(rows(n, 2 * w))
+        near, q = kv.contiguous(), rows(n, w)
+        a, b = torch.empty_like(q), torch.empty_like(q)
+        torch.cuda.synchronize()
+        fb, nb, qb = be.wrap(far), be.wrap(near), be.wrap(q)
+        be.attention(qb, fb, fb, be.wrap(a), n, n, heads, heads, dim, k_stride=stride, v_offset=w, v_stride=stride)
+        be.attention(qb, nb, nb, be.wrap(b), n, n, heads, heads, dim, k_stride=2 * w, v_offset=w, v_stride=2 * w)
+        out = be.download(be.wrap(a))
+        # Strides beyond 2^23 leave the wide kernel: its weights are rounded, 2^-8 of sum p |v| <= 1, and both outputs are.
+        tol = 0 if stride <= 1 << 23 else 2 ** -7
+        assert np.allclose(out, be.download(be.wrap(b)), rtol=tol, atol=tol) and np.abs(out).max() > 0.1
+        del far, kv
+    n, c, last = 1_200_000, 2048, 64
+    x = torch.zeros((n, c), dtype=bf, device=dev)
+    x[-last:] = rows(last, c)
+    tail = x[-last:].clone()
+    y = torch.zeros_like(x)
+    coords = torch.randint(0, 64, (n, 4), dtype=torch.int32, generator=gen).cuda()
+    end = coords[-last:].clone()
+    weight = np.random.default_rng(4).standard_normal((64, c)).astype(np.float32) / 45
+    torch.cuda.synchronize()
+    xb, yb, tb, cb, eb = (be.wrap(t) for t in (x, y, tail, coords, end))
+    alone = be.alloc(last * c)
+
+    def same(width=c):
+        torch.cuda.synchronize()
+        got = y.reshape(-1)[:n * width].reshape(n, width)
+        assert np.array_equal(got[-last:].float().cpu().numpy(), be.download(alone)[:last * width].reshape(last, width))
+        assert not got[:1000].any()
+
+    be.rms_norm(xb, None, yb, n, c, 1e-6, residual=xb)
+    be.rms_norm(tb, None, alone, last, c, 1e-6, residual=tb)
+    same()
+    big8, small8 = be.alloc_rows8(n, c), be.alloc_rows8(last, c)
+    be.rms_norm(xb, None, big8, n, c, 1e-6)
+    be.rms_norm(tb, None, small8, last, c, 1e-6)
+    be.expand_rows8(big8, yb, n, c)
+    be.expand_rows8(small8, alone, last, c)
+    same()
+    be.rotary(xb, cb, yb, n, 16, 128, (21, 21, 21), 10000.0, eps=1e-6)
+    be.rotary(tb, eb, alone, last, 16, 128, (21, 21, 21), 10000.0, eps=1e-6)
+    same()
+    for a, b in ((xb, tb), (big8, small8)):
+        be.linear_act(a, weight, None, yb, n, c, 64)
+        be.linear_act(b, weight, None, alone, last, c, 64)
+        torch.cuda.synchronize()
+        got = y.reshape(-1)[:n * 64].reshape(n, 64)[-last:].float().cpu().numpy()
+        # Other blocks and splits: sums of 2,048 in another order, 8 sqrt(2048) 2^-24 of 4 at most, and a rounding to bf16.
+        assert np.allclose(got, be.download(alone)[:last * 64].reshape(last, 64), rtol=2 ** -7, atol=1e-4)
+
+
 def two_backends_at_once(program):
     """Two backends on two streams, queued in turn with no wait between: each gives its own results."""
     be, blk, n, t, exp = program
@@ -147,7 +279,8 @@ def wrap_refusals(program):
 
 
 if __name__ == "__main__":
-    for check in (tensors_and_streams, graphs, two_backends_at_once, wrap_refusals):
+    for check in (tensors_and_streams, graphs, split_graphs, beyond_32_bits, two_backends_at_once,
+                  wrap_refusals):
         p = program()
         check(p)
         p[0].destroy()

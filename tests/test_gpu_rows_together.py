@@ -178,7 +178,8 @@ def torch_program():
     return r.returncode, r.stdout, r.stderr[-3000:]
 
 
-@pytest.mark.parametrize("what", ["tensors_and_streams", "graphs", "two_backends_at_once", "wrap_refusals"])
+@pytest.mark.parametrize("what", ["tensors_and_streams", "graphs", "split_graphs", "beyond_32_bits", "two_backends_at_once",
+                                  "wrap_refusals"])
 def test_with_torch(torch_program, what):
     rc, out, err = torch_program
     assert f"{what}: ok" in out.splitlines() and rc == 0, f"exit {rc}\n{out}\n{err}"

@@ -15,6 +15,8 @@ def test_null_arguments():
     assert L.trellis_sparse_hip_wrap_i32(None, 16, 1, ctypes.byref(out)) == bad
     assert L.trellis_sparse_hip_set_stream(None, None) == bad
     assert L.trellis_sparse_hip_own_stream(None) == bad
+    assert L.trellis_sparse_hip_set_scratch(None, None) == bad
+    assert L.trellis_sparse_hip_scratch_bytes(None) == 0
     assert L.trellis_sparse_hip_alloc_rows8(None, 1, 1, ctypes.byref(out)) == bad
     assert L.trellis_sparse_hip_pack_rows8(None, None, None, 1, 1) == bad
     assert L.trellis_sparse_hip_expand_rows8(None, None, None, 1, 1) == bad

@@ -80,6 +80,9 @@ struct Backend {
     hipStream_t stream = nullptr;      // where calls enqueue: own_stream, or the caller's (set_stream)
     hipStream_t own_stream = nullptr;
     hipEvent_t stream_left = nullptr;  // orders a new stream behind the one left (created on first use)
+    // Scratch that the caller gave for split sums (set_scratch), and the most that a call wanted.
+    void * scratch = nullptr;
+    size_t scratch_bytes = 0, scratch_most = 0;
     trellis_sparse_hip_policy policy{};
     std::string last_error;
     // Pool: size class -> free device blocks.
@@ -219,15 +222,15 @@ hipError_t device_malloc(Backend * be, void ** p, size_t bytes) {
 // Whether the caller's stream (set_stream) is being captured into a graph: no
 // memory is handed out then.  A fresh allocation cannot be captured, and a pool
 // block would go back to the pool while the graph still writes to it.
-bool capturing(const Backend * be) {
-    if (be->stream == be->own_stream) return false;
+bool stream_captured(hipStream_t stream) {
     hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
-    if (hipStreamIsCapturing(be->stream, &status) != hipSuccess) {
+    if (hipStreamIsCapturing(stream, &status) != hipSuccess) {
         (void) hipGetLastError();
         return true;
     }
     return status != hipStreamCaptureStatusNone;
 }
+bool capturing(const Backend * be) { return be->stream != be->own_stream && stream_captured(be->stream); }
 
 trellis_status dev_alloc(Backend * be, size_t bytes, DevMem * out) {
     out->ptr = nullptr;
@@ -383,7 +386,7 @@ hipEvent_t take_event(Backend * be) {
 }
 
 void stage_begin(Backend * be, int stage) {
-    if (!be->profiling) return;
+    if (!be->profiling || capturing(be)) return;  // (a graph's replays are not timed)
     StageMark & m = be->open[stage];
     m.stage = stage;
     m.a = take_event(be);
@@ -741,6 +744,10 @@ void op_free_buffer(trellis_sparse_backend * backend, trellis_sparse_buffer * bu
     if (backend == nullptr || buffer == nullptr) return;
     Backend * be = as_backend(backend);
     DevMem m{buffer->ptr, buffer->cap};
+    if (buffer->ptr == be->scratch) {
+        be->scratch = nullptr;
+        be->scratch_bytes = 0;
+    }
     if (buffer->cap != 0) dev_release(be, &m);  // a wrapped buffer's memory is the caller's
     free(buffer);
 }
@@ -2080,6 +2087,26 @@ uint8_t * rows8_scale_bytes(const trellis_sparse_buffer * b) {
 // n rows of c channels, with sizes that every address computation holds.
 bool rows_ok(int64_t n, int64_t c) { return n > 0 && c > 0 && n <= INT64_MAX / 64 / c; }
 
+// Scratch for one call's split sums: the caller's (set_scratch), or the pool's,
+// which a captured call does not take, as a graph's replays would share it with
+// the calls after it.  Null where there is none; `from` is what to release.
+void * take_scratch(Backend * be, size_t bytes, DevMem * from) {
+    be->scratch_most = std::max(be->scratch_most, bytes);
+    if (bytes <= be->scratch_bytes) return be->scratch;
+    if (capturing(be)) return nullptr;
+    if (dev_alloc(be, bytes, from) != TRELLIS_STATUS_OK) be->last_error.clear();
+    return from->ptr;
+}
+
+// Whether the caller's scratch, when a call takes `bytes` of it, holds rows of the call.
+bool scratch_clash(const Backend * be, size_t bytes, std::initializer_list<Span> rows) {
+    if (bytes == 0 || bytes > be->scratch_bytes) return false;
+    const Span s{(const char *) be->scratch, 1, (int64_t) bytes, (int64_t) bytes};
+    for (const Span & r : rows)
+        if (r.at != nullptr && r.rows > 0 && r.at < s.end() && s.at < r.end()) return true;
+    return false;
+}
+
 // Runs a call; a failed host allocation (packed weights, the weight table) is a
 // status, not an exception that leaves a C entry point.
 template <class F> trellis_status no_throw(trellis_sparse_backend * backend, F && call) {
@@ -2226,16 +2253,17 @@ trellis_status linear_act_impl(trellis_sparse_backend * backend, const trellis_s
     p.ci = ci;
     p.co = co;
     p.act = act;
-    // Scratch for split sums is the pool's; where none is to be had (also under
-    // capture, where two graphs could share it) a block takes all of K.
+    // Without scratch for split sums a block takes all of K.
     const int x_type = from8 ? kRows8 : dt;
-    LinearActPlan plan = linear_act_plan(dt, x_type, n, co, p.row_bytes, p.w_bytes, be->cus, !capturing(be));
-    DevMem scratch;
-    if (plan.scratch > 0 && dev_alloc(be, plan.scratch, &scratch) != TRELLIS_STATUS_OK) {
-        be->last_error.clear();
-        plan = linear_act_plan(dt, x_type, n, co, p.row_bytes, p.w_bytes, be->cus, false);
+    LinearActPlan plan = linear_act_plan(dt, x_type, n, co, p.row_bytes, p.w_bytes, be->cus, true);
+    if (scratch_clash(be, plan.scratch, {packed(y, n, co), packed(residual, n, co), from8 ? Span{} : packed(x, n, ci)})) {
+        return fail(be, TRELLIS_STATUS_INVALID_ARGUMENT, "linear_act: rows in the scratch");
     }
-    p.partial = (float *) scratch.ptr;
+    DevMem scratch;
+    if (plan.scratch > 0) {
+        p.partial = (float *) take_scratch(be, plan.scratch, &scratch);
+        if (p.partial == nullptr) plan = linear_act_plan(dt, x_type, n, co, p.row_bytes, p.w_bytes, be->cus, false);
+    }
     stage_begin(be, TRELLIS_SPARSE_HIP_STAGE_ELEMENTWISE);
     const hipError_t err = launch_linear_act(dt, x_type, p, plan, be->stream);
     stage_end(be, TRELLIS_SPARSE_HIP_STAGE_ELEMENTWISE);
@@ -2329,7 +2357,8 @@ trellis_status attention_impl(trellis_sparse_backend * backend, const trellis_sp
         return fail(be, TRELLIS_STATUS_INVALID_ARGUMENT, "attention: bad desc");
     }
     const trellis_sparse_hip_attention_desc & d = *desc;
-    if (nq <= 0 || nq > INT32_MAX || nkv < 0 || nkv > INT32_MAX || d.heads <= 0 || d.heads > 65536 ||
+    constexpr int64_t kMostRows = INT32_MAX - 64;  // a tile past the last row is counted in 32 bits
+    if (nq <= 0 || nq > kMostRows || nkv < 0 || nkv > kMostRows || d.heads <= 0 || d.heads > 65536 ||
         d.kv_heads <= 0 || d.heads % d.kv_heads != 0 || d.head_dim <= 0 || !std::isfinite(d.scale) ||
         (q_offsets == nullptr) != (kv_offsets == nullptr) || n_seqs <= 0 || (q_offsets == nullptr && n_seqs != 1)) {
         return fail(be, TRELLIS_STATUS_INVALID_ARGUMENT, "attention: bad argument");
@@ -2355,6 +2384,11 @@ trellis_status attention_impl(trellis_sparse_backend * backend, const trellis_sp
         sk = strided(be, k, nkv, kw, d.k_offset, ks);
         sv = strided(be, v, nkv, kw, d.v_offset, vs);
     }
+    for (const trellis_sparse_buffer * b : {q_offsets, kv_offsets}) {
+        if (b != nullptr && spans_clash(sy, Span{(const char *) b->ptr, n_seqs + 1, 4, 4}, false)) {
+            return fail(be, TRELLIS_STATUS_INVALID_ARGUMENT, "attention: overlapping rows");
+        }
+    }
     // Other blocks still read keys and values where one has written its queries' rows; q itself may be y.
     if (spans_clash(sy, sq, true) || spans_clash(sy, sk, false) || spans_clash(sy, sv, false)) {
         return fail(be, TRELLIS_STATUS_INVALID_ARGUMENT, "attention: overlapping rows");
@@ -2379,14 +2413,15 @@ trellis_status attention_impl(trellis_sparse_backend * backend, const trellis_sp
     p.dim = d.head_dim;
     const double scale = d.scale == 0.0f ? 1.0 / std::sqrt((double) d.head_dim) : (double) d.scale;
     p.scale = (float) (scale * 1.4426950408889634);
-    // Scratch for split keys is the pool's; where none is to be had (also under
-    // capture, where two graphs could share it) one block takes all of a
-    // query's keys.
+    // Without scratch for split keys one block takes all of a query's keys.
     const AttentionShape shape = attention_shape(be->policy.compute_dtype, p, be->cus);
+    if (scratch_clash(be, shape.scratch, {sq, sk, sv, sy})) {
+        return fail(be, TRELLIS_STATUS_INVALID_ARGUMENT, "attention: rows in the scratch");
+    }
     DevMem scratch;
-    if (shape.scratch > 0 && dev_alloc(be, shape.scratch, &scratch) != TRELLIS_STATUS_OK) be->last_error.clear();
+    void * split_keys = shape.scratch > 0 ? take_scratch(be, shape.scratch, &scratch) : nullptr;
     stage_begin(be, TRELLIS_SPARSE_HIP_STAGE_ELEMENTWISE);
-    const hipError_t err = launch_attention(be->policy.compute_dtype, p, shape, scratch.ptr, be->stream);
+    const hipError_t err = launch_attention(be->policy.compute_dtype, p, shape, split_keys, be->stream);
     stage_end(be, TRELLIS_SPARSE_HIP_STAGE_ELEMENTWISE);
     dev_release(be, &scratch);
     return hip_status(be, err, "attention");
@@ -2506,6 +2541,10 @@ trellis_status set_stream_impl(trellis_sparse_backend * backend, hipStream_t str
     Backend * be = as_backend(backend);
     if (stream == be->stream) return TRELLIS_STATUS_OK;
     DeviceScope scope(be);
+    // Events between a captured stream and another would end the capture.
+    if (capturing(be) || (stream != be->own_stream && stream_captured(stream))) {
+        return fail(be, TRELLIS_STATUS_ERROR, "set_stream: a stream is being captured");
+    }
     if (be->stream_left == nullptr) {
         TSH_TRY(be, hipEventCreateWithFlags(&be->stream_left, hipEventDisableTiming));
     }
@@ -3036,6 +3075,21 @@ trellis_status trellis_sparse_hip_wrap_i32(trellis_sparse_backend * backend, voi
 
 trellis_status trellis_sparse_hip_set_stream(trellis_sparse_backend * backend, void * stream) {
     return tsh::set_stream_impl(backend, (hipStream_t) stream);
+}
+
+trellis_status trellis_sparse_hip_set_scratch(trellis_sparse_backend * backend, const trellis_sparse_buffer * scratch) {
+    if (backend == nullptr) return TRELLIS_STATUS_INVALID_ARGUMENT;
+    tsh::Backend * be = tsh::as_backend(backend);
+    if (scratch != nullptr && (scratch->ptr == nullptr || scratch->dtype == tsh::kRows8)) {
+        return tsh::fail(be, TRELLIS_STATUS_INVALID_ARGUMENT, "set_scratch: a buffer of rows or int32");
+    }
+    be->scratch = scratch != nullptr ? scratch->ptr : nullptr;
+    be->scratch_bytes = scratch != nullptr ? scratch->bytes : 0;
+    return TRELLIS_STATUS_OK;
+}
+
+size_t trellis_sparse_hip_scratch_bytes(const trellis_sparse_backend * backend) {
+    return backend != nullptr ? ((const tsh::Backend *) backend)->scratch_most : 0;
 }
 
 trellis_status trellis_sparse_hip_own_stream(trellis_sparse_backend * backend) {

@@ -21,11 +21,15 @@ __device__ __forceinline__ int64_t offset_of(const int32_t * at, int i, int64_t 
     return v < 0 ? 0 : (v > n ? n : v);
 }
 
-// Tile `tile` of TQ queries among all sequences' tiles, in order; nq = 0 past
-// the last.  A query is a row and one of the `group` heads that share a kv head:
-// query i of a sequence is its row i / group, head i % group of them.  Offsets
-// are read on the device, so a grid has an upper bound of tiles; they are
-// clamped to the rows that there are, and a sequence whose offsets fall is empty.
+// Tile `tile` of TQ queries among all sequences' tiles, in order; nq = 0 where
+// there is none.  A query is a row and one of the `group` heads that share a kv
+// head: query i of a sequence is its row i / group, head i % group of them.
+// Offsets are read on the device, so tiles are numbered by what holds for any
+// lengths: sequence s, whose queries begin at a, has its tiles from a / TQ + s
+// on, and never reaches past the next one's first.  They are clamped to the rows
+// that there are, and a sequence whose offsets fall is empty.  The sequence is
+// found 64 offsets at a time: 18,216 rows in 2,024 sequences of 9, 8 heads of 64,
+// took 284 us with all sequences counted up to the tile, 89 so.
 template <int TQ> __device__ Place find_place(const Attention & p, int64_t tile, int group) {
     Place r{0, 0, 0, 0, 0};
     if (p.q_at == nullptr) {
@@ -34,33 +38,25 @@ template <int TQ> __device__ Place find_place(const Attention & p, int64_t tile,
         r.nk = (int) p.nk;
         return r;
     }
-    // 64 sequences at a time: an inclusive scan of their tile counts, then the first that reaches past `tile`.
     const int lane = threadIdx.x & 63;
-    for (int s0 = 0; s0 < p.seqs; s0 += 64) {
-        const int i = s0 + lane;
-        int64_t lo = 0, len = 0;
-        if (i < p.seqs) {
-            lo = offset_of(p.q_at, i, p.nq);
-            len = max((int64_t) 0, offset_of(p.q_at, i + 1, p.nq) - lo) * group;
-        }
-        const int64_t tiles = (len + TQ - 1) / TQ;
-        int64_t sum = tiles;
-        for (int d = 1; d < 64; d <<= 1) {
-            const int64_t o = __shfl_up(sum, d);
-            if (lane >= d) sum += o;
-        }
-        const unsigned long long past = __ballot(sum > tile);
-        if (past != 0) {
-            const int at = __ffsll(past) - 1, seq = s0 + at;
-            r.q0 = uniform((int64_t) __shfl(lo, at));
-            r.first = uniform((tile - __shfl(sum - tiles, at)) * TQ);
-            r.nq = uniform((int) min((int64_t) TQ, __shfl(len, at) - r.first));
-            r.k0 = uniform(offset_of(p.k_at, seq, p.nk));
-            r.nk = uniform((int) max((int64_t) 0, offset_of(p.k_at, seq + 1, p.nk) - r.k0));
-            return r;
-        }
-        tile -= uniform((int64_t) __shfl(sum, 63));
+    const auto first_tile = [&](int s) { return offset_of(p.q_at, s, p.nq) * group / TQ + s; };
+    // The last sequence of [seq, seq + many) whose tiles begin at or before `tile`.
+    int seq = 0, many = p.seqs;
+    while (many > 1) {
+        const int step = (many + 63) / 64, i = lane * step;
+        const unsigned long long before = __ballot(i < many && first_tile(seq + i) <= tile);
+        if (before == 0) return r;
+        const int at = 63 - __clzll(before);
+        seq += at * step;
+        many = min(step, many - at * step);
     }
+    r.q0 = uniform(offset_of(p.q_at, seq, p.nq));
+    r.first = (tile - (r.q0 * group / TQ + seq)) * TQ;
+    const int64_t left = (uniform(offset_of(p.q_at, seq + 1, p.nq)) - r.q0) * group - r.first;
+    if (r.first < 0 || left <= 0) return r;
+    r.nq = (int) min((int64_t) TQ, left);
+    r.k0 = uniform(offset_of(p.k_at, seq, p.nk));
+    r.nk = (int) max((int64_t) 0, uniform(offset_of(p.k_at, seq + 1, p.nk)) - r.k0);
     return r;
 }
 
@@ -145,7 +141,6 @@ template <int DT> __global__ void __launch_bounds__(256) k_attention_any(Attenti
 }
 
 template <int DT> hipError_t launch_any(const Attention & p, hipStream_t s) {
-    // Every sequence may add one partly filled tile.
     const int64_t tiles = p.nq / 16 + (p.q_at != nullptr ? p.seqs : 1);
     const int64_t grid = tiles * p.heads;
     if (grid > 0x7fffffffLL) return hipErrorInvalidValue;
@@ -187,6 +182,44 @@ struct Partial {
     float2 * stat; // [splits][nq * heads]: maximum (log2 units), sum
     int splits;
 };
+
+// Lane (query, half) leaves channels d * 32 + 8 i + 4 half + 0 .. 3: of its split, or of y.
+template <int DT, int N>
+__device__ __forceinline__ void leave(const Attention & p, const Partial & part, const f32x16 (&out)[N], float ref,
+                                      float sum, bool live, bool some, int split, int64_t row, int head, int half) {
+    using T = typename Store<DT>::T;
+    if (!live) return;
+    if (part.splits > 1) {
+        const int64_t at_q = ((int64_t) split * p.nq + row) * p.heads + head;
+        if (half == 0) part.stat[at_q] = float2{ref, sum};
+        if (!some) return;
+        float * o = part.out + at_q * p.dim;
+#pragma unroll
+        for (int d = 0; d < N; ++d)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int c = d * 32 + i * 8 + half * 4;
+                if (c < p.dim)
+                    *(float4 *) (o + c) = float4{out[d][4 * i], out[d][4 * i + 1], out[d][4 * i + 2], out[d][4 * i + 3]};
+            }
+        return;
+    }
+    // No keys (or none above -inf): zeros.
+    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+    T * y = (T *) p.y + row * p.y_stride + (int64_t) head * p.dim;
+#pragma unroll
+    for (int d = 0; d < N; ++d)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int c = d * 32 + i * 8 + half * 4;
+            struct alignas(4 * sizeof(T)) {
+                T h[4];
+            } w;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) w.h[j] = round_to_store<DT>(out[d][4 * i + j] * inv);
+            if (c < p.dim) *(decltype(w) *) (y + c) = w;
+        }
+}
 
 // NW wavefronts of 32 queries each, keys in tiles of 64 straight into LDS, two
 // tiles deep.  Scores are computed transposed (keys x queries, K as the A
@@ -463,42 +496,153 @@ __global__ void __launch_bounds__(64 * NW, DC <= 64 ? 3 : 2) k_attention(Attenti
         }
     }
 
-    float sum = sum0 + sum1;
-    sum = sum_halves(sum);
-    if (!live) return;
-    if (part.splits > 1) {
-        const int64_t at_q = ((int64_t) split * p.nq + row) * p.heads + head;
-        if (half == 0) part.stat[at_q] = float2{ref, sum};
-        if (t0 < t1) {
-            float * o = part.out + at_q * p.dim;
+    leave<DT>(p, part, out, ref, sum_halves(sum0 + sum1), live, t0 < t1, split, row, head, half);
+}
+
+// fp32: as k_attention, with products of two channels, or two keys, at a time.
+// The two halves of a wavefront have 4 channels each of every 8 of K's and q's
+// rows (the order of a sum's terms is free, so a chunk of 16 bytes serves four
+// products as it is read), and score i of a lane, key 8 (i / 4) + 4 half + i % 4, is
+// the B operand of the values' product with the rows of V that the halves read.
+// These products take 64 clocks each, 4,096 of a tile of 32 queries x 32 keys x
+// 64 channels against some 300 of its softmax, which is why nothing is
+// interleaved by hand: 18,216 rows, 8 heads of 64 in 5.7 ms, 118 TFLOP/s (129 at
+// 128 channels; a large fp32 matrix product of the library reaches 136 to 153),
+// where k_attention_any takes 44 ms.  Keys in tiles of 32 straight into LDS, two tiles deep;
+// chunk c of row r at c ^ f(r), so that the 16 lanes of a K read (16 rows, one
+// chunk) touch different banks.
+template <int DC, int NW>
+__global__ void __launch_bounds__(64 * NW, 2) k_attention32(Attention p, Partial part, int tiles) {
+    constexpr int TQ = 32 * NW, TK = 32;
+    constexpr int LP = DC <= 32 ? 32 : (DC <= 64 ? 64 : 128);  // values per LDS row
+    constexpr int ROW = LP * 4, CH = LP / 4;
+    constexpr int KS = DC / 8, DT32 = DC / 32;
+    constexpr int TILE = TK * ROW;
+    constexpr int RPL = 64 / CH;
+    constexpr int PER = TILE / 1024 / NW;
+    static_assert(TILE / 1024 % NW == 0, "whole loads");
+    __shared__ __attribute__((aligned(1024))) unsigned char s_tile[4 * TILE];  // K, V of two tiles
+
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int l32 = lane & 31, half = lane >> 5;
+    const int group = p.heads / p.kv_heads;
+    const int64_t unit = xcd_remap(blockIdx.x, gridDim.x);
+    const int split = (int) (unit % part.splits);
+    const int kv = (int) (unit / part.splits / tiles);
+    const Place at = find_place<TQ>(p, unit / part.splits % tiles, group);
+    if (at.nq <= 0) return;
+    const int all = (at.nk + TK - 1) / TK;
+    const int t0 = (int) ((int64_t) all * split / part.splits), t1 = (int) ((int64_t) all * (split + 1) / part.splits);
+
+    const int qi = wave * 32 + l32;
+    const int64_t vq = at.first + qi;
+    const int64_t row = at.q0 + vq / group;
+    const int head = kv * group + (int) (vq % group);
+    const bool live = qi < at.nq;
+    const float sign = p.scale < 0.0f ? -1.0f : 1.0f, scale = fabsf(p.scale);
+    float q[KS][4];
+    {
+        const float * qr = (const float *) p.q + row * p.q_stride + (int64_t) head * p.dim;
 #pragma unroll
-            for (int d = 0; d < DT32; ++d)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int c = d * 32 + i * 8 + half * 4;
-                    if (c < p.dim)
-                        *(float4 *) (o + c) =
-                            float4{out[d][4 * i], out[d][4 * i + 1], out[d][4 * i + 2], out[d][4 * i + 3]};
-                }
+        for (int k = 0; k < KS; ++k) {
+            const int c = 8 * k + 4 * half;
+            float4 v{0.f, 0.f, 0.f, 0.f};
+            if (live && c < p.dim) v = *(const float4 *) (qr + c);
+            q[k][0] = v.x * sign;
+            q[k][1] = v.y * sign;
+            q[k][2] = v.z * sign;
+            q[k][3] = v.w * sign;
         }
-        return;
     }
-    // No keys (or none above -inf): zeros.
-    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-    T * y = (T *) p.y + row * p.y_stride + (int64_t) head * p.dim;
+
+    const auto swizzle = [](int r) {
+        if constexpr (CH == 8) return (r >> 1) & 7;
+        return ((r & 4) << 1) | ((r & 8) >> 1) | (r & 3);
+    };
+    const char * kb = (const char *) ((const float *) p.k + at.k0 * p.k_stride + (int64_t) kv * p.dim);
+    const char * vb = (const char *) ((const float *) p.v + at.k0 * p.v_stride + (int64_t) kv * p.dim);
+    const int ks = (int) p.k_stride * 4, vs = (int) p.v_stride * 4;
+    constexpr uint32_t kOutside = 0x80000000u;
+    const uint32_t lds0 = (uint32_t) (uintptr_t) (__attribute__((address_space(3))) unsigned char *) s_tile;
+    // Rows past the last and channels past dim are zeros.
+    const auto load = [&](int t) {
+        const int rows = min(TK, at.nk - t * TK);
+        const uint32_t to = lds0 + (uint32_t) (((t - t0) & 1) * TILE);
+        const __amdgpu_buffer_rsrc_t kres = __builtin_amdgcn_make_buffer_rsrc(
+            (void *) (kb + (int64_t) t * TK * ks), 0, (rows - 1) * ks + p.dim * 4, 0x00020000);
+        const __amdgpu_buffer_rsrc_t vres = __builtin_amdgcn_make_buffer_rsrc(
+            (void *) (vb + (int64_t) t * TK * vs), 0, (rows - 1) * vs + p.dim * 4, 0x00020000);
+#pragma unroll
+        for (int j = 0; j < PER; ++j) {
+            const int r = (wave * PER + j) * RPL + lane / CH;
+            const int c = (lane % CH) ^ swizzle(r);
+            const bool in = r < rows && c * 4 < p.dim;
+            dma_b128_m0(kres, to + (wave * PER + j) * 1024u, in ? (uint32_t) (r * ks + c * 16) : kOutside, 0);
+            dma_b128_m0(vres, to + 2 * TILE + (wave * PER + j) * 1024u, in ? (uint32_t) (r * vs + c * 16) : kOutside, 0);
+        }
+    };
+
+    f32x16 out[DT32];
 #pragma unroll
     for (int d = 0; d < DT32; ++d)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int c = d * 32 + i * 8 + half * 4;
-            union {
-                T h[4];
-                int2 v;
-            } w;
+        for (int i = 0; i < 16; ++i) out[d][i] = 0.0f;
+    float ref = -__builtin_inff(), sum0 = 0.0f, sum1 = 0.0f;
+    if (t0 < t1) load(t0);
+    for (int t = t0; t < t1; ++t) {
+        // Tile t has landed; every wavefront is done with tile t - 1.
+        wait_vmcnt<0>();
+        lds_barrier();
+        if (t + 1 < t1) load(t + 1);
+        const unsigned char * sk = s_tile + ((t - t0) & 1) * TILE;
+        const unsigned char * sv = sk + 2 * TILE;
+        f32x16 cur;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) w.h[j] = round_to_store<DT>(out[d][4 * i + j] * inv);
-            if (c < p.dim) *(int2 *) (y + c) = w.v;
+        for (int i = 0; i < 16; ++i) cur[i] = 0.0f;
+#pragma unroll
+        for (int k = 0; k < KS; ++k) {
+            const float4 a = *(const float4 *) (sk + l32 * ROW + (((2 * k + half) ^ swizzle(l32)) * 16));
+            cur = __builtin_amdgcn_mfma_f32_32x32x2f32(a.x, q[k][0], cur, 0, 0, 0);
+            cur = __builtin_amdgcn_mfma_f32_32x32x2f32(a.y, q[k][1], cur, 0, 0, 0);
+            cur = __builtin_amdgcn_mfma_f32_32x32x2f32(a.z, q[k][2], cur, 0, 0, 0);
+            cur = __builtin_amdgcn_mfma_f32_32x32x2f32(a.w, q[k][3], cur, 0, 0, 0);
         }
+        const int left = at.nk - t * TK;
+        if (left < TK) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+                if (8 * (i / 4) + 4 * half + i % 4 >= left) cur[i] = -__builtin_inff();
+        }
+        float m = cur[0];
+#pragma unroll
+        for (int i = 1; i < 16; ++i) m = fmaxf(m, cur[i]);
+        m = max_halves(m) * scale;
+        if (__any(m > ref + 8.0f)) {
+            const float next = fmaxf(ref, m);
+            const float keep = next == -__builtin_inff() ? 1.0f : __builtin_amdgcn_exp2f(ref - next);
+            ref = next;
+            sum0 *= keep;
+            sum1 *= keep;
+#pragma unroll
+            for (int d = 0; d < DT32; ++d)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) out[d][i] *= keep;
+        }
+        const float base = ref == -__builtin_inff() ? 0.0f : ref;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            const float e = __builtin_amdgcn_exp2f(fmaf(cur[i], scale, -base));
+            (i % 2 == 0 ? sum0 : sum1) += e;
+            const int r = 8 * (i / 4) + 4 * half + i % 4;
+#pragma unroll
+            for (int d = 0; d < DT32; ++d) {
+                const float a = *(const float *) (sv + r * ROW + (((8 * d + l32 / 4) ^ swizzle(r)) * 16) + l32 % 4 * 4);
+                out[d] = __builtin_amdgcn_mfma_f32_32x32x2f32(a, e, out[d], 0, 0, 0);
+            }
+        }
+    }
+    leave<kF32>(p, part, out, ref, sum_halves(sum0 + sum1), live, t0 < t1, split, row, head, half);
 }
 
 // Joins the splits, a query to WAVES wavefronts (one with few splits, four with
@@ -570,7 +714,11 @@ template <int DT, int DC, int NW>
 hipError_t launch_nw(const Attention & p, const Partial & part, int64_t tiles, hipStream_t s) {
     const int64_t grid = tiles * p.kv_heads * part.splits;
     if (grid > 0x7fffffffLL) return hipErrorInvalidValue;
-    k_attention<DT, DC, NW><<<(unsigned) grid, 64 * NW, 0, s>>>(p, part, (int) tiles);
+    if constexpr (DT == kF32) {
+        k_attention32<DC, NW><<<(unsigned) grid, 64 * NW, 0, s>>>(p, part, (int) tiles);
+    } else {
+        k_attention<DT, DC, NW><<<(unsigned) grid, 64 * NW, 0, s>>>(p, part, (int) tiles);
+    }
     hipError_t err = hipGetLastError();
     if (err == hipSuccess && part.splits > 1) {
         int qp = 1;
@@ -606,10 +754,11 @@ hipError_t launch_mfma(const Attention & p, const Partial & part, const Attentio
 
 AttentionShape attention_shape(int dtype, const Attention & p, int cus) {
     AttentionShape sh{0, 0, 1, 0};
-    const auto aligned = [](const void * ptr, int64_t stride) { return (uintptr_t) ptr % 16 == 0 && stride % 8 == 0; };
-    // A tile's 64 rows stay within a buffer's 2 GiB of offsets.
+    const int chunk = dtype == kF32 ? 4 : 8;  // of 16 bytes
+    const auto aligned = [&](const void * ptr, int64_t stride) { return (uintptr_t) ptr % 16 == 0 && stride % chunk == 0; };
+    // A tile's rows (64, of fp32 32) stay within a buffer's 2 GiB of offsets.
     constexpr int64_t kMaxStride = 1 << 23;
-    if (dtype == kF32 || p.dim % 8 != 0 || p.dim > 128 || !aligned(p.q, p.q_stride) || !aligned(p.k, p.k_stride) ||
+    if (p.dim % chunk != 0 || p.dim > 128 || !aligned(p.q, p.q_stride) || !aligned(p.k, p.k_stride) ||
         !aligned(p.v, p.v_stride) || !aligned(p.y, p.y_stride) || p.k_stride > kMaxStride || p.v_stride > kMaxStride) {
         return sh;
     }
@@ -618,7 +767,7 @@ AttentionShape attention_shape(int dtype, const Attention & p, int cus) {
     // Sequences of up to 32 queries: one wavefront a block, as the others would only help to load.
     sh.waves = queries <= 32 * seqs ? 1 : 4;
     const int tq = 32 * sh.waves;
-    sh.tiles = queries / tq + seqs;  // every sequence may add one partly filled tile
+    sh.tiles = queries / tq + seqs;
     const int64_t blocks = (queries + tq - 1) / tq * p.kv_heads;
     const int64_t want = (int64_t) cus * 8 / sh.waves;  // two wavefronts per SIMD
     // Few queries: the keys split over more blocks, at least four tiles of 64 each.
@@ -643,7 +792,11 @@ hipError_t launch_attention(int dtype, const Attention & p, const AttentionShape
         part.stat = (float2 *) (part.out + (size_t) sh.splits * p.nq * p.heads * p.dim);
     }
     if (sh.tiles > 0x7fffffffLL) return hipErrorInvalidValue;
-    return dtype == kBF16 ? launch_mfma<kBF16>(p, part, sh, s) : launch_mfma<kF16>(p, part, sh, s);
+    switch (dtype) {
+        case kF32: return launch_mfma<kF32>(p, part, sh, s);
+        case kF16: return launch_mfma<kF16>(p, part, sh, s);
+        default: return launch_mfma<kBF16>(p, part, sh, s);
+    }
 }
 
 }  // namespace tsh

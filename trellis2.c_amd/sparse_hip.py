@@ -161,6 +161,8 @@ ABI = {
     "trellis_sparse_hip_wrap_i32": (c_int, [_p, c_void_p, c_size_t, POINTER(_p)]),
     "trellis_sparse_hip_set_stream": (c_int, [_p, c_void_p]),
     "trellis_sparse_hip_own_stream": (c_int, [_p]),
+    "trellis_sparse_hip_set_scratch": (c_int, [_p, _p]),
+    "trellis_sparse_hip_scratch_bytes": (c_size_t, [_p]),
     "trellis_sparse_hip_alloc_rows8": (c_int, [_p, c_int64, c_int, POINTER(_p)]),
     "trellis_sparse_hip_pack_rows8": (c_int, [_p, _p, _p, c_int64, c_int]),
     "trellis_sparse_hip_expand_rows8": (c_int, [_p, _p, _p, c_int64, c_int]),
@@ -487,6 +489,17 @@ class Backend:
         st = (LIB.trellis_sparse_hip_own_stream(self.ptr) if stream is None else
               LIB.trellis_sparse_hip_set_stream(self.ptr, stream))
         self._check(st, "set_stream")
+
+    def set_scratch(self, scratch: Buffer | None):
+        """Memory for split sums and keys in place of the pool's, in captured calls too (None: the pool again)."""
+        st = LIB.trellis_sparse_hip_set_scratch(self.ptr, None if scratch is None else scratch.handle)
+        self._check(st, "set_scratch")
+        self._scratch = scratch
+
+    @property
+    def scratch_bytes(self) -> int:
+        """The most scratch that a call has asked for so far."""
+        return LIB.trellis_sparse_hip_scratch_bytes(self.ptr)
 
     # -- transformer blocks over voxel rows -----------------------------------------
     def alloc_rows8(self, n: int, c: int) -> Buffer:
