@@ -2253,6 +2253,7 @@ trellis_status linear_act_impl(trellis_sparse_backend * backend, const trellis_s
     p.ci = ci;
     p.co = co;
     p.act = act;
+    p.cus = be->cus;
     // Without scratch for split sums a block takes all of K.
     const int x_type = from8 ? kRows8 : dt;
     LinearActPlan plan = linear_act_plan(dt, x_type, n, co, p.row_bytes, p.w_bytes, be->cus, true);

@@ -51,35 +51,27 @@ typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
 // N (1, 2 or 4) adjacent values at byte voff + soff of a buffer, whole and
 // aligned; beyond the buffer loads give zeros and stores nothing.
+template <int DT, int N> union Adjacent {
+    typename Store<DT>::T h[N];
+    uint16_t b2;
+    uint32_t b4;
+    u32x2 b8;
+    u32x4 b16;
+};
 template <int DT, int N>
-__device__ __forceinline__ void load_adjacent(__amdgpu_buffer_rsrc_t rsrc, uint32_t voff, uint32_t soff, float * v) {
-    using T = typename Store<DT>::T;
-    constexpr int B = N * sizeof(T);
-    union {
-        T h[N];
-        uint16_t b2;
-        uint32_t b4;
-        u32x2 b8;
-        u32x4 b16;
-    } w;
+__device__ __forceinline__ Adjacent<DT, N> load_adjacent(__amdgpu_buffer_rsrc_t rsrc, uint32_t voff, uint32_t soff) {
+    constexpr int B = N * sizeof(typename Store<DT>::T);
+    Adjacent<DT, N> w;
     if constexpr (B == 2) w.b2 = __builtin_amdgcn_raw_buffer_load_b16(rsrc, (int) voff, (int) soff, 0);
     if constexpr (B == 4) w.b4 = __builtin_amdgcn_raw_buffer_load_b32(rsrc, (int) voff, (int) soff, 0);
     if constexpr (B == 8) w.b8 = __builtin_amdgcn_raw_buffer_load_b64(rsrc, (int) voff, (int) soff, 0);
     if constexpr (B == 16) w.b16 = __builtin_amdgcn_raw_buffer_load_b128(rsrc, (int) voff, (int) soff, 0);
-#pragma unroll
-    for (int u = 0; u < N; ++u) v[u] = Store<DT>::ld(w.h, u);
+    return w;
 }
 template <int DT, int N>
 __device__ __forceinline__ void store_adjacent(__amdgpu_buffer_rsrc_t rsrc, uint32_t voff, uint32_t soff, const float * v) {
-    using T = typename Store<DT>::T;
-    constexpr int B = N * sizeof(T);
-    union {
-        T h[N];
-        uint16_t b2;
-        uint32_t b4;
-        u32x2 b8;
-        u32x4 b16;
-    } w;
+    constexpr int B = N * sizeof(typename Store<DT>::T);
+    Adjacent<DT, N> w;
 #pragma unroll
     for (int u = 0; u < N; ++u) w.h[u] = round_to_store<DT>(v[u]);
     if constexpr (B == 2) __builtin_amdgcn_raw_buffer_store_b16(w.b2, rsrc, (int) voff, (int) soff, 0);
@@ -147,6 +139,9 @@ __device__ __forceinline__ void dma_b32(__amdgpu_buffer_rsrc_t rsrc, uint32_t ld
         : "memory");
 }
 
+// The same value in every lane, in a scalar register.
+__device__ __forceinline__ int scalar(int v) { return __builtin_amdgcn_readfirstlane(v); }
+
 constexpr uint32_t kOutside = 0x80000000u;  // beyond every buffer here: loads fetch zeros
 
 // A block of RW x CW wavefronts multiplies BM rows of x by BN rows of W (output
@@ -186,87 +181,112 @@ __global__ void __launch_bounds__(64 * RW * CW, RW * CW * PER_CU / 4) k_linear_a
 
     // An XCD (blocks b, b + 8, ...) takes a contiguous range of the tiles, row
     // block by row block with every channel block in turn: the rows stay in its
-    // L2, and few tiles spread over all XCDs.
+    // L2, and few tiles spread over all XCDs.  More tiles than blocks: its blocks
+    // take every so many of them.
     const int split = kMaySplit ? (int) (blockIdx.x / p.split_blocks) : 0;
-    const int64_t unit = xcd_remap(blockIdx.x - (int64_t) split * p.split_blocks, p.split_blocks);
-    const int64_t tile = unit / p.col_tiles;
-    const int64_t row0 = tile * BM;
-    const int col0 = (int) (unit % p.col_tiles) * BN;
-    const int rows = (int) min((int64_t) BM, p.n - row0);
+    int unit, end, stride = 1;
+    if (p.blocks == p.split_blocks) {
+        unit = scalar((int) xcd_remap(blockIdx.x - (int64_t) split * p.split_blocks, p.split_blocks));
+        end = unit + 1;
+    } else {
+        const int xcd = (int) (blockIdx.x % 8);
+        stride = p.blocks / 8;
+        unit = (int) ((int64_t) p.split_blocks * xcd / 8 + blockIdx.x / 8);
+        end = (int) ((int64_t) p.split_blocks * (xcd + 1) / 8);
+        if (unit >= end) return;
+    }
+    const auto row_of = [&](int u) { return (int64_t) scalar(u / p.col_tiles) * BM; };
+    const auto col_of = [&](int u) { return scalar(u % p.col_tiles) * BN; };
 
-    const __amdgpu_buffer_rsrc_t xres = __builtin_amdgcn_make_buffer_rsrc(
-        (void *) ((const char *) p.x + row0 * p.row_bytes), 0, (int) (rows * p.row_bytes), 0x00020000);
-    const __amdgpu_buffer_rsrc_t wres = __builtin_amdgcn_make_buffer_rsrc(
-        (void *) ((const char *) p.w + (int64_t) col0 * p.w_bytes), 0, (int) (BN * p.w_bytes), 0x00020000);
     const uint32_t slots = (uint32_t) (uintptr_t) (__attribute__((address_space(3))) unsigned char *) s_slot;
 
     // The channel of a row of W in LDS.
     const auto channel_of = [](int r) { return r / (32 * NT) * (32 * NT) + r % 32 * NT + r % (32 * NT) / 32; };
     const auto swizzle = [](int r) { return (((r >> 1) & 1) << 2) | (((r >> 2) & 1) << 1) | ((r >> 3) & 1); };
-    // This lane's piece of a load: 8 lines of 128 bytes.
-    uint32_t x_at[NA], w_at[NB];
-    int x_chunk[NA];
+    // This lane's piece of load g, of 8 rows of 128 bytes: row lane / 8, whose
+    // chunk's lowest bit is g's.  The rest of the place is the same in all lanes
+    // and added at each load (registers are what the largest blocks lack).
+    const int chunk = (lane & 7) ^ swizzle(lane >> 3);
+    uint32_t x_at[2], w_at[2];
 #pragma unroll
-    for (int j = 0; j < NA; ++j) {
-        const int row = (wave * NA + j) * 8 + (lane >> 3);
-        x_chunk[j] = (lane & 7) ^ swizzle(row);
-        x_at[j] = row < rows ? (uint32_t) (row * p.row_bytes) + x_chunk[j] * 16u : kOutside;
-    }
-#pragma unroll
-    for (int j = 0; j < NB; ++j) {
-        const int row = (wave * NB + j) * 8 + (lane >> 3);
-        w_at[j] = (uint32_t) (channel_of(row) * p.w_bytes) + ((lane & 7) ^ swizzle(row)) * 16u;
+    for (int o = 0; o < 2; ++o) {
+        x_at[o] = (uint32_t) ((lane >> 3) * p.row_bytes + (chunk ^ o) * 16);
+        w_at[o] = (uint32_t) ((lane >> 3) * NT * p.w_bytes + (chunk ^ o) * 16);
     }
     // Scales: 64 rows a wavefront (the last ones again for wavefronts beyond them).
     const int scale_load = min(wave, kRows / 64 - 1);
-    uint32_t scale_at = kOutside;
-    __amdgpu_buffer_rsrc_t sres = xres;
-    if constexpr (kScaled) {
-        const bool of_x = scale_load * 64 < BM;
-        const int pitch = (of_x ? p.row_bytes : p.w_bytes) / 32;
-        const uint8_t * base = of_x ? p.x_scales + row0 * pitch : p.w_scales + (int64_t) col0 * pitch;
-        const int row = scale_load * 64 + lane;
-        if (!of_x) {
-            scale_at = (uint32_t) (channel_of(row - BM) * pitch);
-        } else if (row < rows) {
-            scale_at = (uint32_t) (row * pitch);
-        }
-        sres = __builtin_amdgcn_make_buffer_rsrc((void *) base, 0, (of_x ? rows : BN) * pitch, 0x00020000);
-    }
+    const bool scales_of_x = scale_load * 64 < BM;
+    const int scale_pitch = (scales_of_x ? p.row_bytes : p.w_bytes) / 32;
+    const int scale_row = scale_load * 64 + lane;
+    const uint32_t scale_at = (uint32_t) ((scales_of_x ? scale_row : channel_of(scale_row - BM)) * scale_pitch);
 
-    // This split's steps.
+    // This split's steps; and the tile to load, as buffers.  Rows past the last,
+    // and all after the last tile, are beyond them: zeros.
     const int all = p.w_bytes / 128;
-    const int first_step = kMaySplit ? (int) ((int64_t) all * split / p.splits) : 0;
-    const int steps = kMaySplit ? (int) ((int64_t) all * (split + 1) / p.splits) : all;
-    // Past the last step loads fetch zeros; what follows a row of x is the next one.
-    const auto load = [&](int s, uint32_t slot, int j) {
-        if (j < NA) {
-            dma_b128(xres, slot + (wave * NA + j) * 1024u,
-                     (!kMaySplit || s < steps) && s * 128 + x_chunk[j] * 16 < p.row_bytes ? x_at[j] : kOutside, s * 128u);
-        } else {
-            dma_b128(wres, slot + BM * 128 + (wave * NB + j - NA) * 1024u, s < steps ? w_at[j - NA] : kOutside, s * 128u);
+    const int first_step = kMaySplit ? scalar((int) ((int64_t) all * split / p.splits)) : 0;
+    const int steps = kMaySplit ? scalar((int) ((int64_t) all * (split + 1) / p.splits)) : all;
+    __amdgpu_buffer_rsrc_t xres, wres, sres;
+    const auto aim = [&](int u, bool some) {
+        const int64_t r0 = row_of(u);
+        const int c0 = col_of(u), rows = (int) min((int64_t) BM, p.n - r0);
+        xres = __builtin_amdgcn_make_buffer_rsrc((void *) ((const char *) p.x + r0 * p.row_bytes), 0,
+                                                 some ? rows * p.row_bytes : 0, 0x00020000);
+        wres = __builtin_amdgcn_make_buffer_rsrc((void *) ((const char *) p.w + (int64_t) c0 * p.w_bytes), 0,
+                                                 some ? BN * p.w_bytes : 0, 0x00020000);
+        if constexpr (kScaled) {
+            const uint8_t * base = scales_of_x ? p.x_scales + r0 * scale_pitch : p.w_scales + (int64_t) c0 * scale_pitch;
+            sres = __builtin_amdgcn_make_buffer_rsrc((void *) base, 0, some ? (scales_of_x ? rows : BN) * scale_pitch : 0,
+                                                     0x00020000);
         }
     };
-    const auto load_scales = [&](int s, uint32_t slot) {
-        if constexpr (kScaled) dma_b32(sres, slot + kBytes + scale_load * 256u, s < steps ? scale_at : kOutside, s * 4u);
+    aim(unit, true);
+    // (What follows a row of x in memory is the next one.)
+    const auto load = [&](int step, uint32_t slot, int j) {
+        if (j < NA) {
+            const int g = wave * NA + j, o = NA % 2 == 0 ? j % 2 : g % 2;
+            uint32_t row = (uint32_t) (g * 8 * p.row_bytes);
+            asm volatile("" : "+s"(row));
+            dma_b128_m0(xres, slot + g * 1024u,
+                        step * 128 + (chunk ^ o) * 16 < p.row_bytes ? x_at[o] + row : kOutside, step * 128u);
+        } else {
+            const int g = wave * NB + j - NA, o = NB % 2 == 0 ? (j - NA) % 2 : g % 2;
+            uint32_t row = (uint32_t) (channel_of(g * 8) * p.w_bytes);
+            asm volatile("" : "+s"(row));
+            dma_b128_m0(wres, slot + BM * 128 + g * 1024u, w_at[o] + row, step * 128u);
+        }
+    };
+    const auto load_scales = [&](int step, uint32_t slot) {
+        if constexpr (kScaled) dma_b32(sres, slot + kBytes + scale_load * 256u, scale_at, step * 4u);
     };
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
-        load_scales(first_step + s, slots + s * kSlot);
+        if (first_step + s >= steps) aim(unit, false);
+        const int step = first_step + s < steps ? first_step + s : 0;
+        load_scales(step, slots + s * kSlot);
 #pragma unroll
-        for (int j = 0; j < kPer; ++j) load(first_step + s, slots + s * kSlot, j);
+        for (int j = 0; j < kPer; ++j) load(step, slots + s * kSlot, j);
     }
 
-    const int ch = col0 + (cw * 32 + l32) * NT;  // the lane's first channel
+    // The channels of this lane in a tile begin at its col0 + ch0.
+    const int ch0 = (cw * 32 + l32) * NT;
+    const __amdgpu_buffer_rsrc_t bres = __builtin_amdgcn_make_buffer_rsrc(
+        (void *) p.bias, 0, p.bias != nullptr && (!kMaySplit || p.splits == 1) ? p.co * 4 : 0, 0x00020000);
+    Adjacent<kF32, NT> bias;
+    const auto load_bias = [&](int u) { bias = load_adjacent<kF32, NT>(bres, (uint32_t) ((col_of(u) + ch0) * 4), 0); };
+    load_bias(unit);
     f32x16 acc[RB][NT];
+    const auto begin = [&]() {
 #pragma unroll
-    for (int t = 0; t < NT; ++t) {
-        const float bias = p.bias != nullptr && (!kMaySplit || p.splits == 1) && ch + t < p.co ? p.bias[ch + t] : 0.0f;
+        for (int t = 0; t < NT; ++t)
 #pragma unroll
-        for (int q = 0; q < RB; ++q)
+            for (int q = 0; q < RB; ++q) {
+                float b = bias.h[t];
+                asm volatile("" : "+v"(b));  // else 16 copies of it are made with the load, and wait in memory
 #pragma unroll
-            for (int i = 0; i < 16; ++i) acc[q][t][i] = bias;
-    }
+                for (int i = 0; i < 16; ++i) acc[q][t][i] = b;
+            }
+    };
+    begin();
 
     Frag fa[2][RB], fb[2][NT];
     int sa[RB], sb[NT];
@@ -295,7 +315,7 @@ __global__ void __launch_bounds__(64 * RW * CW, RW * CW * PER_CU / 4) k_linear_a
     };
     // The products of half h; between one tile and the next a fragment of the
     // other half is read from `from`, and in the second half a load is issued.
-    const auto products = [&](auto h_c, uint32_t from, int s, uint32_t to) {
+    const auto products = [&](auto h_c, uint32_t from, int step, uint32_t to) {
         constexpr int H = decltype(h_c)::value, READS = RB + NT, TILES = RB * NT;
 #pragma unroll
         for (int k = 0; k < TILES; ++k) {
@@ -308,9 +328,9 @@ __global__ void __launch_bounds__(64 * RW * CW, RW * CW * PER_CU / 4) k_linear_a
                 }
             }
             if constexpr (H == 1) {
-                if (k == 0) load_scales(s, slots + to);
+                if (k == 0) load_scales(step, slots + to);
 #pragma unroll
-                for (int j = kPer * k / TILES; j < kPer * (k + 1) / TILES; ++j) load(s, slots + to, j);
+                for (int j = kPer * k / TILES; j < kPer * (k + 1) / TILES; ++j) load(step, slots + to, j);
             }
             const int q = k / NT, t = k % NT;
             acc[q][t] = mac<MT, 2 * H>(fa[H][q], fb[H][t], acc[q][t], kScaled ? sa[q] : 0, kScaled ? sb[t] : 0);
@@ -318,86 +338,120 @@ __global__ void __launch_bounds__(64 * RW * CW, RW * CW * PER_CU / 4) k_linear_a
         }
     };
 
-    wait_vmcnt<0>();
-    lds_barrier();
-    read_scales(0);
-#pragma unroll
-    for (int q = 0; q < RB; ++q) read_a(0, 0, q);
-#pragma unroll
-    for (int t = 0; t < NT; ++t) read_b(0, 0, t);
-    uint32_t here = 0, there = kSlot;
-    using std::integral_constant;
-    for (int s = first_step; s < steps; ++s) {
-        products(integral_constant<int, 0>(), here, 0, 0);
-        // Step s + 1 has landed, and every wavefront has read all of step s.
-        wait_vmcnt<0>();
-        lds_barrier();
-        __builtin_amdgcn_sched_barrier(0);
-        products(integral_constant<int, 1>(), there, s + 2, here);
-        read_scales(there);
-        const uint32_t swap = here;
-        here = there;
-        there = swap;
-    }
-    wait_vmcnt<0>();
-
     // Lane (l32, half) holds rows 8 (i / 4) + 4 half + i % 4 of each row block.
     // Buffer offsets: the lane's place, and the row's in a scalar; rows past
     // the last and channels past co (a multiple of NT) fall outside.
-    const int pitch = p.co * (int) sizeof(T);
-    const __amdgpu_buffer_rsrc_t yres =
-        __builtin_amdgcn_make_buffer_rsrc((char *) p.y + row0 * pitch, 0, rows * pitch, 0x00020000);
-    const __amdgpu_buffer_rsrc_t rres = __builtin_amdgcn_make_buffer_rsrc(
-        (char *) (p.residual != nullptr ? p.residual : p.y) + row0 * pitch, 0, rows * pitch, 0x00020000);
-    const uint32_t at =
-        ch < p.co ? (uint32_t) ((rw * RB * 32 + 4 * half) * pitch + ch * (int) sizeof(T)) : kOutside;
-    const auto finish = [&](auto act_c, auto res_c) {
+    const auto leave = [&](int u) {
+        const int64_t row0 = row_of(u);
+        const int rows = (int) min((int64_t) BM, p.n - row0), ch = col_of(u) + ch0;
+        if constexpr (kMaySplit) if (p.splits > 1) {
+            // The sums of this split, as they are.
+            const __amdgpu_buffer_rsrc_t pres = __builtin_amdgcn_make_buffer_rsrc(
+                p.partial + ((int64_t) split * p.n + row0) * p.co, 0, rows * p.co * 4, 0x00020000);
+            const uint32_t to = ch < p.co ? (uint32_t) (((rw * RB * 32 + 4 * half) * p.co + ch) * 4) : kOutside;
 #pragma unroll
-        for (int q = 0; q < RB; ++q)
+            for (int q = 0; q < RB; ++q)
 #pragma unroll
-            for (int g = 0; g < 4; ++g) {
-                float r[4][NT];
-                if constexpr (decltype(res_c)::value) {
+                for (int i = 0; i < 16; ++i) {
+                    float v[NT];
 #pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        load_adjacent<DT, NT>(rres, at, (uint32_t) ((q * 32 + g * 8 + i) * pitch), r[i]);
+                    for (int t = 0; t < NT; ++t) v[t] = acc[q][t][i];
+                    store_adjacent<kF32, NT>(pres, to, (uint32_t) ((q * 32 + i / 4 * 8 + i % 4) * p.co * 4), v);
                 }
+            return;
+        }
+        const int pitch = p.co * (int) sizeof(T);
+        const __amdgpu_buffer_rsrc_t yres =
+            __builtin_amdgcn_make_buffer_rsrc((char *) p.y + row0 * pitch, 0, rows * pitch, 0x00020000);
+        const __amdgpu_buffer_rsrc_t rres = __builtin_amdgcn_make_buffer_rsrc(
+            (char *) (p.residual != nullptr ? p.residual : p.y) + row0 * pitch, 0, rows * pitch, 0x00020000);
+        const uint32_t at =
+            ch < p.co ? (uint32_t) ((rw * RB * 32 + 4 * half) * pitch + ch * (int) sizeof(T)) : kOutside;
+        const auto finish = [&](auto act_c, auto res_c) {
+            // Four rows at a time, the next four's residuals on their way.
+            constexpr bool kRes = decltype(res_c)::value;
+            Adjacent<DT, NT> r[2][4];
+            const auto fetch = [&](int k) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if constexpr (kRes)
+                        r[k % 2][i] = load_adjacent<DT, NT>(rres, at, (uint32_t) ((k / 4 * 32 + k % 4 * 8 + i) * pitch));
+            };
+            fetch(0);
+#pragma unroll
+            for (int k = 0; k < 4 * RB; ++k) {
+                if (k + 1 < 4 * RB) fetch(k + 1);
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     float v[NT];
 #pragma unroll
                     for (int t = 0; t < NT; ++t) {
-                        v[t] = activate<DT, decltype(act_c)::value>(acc[q][t][4 * g + i]);
-                        if constexpr (decltype(res_c)::value) v[t] += r[i][t];
+                        v[t] = activate<DT, decltype(act_c)::value>(acc[k / 4][t][4 * (k % 4) + i]);
+                        if constexpr (kRes) v[t] += Store<DT>::ld(r[k % 2][i].h, t);
                     }
-                    store_adjacent<DT, NT>(yres, at, (uint32_t) ((q * 32 + g * 8 + i) * pitch), v);
+                    store_adjacent<DT, NT>(yres, at, (uint32_t) ((k / 4 * 32 + k % 4 * 8 + i) * pitch), v);
                 }
                 __builtin_amdgcn_sched_barrier(0);
             }
-    };
-    if constexpr (kMaySplit) if (p.splits > 1) {
-        // The sums of this split, as they are.
-        const __amdgpu_buffer_rsrc_t pres = __builtin_amdgcn_make_buffer_rsrc(
-            p.partial + ((int64_t) split * p.n + row0) * p.co, 0, rows * p.co * 4, 0x00020000);
-        const uint32_t to = ch < p.co ? (uint32_t) (((rw * RB * 32 + 4 * half) * p.co + ch) * 4) : kOutside;
-#pragma unroll
-        for (int q = 0; q < RB; ++q)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                float v[NT];
-#pragma unroll
-                for (int t = 0; t < NT; ++t) v[t] = acc[q][t][i];
-                store_adjacent<kF32, NT>(pres, to, (uint32_t) ((q * 32 + i / 4 * 8 + i % 4) * p.co * 4), v);
+        };
+        by_act(p.act, [&](auto act_c) {
+            if (p.residual != nullptr) {
+                finish(act_c, std::true_type());
+            } else {
+                finish(act_c, std::false_type());
             }
-        return;
-    }
-    by_act(p.act, [&](auto act_c) {
-        if (p.residual != nullptr) {
-            finish(act_c, std::true_type());
-        } else {
-            finish(act_c, std::false_type());
+        });
+    };
+
+    const auto first_half = [&](uint32_t slot) {
+        read_scales(slot);
+#pragma unroll
+        for (int q = 0; q < RB; ++q) read_a(0, slot, q);
+#pragma unroll
+        for (int t = 0; t < NT; ++t) read_b(0, slot, t);
+    };
+    wait_vmcnt<0>();
+    lds_barrier();
+    first_half(0);
+    uint32_t here = 0, there = kSlot;
+    using std::integral_constant;
+    // Up to the step before the last two of a tile the loads are of its own
+    // steps; those of the last two are of the next tile's first two (a block with
+    // several tiles has at least two steps), which then arrive while it leaves.
+    int s = first_step, stop = max(first_step, steps - 2), load_step = first_step + 2, more = 1;
+    for (;;) {
+        for (; s < stop; ++s) {
+            products(integral_constant<int, 0>(), here, 0, 0);
+            // Step s + 1 (or the next tile's first) has landed, and every wavefront has read all of step s.
+            wait_vmcnt<0>();
+            lds_barrier();
+            __builtin_amdgcn_sched_barrier(0);
+            products(integral_constant<int, 1>(), there, scalar(load_step), here);
+            read_scales(there);
+            load_step += more;
+            const uint32_t swap = here;
+            here = there;
+            there = swap;
         }
-    });
+        if (stop < steps) {
+            stop = steps;
+            more = unit + stride < end ? 1 : 0;
+            aim(more ? unit + stride : unit, more);
+            load_step = more ? first_step : 0;
+            continue;
+        }
+        const int u = unit;
+        unit += stride;
+        if (unit < end) load_bias(unit);
+        leave(u);
+        if (unit >= end) break;
+        s = first_step;
+        stop = steps - 2;
+        load_step = first_step + 2;
+        begin();
+        first_half(here);  // again, as the registers were of use for the outputs
+    }
+    wait_vmcnt<0>();
 }
 
 // Joins the splits' sums in their order, then bias, activation and residual: N
@@ -564,7 +618,11 @@ hipError_t launch_shape(LinearAct p, const Blocks & b, hipStream_t s) {
     const int64_t grid = p.row_tiles * p.col_tiles;
     if (grid * p.splits > 0x7fffffffLL) return hipErrorInvalidValue;
     p.split_blocks = (int) grid;
-    k_linear_act<MT, DT, RW, CW, RB, NT, PER_CU><<<(unsigned) (grid * p.splits), 64 * RW * CW, 0, s>>>(p);
+    p.blocks = (int) grid;
+    // More tiles than fit at once: blocks that stay, each with several of them.
+    const int64_t fit = (int64_t) p.cus / 8 * 8 * PER_CU;
+    if (p.splits == 1 && p.w_bytes >= 256 && fit > 0 && grid > fit) p.blocks = (int) fit;
+    k_linear_act<MT, DT, RW, CW, RB, NT, PER_CU><<<(unsigned) (p.blocks * (int64_t) p.splits), 64 * RW * CW, 0, s>>>(p);
     hipError_t err = hipGetLastError();
     if (err == hipSuccess && p.splits > 1) {
         const bool four = p.co % 4 == 0;

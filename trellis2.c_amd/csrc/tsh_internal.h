@@ -390,7 +390,8 @@ struct LinearAct {
     float * partial;         // [splits][rows][co] sums of a part's splits, or null
     int splits;              // set by the launcher, as are:
     int64_t row_tiles;
-    int col_tiles, split_blocks;
+    int col_tiles, split_blocks, blocks;  // split_blocks: the tiles
+    int cus;                              // compute units of the device
 };
 // How a linear is run: parts of its rows one after the other, each with a block
 // shape and its K in splits (for which the scratch memory is; without it they are
