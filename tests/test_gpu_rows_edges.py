@@ -52,6 +52,24 @@ def test_linear_act_ends_at_its_rows(backends, dtype, n, ci, co, from8):
     assert np.array_equal(rows(), be.download(plain).reshape(n, co))
 
 
+@pytest.mark.parametrize("act", list(sh.ACTS))
+@pytest.mark.parametrize("residual", [False, True])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_linear_act_of_the_largest_blocks(backends, dtype, act, residual):
+    """51 x 4 tiles of 256 x 256, whose outputs are computed while earlier ones are stored; many tiles a block too."""
+    be, rng = backends[dtype], np.random.default_rng(3)
+    for n, ci, co in ((13056, 200, 1024), (40000, 96, 1024)):
+        x, r, w = make(rng, dtype, n, ci), make(rng, dtype, n, co), (rng.standard_normal((co, ci)) / 14).astype(np.float32)
+        b = rng.standard_normal(co).astype(np.float32)
+        y = be.alloc(n * co)
+        be.linear_act(be.upload(x), w, b, y, n, ci, co, act=act, residual=be.upload(r) if residual else None)
+        got = be.download(y).reshape(n, co)
+        rows = np.concatenate([np.arange(300), rng.integers(0, n, 300), np.arange(n - 300, n)])
+        exp, err = ref.linear_act(x[rows].astype(np.float64), sh.storage_round(w, dtype).astype(np.float64),
+                                  b.astype(np.float64), act, r[rows].astype(np.float64) if residual else None)
+        ref.check(got[rows], exp, err + ref.stored(exp, dtype), f"{n} {act}")
+
+
 @pytest.mark.parametrize("n,c", [(1, 64), (33, 100), (7, 512), (130, 1024), (5, 4100)])
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_norm_and_expansion_end_at_their_rows(backends, dtype, n, c):

@@ -77,7 +77,10 @@ __device__ __forceinline__ void store_adjacent(__amdgpu_buffer_rsrc_t rsrc, uint
     if constexpr (B == 2) __builtin_amdgcn_raw_buffer_store_b16(w.b2, rsrc, (int) voff, (int) soff, 0);
     if constexpr (B == 4) __builtin_amdgcn_raw_buffer_store_b32(w.b4, rsrc, (int) voff, (int) soff, 0);
     if constexpr (B == 8) __builtin_amdgcn_raw_buffer_store_b64(w.b8, rsrc, (int) voff, (int) soff, 0);
-    if constexpr (B == 16) __builtin_amdgcn_raw_buffer_store_b128(w.b16, rsrc, (int) voff, (int) soff, 0);
+    // 16 bytes: no scalar offset.  With one, the compiler leaves out the wait
+    // before the data's registers are written again, and lanes 12-15 and 28-31 of
+    // a half have stored values that were written after the store (measured).
+    if constexpr (B == 16) __builtin_amdgcn_raw_buffer_store_b128(w.b16, rsrc, (int) (voff + soff), 0, 0);
 }
 
 // ---- MFMA GEMM ----------------------------------------------------------------------------------
@@ -559,19 +562,21 @@ template <int DT> __global__ void __launch_bounds__(256) k_linear_act_any(Linear
 // Block shapes: rows, channels, adjacent channels per lane (which divide co),
 // blocks per CU, and what a step of 128 bytes and the rest of a block take with
 // all CUs busy, in us (measured on whole rounds of blocks, 1,024 channels, K of 4
-// and of 32 steps).
+// and of 32 steps, four rounds of 16 or 8 bits and two of fp32; the first loads and
+// the last outputs of all, kOnce, are not in it).
 struct Blocks {
     int rows, channels, adjacent, per_cu;
     float step16, step8, step32, rest, rest32;
 };
 constexpr Blocks kBlocks[] = {
-    {256, 256, 4, 1, 1.77f, 2.05f, 7.1f, 5.4f, 16.0f},
-    {192, 256, 2, 1, 1.50f, 1.80f, 5.4f, 3.7f, 12.5f},
-    {128, 128, 2, 2, 1.25f, 1.55f, 3.8f, 2.1f, 7.8f},
-    {64, 128, 2, 3, 1.15f, 1.53f, 3.0f, 2.0f, 5.4f},
-    {128, 128, 1, 2, 1.26f, 1.67f, 3.8f, 2.6f, 7.3f},
-    {64, 64, 1, 4, 0.80f, 1.26f, 2.2f, 2.5f, 4.4f},
+    {256, 256, 4, 1, 1.78f, 2.10f, 7.1f, 4.2f, 13.7f},
+    {192, 256, 2, 1, 1.52f, 1.75f, 5.4f, 2.7f, 12.0f},
+    {128, 128, 2, 2, 1.27f, 1.58f, 3.85f, 1.1f, 7.3f},
+    {64, 128, 2, 3, 1.20f, 1.57f, 3.1f, 0.9f, 5.5f},
+    {128, 128, 1, 2, 1.31f, 1.70f, 3.9f, 1.8f, 7.5f},
+    {64, 64, 1, 4, 0.88f, 1.24f, 2.3f, 1.6f, 4.7f},
 };
+constexpr double kOnce = 1.5;
 constexpr int kShapes = sizeof(kBlocks) / sizeof(kBlocks[0]);
 
 inline float step_us(const Blocks & b, int mt) { return mt == kF32 ? b.step32 : (mt == kRows8 ? b.step8 : b.step16); }
@@ -597,7 +602,7 @@ Choice choose(int mt, int64_t n, int co, int w_bytes, int cus, bool may_split) {
             // A last round of few blocks leaves each more of its CU where several share one.
             const double last = rounds - whole;
             const double tail = last == 0.0 ? 0.0 : (b.per_cu == 1 || whole > 0 ? 1.0 : 0.6 + 0.4 * last);
-            double us = (whole + tail) * ((steps + s - 1) / s * step + rest);
+            double us = kOnce + (whole + tail) * ((steps + s - 1) / s * step + rest);
             if (s > 1) us += 4.0 + (double) s * n * co * 8.0 / 4.5e6;
             if (best.shape < 0 || us < best.us) {
                 best.shape = i;
@@ -708,7 +713,7 @@ LinearActPlan linear_act_plan(int dtype, int x_type, int64_t n, int co, int row_
         if (rounds < 1 || rows <= 0 || rows >= n) continue;
         const Choice rest = choose(mt, n - rows, co, w_bytes, cus, may_split);
         const double block = w_bytes / 128 * step_us(b, mt) + (mt == kF32 ? b.rest32 : b.rest);
-        const float us = (float) (rounds * block) + rest.us + 3.0f;
+        const float us = (float) (kOnce + rounds * block) + rest.us + 3.0f;
         if (us >= least) continue;
         least = us;
         plan.parts = 2;
