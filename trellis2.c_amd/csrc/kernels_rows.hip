@@ -335,9 +335,10 @@ hipError_t norm_dt(const void * x, const void * residual, const float * gamma, v
 // is 5,215 turns, of which 32 bits keep 2^-12).  A block turns RB rows: sine and
 // cosine of a row's pairs are computed once, into LDS, and used by all of its
 // heads; then lanes of 4 pairs (two 8-byte or one 16-byte load) take one head
-// each over all rows, gamma in registers.  Bound by memory: 79,523 rows, q and k of 8
-// heads of 64, bf16 with norm 75 us, 4.4 TB/s (a copy of the size 5.3; the sines come before
-// a block's rows and leave its loads idle meanwhile); 997 rows of 6 x 48 in fp32 4 us.
+// each over all rows, gamma in registers, two items ahead of the one in hand (one:
+// 79 us).  Bound by memory: 79,523 rows, q and k of 8 heads of 64 in a buffer of q, k
+// and v, bf16 with norm 72 us, 4.5 TB/s (a copy of the size 5.3); packed fp32 rows of 8
+// heads 66 us, 4.9 TB/s; 997 rows of 6 x 48 in fp32 4 us.
 struct RotaryShape {
     int64_t n, x_stride, y_stride;
     int heads, dim, total;  // total: turned pairs
@@ -368,22 +369,24 @@ __global__ void __launch_bounds__(256) k_rotary(const typename Store<DT>::T * x,
     const bool on = l < lanes && ri < step;
     // A lane's two runs of four channels, and its first pair.
     const int a_at = SPLIT ? 4 * l : 8 * l, b_at = SPLIT ? half + 4 * l : 8 * l + 4, pair = 4 * l;
-    // Two runs as they are in memory; the next item's are on their way while one is turned.
+    // Two runs as they are in memory; the next two items' are on their way while one is turned.
     using Run = typename std::conditional<DT == kF32, int4, int2>::type;
-    Run na{}, nb{};
-    const auto fetch = [&](int h, int r) {
+    struct Item {
+        Run a, b;
+    } next[2];
+    const auto fetch = [&](Item & to, int h, int r) {
+        to = Item{};
         if (!on || h >= p.heads || r >= rows) return;
         const T * xr = x + (row0 + r) * p.x_stride + (int64_t) h * p.dim;
         if constexpr (DT != kF32 && !SPLIT) {
             const int4 c = *(const int4 *) (xr + a_at);
-            na = int2{c.x, c.y};
-            nb = int2{c.z, c.w};
+            to = Item{int2{c.x, c.y}, int2{c.z, c.w}};
         } else {
-            na = *(const Run *) (xr + a_at);
-            nb = *(const Run *) (xr + b_at);
+            to = Item{*(const Run *) (xr + a_at), *(const Run *) (xr + b_at)};
         }
     };
-    fetch(hi, ri);
+    fetch(next[0], hi, ri);
+    fetch(next[1], hi, ri + step);
     for (int i = threadIdx.x; i < rows * half; i += 256) {
         const int r = i / half, j = i % half;
         float sn = 0.0f, cs = 1.0f;
@@ -403,21 +406,16 @@ __global__ void __launch_bounds__(256) k_rotary(const typename Store<DT>::T * x,
             for (int u = 0; u < 8; ++u)
                 g[u] = on && gamma != nullptr ? gamma[(int64_t) h * p.dim + (u < 4 ? a_at + u : b_at + u - 4)] : 1.0f;
         }
-        for (int r = ri; r < rows; r += step) {
-            float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-            if (on) {
-                if constexpr (DT == kF32) {
-                    unpack_chunk_of<DT>(na, v);
-                    unpack_chunk_of<DT>(nb, v + 4);
-                } else {
-                    unpack_chunk<DT>(int4{na.x, na.y, nb.x, nb.y}, v);
-                }
-            }
-            if (r + step < rows) {
-                fetch(h, r + step);
+        const auto turn = [&](Item & item, int r) {
+            if (r >= rows) return;
+            float v[8];
+            if constexpr (DT == kF32) {
+                unpack_chunk_of<DT>(item.a, v);
+                unpack_chunk_of<DT>(item.b, v + 4);
             } else {
-                fetch(h + heads, ri);
+                unpack_chunk<DT>(int4{item.a.x, item.a.y, item.b.x, item.b.y}, v);
             }
+            fetch(item, h, r + 2 * step);
             if constexpr (NORM) {
                 float sum = 0.0f;
 #pragma unroll
@@ -450,7 +448,13 @@ __global__ void __launch_bounds__(256) k_rotary(const typename Store<DT>::T * x,
                     }
                 }
             }
+        };
+        for (int r = ri; r < rows; r += 2 * step) {
+            turn(next[0], r);
+            turn(next[1], r + step);
         }
+        fetch(next[0], h + heads, ri);
+        fetch(next[1], h + heads, ri + step);
     }
 }
 
