@@ -166,6 +166,26 @@ LINEAR_SHAPES = [(1, 1, 1), (1, 1024, 4096), (2, 7, 5), (3, 64, 128), (63, 40, 1
                  (257, 136, 300), (300, 1000, 200), (17, 4096, 64), (1000, 72, 1000), (5003, 512, 256)]
 
 
+@pytest.mark.parametrize("dtype", [sh.F16, sh.BF16])
+@pytest.mark.parametrize("c", [64, 512, 1000, 1024])
+def test_rms_norm_to_rows8_codes(backends, dtype, c):
+    """Codes are those of the 64-bit norm.  The sum of squares carries 8 squares' fp32 roundings, 3 E of the sum at most, and
+    half of it reaches the inverse: 1.5 E, and the two floats' products 2^-45.  A code differs only where a border lies
+    between: of 8 borders an octave (uniform values within it) that is 8 x 2 x 1.5 E / ln 2 of the values at most, twice
+    for e4m3's coarser steps near zero; 8 standard deviations of that count beside it.  (x + r is exact in fp32 unless one is
+    2^13 times the other, which is rarer.)"""
+    be, rng, n = backends[dtype], np.random.default_rng(c), 2_000_000 // c
+    x, r, g = make(rng, dtype, n, c), make(rng, dtype, n, c), (1 + 0.1 * rng.standard_normal(c)).astype(np.float32)
+    q, y = be.alloc_rows8(n, c), be.alloc(n * c)
+    be.rms_norm(be.upload(x), g, q, n, c, 1e-6, residual=be.upload(r))
+    be.expand_rows8(q, y, n, c)
+    exp = ref.rows8(ref.rms_norm(x.astype(np.float64) + r, g.astype(np.float64), 1e-6))
+    if dtype == sh.F16:
+        exp = exp.astype(np.float16).astype(np.float64)  # the smallest codes are below fp16's normal numbers
+    most = n * c * 2 * 8 * 2 * 1.5 * ref.E / math.log(2)
+    assert (be.download(y).reshape(n, c) != exp).sum() <= most + 8 * math.sqrt(most)
+
+
 def linear_case(be, dtype, n, ci, co, act, bias, residual, from8=False):
     rng = np.random.default_rng(n + 3 * ci + 7 * co)
     x, r = make(rng, dtype, n, ci), make(rng, dtype, n, co)

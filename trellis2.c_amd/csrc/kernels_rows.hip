@@ -30,8 +30,6 @@ template <int DT> __device__ __forceinline__ void store_chunk(typename Store<DT>
     }
 }
 
-__device__ __forceinline__ float wave_sum(float v) { return group_sum<64>(v); }
-
 // ---- 8-bit rows ---------------------------------------------------------------------------------
 
 // A block of 32 channels has one scale 2^e, e >= -126 the least with
@@ -67,15 +65,18 @@ __device__ __forceinline__ uint32_t abs_bits(float v) { return __builtin_bit_cas
 
 // 1 / sqrt(sum / c + eps), for 8-bit outputs as two floats from 64 bits: there a
 // value on the other side of a code's border is off by a whole code, so the last
-// bit of the norm counts (a value then carries two roundings less than in fp32,
-// at three more operations).
+// bit of the norm counts.  The sum joins 8 squares at a time in 64 bits, and a
+// value is not rounded to nearest before it is rounded to its code, but cut and
+// made odd where something was cut (twice to nearest had 10 of 12 M codes beside the
+// exact ones, so 2).
 struct Inverse {
     float hi, lo;
 };
-template <bool FINE> __device__ __forceinline__ Inverse inverse_rms(float sum, int c, float eps) {
+template <bool FINE> using NormSum = typename std::conditional<FINE, double, float>::type;
+template <bool FINE> __device__ __forceinline__ Inverse inverse_rms(NormSum<FINE> sum, int c, double per_c, float eps) {
     if constexpr (FINE) {
         // The hardware's estimate and one Newton step in 64 bits (1e-13).
-        const double m = (double) sum / (double) c + (double) eps;
+        const double m = sum * per_c + (double) eps;  // (per_c: 1 / c)
         const double y = (double) __builtin_amdgcn_rsqf((float) m);
         double d = fma(0.5 * y, fma(-m * y, y, 1.0), y);
         if (!(m > 1e-30 && m < 1e38)) d = 1.0 / sqrt(m);
@@ -84,12 +85,18 @@ template <bool FINE> __device__ __forceinline__ Inverse inverse_rms(float sum, i
     }
     return {1.0f / sqrtf(sum / (float) c + eps), 0.0f};
 }
-// v * inv * g, rounded about once where FINE.
+// v * inv * g; where FINE to odd: what a later rounding to fewer bits sees is the exact value's side.
 template <bool FINE> __device__ __forceinline__ float scaled(float v, const Inverse & inv, float g) {
     if constexpr (FINE) {
         const float p = v * g;
         const float low = fmaf(fmaf(v, g, -p), inv.hi, p * inv.lo);
-        return fmaf(p, inv.hi, low);
+        const float h = fmaf(p, inv.hi, low);
+        const float rest = fmaf(p, inv.hi, -h) + low;
+        const uint32_t b = __builtin_bit_cast(uint32_t, h);
+        // Nearest went past the value: one step back towards zero.
+        const uint32_t past = (__builtin_bit_cast(uint32_t, rest) ^ b) >> 31;
+        constexpr int kNonzeroFinite = 0x198;
+        return __builtin_amdgcn_classf(rest, kNonzeroFinite) ? __builtin_bit_cast(float, (b - past) | 1u) : h;
     }
     return v * inv.hi * g;
 }
@@ -127,6 +134,7 @@ __global__ void __launch_bounds__(256) k_norm_vec(const typename Store<DT>::T * 
             const int at = (i * LPR + l) * V + u;
             g[i][u] = NORM && gamma != nullptr && at < c ? gamma[at] : 1.0f;
         }
+    const double per_c = 1.0 / c;
     // The next row's loads run under this one's sums and stores.
     int4 xc[CPL], rc[CPL];
     const auto fetch = [&](int64_t row) {
@@ -145,7 +153,7 @@ __global__ void __launch_bounds__(256) k_norm_vec(const typename Store<DT>::T * 
     if (row < n) fetch(row);
     for (; row < n; row += stride) {
         float v[CPL][V];
-        float sum = 0.0f;
+        NormSum<Q8> sum = 0;
 #pragma unroll
         for (int i = 0; i < CPL; ++i) {
             unpack_chunk_of<DT>(xc[i], v[i]);
@@ -172,7 +180,7 @@ __global__ void __launch_bounds__(256) k_norm_vec(const typename Store<DT>::T * 
                 for (int u = 0; u < V; ++u) part += v[i][u] * v[i][u];
                 sum += part;
             }
-            const Inverse inv = inverse_rms<Q8>(group_sum<LPR>(sum), c, eps);
+            const Inverse inv = inverse_rms<Q8>(group_sum<LPR>(sum), c, per_c, eps);
 #pragma unroll
             for (int i = 0; i < CPL; ++i)
 #pragma unroll
@@ -182,16 +190,14 @@ __global__ void __launch_bounds__(256) k_norm_vec(const typename Store<DT>::T * 
         for (int i = 0; i < CPL; ++i) {
             const int at = (i * LPR + l) * V;
             if constexpr (Q8) {
-                // The 32 / V lanes of a block are neighbours.
+                // The 32 / V lanes of a block are neighbours; values beyond c are zeros (or NaN, as all of the row).
                 uint32_t m = 0;
 #pragma unroll
-                for (int u = 0; u < V; ++u) m = max(m, at < c ? abs_bits(v[i][u]) : 0u);
+                for (int u = 0; u < V; ++u) m = max(m, abs_bits(v[i][u]));
                 const uint32_t scale = block_scale(group_max<32 / V>(m));
                 const float inv = inverse_scale(scale);
                 if (at < out.cp) {
-                    float z[V];
-#pragma unroll
-                    for (int u = 0; u < V; ++u) z[u] = at < c ? v[i][u] : 0.0f;
+                    const float * z = v[i];
                     uint8_t * p = out.codes + row * out.cp + at;
                     if constexpr (V == 8) {
                         *(uint2 *) p = uint2{codes4(z, inv, scale), codes4(z + 4, inv, scale)};
@@ -225,12 +231,12 @@ __global__ void __launch_bounds__(256) k_norm_any(const typename Store<DT>::T * 
     };
     Inverse inv{1.0f, 0.0f};
     if constexpr (NORM) {
-        float sum = 0.0f;
+        NormSum<Q8> sum = 0;
         for (int i = lane; i < c; i += 64) {
             const float v = at(i);
             sum += v * v;
         }
-        inv = inverse_rms<Q8>(wave_sum(sum), c, eps);
+        inv = inverse_rms<Q8>(group_sum<64>(sum), c, 1.0 / c, eps);
     }
     const int end = Q8 ? out.cp : c;
     for (int i = lane; i < end; i += 64) {
@@ -314,9 +320,16 @@ hipError_t norm_dt(const void * x, const void * residual, const float * gamma, v
     };
     using std::integral_constant;
     if (chunks <= 8) return launch(integral_constant<int, 8>(), integral_constant<int, 1>());
-    if (chunks <= 16) return launch(integral_constant<int, 16>(), integral_constant<int, 1>());
-    if (chunks <= 32) return launch(integral_constant<int, 32>(), integral_constant<int, 1>());
-    if (chunks <= 64) return launch(integral_constant<int, 64>(), integral_constant<int, 1>());
+    if constexpr (Q8) {
+        // The inverse's 64-bit arithmetic counts: two rows a wavefront share it (79,523 rows of 512 in bf16 43 -> 38 us).
+        if (chunks <= 16) return launch(integral_constant<int, 8>(), integral_constant<int, 2>());
+        if (chunks <= 32) return launch(integral_constant<int, 16>(), integral_constant<int, 2>());
+        if (chunks <= 64) return launch(integral_constant<int, 32>(), integral_constant<int, 2>());
+    } else {
+        if (chunks <= 16) return launch(integral_constant<int, 16>(), integral_constant<int, 1>());
+        if (chunks <= 32) return launch(integral_constant<int, 32>(), integral_constant<int, 1>());
+        if (chunks <= 64) return launch(integral_constant<int, 64>(), integral_constant<int, 1>());
+    }
     if (chunks <= 128) return launch(integral_constant<int, 64>(), integral_constant<int, 2>());
     if (chunks <= 256) return launch(integral_constant<int, 64>(), integral_constant<int, 4>());
     return launch(integral_constant<int, 64>(), integral_constant<int, 8>());
