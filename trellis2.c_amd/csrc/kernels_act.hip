@@ -210,8 +210,17 @@ __global__ void __launch_bounds__(64 * RW * CW, RW * CW * PER_CU / 4) k_linear_a
         end = (int) ((int64_t) p.split_blocks * (xcd + 1) / 8);
         if (unit >= end) return;
     }
-    const auto row_of = [&](int u) { return (int64_t) scalar(u / p.col_tiles) * BM; };
-    const auto col_of = [&](int u) { return scalar(u % p.col_tiles) * BN; };
+    // This tile's first row and channel, and those of the one to load.
+    int64_t row0, next_row0;
+    int col0, next_col0;
+    const auto place = [&](int u) {
+        const int r = scalar(u / p.col_tiles);
+        next_row0 = (int64_t) r * BM;
+        next_col0 = (u - r * p.col_tiles) * BN;
+    };
+    place(unit);
+    row0 = next_row0;
+    col0 = next_col0;
 
     const uint32_t slots = (uint32_t) (uintptr_t) (__attribute__((address_space(3))) unsigned char *) s_slot;
 
@@ -238,23 +247,23 @@ __global__ void __launch_bounds__(64 * RW * CW, RW * CW * PER_CU / 4) k_linear_a
     // This split's steps; and the tile to load, as buffers.  Rows past the last,
     // and all after the last tile, are beyond them: zeros.
     const int all = p.w_bytes / 128;
-    const int first_step = kMaySplit ? scalar((int) ((int64_t) all * split / p.splits)) : 0;
-    const int steps = kMaySplit ? scalar((int) ((int64_t) all * (split + 1) / p.splits)) : all;
+    const int first_step = kMaySplit ? scalar(all * split / p.splits) : 0;
+    const int steps = kMaySplit ? scalar(all * (split + 1) / p.splits) : all;
     __amdgpu_buffer_rsrc_t xres, wres, sres;
-    const auto aim = [&](int u, bool some) {
-        const int64_t r0 = row_of(u);
-        const int c0 = col_of(u), rows = (int) min((int64_t) BM, p.n - r0);
-        xres = __builtin_amdgcn_make_buffer_rsrc((void *) ((const char *) p.x + r0 * p.row_bytes), 0,
+    const auto aim = [&](bool some) {
+        const int rows = (int) min((int64_t) BM, p.n - next_row0);
+        xres = __builtin_amdgcn_make_buffer_rsrc((void *) ((const char *) p.x + next_row0 * p.row_bytes), 0,
                                                  some ? rows * p.row_bytes : 0, 0x00020000);
-        wres = __builtin_amdgcn_make_buffer_rsrc((void *) ((const char *) p.w + (int64_t) c0 * p.w_bytes), 0,
+        wres = __builtin_amdgcn_make_buffer_rsrc((void *) ((const char *) p.w + (int64_t) next_col0 * p.w_bytes), 0,
                                                  some ? BN * p.w_bytes : 0, 0x00020000);
         if constexpr (kScaled) {
-            const uint8_t * base = scales_of_x ? p.x_scales + r0 * scale_pitch : p.w_scales + (int64_t) c0 * scale_pitch;
+            const uint8_t * base =
+                scales_of_x ? p.x_scales + next_row0 * scale_pitch : p.w_scales + (int64_t) next_col0 * scale_pitch;
             sres = __builtin_amdgcn_make_buffer_rsrc((void *) base, 0, some ? (scales_of_x ? rows : BN) * scale_pitch : 0,
                                                      0x00020000);
         }
     };
-    aim(unit, true);
+    aim(true);
     // (What follows a row of x in memory is the next one.)
     const auto load = [&](int step, uint32_t slot, int j) {
         if (j < NA) {
@@ -275,7 +284,7 @@ __global__ void __launch_bounds__(64 * RW * CW, RW * CW * PER_CU / 4) k_linear_a
     };
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
-        if (first_step + s >= steps) aim(unit, false);
+        if (first_step + s >= steps) aim(false);
         const int step = first_step + s < steps ? first_step + s : 0;
         load_scales(step, slots + s * kSlot);
 #pragma unroll
@@ -287,8 +296,8 @@ __global__ void __launch_bounds__(64 * RW * CW, RW * CW * PER_CU / 4) k_linear_a
     const __amdgpu_buffer_rsrc_t bres = __builtin_amdgcn_make_buffer_rsrc(
         (void *) p.bias, 0, p.bias != nullptr && (!kMaySplit || p.splits == 1) ? p.co * 4 : 0, 0x00020000);
     Adjacent<kF32, NT> bias;
-    const auto load_bias = [&](int u) { bias = load_adjacent<kF32, NT>(bres, (uint32_t) ((col_of(u) + ch0) * 4), 0); };
-    load_bias(unit);
+    const auto load_bias = [&]() { bias = load_adjacent<kF32, NT>(bres, (uint32_t) ((col0 + ch0) * 4), 0); };
+    load_bias();
     f32x16 acc[RB][NT];
     const auto begin = [&]() {
 #pragma unroll
@@ -356,9 +365,8 @@ __global__ void __launch_bounds__(64 * RW * CW, RW * CW * PER_CU / 4) k_linear_a
     // Lane (l32, half) holds rows 8 (i / 4) + 4 half + i % 4 of each row block.
     // Buffer offsets: the lane's place, and the row's in a scalar; rows past
     // the last and channels past co (a multiple of NT) fall outside.
-    const auto leave = [&](int u) {
-        const int64_t row0 = row_of(u);
-        const int rows = (int) min((int64_t) BM, p.n - row0), ch = col_of(u) + ch0;
+    const auto leave = [&](int64_t row0, int col0) {
+        const int rows = (int) min((int64_t) BM, p.n - row0), ch = col0 + ch0;
         if constexpr (kMaySplit) if (p.splits > 1) {
             // The sums of this split, as they are.
             const __amdgpu_buffer_rsrc_t pres = __builtin_amdgcn_make_buffer_rsrc(
@@ -451,14 +459,18 @@ __global__ void __launch_bounds__(64 * RW * CW, RW * CW * PER_CU / 4) k_linear_a
         if (stop < steps) {
             stop = steps;
             more = unit + stride < end ? 1 : 0;
-            aim(more ? unit + stride : unit, more);
+            if (more) place(unit + stride);
+            aim(more);
             load_step = more ? first_step : 0;
             continue;
         }
-        const int u = unit;
+        const int64_t row = row0;
+        const int col = col0;
+        row0 = next_row0;
+        col0 = next_col0;
         unit += stride;
-        if (unit < end) load_bias(unit);
-        leave(u);
+        if (unit < end) load_bias();
+        leave(row, col);
         if (unit >= end) break;
         s = first_step;
         stop = steps - 2;
