@@ -615,10 +615,11 @@ struct Choice {
 // The shape and splits with the least estimated time for n rows.  Of a round that
 // is not full each CU has its share of blocks, which take their part of a full
 // round's time, but not less than kAlone (one block of three or four a CU: 0.33 to
-// 0.45 measured).  Splits pay for their sums' way out and back, which the caches
+// 0.45 measured), nor a step less than its loads' way, kWay (warm 0.5 us, from
+// memory 1).  Splits pay for their sums' way out and back, which the caches
 // hold, and for the join's launch: 5,003 x 300 -> 77 fp32 unsplit 10.7 us, in four 14.1;
 // 1,832 x 4096 -> 1024 bf16 in four 28.
-constexpr double kAlone = 0.4, kJoin = 3.0, kJoinBytesPerUs = 2.4e7;
+constexpr double kAlone = 0.4, kWay = 0.7, kJoin = 3.0, kJoinBytesPerUs = 2.4e7;
 Choice choose(int mt, int64_t n, int co, int w_bytes, int cus, bool may_split) {
     const int steps = w_bytes / 128;
     Choice best;
@@ -631,8 +632,10 @@ Choice choose(int mt, int64_t n, int co, int w_bytes, int cus, bool may_split) {
             if (s > 1 && (s > steps / 2 || i == 0)) break;  // (the largest blocks do not split)
             const double rounds = blocks * s / ((double) cus * b.per_cu), whole = std::floor(rounds);
             const double last = rounds - whole;
-            const double tail = last == 0.0 ? 0.0 : std::max(kAlone, std::ceil(last * b.per_cu) / b.per_cu);
-            double us = kOnce + (whole + tail) * ((steps + s - 1) / s * step + rest);
+            const double tail = std::max(kAlone, std::ceil(last * b.per_cu) / b.per_cu);
+            const int each = (steps + s - 1) / s;
+            double us = kOnce + whole * (each * step + rest);
+            if (last > 0.0) us += each * std::max(tail * step, kWay) + tail * rest;
             if (s > 1) us += kJoin + (double) s * n * co * 8.0 / kJoinBytesPerUs;
             if (best.shape < 0 || us < best.us) {
                 best.shape = i;
