@@ -619,7 +619,7 @@ struct Choice {
 // memory 1).  Splits pay for their sums' way out and back, which the caches
 // hold, and for the join's launch: 5,003 x 300 -> 77 fp32 unsplit 10.7 us, in four 14.1;
 // 1,832 x 4096 -> 1024 bf16 in four 28.
-constexpr double kAlone = 0.4, kWay = 0.7, kJoin = 3.0, kJoinBytesPerUs = 2.4e7;
+constexpr double kAlone = 0.4, kWay = 0.85, kJoin = 3.0, kJoinBytesPerUs = 8e6;
 Choice choose(int mt, int64_t n, int co, int w_bytes, int cus, bool may_split) {
     const int steps = w_bytes / 128;
     Choice best;
