@@ -10,22 +10,42 @@ namespace {
 // ---- activations --------------------------------------------------------------------------------
 
 // For 16-bit outputs the hardware exponential and reciprocal (about 2^-21
-// relative) stay far below the output's rounding; fp32 outputs take the accurate
-// functions.  All are v times a logistic function of v: SiLU of v itself, GELU with
-// tanh of 2 sqrt(2 / pi) (v + 0.044715 v^3), and the normal distribution function
-// of GELU of v R(v^2), R a minimax polynomial of its logit (in log2 units) on
-// [0, 6]: 1.5e-6 off, and six operations less than a rational erf, which count:
-// a 256 x 256 block's GELU takes as long as 1,000 K values of its products.
-constexpr float kG0 = 2.30216527f, kG1 = 0.105008416f, kG2 = -2.55234947e-4f, kG3 = -1.0548038e-4f, kG4 = 4.0871505e-6f;
+// relative) stay far below the output's rounding; fp32 outputs of SiLU and of GELU
+// with tanh take the accurate functions.  Both are v times a logistic function: of v,
+// and of 2 sqrt(2 / pi) (v + 0.044715 v^3).
+//
+// GELU is v Phi(v), and below zero Phi is small beside 1: one minus an erf, or a
+// polynomial that is right to some 1e-6 of 1, loses it.  So Phi(-a) = exp(-a^2 / 2)
+// M(a), a = |v|, where M falls like 1 / a: t Q(t), t = 1 / (1 + p a), Q fitted to the
+// least relative error.  bf16: cubic, 2^-12 down to v = -13.2, below which the
+// exponential is zero.  fp16: cubic, 2^-14.5 down to -4.05, and below that 2^-28
+// or less, an eighth of the output's half step there as well.  fp32: degree 8, 2^-25.2;
+// t, Q, their products and the exponential add some 16 roundings, the exponential's
+// argument 1.5 a^2.
+template <int DT> struct GeluTail {
+    static constexpr int degree = 3;
+    static constexpr float p = DT == kF16 ? 0.28f : 0.3f;
+    static constexpr float q[4] = {DT == kF16 ? 0.0977476385f : 0.118204356f, DT == kF16 ? 0.205788678f : 0.137478365f,
+                                   DT == kF16 ? -0.13003297f : 0.0355873705f, DT == kF16 ? 0.326480256f : 0.208844977f};
+};
+template <> struct GeluTail<kF32> {
+    static constexpr int degree = 8;
+    static constexpr float p = 0.34f;
+    static constexpr float q[9] = {0.135618851f, 0.136142388f, 0.11496748f, 0.116314463f, -0.0470853858f,
+                                   0.205778807f, -0.276415288f, 0.141150713f, -0.0264720283f};
+};
 template <int DT, int ACT> __device__ __forceinline__ float activate(float v) {
     if constexpr (ACT == TRELLIS_SPARSE_HIP_ACT_SILU) {
         if constexpr (DT == kF32) return v / (1.0f + expf(-v));
         return v * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-1.4426950408889634f * v));
     } else if constexpr (ACT == TRELLIS_SPARSE_HIP_ACT_GELU) {
-        if constexpr (DT == kF32) return 0.5f * v * (1.0f + erff(v * 0.70710678118654752f));
-        const float t = v * v;
-        const float r = kG0 + t * (kG1 + t * (kG2 + t * (kG3 + t * kG4)));
-        return v * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-v * r));
+        using G = GeluTail<DT>;
+        const float t = __builtin_amdgcn_rcpf(fmaf(G::p, fabsf(v), 1.0f));
+        float m = G::q[G::degree];
+#pragma unroll
+        for (int i = G::degree - 1; i >= 0; --i) m = fmaf(m, t, G::q[i]);
+        const float tail = m * t * __builtin_amdgcn_exp2f(v * (v * -0.72134752f));
+        return v * (v > 0.0f ? 1.0f - tail : tail);
     } else if constexpr (ACT == TRELLIS_SPARSE_HIP_ACT_GELU_TANH) {
         // (1 + tanh(u)) / 2 = 1 / (1 + exp(-2u))
         const float r = 1.5957691216057308f + 0.0713548162726f * v * v;
