@@ -1,0 +1,49 @@
+"""Scratch that the caller gives: what may not lie in it, and which handle it belongs to."""
+import ctypes
+
+import numpy as np
+import pytest
+
+import sparse_hip as sh
+from test_gpu_rows import make, refused
+
+pytestmark = pytest.mark.gpu
+
+
+def attention_of_offsets(be, q, k, v, y, nq, nk, q_at, k_at, seqs, heads, dim):
+    """The call itself: buffers of offsets may be longer than the sequences need."""
+    d = sh.AttentionDesc(ctypes.sizeof(sh.AttentionDesc), heads, heads, dim)
+    be._check(sh.LIB.trellis_sparse_hip_attention(be.ptr, q.handle, k.handle, v.handle, y.handle, nq, nk, q_at.handle,
+                                                  k_at.handle, seqs, ctypes.byref(d)), "attention")
+
+
+@pytest.mark.parametrize("dtype", [sh.F32, sh.BF16])
+def test_offsets_in_the_scratch(dtype):
+    """Offsets are read while other blocks write the scratch: refused where the call takes it, and the output as it was;
+    fine where it does not, or lies elsewhere."""
+    be, rng, nk = sh.Backend(0, dtype), np.random.default_rng(1), 9000
+    try:
+        q, k, v = (be.upload(make(rng, dtype, m, 128)) for m in (2, nk, nk))
+        at = np.zeros(1 << 20, np.int32)
+        at[:3] = 0, 1, 2
+        kat = at.copy()
+        kat[:3] = 0, 4000, nk
+        qo, ko, small_q, small_k = (be.upload_i32(a) for a in (at, kat, at[:3], kat[:3]))
+        y = be.alloc(2 * 128)
+        attention_of_offsets(be, q, k, v, y, 2, nk, qo, ko, 2, 2, 64)
+        exp = be.download(y)
+        assert 0 < be.scratch_bytes <= 4 * at.size
+        for scratch, a, b in ((qo, qo, small_k), (ko, small_q, ko), (qo, qo, qo)):
+            be.set_scratch(scratch)
+            y = be.upload(np.full(2 * 128, 7, np.float32))
+            refused(sh.INVALID_ARGUMENT, attention_of_offsets, be, q, k, v, y, 2, nk, a, b, 2, 2, 64)
+            assert np.all(be.download(y) == 7)
+        assert np.array_equal(be.download_i32(qo), at) and np.array_equal(be.download_i32(ko), kat)
+        be.set_scratch(small_q)  # too small: the pool's serves
+        attention_of_offsets(be, q, k, v, y, 2, nk, small_q, small_k, 2, 2, 64)
+        assert np.array_equal(be.download(y), exp)
+        be.set_scratch(qo)
+        attention_of_offsets(be, q, k, v, y, 2, nk, small_q, small_k, 2, 2, 64)
+        assert np.array_equal(be.download(y), exp)
+    finally:
+        be.destroy()

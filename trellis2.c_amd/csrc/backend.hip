@@ -2273,7 +2273,7 @@ trellis_status linear_act_impl(trellis_sparse_backend * backend, const trellis_s
 }
 
 // Rows of `width` elements at `offset`, `stride` apart (0: packed), within a
-// float buffer; 16-byte aligned when `aligned`.
+// float buffer.
 bool strided_ok(const Backend * be, const trellis_sparse_buffer * b, int64_t n, int64_t width, int64_t offset,
                 int64_t * stride) {
     if (offset < 0 || *stride < 0 || (*stride != 0 && *stride < width)) return false;
@@ -2286,6 +2286,12 @@ Span strided(const Backend * be, const trellis_sparse_buffer * b, int64_t n, int
              int64_t stride) {
     const int64_t e = (int64_t) dtype_bytes(be->policy.compute_dtype);
     return Span{(const char *) b->ptr + offset * e, n, width * e, stride * e};
+}
+
+// The offsets of n_seqs sequences (none: nullptr).
+Span offset_span(const trellis_sparse_buffer * b, int n_seqs) {
+    if (b == nullptr) return Span{nullptr, 0, 0, 0};
+    return Span{(const char *) b->ptr, (int64_t) n_seqs + 1, 4, 4};
 }
 
 trellis_status rotary_impl(trellis_sparse_backend * backend, const trellis_sparse_buffer * x,
@@ -2385,10 +2391,9 @@ trellis_status attention_impl(trellis_sparse_backend * backend, const trellis_sp
         sk = strided(be, k, nkv, kw, d.k_offset, ks);
         sv = strided(be, v, nkv, kw, d.v_offset, vs);
     }
-    for (const trellis_sparse_buffer * b : {q_offsets, kv_offsets}) {
-        if (b != nullptr && spans_clash(sy, Span{(const char *) b->ptr, n_seqs + 1, 4, 4}, false)) {
-            return fail(be, TRELLIS_STATUS_INVALID_ARGUMENT, "attention: overlapping rows");
-        }
+    const Span sqo = offset_span(q_offsets, n_seqs), sko = offset_span(kv_offsets, n_seqs);
+    if (spans_clash(sy, sqo, false) || spans_clash(sy, sko, false)) {
+        return fail(be, TRELLIS_STATUS_INVALID_ARGUMENT, "attention: overlapping rows");
     }
     // Other blocks still read keys and values where one has written its queries' rows; q itself may be y.
     if (spans_clash(sy, sq, true) || spans_clash(sy, sk, false) || spans_clash(sy, sv, false)) {
@@ -2416,7 +2421,7 @@ trellis_status attention_impl(trellis_sparse_backend * backend, const trellis_sp
     p.scale = (float) (scale * 1.4426950408889634);
     // Without scratch for split keys one block takes all of a query's keys.
     const AttentionShape shape = attention_shape(be->policy.compute_dtype, p, be->cus);
-    if (scratch_clash(be, shape.scratch, {sq, sk, sv, sy})) {
+    if (scratch_clash(be, shape.scratch, {sq, sk, sv, sy, sqo, sko})) {
         return fail(be, TRELLIS_STATUS_INVALID_ARGUMENT, "attention: rows in the scratch");
     }
     DevMem scratch;
