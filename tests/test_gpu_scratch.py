@@ -47,3 +47,37 @@ def test_offsets_in_the_scratch(dtype):
         assert np.array_equal(be.download(y), exp)
     finally:
         be.destroy()
+
+
+def wrap_again(be, buf):
+    """Another buffer over a buffer's memory, as int32 (a buffer's first field is its address)."""
+    h = sh.c_void_p()
+    at = ctypes.cast(buf.handle, ctypes.POINTER(ctypes.c_void_p))[0]
+    be._check(sh.LIB.trellis_sparse_hip_wrap_i32(be.ptr, at, buf.count, ctypes.byref(h)), "wrap")
+    return sh.Buffer(be, h, buf.count)
+
+
+def test_another_buffer_over_the_scratch():
+    """Freeing another buffer over the same memory leaves the scratch set; freeing the buffer that it is unsets it."""
+    be, rng = sh.Backend(0, sh.BF16), np.random.default_rng(2)
+    try:
+        w = make(rng, sh.BF16, 512, 4096)
+        x, y = be.upload(make(rng, sh.BF16, 1, 4096)), be.alloc(512)
+        be.linear_act(x, w, None, y, 1, 4096, 512)
+        exp, need = be.download(y), be.scratch_bytes
+        assert need > 0
+        words = np.full(need // 4, 7, np.int32)
+        memory = be.upload_i32(words)
+        scratch, other = wrap_again(be, memory), wrap_again(be, memory)
+        be.set_scratch(scratch)
+        other.free()
+        be.linear_act(x, w, None, y, 1, 4096, 512)
+        assert np.array_equal(be.download(y), exp) and not np.array_equal(be.download_i32(memory), words)
+        memory = be.upload_i32(words)
+        scratch, other = wrap_again(be, memory), wrap_again(be, memory)
+        be.set_scratch(scratch)
+        scratch.free()
+        be.linear_act(x, w, None, y, 1, 4096, 512)
+        assert np.array_equal(be.download(y), exp) and np.array_equal(be.download_i32(memory), words)
+    finally:
+        be.destroy()

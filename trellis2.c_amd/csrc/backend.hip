@@ -80,8 +80,9 @@ struct Backend {
     hipStream_t stream = nullptr;      // where calls enqueue: own_stream, or the caller's (set_stream)
     hipStream_t own_stream = nullptr;
     hipEvent_t stream_left = nullptr;  // orders a new stream behind the one left (created on first use)
-    // Scratch that the caller gave for split sums (set_scratch), and the most that a call wanted.
+    // Scratch that the caller gave for split sums (set_scratch) and the buffer that it is, and the most that a call wanted.
     void * scratch = nullptr;
+    const trellis_sparse_buffer * scratch_of = nullptr;
     size_t scratch_bytes = 0, scratch_most = 0;
     trellis_sparse_hip_policy policy{};
     std::string last_error;
@@ -740,14 +741,18 @@ trellis_status op_download_f32(trellis_sparse_backend * backend, const trellis_s
     return hip_status(be, err, "download_f32");
 }
 
+void set_scratch(Backend * be, const trellis_sparse_buffer * b) {
+    be->scratch_of = b;
+    be->scratch = b != nullptr ? b->ptr : nullptr;
+    be->scratch_bytes = b != nullptr ? b->bytes : 0;
+}
+
 void op_free_buffer(trellis_sparse_backend * backend, trellis_sparse_buffer * buffer) {
     if (backend == nullptr || buffer == nullptr) return;
     Backend * be = as_backend(backend);
     DevMem m{buffer->ptr, buffer->cap};
-    if (buffer->ptr == be->scratch) {
-        be->scratch = nullptr;
-        be->scratch_bytes = 0;
-    }
+    // (Other buffers may be over the same memory: wrapped ones.)
+    if (buffer == be->scratch_of) set_scratch(be, nullptr);
     if (buffer->cap != 0) dev_release(be, &m);  // a wrapped buffer's memory is the caller's
     free(buffer);
 }
@@ -3089,8 +3094,7 @@ trellis_status trellis_sparse_hip_set_scratch(trellis_sparse_backend * backend, 
     if (scratch != nullptr && (scratch->ptr == nullptr || scratch->dtype == tsh::kRows8)) {
         return tsh::fail(be, TRELLIS_STATUS_INVALID_ARGUMENT, "set_scratch: a buffer of rows or int32");
     }
-    be->scratch = scratch != nullptr ? scratch->ptr : nullptr;
-    be->scratch_bytes = scratch != nullptr ? scratch->bytes : 0;
+    tsh::set_scratch(be, scratch);
     return TRELLIS_STATUS_OK;
 }
 
