@@ -543,7 +543,7 @@ trellis_status trellis_sparse_hip_own_stream(trellis_sparse_backend * backend);
  * another order.  With `scratch` set (NULL: the pool again) such calls use its
  * memory where it is large enough, captured ones too: graphs, streams or backends
  * that may run at the same time need scratch of their own.  It is the caller's, and
- * free_buffer of this very buffer unsets it; rows or offsets in it ->
+ * free_buffer of this very buffer unsets it; rows, coordinates or offsets in it ->
  * INVALID_ARGUMENT.  scratch_bytes: the most that a call has asked for so far. */
 trellis_status trellis_sparse_hip_set_scratch(trellis_sparse_backend * backend, const trellis_sparse_buffer * scratch);
 size_t trellis_sparse_hip_scratch_bytes(const trellis_sparse_backend * backend);

@@ -1,11 +1,13 @@
-"""Scratch that the caller gives: what may not lie in it, and which handle it belongs to."""
+"""Scratch that the caller gives: what may not lie in it, and which buffer it is."""
 import ctypes
 
 import numpy as np
 import pytest
 
+import rows_block
 import sparse_hip as sh
 from test_gpu_rows import make, refused
+from test_gpu_rows_together import block_args
 
 pytestmark = pytest.mark.gpu
 
@@ -79,5 +81,41 @@ def test_another_buffer_over_the_scratch():
         scratch.free()
         be.linear_act(x, w, None, y, 1, 4096, 512)
         assert np.array_equal(be.download(y), exp) and np.array_equal(be.download_i32(memory), words)
+    finally:
+        be.destroy()
+
+
+@pytest.mark.parametrize("dtype", [sh.F32, sh.BF16])
+def test_block_with_rows_in_the_scratch(dtype):
+    """The block's first linear writes its partial sums while h, the coordinates and the offsets are still to be read:
+    none of the block's buffers may be the scratch, and beside it they give what they give without."""
+    be, rng, n = sh.Backend(0, dtype), np.random.default_rng(3), 40
+    try:
+        blk = rows_block.Block(dtype, heads=16, dim=64, hidden=256)
+        coords, at = rows_block.voxels(n, rng)
+        x = sh.storage_round(rng.standard_normal((n, blk.c)).astype(np.float32), dtype)
+        xb, cb, ab, out = be.upload(x), be.upload_i32(coords), be.upload_i32(at), be.alloc(n * blk.c)
+
+        def block(h=xb, coords=cb, offsets=ab, y=out):
+            be.transformer_block(h, coords, y, n, offsets=offsets, **block_args(blk))
+
+        block()
+        exp, need = be.download(out), be.scratch_bytes
+        assert need > 0
+        big = be.alloc(max(need, x.size * 4))
+        big_i32 = be.upload_i32(np.pad(coords.ravel(), (0, need // 4)))
+        be.set_scratch(big)
+        for more in (dict(h=big), dict(y=big), dict(h=big, y=big)):
+            refused(sh.INVALID_ARGUMENT, block, **more)
+        be.set_scratch(big_i32)
+        refused(sh.INVALID_ARGUMENT, block, coords=big_i32)
+        assert np.array_equal(be.download_i32(big_i32)[:4 * n], coords.ravel())
+        be.set_scratch(ab)
+        refused(sh.INVALID_ARGUMENT, block)
+        be.set_scratch(cb)
+        refused(sh.INVALID_ARGUMENT, block)
+        be.set_scratch(big)
+        block()
+        assert np.array_equal(be.download(out), exp)
     finally:
         be.destroy()

@@ -2460,6 +2460,13 @@ trellis_status transformer_block_impl(trellis_sparse_backend * backend, const tr
         return fail(be, TRELLIS_STATUS_INVALID_ARGUMENT, "transformer_block: bad argument");
     }
     const int c = (int) wide;
+    // What the call reads after its first linear may not be where that one's sums go.  (A call's own check is of its rows.)
+    const Span at = coords_map != nullptr ? Span{(const char *) coords_map->coords.ptr, n, 16, 16}
+                    : coords != nullptr   ? Span{(const char *) coords->ptr, n, 16, 16}
+                                          : Span{nullptr, 0, 0, 0};
+    if (scratch_clash(be, be->scratch_bytes, {packed(h, n, c), packed(out, n, c), at, offset_span(offsets, n_seqs)})) {
+        return fail(be, TRELLIS_STATUS_INVALID_ARGUMENT, "transformer_block: rows in the scratch");
+    }
     trellis_sparse_buffer *row = nullptr, *qkv = nullptr, *hid = nullptr, *row8 = nullptr, *hid8 = nullptr;
     trellis_status st = op_alloc_f32(backend, (size_t) n * c, &row);
     if (st == TRELLIS_STATUS_OK) st = op_alloc_f32(backend, (size_t) n * 3 * c, &qkv);
