@@ -2438,6 +2438,16 @@ trellis_status attention_impl(trellis_sparse_backend * backend, const trellis_sp
     return hip_status(be, err, "attention");
 }
 
+// A buffer that goes back to the pool however the call ends.
+struct PoolBuffer {
+    trellis_sparse_backend * backend;
+    trellis_sparse_buffer * b = nullptr;
+    explicit PoolBuffer(trellis_sparse_backend * be) : backend(be) {}
+    ~PoolBuffer() { op_free_buffer(backend, b); }
+    PoolBuffer(const PoolBuffer &) = delete;
+    PoolBuffer & operator=(const PoolBuffer &) = delete;
+};
+
 // A transformer block over voxel rows, from the calls above: each half is a norm,
 // its linears and the residual, added in the last linear's epilogue.
 trellis_status transformer_block_impl(trellis_sparse_backend * backend, const trellis_sparse_buffer * h,
@@ -2467,13 +2477,13 @@ trellis_status transformer_block_impl(trellis_sparse_backend * backend, const tr
     if (scratch_clash(be, be->scratch_bytes, {packed(h, n, c), packed(out, n, c), at, offset_span(offsets, n_seqs)})) {
         return fail(be, TRELLIS_STATUS_INVALID_ARGUMENT, "transformer_block: rows in the scratch");
     }
-    trellis_sparse_buffer *row = nullptr, *qkv = nullptr, *hid = nullptr, *row8 = nullptr, *hid8 = nullptr;
-    trellis_status st = op_alloc_f32(backend, (size_t) n * c, &row);
-    if (st == TRELLIS_STATUS_OK) st = op_alloc_f32(backend, (size_t) n * 3 * c, &qkv);
-    if (st == TRELLIS_STATUS_OK) st = op_alloc_f32(backend, (size_t) n * d.hidden, &hid);
-    if (st == TRELLIS_STATUS_OK && d.rows8) st = alloc_rows8_impl(backend, n, c, &row8);
-    if (st == TRELLIS_STATUS_OK && d.rows8) st = alloc_rows8_impl(backend, n, d.hidden, &hid8);
-    trellis_sparse_buffer * normed = d.rows8 ? row8 : row;
+    PoolBuffer row(backend), qkv(backend), hid(backend), row8(backend), hid8(backend);
+    trellis_status st = op_alloc_f32(backend, (size_t) n * c, &row.b);
+    if (st == TRELLIS_STATUS_OK) st = op_alloc_f32(backend, (size_t) n * 3 * c, &qkv.b);
+    if (st == TRELLIS_STATUS_OK) st = op_alloc_f32(backend, (size_t) n * d.hidden, &hid.b);
+    if (st == TRELLIS_STATUS_OK && d.rows8) st = alloc_rows8_impl(backend, n, c, &row8.b);
+    if (st == TRELLIS_STATUS_OK && d.rows8) st = alloc_rows8_impl(backend, n, d.hidden, &hid8.b);
+    trellis_sparse_buffer * normed = d.rows8 ? row8.b : row.b;
 
     trellis_sparse_hip_rotary_desc rot{};
     rot.struct_size = sizeof(rot);
@@ -2497,26 +2507,25 @@ trellis_status transformer_block_impl(trellis_sparse_backend * backend, const tr
         if (st == TRELLIS_STATUS_OK) st = call();
     };
     run([&] { return rms_norm_impl(backend, h, nullptr, d.norm1_gamma, nullptr, normed, n, c, d.eps); });
-    run([&] { return linear_act_impl(backend, normed, d.qkv_w, d.qkv_b, 0, nullptr, qkv, n, c, 3 * c); });
-    run([&] { return rotary_impl(backend, qkv, coords, coords_map, qkv, n, &rot); });
+    run([&] { return linear_act_impl(backend, normed, d.qkv_w, d.qkv_b, 0, nullptr, qkv.b, n, c, 3 * c); });
+    run([&] { return rotary_impl(backend, qkv.b, coords, coords_map, qkv.b, n, &rot); });
     // Attention leaves rows in no sequence as they are: zeros.
     if (offsets != nullptr) {
         run([&] {
             DeviceScope scope(be);
-            return hip_status(be, launch_fill_i32((int32_t *) row->ptr, (int64_t) (row->cap / 4), 0, be->stream), "fill");
+            const hipError_t err = launch_fill_i32((int32_t *) row.b->ptr, (int64_t) (row.b->cap / 4), 0, be->stream);
+            return hip_status(be, err, "fill");
         });
     }
-    run([&] { return attention_impl(backend, qkv, qkv, qkv, row, n, n, offsets, offsets, n_seqs, &att); });
-    if (d.rows8) run([&] { return pack_rows8_impl(backend, row, row8, n, c); });
+    run([&] { return attention_impl(backend, qkv.b, qkv.b, qkv.b, row.b, n, n, offsets, offsets, n_seqs, &att); });
+    if (d.rows8) run([&] { return pack_rows8_impl(backend, row.b, row8.b, n, c); });
     run([&] { return linear_act_impl(backend, normed, d.out_w, d.out_b, 0, h, out, n, c, c); });
     run([&] { return rms_norm_impl(backend, out, nullptr, d.norm2_gamma, nullptr, normed, n, c, d.eps); });
-    run([&] { return linear_act_impl(backend, normed, d.mlp0_w, d.mlp0_b, d.act, nullptr, hid, n, c, d.hidden); });
-    if (d.rows8) run([&] { return pack_rows8_impl(backend, hid, hid8, n, d.hidden); });
+    run([&] { return linear_act_impl(backend, normed, d.mlp0_w, d.mlp0_b, d.act, nullptr, hid.b, n, c, d.hidden); });
+    if (d.rows8) run([&] { return pack_rows8_impl(backend, hid.b, hid8.b, n, d.hidden); });
     run([&] {
-        return linear_act_impl(backend, d.rows8 ? hid8 : hid, d.mlp2_w, d.mlp2_b, 0, out, out, n, d.hidden, c);
+        return linear_act_impl(backend, d.rows8 ? hid8.b : hid.b, d.mlp2_w, d.mlp2_b, 0, out, out, n, d.hidden, c);
     });
-    for (trellis_sparse_buffer * b : {hid8, row8, hid, qkv, row})
-        if (b != nullptr) op_free_buffer(backend, b);
     return st;
 }
 
