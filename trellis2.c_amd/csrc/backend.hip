@@ -2477,6 +2477,7 @@ trellis_status transformer_block_impl(trellis_sparse_backend * backend, const tr
     if (scratch_clash(be, be->scratch_bytes, {packed(h, n, c), packed(out, n, c), at, offset_span(offsets, n_seqs)})) {
         return fail(be, TRELLIS_STATUS_INVALID_ARGUMENT, "transformer_block: rows in the scratch");
     }
+    DeviceScope scope(be);  // (the allocations alone would leave the thread on this device)
     PoolBuffer row(backend), qkv(backend), hid(backend), row8(backend), hid8(backend);
     trellis_status st = op_alloc_f32(backend, (size_t) n * c, &row.b);
     if (st == TRELLIS_STATUS_OK) st = op_alloc_f32(backend, (size_t) n * 3 * c, &qkv.b);
@@ -2512,7 +2513,6 @@ trellis_status transformer_block_impl(trellis_sparse_backend * backend, const tr
     // Attention leaves rows in no sequence as they are: zeros.
     if (offsets != nullptr) {
         run([&] {
-            DeviceScope scope(be);
             const hipError_t err = launch_fill_i32((int32_t *) row.b->ptr, (int64_t) (row.b->cap / 4), 0, be->stream);
             return hip_status(be, err, "fill");
         });
