@@ -17,16 +17,20 @@ namespace {
 // GELU is v Phi(v), and below zero Phi is small beside 1: one minus an erf, or a
 // polynomial that is right to some 1e-6 of 1, loses it.  So Phi(-a) = exp(-a^2 / 2)
 // M(a), a = |v|, where M falls like 1 / a: t Q(t), t = 1 / (1 + p a), Q fitted to the
-// least relative error.  bf16: cubic, 2^-12 down to v = -13.2, below which the
-// exponential is zero.  fp16: cubic, 2^-14.5 down to -4.05, and below that 2^-28
-// or less, an eighth of the output's half step there as well.  fp32: degree 8, 2^-25.2;
-// t, Q, their products and the exponential add some 16 roundings, the exponential's
-// argument 1.5 a^2.
+// least error, relative and of Phi, as the output's rounding needs it.  bf16: 2^-13.8
+// relative down to v = -13.2, below which the exponential is zero, and 2^-22 of Phi.
+// fp16: 2^-16 down to -4.05, below that 2^-29.9 of GELU (half a step is 2^-25), and 2^-21
+// of Phi.  fp32: 2^-25.2; t, Q, their products and the exponential add some 16 roundings,
+// the exponential's argument 1.5 a^2.
 template <int DT> struct GeluTail {
-    static constexpr int degree = 3;
-    static constexpr float p = DT == kF16 ? 0.28f : 0.3f;
-    static constexpr float q[4] = {DT == kF16 ? 0.0977476385f : 0.118204356f, DT == kF16 ? 0.205788678f : 0.137478365f,
-                                   DT == kF16 ? -0.13003297f : 0.0355873705f, DT == kF16 ? 0.326480256f : 0.208844977f};
+    static constexpr int degree = 5;
+    static constexpr float p = 0.42f;
+    static constexpr float q[6] = {0.166797221f, 0.178975746f, 0.073189348f, 0.257076681f, -0.233487561f, 0.0574485436f};
+};
+template <> struct GeluTail<kF16> {
+    static constexpr int degree = 4;
+    static constexpr float p = 0.34f;
+    static constexpr float q[5] = {0.130050302f, 0.182318762f, -0.0322297364f, 0.32397607f, -0.104115553f};
 };
 template <> struct GeluTail<kF32> {
     static constexpr int degree = 8;
