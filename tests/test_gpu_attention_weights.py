@@ -1,0 +1,41 @@
+"""Attention over many keys whose weights are small beside the largest: what they add up to is not lost."""
+import numpy as np
+import pytest
+
+import rows64 as ref
+import sparse_hip as sh
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("dtype", [sh.F32, sh.F16, sh.BF16])
+@pytest.mark.parametrize("nq", [1, 40, 3000, 70000])
+@pytest.mark.parametrize("below", [17.375, 17.0, 13.0])
+@pytest.mark.parametrize("value", [0, 2])
+@pytest.mark.parametrize("first", [True, False])
+def test_many_small_weights(dtype, nq, below, value, first):
+    """One key of score 0 with the value 0 or 2, and 80,000 of -17.375 (weights of 2^-25.07), -17 or -13 with the value 1:
+    split over the keys and not (70,000 queries), the largest met first or last.  With S = 80,000 exp(-below) the exact result
+    is (value + S) / (1 + S).
+
+    A weight is rounded by half a step relative, or by 2^-32 of the largest where fp16 has no finer steps; all of them
+    alike here, so the errors add up: (half a step + 4 E below) S + 80,000 x 2^-32 beside weights that sum to 1 + S.  A sum
+    of N terms one after the other takes N roundings, each at most E of the sum, and of equal terms all may be the same way:
+    with at least one key at a time N = n for the values' products; a lane adds a quarter of the weights: n / 4.  (The value 0
+    shows the small weights alone: weights that fp16 loses leave nothing of S / (1 + S) = 0.0023, of which this is 1 %.)"""
+    be, n, dim = sh.Backend(0, dtype), 80001, 32
+    try:
+        q, k, v = np.zeros((nq, dim), np.float32), np.zeros((n, dim), np.float32), np.ones((n, dim), np.float32)
+        q[:, 0], k[:, 0] = 1, -below
+        top = 0 if first else n - 1
+        k[top, 0], v[top] = 0, value
+        y = be.alloc(nq * dim)
+        be.attention(be.upload(q), be.upload(k), be.upload(v), y, nq, n, 1, 1, dim, scale=1.0)
+        s = (n - 1) * np.exp(-below)
+        exp = np.full(nq * dim, (value + s) / (1 + s))
+        half = ref.HALF[dtype] if dtype != sh.F32 else 0.0
+        err = ((half + 4 * ref.E * below) * s + (80000 * 2.0 ** -32 if dtype == sh.F16 else 0.0)) / (1 + s)
+        err = err + 1.25 * n * ref.E * exp
+        ref.check(be.download(y), exp, err + ref.stored(exp, dtype), "y")
+    finally:
+        be.destroy()

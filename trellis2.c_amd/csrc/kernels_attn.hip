@@ -175,8 +175,9 @@ __device__ __forceinline__ float sum_halves(float v) {
     return a + b;
 }
 
-// Where the keys are split over blocks: each split's running maximum, sum and
+// Where the keys are split over blocks: each split's reference, sum and
 // unnormalised output of every query (row * heads + head), joined by k_join.
+// (Sums and outputs of all splits are lifted alike.)
 struct Partial {
     float * out;   // [splits][nq * heads][dim]
     float2 * stat; // [splits][nq * heads]: maximum (log2 units), sum
@@ -232,7 +233,12 @@ __device__ __forceinline__ void leave(const Attention & p, const Partial & part,
 //
 // Weights are 2^(score - reference), in [0, 2^8]: the reference is a running
 // maximum that moves only when some query's scores exceed it by 8, so most
-// tiles leave the output unscaled.
+// tiles leave the output unscaled.  They meet the values in the storage type, as the
+// matrix unit takes no other, each rounded by half a step at most; their sum is
+// that of the fp32 weights.  (With random values some 1.4 times the output's own
+// rounding in all.)  fp16's steps end at 2^-24, which many keys far below the maximum
+// would feel (80,000 of them 25.05 below it: 0.0023 of the result, five half steps):
+// its weights are 2^7 times as large, up to 2^15, and what is lost is 2^-32 a key.
 //
 // Bound by issue: a tile of 32 queries x 64 keys x 64 channels is 16 products, 512
 // clocks of the matrix unit, and its softmax about 580 of the vector unit (per
@@ -408,7 +414,8 @@ __global__ void __launch_bounds__(64 * NW, DC <= 64 ? 3 : 2) k_attention(Attenti
 #pragma unroll
                 for (int i = 0; i < 16; ++i) out[d][i] *= keep;
         }
-        const float base = ref == -__builtin_inff() ? 0.0f : ref;
+        constexpr float kLift = DT == kF16 ? 7.0f : 0.0f;
+        const float base = ref == -__builtin_inff() ? 0.0f : ref - kLift;
         // Keys of t + 1 and values of t have landed; every wavefront is done with
         // the keys of t and the values of t - 1.
         wait_vmcnt<0>();
