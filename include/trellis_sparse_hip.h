@@ -636,7 +636,7 @@ typedef struct trellis_sparse_hip_attention_desc {
     int32_t heads;
     int32_t kv_heads;      /* divides heads */
     int32_t head_dim;      /* up to 192 */
-    float scale;           /* 0: 1 / sqrt(head_dim) */
+    float scale;           /* 0: 1 / sqrt(head_dim); log2(e) times it is finite */
     int64_t q_offset, q_stride;  /* row i's first head at q_offset + i * q_stride; stride 0: packed */
     int64_t k_offset, k_stride;
     int64_t v_offset, v_stride;

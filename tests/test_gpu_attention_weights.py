@@ -1,9 +1,10 @@
-"""Attention over many keys whose weights are small beside the largest: what they add up to is not lost."""
+"""Attention where its softmax is extreme: many keys whose weights are small beside the largest, and the largest scales."""
 import numpy as np
 import pytest
 
 import rows64 as ref
 import sparse_hip as sh
+from test_gpu_rows import refused
 
 pytestmark = pytest.mark.gpu
 
@@ -37,5 +38,22 @@ def test_many_small_weights(dtype, nq, below, value, first):
         err = ((half + 4 * ref.E * below) * s + (80000 * 2.0 ** -32 if dtype == sh.F16 else 0.0)) / (1 + s)
         err = err + 1.25 * n * ref.E * exp
         ref.check(be.download(y), exp, err + ref.stored(exp, dtype), "y")
+    finally:
+        be.destroy()
+
+
+@pytest.mark.parametrize("dtype", [sh.F32, sh.BF16])
+def test_largest_scales(dtype):
+    """The kernels' scale is log2(e) times the caller's: refused where fp32 has no such number (scores of 0 would be NaN),
+    one-hot weights just below that."""
+    be = sh.Backend(0, dtype)
+    try:
+        q = be.upload(np.eye(2, 32, dtype=np.float32))
+        k, v = be.upload(np.eye(2, 32, dtype=np.float32)), be.upload(np.arange(64, dtype=np.float32).reshape(2, 32))
+        y = be.alloc(64)
+        for scale in (2.4e38, -2.4e38, float(np.finfo(np.float32).max)):
+            refused(sh.INVALID_ARGUMENT, be.attention, q, k, v, y, 2, 2, 1, 1, 32, scale=scale)
+        be.attention(q, k, v, y, 2, 2, 1, 1, 32, scale=2.3e38)
+        assert np.array_equal(be.download(y), np.arange(64))
     finally:
         be.destroy()

@@ -2375,6 +2375,11 @@ trellis_status attention_impl(trellis_sparse_backend * backend, const trellis_sp
         (q_offsets == nullptr) != (kv_offsets == nullptr) || n_seqs <= 0 || (q_offsets == nullptr && n_seqs != 1)) {
         return fail(be, TRELLIS_STATUS_INVALID_ARGUMENT, "attention: bad argument");
     }
+    const double natural = d.scale == 0.0f ? 1.0 / std::sqrt((double) d.head_dim) : (double) d.scale;
+    const float scale = (float) (natural * 1.4426950408889634);
+    if (!std::isfinite(scale)) {
+        return fail(be, TRELLIS_STATUS_INVALID_ARGUMENT, "attention: scale beyond 2^128 / log2(e)");
+    }
     if (d.head_dim > kAttentionMaxDim) {
         return fail(be, TRELLIS_STATUS_NOT_IMPLEMENTED, "attention: head_dim up to 192");
     }
@@ -2422,8 +2427,7 @@ trellis_status attention_impl(trellis_sparse_backend * backend, const trellis_sp
     p.heads = d.heads;
     p.kv_heads = d.kv_heads;
     p.dim = d.head_dim;
-    const double scale = d.scale == 0.0f ? 1.0 / std::sqrt((double) d.head_dim) : (double) d.scale;
-    p.scale = (float) (scale * 1.4426950408889634);
+    p.scale = scale;
     // Without scratch for split keys one block takes all of a query's keys.
     const AttentionShape shape = attention_shape(be->policy.compute_dtype, p, be->cus);
     if (scratch_clash(be, shape.scratch, {sq, sk, sv, sy, sqo, sko})) {
