@@ -1268,7 +1268,8 @@ trellis_status conv_impl(trellis_sparse_backend * backend, const trellis_sparse_
         if (sorted) {
             // Where the order's memory does not fit, the rows are taken in their
             // own: the same sums, more of the multiplied rows absent.
-            if (rulebook_order_pays(rulebook, ci, co)) st = rulebook_ensure_order(be, rulebook);
+            // A captured conv takes them in the order that there is: no memory is handed out then.
+            if (!capturing(be) && rulebook_order_pays(rulebook, ci, co)) st = rulebook_ensure_order(be, rulebook);
             if (st == TRELLIS_STATUS_OUT_OF_MEMORY) {
                 be->last_error.clear();
                 st = TRELLIS_STATUS_OK;
