@@ -529,11 +529,12 @@ trellis_status trellis_sparse_hip_wrap_i32(trellis_sparse_backend * backend, voi
  * the backend's device; NULL is the default stream), behind what it has queued
  * before; own_stream goes back to the stream it was created with.  The stream
  * outlives its use here: go back, or destroy the backend, before destroying it.
- * While the stream is captured into a graph, calls that need no memory can be
- * captured: buffers exist before, weights are on the device from an earlier
- * call, and all stay until the last replay; a call that would allocate
- * (transformer_block does) returns TRELLIS_STATUS_ERROR, and so does set_stream
- * while either stream is captured. */
+ * While the stream is captured into a graph, calls that need no memory and wait
+ * for nothing can be captured: buffers exist before, weights are on the device
+ * from an earlier call, and all stay until the last replay; a call that would
+ * allocate (transformer_block does) or wait (downloads, build_c2s_map_into,
+ * synchronize, trim, the timing calls) returns TRELLIS_STATUS_ERROR and leaves the
+ * capture as it was, and so does set_stream while either stream is captured. */
 trellis_status trellis_sparse_hip_set_stream(trellis_sparse_backend * backend, void * stream);
 trellis_status trellis_sparse_hip_own_stream(trellis_sparse_backend * backend);
 

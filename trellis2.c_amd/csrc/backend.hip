@@ -233,6 +233,17 @@ bool stream_captured(hipStream_t stream) {
 }
 bool capturing(const Backend * be) { return be->stream != be->own_stream && stream_captured(be->stream); }
 
+// A call that waits for the stream cannot be captured; tried, it would end the capture.
+trellis_status may_wait(Backend * be) {
+    if (!capturing(be)) return TRELLIS_STATUS_OK;
+    return fail(be, TRELLIS_STATUS_ERROR, "the call waits for the stream, which is being captured");
+}
+#define TSH_MAY_WAIT(be)                                                       \
+    do {                                                                       \
+        const trellis_status tsh_st_ = tsh::may_wait(be);                      \
+        if (tsh_st_ != TRELLIS_STATUS_OK) return tsh_st_;                      \
+    } while (0)
+
 trellis_status dev_alloc(Backend * be, size_t bytes, DevMem * out) {
     out->ptr = nullptr;
     out->bytes = 0;
@@ -726,6 +737,7 @@ trellis_status op_download_f32(trellis_sparse_backend * backend, const trellis_s
     Backend * be = as_backend(backend);
     CallScope scope(be);
     if (count == 0) return TRELLIS_STATUS_OK;
+    TSH_MAY_WAIT(be);
     if (src->dtype == kF32 || src->dtype < 0) {
         TSH_TRY(be, hipMemcpyAsync(dst, src->ptr, count * 4, hipMemcpyDeviceToHost, be->stream));
         TSH_TRY(be, hipStreamSynchronize(be->stream));
@@ -1687,6 +1699,7 @@ trellis_status op_download_c2s_coords(trellis_sparse_backend * backend, const tr
         return fail(be, TRELLIS_STATUS_INVALID_ARGUMENT, "download_c2s_coords: bad argument");
     }
     CallScope scope(be);
+    TSH_MAY_WAIT(be);
     TSH_TRY(be, hipMemcpyAsync(coords_out, map->coords.ptr, (size_t) n * 16, hipMemcpyDeviceToHost, be->stream));
     TSH_TRY(be, hipStreamSynchronize(be->stream));
     return TRELLIS_STATUS_OK;
@@ -1701,6 +1714,7 @@ trellis_status op_download_c2s_map(trellis_sparse_backend * backend, const trell
         return fail(be, TRELLIS_STATUS_INVALID_ARGUMENT, "download_c2s_map: bad argument");
     }
     CallScope scope(be);
+    TSH_MAY_WAIT(be);
     TSH_TRY(be, hipMemcpyAsync(coords_out, map->coords.ptr, (size_t) n * 16, hipMemcpyDeviceToHost, be->stream));
     TSH_TRY(be, hipMemcpyAsync(parent_out, map->parent.ptr, (size_t) n * 4, hipMemcpyDeviceToHost, be->stream));
     TSH_TRY(be, hipMemcpyAsync(subidx_out, map->subidx.ptr, (size_t) n * 4, hipMemcpyDeviceToHost, be->stream));
@@ -2596,6 +2610,7 @@ trellis_status op_trim(trellis_sparse_backend * backend, unsigned flags, size_t 
     if (flags == 0) return TRELLIS_STATUS_OK;
     Backend * be = as_backend(backend);
     CallScope scope(be);
+    TSH_MAY_WAIT(be);
     TSH_TRY(be, hipStreamSynchronize(be->stream));
     size_t released = 0;
     if (flags & TRELLIS_SPARSE_TRIM_WEIGHTS) {
@@ -2810,6 +2825,7 @@ trellis_status trellis_sparse_hip_synchronize(trellis_sparse_backend * backend) 
     if (backend == nullptr) return TRELLIS_STATUS_INVALID_ARGUMENT;
     Backend * be = tsh::as_backend(backend);
     tsh::select_device(be);
+    TSH_MAY_WAIT(be);
     return tsh::hip_status(be, hipStreamSynchronize(be->stream), "synchronize");
 }
 
@@ -2819,6 +2835,7 @@ trellis_status trellis_sparse_hip_rulebook_stats(trellis_sparse_backend * backen
     if (backend == nullptr || rulebook == nullptr) return TRELLIS_STATUS_INVALID_ARGUMENT;
     Backend * be = tsh::as_backend(backend);
     tsh::select_device(be);
+    TSH_MAY_WAIT(be);
     const trellis_status lst = tsh::rulebook_ensure_lists(be, rulebook);
     if (lst != TRELLIS_STATUS_OK) return lst;
     int32_t ctr[tsh::kCounterInts];
@@ -2847,6 +2864,7 @@ trellis_status trellis_sparse_hip_download_neighbors(trellis_sparse_backend * ba
     }
     Backend * be = tsh::as_backend(backend);
     tsh::select_device(be);
+    TSH_MAY_WAIT(be);
     tsh::DevMem nbr;
     trellis_status st = tsh::rulebook_ensure_rows(be, rulebook);
     if (st == TRELLIS_STATUS_OK) st = tsh::dev_alloc(be, (size_t) n * 27 * 4, &nbr);
@@ -2865,6 +2883,7 @@ trellis_status trellis_sparse_hip_download_pairs(trellis_sparse_backend * backen
     if (backend == nullptr || rulebook == nullptr || counts_out == nullptr) return TRELLIS_STATUS_INVALID_ARGUMENT;
     Backend * be = tsh::as_backend(backend);
     tsh::select_device(be);
+    TSH_MAY_WAIT(be);
     const trellis_status lst = tsh::rulebook_ensure_lists(be, rulebook);
     if (lst != TRELLIS_STATUS_OK) return lst;
     // Per-offset totals are the column sums of the per-(tile, offset) counts.
@@ -2939,6 +2958,7 @@ trellis_status trellis_sparse_hip_download_raw(trellis_sparse_backend * backend,
     }
     Backend * be = tsh::as_backend(backend);
     tsh::select_device(be);
+    TSH_MAY_WAIT(be);
     const size_t elem = src->dtype < 0 ? 4u : tsh::dtype_bytes(src->dtype);
     hipError_t err = hipMemcpyAsync(dst, src->ptr, count * elem, hipMemcpyDeviceToHost, be->stream);
     if (err == hipSuccess) err = hipStreamSynchronize(be->stream);
@@ -3002,6 +3022,7 @@ trellis_status trellis_sparse_hip_build_c2s_map_into(trellis_sparse_backend * ba
         return fail(be, TRELLIS_STATUS_ERROR, "build_c2s_map_into: scratch address unavailable on this device");
     }
     select_device(be);
+    TSH_MAY_WAIT(be);
     hipStream_t s = be->stream;
     IntoScratch & sc = *be->into;
     // One call at a time per device; this call's kernels start after the
@@ -3208,6 +3229,7 @@ trellis_status trellis_sparse_hip_profile_read(trellis_sparse_backend * backend,
     if (backend == nullptr || out == nullptr) return TRELLIS_STATUS_INVALID_ARGUMENT;
     Backend * be = tsh::as_backend(backend);
     tsh::select_device(be);
+    TSH_MAY_WAIT(be);
     const hipError_t err = hipStreamSynchronize(be->stream);
     if (err != hipSuccess) return tsh::hip_status(be, err, "profile_read");
     for (auto & m : be->pending) {
@@ -3231,6 +3253,7 @@ trellis_status trellis_sparse_hip_event_record(trellis_sparse_backend * backend,
     if (backend == nullptr || slot < 0 || slot >= 16) return TRELLIS_STATUS_INVALID_ARGUMENT;
     Backend * be = tsh::as_backend(backend);
     tsh::select_device(be);
+    TSH_MAY_WAIT(be);
     if (be->user_events[slot] == nullptr) {
         const hipError_t err = hipEventCreate(&be->user_events[slot]);
         if (err != hipSuccess) return tsh::hip_status(be, err, "event_create");
@@ -3244,6 +3267,7 @@ trellis_status trellis_sparse_hip_event_elapsed(trellis_sparse_backend * backend
     }
     Backend * be = tsh::as_backend(backend);
     tsh::select_device(be);
+    TSH_MAY_WAIT(be);
     if (be->user_events[slot_a] == nullptr || be->user_events[slot_b] == nullptr) {
         return TRELLIS_STATUS_INVALID_ARGUMENT;
     }
