@@ -21,8 +21,8 @@ namespace {
 // exponential is zero there.  bf16: degree 9, 2^-12.4 relative down to v = -13.2 (below
 // that bf16 has no normal numbers for the result), 2^-20.2 absolute.  fp16: degree 7,
 // 2^-16 relative down to -4.05, below that 2^-29.6 of GELU (half a step is 2^-25), 2^-21
-// absolute.  Of 79,523 x 512 -> 2048 from 8-bit rows, norm included, 200 us; with the form
-// of fp32 below 203; as a logistic function of v R(v^2), which is 5.7e-6 off, 183.
+// absolute.  14 instructions a value: 79,523 x 512 -> 2048 from 8-bit rows 181 us; with the
+// form of fp32 below 184; as a logistic function of v R(v^2), which is 5.7e-6 off, 165.
 // fp32: exp(-a^2 / 2) t Q(t), t = 1 / (1 + p a), as the tail falls like 1 / a beside the
 // exponential; Q of degree 8, 2^-25.2 relative.  t, Q, their products and the exponential
 // add some 16 roundings, the exponential's argument 1.5 a^2.
@@ -204,13 +204,13 @@ constexpr uint32_t kOutside = 0x80000000u;  // beyond every buffer here: loads f
 //
 // More tiles than fit at once are walked by blocks that stay: the loads of a tile's
 // last two steps are those of the next one's first two, so that they arrive while
-// outputs are activated and stored (79,523 rows 512 -> 2048 of 8-bit rows with GELU
-// 188 -> 167 us, 18,216 rows 1024 -> 4096 in bf16 151 -> 139).
+// outputs are activated and stored (79,523 rows 512 -> 2048 with GELU of 8-bit rows
+// 201 -> 181 us, in bf16 259 -> 239).
 //
 // Bound by the matrix unit and what feeds it where K is long: 16,384 x 4096 ->
-// 4096 bf16 434 us, 1,267 TFLOP/s (the library's largest product 1,570); of 8-bit rows
-// 264 us, 2,083 TFLOP/s (2,807), where a step's reads of LDS take as long as its
-// products.  With short K by the outputs: their activation (GELU some 43 clocks for 64
+// 4096 bf16 430 us, 1,280 TFLOP/s (the library's largest product 1,590); of 8-bit rows
+// 268 us, 2,050 TFLOP/s (2,790), where a step's reads of LDS take as long as its
+// products.  With short K by the outputs: their activation (GELU some 60 clocks for 64
 // values) and their way to memory run while nothing is multiplied, as there are
 // registers for one block of 256 x 256 per CU only.
 template <int MT, int DT, int RW, int CW, int RB, int NT, int PER_CU>
@@ -519,8 +519,8 @@ __global__ void __launch_bounds__(64 * RW * CW, RW * CW * PER_CU / 4) k_linear_a
 }
 
 // Joins the splits' sums in their order, then bias, activation and residual: N
-// adjacent outputs a thread (N divides co).  One row 1024 -> 4096 fp16: 4.5 us of products
-// and 2.4 here.
+// adjacent outputs a thread (N divides co).  One row 1024 -> 4096 fp16: 4.8 us of products
+// and 2.6 here.
 template <int DT, int N> __global__ void __launch_bounds__(256) k_linear_join(LinearAct p) {
     using T = typename Store<DT>::T;
     const int64_t e = ((int64_t) blockIdx.x * 256 + threadIdx.x) * N, count = p.n * p.co;

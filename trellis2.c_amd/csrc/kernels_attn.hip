@@ -243,10 +243,11 @@ __device__ __forceinline__ void leave(const Attention & p, const Partial & part,
 // Bound by issue: a tile of 32 queries x 64 keys x 64 channels is 16 products, 512
 // clocks of the matrix unit, and its softmax about 580 of the vector unit (per
 // value an exponential 8.3, scale and sum 2.7 each, maximum and rounding 2.2), which
-// stands still for half of each product's 32.  18,216 rows, 8 heads of 64, bf16 783 us
-// (867 TFLOP/s, some 1,200 clocks a tile); 16,384 rows of 128 channels 990 us, 1,110 TFLOP/s,
-// with twice the products to the same softmax.  Products and exponentials written
-// down in turns, and the next tile's scores under this one's softmax: 812 -> 791 us.
+// stands still for half of each product's 32.  Counted: 1,060 clocks a tile, and CUs without
+// a block for 15 % of the time.  18,216 rows, 8 heads of 64, bf16 768 us (885 TFLOP/s);
+// 16,384 rows of 128 channels 986 us, 1,115 TFLOP/s, with twice the products to the same
+// softmax.  Products and exponentials written down in turns, and the next tile's scores
+// under this one's softmax: 812 -> 791 us.
 //
 // LDS: rows of 64 or 128 values, chunk c of row r at c ^ f(r): the 16 lanes of
 // a K read (16 rows, one chunk) and the 32 of a V read (4 rows x 4 chunks, two of

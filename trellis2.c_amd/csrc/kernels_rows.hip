@@ -350,7 +350,7 @@ hipError_t norm_dt(const void * x, const void * residual, const float * gamma, v
 // heads; then lanes of 4 pairs (two 8-byte or one 16-byte load) take one head
 // each over all rows, gamma in registers, two items ahead of the one in hand (one:
 // 79 us).  Bound by memory: 79,523 rows, q and k of 8 heads of 64 in a buffer of q, k
-// and v, bf16 with norm 72 us, 4.5 TB/s (a copy of the size 5.3); packed fp32 rows of 8
+// and v, bf16 with norm 67.5 us, 4.8 TB/s (a copy of the size 5.4); packed fp32 rows of 8
 // heads 66 us, 4.9 TB/s; 997 rows of 6 x 48 in fp32 4 us.
 struct RotaryShape {
     int64_t n, x_stride, y_stride;
