@@ -651,8 +651,10 @@ typedef struct trellis_sparse_hip_attention_desc {
  * (of others every access stays within the buffers).  A sequence without keys
  * gives zeros; rows of y in no sequence are left as they were.  y may be the rows of q.  In 16
  * bits on the matrix unit (head_dim up to 128 and a multiple of 8, rows of whole 16
- * bytes) a weight is rounded to the storage type before it meets v, the sum of the
- * weights is not: some 1.4 times the error of the output's own rounding in all. */
+ * bytes) the weights meet v in the storage type.  Where the queries are few (up to
+ * some 16,384 / kv_heads rows and heads that share one) in two parts, exact to 2^-15
+ * (bf16) or 2^-21; else rounded once, the error of which is as large as
+ * that of the output's own rounding. */
 trellis_status trellis_sparse_hip_attention(trellis_sparse_backend * backend, const trellis_sparse_buffer * q,
                                             const trellis_sparse_buffer * k, const trellis_sparse_buffer * v,
                                             trellis_sparse_buffer * y, int64_t nq, int64_t nkv,

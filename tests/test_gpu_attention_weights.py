@@ -57,3 +57,26 @@ def test_largest_scales(dtype):
         assert np.array_equal(be.download(y), np.arange(64))
     finally:
         be.destroy()
+
+
+@pytest.mark.parametrize("dtype", [sh.F32, sh.F16, sh.BF16])
+@pytest.mark.parametrize("nq,nk,heads,kv_heads,dim", [(1, 300, 2, 2, 64), (3, 20000, 4, 1, 64), (20, 700, 6, 2, 32),
+                                                      (64, 64, 3, 3, 96), (500, 900, 2, 2, 128), (1500, 1500, 2, 2, 64)])
+def test_few_queries_cost_no_precision(dtype, nq, nk, heads, kv_heads, dim):
+    """Nothing but fp32's errors and the output's one rounding: weights of 16 bits are in two parts, the first cut, so that
+    up to a step is left, 2 HALF of the weight, and the second rounded by half a step of that: 2 HALF^2 (and 2^-31 of the
+    largest at most where fp16 has no finer steps)."""
+    be, rng = sh.Backend(0, dtype), np.random.default_rng(nq + nk)
+    try:
+        q, k, v = (sh.storage_round(rng.standard_normal((n, h, dim)).astype(np.float32), dtype)
+                   for n, h in ((nq, heads), (nk, kv_heads), (nk, kv_heads)))
+        y = be.alloc(nq * heads * dim)
+        be.attention(be.upload(q), be.upload(k), be.upload(v), y, nq, nk, heads, kv_heads, dim)
+        half = ref.E if dtype == sh.F32 else 2 * ref.HALF[dtype] ** 2
+        exp, err, _ = ref.attention(*(a.astype(np.float64) for a in (q, k, v)), dim ** -0.5, heads // kv_heads, [0, nq],
+                                    [0, nk], half)
+        if dtype == sh.F16:
+            err = err + 2.0 ** -31 * nk * np.abs(v).max()
+        ref.check(be.download(y).reshape(exp.shape), exp, err + ref.stored(exp, dtype), "y")
+    finally:
+        be.destroy()

@@ -154,6 +154,8 @@ template <int DT> hipError_t launch_any(const Attention & p, hipStream_t s) {
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef short s16x8 __attribute__((ext_vector_type(8)));
+typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 
 template <int DT> __device__ __forceinline__ f32x16 mac32(s16x8 a, s16x8 b, f32x16 c) {
     using V = typename Mfma<DT>::V;
@@ -161,6 +163,42 @@ template <int DT> __device__ __forceinline__ f32x16 mac32(s16x8 a, s16x8 b, f32x
         return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(V, a), __builtin_bit_cast(V, b), c, 0, 0, 0);
     } else {
         return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(V, a), __builtin_bit_cast(V, b), c, 0, 0, 0);
+    }
+}
+
+// Weights e >= 0 as two each of the storage type: e cut, and what is left, rounded.  The
+// second is above zero wherever the first is, so that an infinite value's products agree.
+template <int DT> __device__ __forceinline__ void two_parts(const float * e, s16x8 & w, s16x8 & rest) {
+    if constexpr (DT == kBF16) {
+        union {
+            uint32_t c[4];
+            s16x8 v;
+        } cut;
+#pragma unroll
+        for (int i = 0; i < 8; i += 2) {
+            const uint32_t b0 = __builtin_bit_cast(uint32_t, e[i]), b1 = __builtin_bit_cast(uint32_t, e[i + 1]);
+            cut.c[i / 2] = __builtin_amdgcn_perm(b1, b0, 0x07060302);  // the upper halves
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                // A step of fp32 more than what is left.
+                const float h = __builtin_bit_cast(float, (j == 0 ? b0 : b1) & 0xffff0000u);
+                rest[i + j] = __builtin_bit_cast(short, round_to_store<DT>(fmaf(e[i + j], 1.00000012f, -h)));
+            }
+        }
+        w = cut.v;
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; i += 2) {
+            const auto cut = __builtin_amdgcn_cvt_pkrtz(e[i], e[i + 1]);
+            const f16x2 left{(_Float16) (e[i] - (float) cut[0]), (_Float16) (e[i + 1] - (float) cut[1])};
+            const u16x2 h = __builtin_bit_cast(u16x2, cut);
+            const u16x2 l = __builtin_elementwise_max(__builtin_bit_cast(u16x2, left),
+                                                      __builtin_elementwise_min(h, u16x2{1, 1}));  // 2^-24 at least
+            w[i] = (short) h[0];
+            w[i + 1] = (short) h[1];
+            rest[i] = (short) l[0];
+            rest[i + 1] = (short) l[1];
+        }
     }
 }
 
@@ -234,11 +272,14 @@ __device__ __forceinline__ void leave(const Attention & p, const Partial & part,
 // Weights are 2^(score - reference), in [0, 2^8]: the reference is a running
 // maximum that moves only when some query's scores exceed it by 8, so most
 // tiles leave the output unscaled.  They meet the values in the storage type, as the
-// matrix unit takes no other, each rounded by half a step at most; their sum is
-// that of the fp32 weights.  (With random values some 1.4 times the output's own
-// rounding in all.)  fp16's steps end at 2^-24, which many keys far below the maximum
-// would feel (80,000 of them 25.05 below it: 0.0023 of the result, five half steps):
-// its weights are 2^7 times as large, up to 2^15, and what is lost is 2^-32 a key.
+// matrix unit takes no other; their sum is that of the fp32 weights.  Rounded once, by
+// half a step, they have as much error as the output's own rounding (with random values
+// 0.0023 of the output's root mean square against 0.0017 in bf16, 0.00029 against
+// 0.00021 in fp16); FINE takes what is left of each as a second weight, and the output's
+// rounding is all (0.0017), for products twice and a third more vector instructions.
+// fp16's steps end at 2^-24, which many keys far below the maximum would feel (80,000 of
+// them 25.05 below it: 0.0023 of the result, five half steps): its weights are 2^7 times
+// as large, up to 2^15, and what is lost is 2^-32 a key.
 //
 // Bound by issue: a tile of 32 queries x 64 keys x 64 channels is 16 products, 512
 // clocks of the matrix unit, and its softmax about 580 of the vector unit (per
@@ -252,7 +293,7 @@ __device__ __forceinline__ void leave(const Attention & p, const Partial & part,
 // LDS: rows of 64 or 128 values, chunk c of row r at c ^ f(r): the 16 lanes of
 // a K read (16 rows, one chunk) and the 32 of a V read (4 rows x 4 chunks, two of
 // them) touch different banks.
-template <int DT, int DC, int NW>
+template <int DT, int DC, int NW, bool FINE>
 __global__ void __launch_bounds__(64 * NW, DC <= 64 ? 3 : 2) k_attention(Attention p, Partial part, int tiles) {
     using T = typename Store<DT>::T;
     constexpr int TQ = 32 * NW, TK = 64;
@@ -429,8 +470,11 @@ __global__ void __launch_bounds__(64 * NW, DC <= 64 ? 3 : 2) k_attention(Attenti
         zero(nxt[0]);
         zero(nxt[1]);
         constexpr int QPS = KS / 2;  // products of the next scores per step
-        s16x8 kf[QPS], vf[DT32], w;
-        const auto values = [&](int d) { out[d] = mac32<DT>(vf[d], w, out[d]); };
+        s16x8 kf[QPS], vf[DT32], w, rest;
+        const auto values = [&](int d) {
+            out[d] = mac32<DT>(vf[d], w, out[d]);
+            if constexpr (FINE) out[d] = mac32<DT>(vf[d], rest, out[d]);
+        };
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
             float e[8];
@@ -479,14 +523,18 @@ __global__ void __launch_bounds__(64 * NW, DC <= 64 ? 3 : 2) k_attention(Attenti
             } r;
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                r.h[i] = round_to_store<DT>(e[i]);
+                if constexpr (!FINE) r.h[i] = round_to_store<DT>(e[i]);
                 if (i % 2 == 0) {
                     sum0 += e[i];
                 } else {
                     sum1 += e[i];
                 }
             }
-            w = r.v;
+            if constexpr (FINE) {
+                two_parts<DT>(e, w, rest);
+            } else {
+                w = r.v;
+            }
         }
 #pragma unroll
         for (int d = 0; d < DT32; ++d) values(d);
@@ -727,13 +775,17 @@ __global__ void __launch_bounds__(256) k_join(Attention p, Partial part, int til
 }
 
 template <int DT, int DC, int NW>
-hipError_t launch_nw(const Attention & p, const Partial & part, int64_t tiles, hipStream_t s) {
+hipError_t launch_nw(const Attention & p, const Partial & part, int64_t tiles, bool fine, hipStream_t s) {
     const int64_t grid = tiles * p.kv_heads * part.splits;
     if (grid > 0x7fffffffLL) return hipErrorInvalidValue;
     if constexpr (DT == kF32) {
         k_attention32<DC, NW><<<(unsigned) grid, 64 * NW, 0, s>>>(p, part, (int) tiles);
     } else {
-        k_attention<DT, DC, NW><<<(unsigned) grid, 64 * NW, 0, s>>>(p, part, (int) tiles);
+        if (fine) {
+            k_attention<DT, DC, NW, true><<<(unsigned) grid, 64 * NW, 0, s>>>(p, part, (int) tiles);
+        } else {
+            k_attention<DT, DC, NW, false><<<(unsigned) grid, 64 * NW, 0, s>>>(p, part, (int) tiles);
+        }
     }
     hipError_t err = hipGetLastError();
     if (err == hipSuccess && part.splits > 1) {
@@ -755,7 +807,8 @@ hipError_t launch_nw(const Attention & p, const Partial & part, int64_t tiles, h
 
 template <int DT, int DC>
 hipError_t launch_dc(const Attention & p, const Partial & part, const AttentionShape & sh, hipStream_t s) {
-    return sh.waves == 1 ? launch_nw<DT, DC, 1>(p, part, sh.tiles, s) : launch_nw<DT, DC, 4>(p, part, sh.tiles, s);
+    return sh.waves == 1 ? launch_nw<DT, DC, 1>(p, part, sh.tiles, sh.fine, s)
+                         : launch_nw<DT, DC, 4>(p, part, sh.tiles, sh.fine, s);
 }
 
 template <int DT>
@@ -769,7 +822,7 @@ hipError_t launch_mfma(const Attention & p, const Partial & part, const Attentio
 }  // namespace
 
 AttentionShape attention_shape(int dtype, const Attention & p, int cus) {
-    AttentionShape sh{0, 0, 1, 0};
+    AttentionShape sh{0, 0, 1, 0, false};
     const int chunk = dtype == kF32 ? 4 : 8;  // of 16 bytes
     const auto aligned = [&](const void * ptr, int64_t stride) { return (uintptr_t) ptr % 16 == 0 && stride % chunk == 0; };
     // A tile's rows (64, of fp32 32) stay within a buffer's 2 GiB of offsets.
@@ -789,6 +842,11 @@ AttentionShape attention_shape(int dtype, const Attention & p, int cus) {
     // Few queries: the keys split over more blocks, at least four tiles of 64 each.
     const int64_t key_tiles = (p.nk / seqs + 63) / 64;
     if (blocks < want) sh.splits = (int) std::max<int64_t>(1, std::min(want / std::max<int64_t>(blocks, 1), key_tiles / 4));
+    // Few blocks: weights in two parts, for the output's own rounding alone.  Their time is
+    // that of loads and latencies: 4 queries on 79,523 keys 33.5 -> 34.9 us, in four sequences
+    // 26 -> 29, 1,000 rows of 8 x 64 17.8 -> 18.9, 2,000 30.3 -> 33.6, but 5,003 85 -> 120 and
+    // 18,216 792 -> 1,097.
+    sh.fine = blocks <= cus / 2;
     if (sh.splits > 1) sh.scratch = (size_t) sh.splits * p.nq * p.heads * (p.dim + 2) * sizeof(float);
     return sh;
 }

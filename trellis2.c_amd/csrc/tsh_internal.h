@@ -426,12 +426,13 @@ struct Attention {
 constexpr int kAttentionMaxDim = 192;
 // How attention is run: wavefronts per block of the MFMA kernel (0: the general
 // kernel), blocks of queries, parts of the keys and the scratch memory to join
-// them (without it they are not split).
+// them (without it they are not split), 16-bit weights in two parts or in one.
 struct AttentionShape {
     int waves;
     int64_t tiles;
     int splits;
     size_t scratch;
+    bool fine;
 };
 AttentionShape attention_shape(int dtype, const Attention & p, int cus);
 hipError_t launch_attention(int dtype, const Attention & p, const AttentionShape & shape, void * scratch,
