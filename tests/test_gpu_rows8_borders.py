@@ -31,27 +31,50 @@ def plain(s, g, eps):
     return ((s.astype(f) * inv).astype(f) * g).astype(f).astype(np.float64)
 
 
-@pytest.mark.parametrize("dtype", [sh.F32, sh.F16, sh.BF16])
-@pytest.mark.parametrize("c", [64, 128, 256, 512, 1000, 1024, 2048, 4096, 1001, 4100])
-def test_norms_beside_borders(dtype, c):
-    """Rows of small whole numbers, whose squares' sums are exact, so that the norm in two floats is right to 2^-45 and the
-    border at least some 2^-30 away: every code is that of the float64 norm (no tolerance), where a norm with fp32's
-    roundings gives the code on the other side at many of these places."""
-    be, rng, n, eps = sh.Backend(0, dtype), np.random.default_rng(c), 21, 1e-6
+def check_codes(dtype, x, r, eps, least):
+    """The norm of x + r to 8-bit rows, gamma beside borders: the float64 norm's codes, which fp32's roundings miss at `least`
+    places or more."""
+    n, c = x.shape
+    s = x.astype(np.float64) + r
+    g = beside_borders(s, float(np.float32(eps)))
+    exp = ref.rows8(ref.rms_norm(s, g.astype(np.float64), float(np.float32(eps))))
+    be = sh.Backend(0, dtype)
     try:
-        x, r = (rng.integers(-8, 9, (n, c)).astype(np.float32) for _ in range(2))
-        s = x.astype(np.float64) + r
-        s[:, 0] += s[:, 0] == 0
-        x[:, 0] = s[:, 0] - r[:, 0]
-        g = beside_borders(s, float(np.float32(eps)))
-        v = ref.rms_norm(s, g.astype(np.float64), float(np.float32(eps)))
-        exp = ref.rows8(v)
         q, y, t = be.alloc_rows8(n, c), be.alloc(n * c), be.alloc(n * c)
         be.rms_norm(be.upload(x), g, q, n, c, eps, residual=be.upload(r), total=t)
         be.expand_rows8(q, y, n, c)
         got = be.download(y).reshape(n, c).astype(np.float64)
         assert np.array_equal(got, sh.storage_round(exp.astype(np.float32), dtype))
-        assert np.array_equal(be.download(t).reshape(n, c), s)
-        assert (ref.rows8(plain(s, g, eps)) != exp).sum() > c / 10
+        assert np.array_equal(be.download(t).reshape(n, c), sh.storage_round(s.astype(np.float32), dtype))
+        assert (ref.rows8(plain(s, g, eps)) != exp).sum() > least
     finally:
         be.destroy()
+
+
+WIDTHS = [64, 128, 256, 512, 1000, 1024, 2048, 4096, 1001, 4100]
+
+
+@pytest.mark.parametrize("dtype", [sh.F32, sh.F16, sh.BF16])
+@pytest.mark.parametrize("c", WIDTHS)
+def test_norms_beside_borders(dtype, c):
+    """Rows of small whole numbers, whose squares' sums are exact, so that the norm in two floats is right to 2^-45 and the
+    border at least some 2^-36 away: every code is that of the float64 norm (no tolerance), where a norm with fp32's
+    roundings gives the code on the other side at many of these places."""
+    rng, n = np.random.default_rng(c), 21
+    x, r = (rng.integers(-8, 9, (n, c)).astype(np.float32) for _ in range(2))
+    s = x.astype(np.float64) + r
+    s[:, 0] += s[:, 0] == 0
+    x[:, 0] = s[:, 0] - r[:, 0]
+    check_codes(dtype, x, r, 1e-6, c / 10)
+
+
+@pytest.mark.parametrize("dtype", [sh.F32, sh.F16, sh.BF16])
+@pytest.mark.parametrize("c", WIDTHS + [330])
+def test_norms_beside_borders_of_many_digits(dtype, c):
+    """Rows whose sums x + r are exact (multiples of 2^-8, 2^-10, 2^-12) but whose squares, or their sums, have more digits
+    than fp32: those of the norm are exact too."""
+    rng, n = np.random.default_rng(c + 1), 21
+    step = {sh.BF16: 2.0 ** -8, sh.F16: 2.0 ** -10, sh.F32: 2.0 ** -12}[dtype]
+    x, r = (sh.storage_round((np.rint(rng.standard_normal((n, c)) / step) * step).astype(np.float32), dtype)
+            for _ in range(2))
+    check_codes(dtype, x, r, 1e-6, c / 20)

@@ -65,14 +65,16 @@ __device__ __forceinline__ uint32_t abs_bits(float v) { return __builtin_bit_cas
 
 // 1 / sqrt(sum / c + eps), for 8-bit outputs as two floats from 64 bits: there a
 // value on the other side of a code's border is off by a whole code, so the last
-// bit of the norm counts.  The sum joins 8 squares at a time in 64 bits, and a
+// bit of the norm counts.  The squares are exact and summed in 64 bits (with squares
+// in fp32, joined 8 at a time, 2 of 12 M codes were beside the exact ones), and a
 // value is not rounded to nearest before it is rounded to its code, but cut and
-// made odd where something was cut (twice to nearest had 10 of 12 M codes beside the
-// exact ones, so 2).
+// made odd where something was cut (twice to nearest had 10 of 12 M).
 struct Inverse {
     float hi, lo;
 };
 template <bool FINE> using NormSum = typename std::conditional<FINE, double, float>::type;
+__device__ __forceinline__ float add_square(float sum, float v) { return sum + v * v; }
+__device__ __forceinline__ double add_square(double sum, float v) { return fma((double) v, (double) v, sum); }
 template <bool FINE> __device__ __forceinline__ Inverse inverse_rms(NormSum<FINE> sum, int c, double per_c, float eps) {
     if constexpr (FINE) {
         // The hardware's estimate and one Newton step in 64 bits (1e-13).
@@ -175,9 +177,9 @@ __global__ void __launch_bounds__(256) k_norm_vec(const typename Store<DT>::T * 
         if constexpr (NORM) {
 #pragma unroll
             for (int i = 0; i < CPL; ++i) {
-                float part = 0.0f;
+                NormSum<Q8> part = 0;
 #pragma unroll
-                for (int u = 0; u < V; ++u) part += v[i][u] * v[i][u];
+                for (int u = 0; u < V; ++u) part = add_square(part, v[i][u]);
                 sum += part;
             }
             const Inverse inv = inverse_rms<Q8>(group_sum<LPR>(sum), c, per_c, eps);
@@ -233,8 +235,7 @@ __global__ void __launch_bounds__(256) k_norm_any(const typename Store<DT>::T * 
     if constexpr (NORM) {
         NormSum<Q8> sum = 0;
         for (int i = lane; i < c; i += 64) {
-            const float v = at(i);
-            sum += v * v;
+            sum = add_square(sum, at(i));
         }
         inv = inverse_rms<Q8>(group_sum<64>(sum), c, 1.0 / c, eps);
     }
