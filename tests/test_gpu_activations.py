@@ -38,9 +38,11 @@ def exact(z, act):
 
     E is half a step of fp32; the hardware's reciprocal and exponential are within 2 E each.  SiLU: those two, the sum, the
     product, and the exponential's argument, |z| with two roundings: (6 + 2 |z|) E, doubled.  GELU with tanh: the argument
-    2 u passes six roundings: (6 + 6 |2 u|) E.  GELU: t = 1 / (1 + p a) 3 E, times up to 2.4 where the tail's factor t Q(t)
-    is steepest, a cubic or its last eight steps 3 E, three products 3 E, an exponential 2 E: 16 E; its argument a^2 / 2 three
-    roundings; and the fit, 2^-12 in bf16, 2^-14.5 in fp16 or 2^-28, 2^-25.2 in fp32.  Exponentials and reciprocals
+    2 u passes six roundings: (6 + 6 |2 u|) E.  GELU of fp32: t = 1 / (1 + p a) 3 E, times up to 2.4 where the tail's factor
+    t Q(t) is steepest, Q's last steps 3 E, three products 3 E, an exponential 2 E: 16 E; its argument a^2 / 2 three roundings.
+    Of 16 bits: an exponential 2 E, one minus it and the product 2 E, and the polynomial that is its argument, whose last
+    two steps or three are as large as itself, some a^2 / 2 + 3: within the same.  And the fit, 2^-12 in bf16, 2^-14.5 in
+    fp16 or 2^-28, 2^-25.2 in fp32.  Exponentials and reciprocals
     below 2^-126 may be zero, which |z| multiplies."""
     a, z = np.abs(z.astype(np.float64)), z.astype(np.float64)
     if act == "silu":
