@@ -566,8 +566,14 @@ size_t trellis_sparse_hip_scratch_bytes(const trellis_sparse_backend * backend);
  * NaN.  A buffer for free_buffer; the slots, uploads and downloads do not take it. */
 trellis_status trellis_sparse_hip_alloc_rows8(trellis_sparse_backend * backend, int64_t n, int c,
                                               trellis_sparse_buffer ** out);
+/* 8-bit integer rows, which the calls below take wherever they take 8-bit rows: n
+ * rows of c channels as whole numbers -127 .. 127, a row with one scale, its largest
+ * magnitude / 127 in fp32.  A row with an infinity or a NaN becomes NaN. */
+trellis_status trellis_sparse_hip_alloc_rows_int8(trellis_sparse_backend * backend, int64_t n, int c,
+                                                  trellis_sparse_buffer ** out);
 /* rows8 = x, rounded to nearest even; y = the values of rows8 (exact in
- * bf16 and fp32 but for 2^128, the code nearest fp32's largest). */
+ * bf16 and fp32 but for 2^128, the code nearest fp32's largest; of integer rows the
+ * product with the scale, rounded). */
 trellis_status trellis_sparse_hip_pack_rows8(trellis_sparse_backend * backend, const trellis_sparse_buffer * x,
                                              trellis_sparse_buffer * rows8, int64_t n, int c);
 trellis_status trellis_sparse_hip_expand_rows8(trellis_sparse_backend * backend, const trellis_sparse_buffer * rows8,
@@ -592,12 +598,24 @@ typedef enum trellis_sparse_hip_act {
     TRELLIS_SPARSE_HIP_ACT_GELU_TANH = 3 /* v (1 + tanh(sqrt(2 / pi) (v + 0.044715 v^3))) / 2 */
 } trellis_sparse_hip_act;
 
+/* Group norm over the rows of each sequence, channels last: the c / groups channels of
+ * a group over a sequence's rows have mean m and variance v (of all values, not one
+ * less), and y = act((x - m) / sqrt(v + eps) * gamma + beta).  offsets: an int32 buffer
+ * [n_seqs + 1] as in attention, or NULL for one sequence of all rows (n_seqs 1); rows
+ * of y in no sequence are left as they were.  gamma, beta (fp32 [c]) may be NULL, y may
+ * be x; groups divides c, eps > 0, act a trellis_sparse_hip_act.  Sums are of 64 bits. */
+trellis_status trellis_sparse_hip_group_norm(trellis_sparse_backend * backend, const trellis_sparse_buffer * x,
+                                             const trellis_sparse_buffer * offsets, int n_seqs, const float * gamma,
+                                             const float * beta, trellis_sparse_buffer * y, int64_t n, int c, int groups,
+                                             float eps, int act);
+
 /* y = act(x W^T + bias) + residual: weight fp32 [co][ci], bias fp32 [co] and
  * residual [n][co] may be NULL, y may be residual.  x is rows of the
  * compute_dtype, with the weights rounded to it, or 8-bit rows (n, ci), with the
  * weights in the same 8-bit format; sums are fp32.  (Of 8-bit rows the matrix unit
  * first adds eight neighbouring products, each cut at 2^-13 of the largest: some
- * 2e-5 of an output's size.)  Always this library's kernels, whatever linear_algo
+ * 2e-5 of an output's size.)  Of 8-bit integer rows the weights are such rows too, a
+ * scale for each output channel, and their sums are exact (ci up to 131,072).  Always this library's kernels, whatever linear_algo
  * says.  ci and co up to 1,048,576. */
 trellis_status trellis_sparse_hip_linear_act(trellis_sparse_backend * backend, const trellis_sparse_buffer * x,
                                              const float * weight, const float * bias, int act,
@@ -662,6 +680,32 @@ trellis_status trellis_sparse_hip_attention(trellis_sparse_backend * backend, co
                                             const trellis_sparse_buffer * kv_offsets, int n_seqs,
                                             const trellis_sparse_hip_attention_desc * desc);
 
+/* Attention whose scores z = scale q_i . k_j are changed before the softmax, in this order:
+ *   cap > 0     z = cap tanh(z / cap)
+ *   slopes      z = z - slopes[h] * d(i, j): the Euclidean distance of the rows'
+ *               coordinates where they are given, else |p_i - j|, p_i = i + keys - queries
+ *               the query's place among its sequence's keys (the last query's the last's)
+ *   causal      keys j > p_i are not seen, but for the first prefix[s] of the sequence
+ * i and j count from the sequence's first row.  A query that sees no key gets zeros;
+ * what a key or a value that is not seen holds reaches nothing. */
+typedef struct trellis_sparse_hip_scores_desc {
+    uint32_t struct_size;  /* sizeof(trellis_sparse_hip_scores_desc) */
+    int32_t causal;        /* 0 or 1 */
+    float cap;             /* 0: none */
+    const float * slopes;  /* fp32 [heads] on the host, up to 2^64, or NULL */
+    const trellis_sparse_buffer * q_coords;  /* int32 [nq][4] (b, x, y, z; b is not read), or NULL */
+    const trellis_sparse_buffer * k_coords;  /* int32 [nkv][4]; both within +-2^29 */
+    const trellis_sparse_buffer * prefix;    /* int32 [n_seqs], read on the device, or NULL: 0 */
+} trellis_sparse_hip_scores_desc;
+/* The rest as in trellis_sparse_hip_attention. */
+trellis_status trellis_sparse_hip_attention_scored(trellis_sparse_backend * backend, const trellis_sparse_buffer * q,
+                                                   const trellis_sparse_buffer * k, const trellis_sparse_buffer * v,
+                                                   trellis_sparse_buffer * y, int64_t nq, int64_t nkv,
+                                                   const trellis_sparse_buffer * q_offsets,
+                                                   const trellis_sparse_buffer * kv_offsets, int n_seqs,
+                                                   const trellis_sparse_hip_attention_desc * desc,
+                                                   const trellis_sparse_hip_scores_desc * scores);
+
 /* A whole block over voxel rows, c = heads * head_dim channels:
  *   a   = attention over rotary(qkv(norm1(h))), q and k turned (and normed per
  *         head where qk_eps > 0)
@@ -669,7 +713,7 @@ trellis_status trellis_sparse_hip_attention(trellis_sparse_backend * backend, co
  *   out = mid + act(norm2(mid) mlp0_w^T + mlp0_b) mlp2_w^T + mlp2_b
  * from the calls above, bit for bit, through intermediates of the backend's
  * pool (n x c, n x 3c, n x hidden).  rows8: each of the four linears reads
- * 8-bit rows.  Weights fp32 on the host: qkv_w [3c][c], out_w [c][c], mlp0_w
+ * 8-bit rows (1) or 8-bit integer rows (2).  Weights fp32 on the host: qkv_w [3c][c], out_w [c][c], mlp0_w
  * [hidden][c], mlp2_w [c][hidden]; gammas [c], qk_gamma [2 heads][head_dim] (q's
  * heads, then k's); biases, gammas and qk_gamma may be NULL. */
 typedef struct trellis_sparse_hip_block_desc {
@@ -678,7 +722,7 @@ typedef struct trellis_sparse_hip_block_desc {
     int32_t head_dim;      /* a multiple of 8, up to 192 */
     int32_t hidden;
     int32_t act;           /* trellis_sparse_hip_act */
-    int32_t rows8;         /* 0 or 1 */
+    int32_t rows8;         /* 0, 1 or 2 */
     int32_t pairs[3];      /* as in trellis_sparse_hip_rotary_desc */
     int32_t split;
     float eps;             /* of norm1 and norm2, > 0 */

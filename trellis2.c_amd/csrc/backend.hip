@@ -63,7 +63,8 @@ enum WeightLayout : int {
     kLayoutLinear16 = 9,         // storage type [co][ci] (narrow MFMA linear)
     kLayoutGemm = 10,            // as kLayoutLinearMfma, groups of 128 columns, 8 adjacent channels per lane
     kLayoutAct = 11,             // storage type [linear_act_rows(co)][ci to whole 128 bytes], zeros beyond co and ci
-    kLayoutAct8 = 12             // 8-bit rows [linear_act_rows(co)] of ci channels
+    kLayoutAct8 = 12,            // 8-bit rows [linear_act_rows(co)] of ci channels
+    kLayoutActInt8 = 13          // 8-bit integer rows, the same
 };
 
 struct StageMark {
@@ -494,6 +495,23 @@ void pack8_row(const float * v, int c, uint8_t * codes, uint8_t * scales) {
     }
 }
 
+// One row of 8-bit integer rows on the host, as the device packs features.
+void pack_int8_row(const float * v, int c, int8_t * codes, float * scale) {
+    memset(codes, 0, (size_t) rows8_width(c));
+    float most = 0.0f;
+    for (int i = 0; i < c; ++i) {
+        if (!std::isfinite(v[i])) {
+            *scale = std::nanf("");
+            return;
+        }
+        most = std::max(most, std::fabs(v[i]));
+    }
+    *scale = (float) ((double) most / 127.0);
+    if (most == 0.0f) return;
+    // (127 v is exact in 64 bits, so that a half comes out of the division as one.)
+    for (int i = 0; i < c; ++i) codes[i] = (int8_t) std::nearbyint(127.0 * (double) v[i] / (double) most);
+}
+
 int linear_act_bytes(int dt, int ci) { return (int) (((size_t) ci * dtype_bytes(dt) + 127) / 128 * 128); }
 
 trellis_status get_weight(Backend * be, const float * host, size_t count, int layout, int ci, int co,
@@ -625,6 +643,14 @@ trellis_status get_weight(Backend * be, const float * host, size_t count, int la
                           staged.data() + rows8_scales(rows, ci) + (size_t) o * (cp / 32));
             break;
         }
+        case kLayoutActInt8: {
+            const int rows = linear_act_rows(co), cp = rows8_width(ci);
+            staged.resize(rows_int8_bytes(rows, ci));
+            float * scales = (float *) (staged.data() + rows8_scales(rows, ci));
+            for (int o = 0; o < co; ++o)
+                pack_int8_row(host + (size_t) o * ci, ci, (int8_t *) staged.data() + (size_t) o * cp, scales + o);
+            break;
+        }
         case kLayoutVector: {
             staged.resize(count * sizeof(float));
             memcpy(staged.data(), host, count * sizeof(float));
@@ -731,7 +757,7 @@ trellis_status op_upload_i32(trellis_sparse_backend * backend, const int32_t * s
 
 trellis_status op_download_f32(trellis_sparse_backend * backend, const trellis_sparse_buffer * src, float * dst,
                                size_t count) {
-    if (backend == nullptr || src == nullptr || dst == nullptr || count > src->count || src->dtype == kRows8) {
+    if (backend == nullptr || src == nullptr || dst == nullptr || count > src->count || is_rows8(src->dtype)) {
         return TRELLIS_STATUS_INVALID_ARGUMENT;
     }
     Backend * be = as_backend(backend);
@@ -2095,9 +2121,17 @@ Span packed(const trellis_sparse_buffer * b, int64_t n, int64_t c) {
     return Span{(const char *) b->ptr, n, w, w};
 }
 
-bool rows8_ok(const trellis_sparse_buffer * b, int64_t n, int c) {
-    return b != nullptr && b->dtype == kRows8 && b->rows == n && b->width == c;
+// The offsets of n_seqs sequences (none: nullptr).
+Span offset_span(const trellis_sparse_buffer * b, int n_seqs) {
+    if (b == nullptr) return Span{nullptr, 0, 0, 0};
+    return Span{(const char *) b->ptr, (int64_t) n_seqs + 1, 4, 4};
 }
+
+// 8-bit rows (n, c) of either kind.
+bool rows8_ok(const trellis_sparse_buffer * b, int64_t n, int c) {
+    return b != nullptr && is_rows8(b->dtype) && b->rows == n && b->width == c;
+}
+bool integer_rows(const trellis_sparse_buffer * b) { return b->dtype == kRowsInt8; }
 
 uint8_t * rows8_codes(const trellis_sparse_buffer * b) { return (uint8_t *) b->ptr; }
 uint8_t * rows8_scale_bytes(const trellis_sparse_buffer * b) {
@@ -2137,7 +2171,8 @@ template <class F> trellis_status no_throw(trellis_sparse_backend * backend, F &
     }
 }
 
-trellis_status alloc_rows8_impl(trellis_sparse_backend * backend, int64_t n, int c, trellis_sparse_buffer ** out) {
+trellis_status alloc_rows8_impl(trellis_sparse_backend * backend, int64_t n, int c, trellis_sparse_buffer ** out,
+                                int dtype = kRows8) {
     if (backend == nullptr || out == nullptr) return TRELLIS_STATUS_INVALID_ARGUMENT;
     *out = nullptr;
     Backend * be = as_backend(backend);
@@ -2148,16 +2183,17 @@ trellis_status alloc_rows8_impl(trellis_sparse_backend * backend, int64_t n, int
     auto * b = (trellis_sparse_buffer *) calloc(1, sizeof(trellis_sparse_buffer));
     if (b == nullptr) return fail(be, TRELLIS_STATUS_OUT_OF_MEMORY, "host allocation");
     DevMem m;
-    const trellis_status st = dev_alloc(be, rows8_bytes(n, c), &m);
+    const size_t bytes = dtype == kRowsInt8 ? rows_int8_bytes(n, c) : rows8_bytes(n, c);
+    const trellis_status st = dev_alloc(be, bytes, &m);
     if (st != TRELLIS_STATUS_OK) {
         free(b);
         return st;
     }
     b->ptr = m.ptr;
     b->count = (size_t) n * c;
-    b->bytes = rows8_bytes(n, c);
+    b->bytes = bytes;
     b->cap = m.bytes;
-    b->dtype = kRows8;
+    b->dtype = dtype;
     b->rows = n;
     b->width = c;
     *out = b;
@@ -2170,7 +2206,7 @@ trellis_status rms_norm_impl(trellis_sparse_backend * backend, const trellis_spa
     if (backend == nullptr) return TRELLIS_STATUS_INVALID_ARGUMENT;
     Backend * be = as_backend(backend);
     const int dt = be->policy.compute_dtype;
-    const bool to8 = y != nullptr && y->dtype == kRows8;
+    const bool to8 = y != nullptr && is_rows8(y->dtype);
     if (c <= 0 || !rows_ok(n, c) || !(eps > 0.0f) || !std::isfinite(eps) || !float_buffer_ok(be, x, (size_t) n * c) ||
         (residual != nullptr && !float_buffer_ok(be, residual, (size_t) n * c)) ||
         (total != nullptr && !float_buffer_ok(be, total, (size_t) n * c)) ||
@@ -2191,11 +2227,55 @@ trellis_status rms_norm_impl(trellis_sparse_backend * backend, const trellis_spa
     const void * r = residual != nullptr ? residual->ptr : nullptr;
     void * t = total != nullptr ? total->ptr : nullptr;
     const hipError_t err =
-        to8 ? launch_rms_norm8(dt, x->ptr, r, (const float *) g, t, rows8_codes(y), rows8_scale_bytes(y), n, c, eps,
+        to8 && integer_rows(y)
+            ? launch_rows_int8(dt, true, x->ptr, r, (const float *) g, t, (int8_t *) y->ptr, (float *) rows8_scale_bytes(y), n,
+                               c, eps, be->cus, be->stream)
+        : to8 ? launch_rms_norm8(dt, x->ptr, r, (const float *) g, t, rows8_codes(y), rows8_scale_bytes(y), n, c, eps,
                                be->cus, be->stream)
             : launch_rms_norm(dt, x->ptr, r, (const float *) g, t, y->ptr, n, c, eps, be->cus, be->stream);
     stage_end(be, TRELLIS_SPARSE_HIP_STAGE_ELEMENTWISE);
     return hip_status(be, err, "rms_norm");
+}
+
+trellis_status group_norm_impl(trellis_sparse_backend * backend, const trellis_sparse_buffer * x,
+                               const trellis_sparse_buffer * offsets, int n_seqs, const float * gamma, const float * beta,
+                               trellis_sparse_buffer * y, int64_t n, int c, int groups, float eps, int act) {
+    if (backend == nullptr) return TRELLIS_STATUS_INVALID_ARGUMENT;
+    Backend * be = as_backend(backend);
+    if (c <= 0 || !rows_ok(n, c) || groups <= 0 || c % groups != 0 || !(eps > 0.0f) || !std::isfinite(eps) ||
+        act < TRELLIS_SPARSE_HIP_ACT_NONE || act > TRELLIS_SPARSE_HIP_ACT_GELU_TANH || n_seqs <= 0 ||
+        (offsets == nullptr && n_seqs != 1) || !float_buffer_ok(be, x, (size_t) n * c) ||
+        !float_buffer_ok(be, y, (size_t) n * c)) {
+        return fail(be, TRELLIS_STATUS_INVALID_ARGUMENT, "group_norm: bad argument");
+    }
+    if (offsets != nullptr && (offsets->dtype >= 0 || offsets->count < (size_t) n_seqs + 1)) {
+        return fail(be, TRELLIS_STATUS_INVALID_ARGUMENT, "group_norm: offsets are int32 [n_seqs + 1]");
+    }
+    const Span sx = packed(x, n, c), sy = packed(y, n, c), so = offset_span(offsets, n_seqs);
+    if (spans_clash(sy, sx, true) || spans_clash(sy, so, false)) {
+        return fail(be, TRELLIS_STATUS_INVALID_ARGUMENT, "group_norm: overlapping rows");
+    }
+    DeviceScope scope(be);
+    const void *g = nullptr, *b = nullptr;
+    trellis_status st = get_weight(be, gamma, (size_t) c, kLayoutVector, 0, c, &g);
+    if (st == TRELLIS_STATUS_OK) st = get_weight(be, beta, (size_t) c, kLayoutVector, 0, c, &b);
+    if (st != TRELLIS_STATUS_OK) return st;
+    GroupNorm p{};
+    p.x = x->ptr;
+    p.y = y->ptr;
+    p.at = offsets != nullptr ? (const int32_t *) offsets->ptr : nullptr;
+    p.gamma = (const float *) g;
+    p.beta = (const float *) b;
+    p.n = n;
+    p.seqs = n_seqs;
+    p.c = c;
+    p.groups = groups;
+    p.act = act;
+    p.eps = eps;
+    stage_begin(be, TRELLIS_SPARSE_HIP_STAGE_ELEMENTWISE);
+    const hipError_t err = launch_group_norm(be->policy.compute_dtype, p, be->stream);
+    stage_end(be, TRELLIS_SPARSE_HIP_STAGE_ELEMENTWISE);
+    return hip_status(be, err, "group_norm");
 }
 
 trellis_status pack_rows8_impl(trellis_sparse_backend * backend, const trellis_sparse_buffer * x,
@@ -2207,8 +2287,12 @@ trellis_status pack_rows8_impl(trellis_sparse_backend * backend, const trellis_s
     }
     DeviceScope scope(be);
     stage_begin(be, TRELLIS_SPARSE_HIP_STAGE_ELEMENTWISE);
-    const hipError_t err = launch_pack8(be->policy.compute_dtype, x->ptr, rows8_codes(rows8),
-                                        rows8_scale_bytes(rows8), n, c, be->cus, be->stream);
+    const int dt = be->policy.compute_dtype;
+    const hipError_t err =
+        integer_rows(rows8) ? launch_rows_int8(dt, false, x->ptr, nullptr, nullptr, nullptr, (int8_t *) rows8->ptr,
+                                               (float *) rows8_scale_bytes(rows8), n, c, 0.0f, be->cus, be->stream)
+                            : launch_pack8(dt, x->ptr, rows8_codes(rows8), rows8_scale_bytes(rows8), n, c, be->cus,
+                                           be->stream);
     stage_end(be, TRELLIS_SPARSE_HIP_STAGE_ELEMENTWISE);
     return hip_status(be, err, "pack_rows8");
 }
@@ -2222,8 +2306,11 @@ trellis_status expand_rows8_impl(trellis_sparse_backend * backend, const trellis
     }
     DeviceScope scope(be);
     stage_begin(be, TRELLIS_SPARSE_HIP_STAGE_ELEMENTWISE);
-    const hipError_t err = launch_expand8(be->policy.compute_dtype, rows8_codes(rows8), rows8_scale_bytes(rows8),
-                                          y->ptr, n, c, be->stream);
+    const int dt = be->policy.compute_dtype;
+    const hipError_t err =
+        integer_rows(rows8) ? launch_expand_int8(dt, (const int8_t *) rows8->ptr, (const float *) rows8_scale_bytes(rows8),
+                                                 y->ptr, n, c, be->stream)
+                            : launch_expand8(dt, rows8_codes(rows8), rows8_scale_bytes(rows8), y->ptr, n, c, be->stream);
     stage_end(be, TRELLIS_SPARSE_HIP_STAGE_ELEMENTWISE);
     return hip_status(be, err, "expand_rows8");
 }
@@ -2234,7 +2321,7 @@ trellis_status linear_act_impl(trellis_sparse_backend * backend, const trellis_s
     if (backend == nullptr) return TRELLIS_STATUS_INVALID_ARGUMENT;
     Backend * be = as_backend(backend);
     const int dt = be->policy.compute_dtype;
-    const bool from8 = x != nullptr && x->dtype == kRows8;
+    const bool from8 = x != nullptr && is_rows8(x->dtype);
     if (weight == nullptr || ci <= 0 || co <= 0 || !rows_ok(n, ci) || !rows_ok(n, co) ||
         act < TRELLIS_SPARSE_HIP_ACT_NONE || act > TRELLIS_SPARSE_HIP_ACT_GELU_TANH ||
         !(from8 ? rows8_ok(x, n, ci) : float_buffer_ok(be, x, (size_t) n * ci)) ||
@@ -2245,6 +2332,10 @@ trellis_status linear_act_impl(trellis_sparse_backend * backend, const trellis_s
     if ((int64_t) ci * 4 > kLinearActMaxBytes || (int64_t) co * 4 > kLinearActMaxBytes) {
         return fail(be, TRELLIS_STATUS_INVALID_ARGUMENT, "linear_act: rows too wide");
     }
+    const int x_type = from8 ? x->dtype : dt;
+    if (x_type == kRowsInt8 && ci > kIntMostTerms) {
+        return fail(be, TRELLIS_STATUS_INVALID_ARGUMENT, "linear_act: sums of integers beyond 32 bits");
+    }
     if ((!from8 && spans_clash(packed(y, n, co), packed(x, n, ci), false)) ||
         spans_clash(packed(y, n, co), packed(residual, n, co), true)) {
         return fail(be, TRELLIS_STATUS_INVALID_ARGUMENT, "linear_act: overlapping rows");
@@ -2253,7 +2344,8 @@ trellis_status linear_act_impl(trellis_sparse_backend * backend, const trellis_s
     LinearAct p{};
     const void *w = nullptr, *b = nullptr;
     trellis_status st =
-        get_weight(be, weight, (size_t) ci * co, from8 ? kLayoutAct8 : kLayoutAct, ci, co, &w);
+        get_weight(be, weight, (size_t) ci * co,
+                   !from8 ? kLayoutAct : (x_type == kRowsInt8 ? kLayoutActInt8 : kLayoutAct8), ci, co, &w);
     if (st == TRELLIS_STATUS_OK) st = get_weight(be, bias, (size_t) co, kLayoutVector, 0, co, &b);
     if (st != TRELLIS_STATUS_OK) return st;
     p.x = x->ptr;
@@ -2275,7 +2367,6 @@ trellis_status linear_act_impl(trellis_sparse_backend * backend, const trellis_s
     p.act = act;
     p.cus = be->cus;
     // Without scratch for split sums a block takes all of K.
-    const int x_type = from8 ? kRows8 : dt;
     LinearActPlan plan = linear_act_plan(dt, x_type, n, co, p.row_bytes, p.w_bytes, be->cus, true);
     if (scratch_clash(be, plan.scratch, {packed(y, n, co), packed(residual, n, co), from8 ? Span{} : packed(x, n, ci)})) {
         return fail(be, TRELLIS_STATUS_INVALID_ARGUMENT, "linear_act: rows in the scratch");
@@ -2306,12 +2397,6 @@ Span strided(const Backend * be, const trellis_sparse_buffer * b, int64_t n, int
              int64_t stride) {
     const int64_t e = (int64_t) dtype_bytes(be->policy.compute_dtype);
     return Span{(const char *) b->ptr + offset * e, n, width * e, stride * e};
-}
-
-// The offsets of n_seqs sequences (none: nullptr).
-Span offset_span(const trellis_sparse_buffer * b, int n_seqs) {
-    if (b == nullptr) return Span{nullptr, 0, 0, 0};
-    return Span{(const char *) b->ptr, (int64_t) n_seqs + 1, 4, 4};
 }
 
 trellis_status rotary_impl(trellis_sparse_backend * backend, const trellis_sparse_buffer * x,
@@ -2373,11 +2458,40 @@ trellis_status rotary_impl(trellis_sparse_backend * backend, const trellis_spars
     return hip_status(be, err, "rotary");
 }
 
+// What attention_scored adds to a call's checks; `scale` is the products', times log2(e).
+trellis_status check_scores(Backend * be, const trellis_sparse_hip_scores_desc & d, int64_t nq, int64_t nkv, int n_seqs,
+                            int heads, float scale) {
+    if (d.struct_size != sizeof(d)) return fail(be, TRELLIS_STATUS_INVALID_ARGUMENT, "attention: bad scores desc");
+    if ((d.causal != 0 && d.causal != 1) || !(d.cap >= 0.0f) || (d.prefix != nullptr && d.causal == 0) ||
+        ((d.q_coords != nullptr || d.k_coords != nullptr) && d.slopes == nullptr) ||
+        (d.q_coords == nullptr && d.k_coords != nullptr) || (d.q_coords != nullptr && d.k_coords == nullptr && nkv > 0)) {
+        return fail(be, TRELLIS_STATUS_INVALID_ARGUMENT, "attention: bad scores");
+    }
+    // Twice the tanh's argument and the cap, both in log2 units, are taken with numbers of fp32.
+    if (!std::isfinite(d.cap * 1.4426950f) || (d.cap > 0.0f && !std::isfinite(2.0f * scale / d.cap))) {
+        return fail(be, TRELLIS_STATUS_INVALID_ARGUMENT, "attention: cap beyond fp32's range");
+    }
+    if (d.slopes != nullptr) {
+        for (int h = 0; h < heads; ++h)
+            if (!(std::fabs(d.slopes[h]) <= 0x1p+64f))
+                return fail(be, TRELLIS_STATUS_INVALID_ARGUMENT, "attention: slopes up to 2^64");
+    }
+    const auto ints = [](const trellis_sparse_buffer * b, size_t count) {
+        return b == nullptr || (b->dtype < 0 && b->count >= count);
+    };
+    if (!ints(d.q_coords, (size_t) nq * 4) || !ints(d.k_coords, (size_t) nkv * 4) || !ints(d.prefix, (size_t) n_seqs)) {
+        return fail(be, TRELLIS_STATUS_INVALID_ARGUMENT, "attention: coordinates are int32 [rows][4], prefixes int32 [n_seqs]");
+    }
+    return TRELLIS_STATUS_OK;
+}
+
+// attention, and with `scores` attention_scored.
 trellis_status attention_impl(trellis_sparse_backend * backend, const trellis_sparse_buffer * q,
                               const trellis_sparse_buffer * k, const trellis_sparse_buffer * v,
                               trellis_sparse_buffer * y, int64_t nq, int64_t nkv,
                               const trellis_sparse_buffer * q_offsets, const trellis_sparse_buffer * kv_offsets,
-                              int n_seqs, const trellis_sparse_hip_attention_desc * desc) {
+                              int n_seqs, const trellis_sparse_hip_attention_desc * desc,
+                              const trellis_sparse_hip_scores_desc * scores = nullptr) {
     if (backend == nullptr) return TRELLIS_STATUS_INVALID_ARGUMENT;
     Backend * be = as_backend(backend);
     if (desc == nullptr || desc->struct_size != sizeof(*desc)) {
@@ -2403,6 +2517,10 @@ trellis_status attention_impl(trellis_sparse_backend * backend, const trellis_sp
             return fail(be, TRELLIS_STATUS_INVALID_ARGUMENT, "attention: offsets are int32 [n_seqs + 1]");
         }
     }
+    if (scores != nullptr) {
+        const trellis_status st = check_scores(be, *scores, nq, nkv, n_seqs, d.heads, scale);
+        if (st != TRELLIS_STATUS_OK) return st;
+    }
     const int64_t qw = (int64_t) d.heads * d.head_dim, kw = (int64_t) d.kv_heads * d.head_dim;
     const int64_t nk = nkv > 0 ? nkv : 1;
     int64_t qs = d.q_stride, ks = d.k_stride, vs = d.v_stride, ys = d.y_stride;
@@ -2424,7 +2542,32 @@ trellis_status attention_impl(trellis_sparse_backend * backend, const trellis_sp
     if (spans_clash(sy, sq, true) || spans_clash(sy, sk, false) || spans_clash(sy, sv, false)) {
         return fail(be, TRELLIS_STATUS_INVALID_ARGUMENT, "attention: overlapping rows");
     }
+    Span sqc{}, skc{}, spf{};
+    if (scores != nullptr) {
+        const auto whole = [](const trellis_sparse_buffer * b, int64_t bytes) {
+            return b != nullptr ? Span{(const char *) b->ptr, 1, bytes, bytes} : Span{};
+        };
+        sqc = whole(scores->q_coords, nq * 16);
+        skc = whole(scores->k_coords, nkv * 16);
+        spf = whole(scores->prefix, (int64_t) n_seqs * 4);
+        if (spans_clash(sy, sqc, false) || spans_clash(sy, skc, false) || spans_clash(sy, spf, false)) {
+            return fail(be, TRELLIS_STATUS_INVALID_ARGUMENT, "attention: overlapping rows");
+        }
+    }
     DeviceScope scope(be);
+    Scores sc{};
+    if (scores != nullptr) {
+        const void * slopes = nullptr;
+        const trellis_status st = get_weight(be, scores->slopes, (size_t) d.heads, kLayoutVector, 0, d.heads, &slopes);
+        if (st != TRELLIS_STATUS_OK) return st;
+        sc.slopes = (const float *) slopes;
+        sc.cap = scores->cap * 1.4426950408889634f;
+        sc.cap_scale = scores->cap > 0.0f ? (float) (natural / (double) scores->cap) : 0.0f;
+        sc.q_xyz = (const int32_t *) sqc.at;
+        sc.k_xyz = (const int32_t *) skc.at;
+        sc.prefix = (const int32_t *) spf.at;
+        sc.causal = scores->causal;
+    }
     Attention p{};
     p.q = sq.at;
     p.k = sk.at;
@@ -2443,6 +2586,12 @@ trellis_status attention_impl(trellis_sparse_backend * backend, const trellis_sp
     p.kv_heads = d.kv_heads;
     p.dim = d.head_dim;
     p.scale = scale;
+    if (scores != nullptr) {
+        stage_begin(be, TRELLIS_SPARSE_HIP_STAGE_ELEMENTWISE);
+        const hipError_t err = launch_attention_scored(be->policy.compute_dtype, p, sc, be->stream);
+        stage_end(be, TRELLIS_SPARSE_HIP_STAGE_ELEMENTWISE);
+        return hip_status(be, err, "attention_scored");
+    }
     // Without scratch for split keys one block takes all of a query's keys.
     const AttentionShape shape = attention_shape(be->policy.compute_dtype, p, be->cus);
     if (scratch_clash(be, shape.scratch, {sq, sk, sv, sy, sqo, sko})) {
@@ -2484,7 +2633,7 @@ trellis_status transformer_block_impl(trellis_sparse_backend * backend, const tr
     const int64_t wide = (int64_t) d.heads * d.head_dim;
     if (n <= 0 || n > INT32_MAX || d.heads <= 0 || d.heads > 32768 || d.head_dim <= 0 || d.hidden <= 0 ||
         wide > (1 << 18) || d.hidden > (1 << 20) || d.qkv_w == nullptr || d.out_w == nullptr || d.mlp0_w == nullptr ||
-        d.mlp2_w == nullptr || (d.rows8 != 0 && d.rows8 != 1) || !float_buffer_ok(be, h, (size_t) (n * wide)) ||
+        d.mlp2_w == nullptr || d.rows8 < 0 || d.rows8 > 2 || !float_buffer_ok(be, h, (size_t) (n * wide)) ||
         !float_buffer_ok(be, out, (size_t) (n * wide)) || spans_clash(packed(out, n, wide), packed(h, n, wide), true)) {
         return fail(be, TRELLIS_STATUS_INVALID_ARGUMENT, "transformer_block: bad argument");
     }
@@ -2501,8 +2650,9 @@ trellis_status transformer_block_impl(trellis_sparse_backend * backend, const tr
     trellis_status st = op_alloc_f32(backend, (size_t) n * c, &row.b);
     if (st == TRELLIS_STATUS_OK) st = op_alloc_f32(backend, (size_t) n * 3 * c, &qkv.b);
     if (st == TRELLIS_STATUS_OK) st = op_alloc_f32(backend, (size_t) n * d.hidden, &hid.b);
-    if (st == TRELLIS_STATUS_OK && d.rows8) st = alloc_rows8_impl(backend, n, c, &row8.b);
-    if (st == TRELLIS_STATUS_OK && d.rows8) st = alloc_rows8_impl(backend, n, d.hidden, &hid8.b);
+    const int kind8 = d.rows8 == 2 ? kRowsInt8 : kRows8;
+    if (st == TRELLIS_STATUS_OK && d.rows8) st = alloc_rows8_impl(backend, n, c, &row8.b, kind8);
+    if (st == TRELLIS_STATUS_OK && d.rows8) st = alloc_rows8_impl(backend, n, d.hidden, &hid8.b, kind8);
     trellis_sparse_buffer * normed = d.rows8 ? row8.b : row.b;
 
     trellis_sparse_hip_rotary_desc rot{};
@@ -2953,7 +3103,7 @@ trellis_status trellis_sparse_hip_upload_raw(trellis_sparse_backend * backend, c
 
 trellis_status trellis_sparse_hip_download_raw(trellis_sparse_backend * backend, const trellis_sparse_buffer * src,
                                                void * dst, size_t count) {
-    if (backend == nullptr || src == nullptr || dst == nullptr || count > src->count || src->dtype == tsh::kRows8) {
+    if (backend == nullptr || src == nullptr || dst == nullptr || count > src->count || tsh::is_rows8(src->dtype)) {
         return TRELLIS_STATUS_INVALID_ARGUMENT;
     }
     Backend * be = tsh::as_backend(backend);
@@ -3133,7 +3283,7 @@ trellis_status trellis_sparse_hip_set_stream(trellis_sparse_backend * backend, v
 trellis_status trellis_sparse_hip_set_scratch(trellis_sparse_backend * backend, const trellis_sparse_buffer * scratch) {
     if (backend == nullptr) return TRELLIS_STATUS_INVALID_ARGUMENT;
     tsh::Backend * be = tsh::as_backend(backend);
-    if (scratch != nullptr && (scratch->ptr == nullptr || scratch->dtype == tsh::kRows8)) {
+    if (scratch != nullptr && (scratch->ptr == nullptr || tsh::is_rows8(scratch->dtype))) {
         return tsh::fail(be, TRELLIS_STATUS_INVALID_ARGUMENT, "set_scratch: a buffer of rows or int32");
     }
     tsh::set_scratch(be, scratch);
@@ -3152,6 +3302,22 @@ trellis_status trellis_sparse_hip_alloc_rows8(trellis_sparse_backend * backend, 
                                               trellis_sparse_buffer ** out) {
     return tsh::no_throw(backend, [&] {
         return tsh::alloc_rows8_impl(backend, n, c, out);
+    });
+}
+
+trellis_status trellis_sparse_hip_alloc_rows_int8(trellis_sparse_backend * backend, int64_t n, int c,
+                                                  trellis_sparse_buffer ** out) {
+    return tsh::no_throw(backend, [&] {
+        return tsh::alloc_rows8_impl(backend, n, c, out, tsh::kRowsInt8);
+    });
+}
+
+trellis_status trellis_sparse_hip_group_norm(trellis_sparse_backend * backend, const trellis_sparse_buffer * x,
+                                             const trellis_sparse_buffer * offsets, int n_seqs, const float * gamma,
+                                             const float * beta, trellis_sparse_buffer * y, int64_t n, int c, int groups,
+                                             float eps, int act) {
+    return tsh::no_throw(backend, [&] {
+        return tsh::group_norm_impl(backend, x, offsets, n_seqs, gamma, beta, y, n, c, groups, eps, act);
     });
 }
 
@@ -3204,6 +3370,21 @@ trellis_status trellis_sparse_hip_attention(trellis_sparse_backend * backend, co
                                             const trellis_sparse_hip_attention_desc * desc) {
     return tsh::no_throw(backend, [&] {
         return tsh::attention_impl(backend, q, k, v, y, nq, nkv, q_offsets, kv_offsets, n_seqs, desc);
+    });
+}
+
+trellis_status trellis_sparse_hip_attention_scored(trellis_sparse_backend * backend, const trellis_sparse_buffer * q,
+                                                   const trellis_sparse_buffer * k, const trellis_sparse_buffer * v,
+                                                   trellis_sparse_buffer * y, int64_t nq, int64_t nkv,
+                                                   const trellis_sparse_buffer * q_offsets,
+                                                   const trellis_sparse_buffer * kv_offsets, int n_seqs,
+                                                   const trellis_sparse_hip_attention_desc * desc,
+                                                   const trellis_sparse_hip_scores_desc * scores) {
+    return tsh::no_throw(backend, [&] {
+        if (backend != nullptr && scores == nullptr) {
+            return tsh::fail(tsh::as_backend(backend), TRELLIS_STATUS_INVALID_ARGUMENT, "attention: bad scores desc");
+        }
+        return tsh::attention_impl(backend, q, k, v, y, nq, nkv, q_offsets, kv_offsets, n_seqs, desc, scores);
     });
 }
 

@@ -122,7 +122,9 @@ __device__ __forceinline__ void store_adjacent(__amdgpu_buffer_rsrc_t rsrc, uint
 
 // ---- MFMA GEMM ----------------------------------------------------------------------------------
 
+typedef int i32x4 __attribute__((ext_vector_type(4)));
 typedef int i32x8 __attribute__((ext_vector_type(8)));
+typedef int i32x16 __attribute__((ext_vector_type(16)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 
 // A fragment is two 16-byte chunks, h and h + 2 for lane half h = lane / 32, of
@@ -137,9 +139,19 @@ struct Frag {
     int4 c[2];
 };
 
+// Sums of integer rows are whole numbers of 32 bits, exact for up to 131,072 products.
+template <int MT> using Sums = typename std::conditional<MT == kRowsInt8, i32x16, f32x16>::type;
+
 // SEL: which of a scale register's bytes counts (0 or 2).
-template <int MT, int SEL> __device__ __forceinline__ f32x16 mac(const Frag & a, const Frag & b, f32x16 c, int sa, int sb) {
-    if constexpr (MT == kF32) {
+template <int MT, int SEL>
+__device__ __forceinline__ Sums<MT> mac(const Frag & a, const Frag & b, Sums<MT> c, int sa, int sb) {
+    if constexpr (MT == kRowsInt8) {
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+            c = __builtin_amdgcn_mfma_i32_32x32x32_i8(__builtin_bit_cast(i32x4, a.c[e]), __builtin_bit_cast(i32x4, b.c[e]), c,
+                                                      0, 0, 0);
+        return c;
+    } else if constexpr (MT == kF32) {
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
             const f32x4 x = __builtin_bit_cast(f32x4, a.c[e]), w = __builtin_bit_cast(f32x4, b.c[e]);
@@ -217,7 +229,7 @@ template <int MT, int DT, int RW, int CW, int RB, int NT, int PER_CU>
 __global__ void __launch_bounds__(64 * RW * CW, RW * CW * PER_CU / 4) k_linear_act(LinearAct p) {
     using T = typename Store<DT>::T;
     constexpr int NW = RW * CW, BM = RW * RB * 32, BN = CW * NT * 32;
-    constexpr bool kScaled = MT == kRows8;
+    constexpr bool kScaled = MT == kRows8, kInt = MT == kRowsInt8;
     constexpr bool kMaySplit = BM * BN < 256 * 256;  // the largest blocks have no registers for it
     constexpr int kRows = BM + BN, kBytes = kRows * 128, kSlot = kBytes + (kScaled ? kRows * 4 : 0);
     // Loads of 1 KB (8 rows) per step and wavefront, of x and of W.
@@ -295,7 +307,8 @@ __global__ void __launch_bounds__(64 * RW * CW, RW * CW * PER_CU / 4) k_linear_a
                                                  some ? BN * p.w_bytes : 0, 0x00020000);
         if constexpr (kScaled) {
             const uint8_t * base =
-                scales_of_x ? p.x_scales + next_row0 * scale_pitch : p.w_scales + (int64_t) next_col0 * scale_pitch;
+                scales_of_x ? (const uint8_t *) p.x_scales + next_row0 * scale_pitch
+                            : (const uint8_t *) p.w_scales + (int64_t) next_col0 * scale_pitch;
             sres = __builtin_amdgcn_make_buffer_rsrc((void *) base, 0, some ? (scales_of_x ? rows : BN) * scale_pitch : 0,
                                                      0x00020000);
         }
@@ -332,19 +345,30 @@ __global__ void __launch_bounds__(64 * RW * CW, RW * CW * PER_CU / 4) k_linear_a
     const int ch0 = (cw * 32 + l32) * NT;
     const __amdgpu_buffer_rsrc_t bres = __builtin_amdgcn_make_buffer_rsrc(
         (void *) p.bias, 0, p.bias != nullptr && (!kMaySplit || p.splits == 1) ? p.co * 4 : 0, 0x00020000);
-    Adjacent<kF32, NT> bias;
-    const auto load_bias = [&]() { bias = load_adjacent<kF32, NT>(bres, (uint32_t) ((col0 + ch0) * 4), 0); };
-    load_bias();
-    f32x16 acc[RB][NT];
+    // (Channels past co have scales too: those of w's rows up to whole blocks.)
+    const __amdgpu_buffer_rsrc_t cres = __builtin_amdgcn_make_buffer_rsrc(
+        (void *) p.w_scales, 0, kInt ? p.col_tiles * BN * 4 : 0, 0x00020000);
+    Adjacent<kF32, NT> bias, channel_scale;
+    const auto load_bias = [&]() {
+        bias = load_adjacent<kF32, NT>(bres, (uint32_t) ((col0 + ch0) * 4), 0);
+        if constexpr (kInt) channel_scale = load_adjacent<kF32, NT>(cres, (uint32_t) ((col0 + ch0) * 4), 0);
+    };
+    if constexpr (!kInt) load_bias();
+    Sums<MT> acc[RB][NT];
     const auto begin = [&]() {
 #pragma unroll
         for (int t = 0; t < NT; ++t)
 #pragma unroll
             for (int q = 0; q < RB; ++q) {
-                float b = bias.h[t];
-                asm volatile("" : "+v"(b));  // else 16 copies of it are made with the load, and wait in memory
+                if constexpr (kInt) {
 #pragma unroll
-                for (int i = 0; i < 16; ++i) acc[q][t][i] = b;
+                    for (int i = 0; i < 16; ++i) acc[q][t][i] = 0;
+                } else {
+                    float b = bias.h[t];
+                    asm volatile("" : "+v"(b));  // else 16 copies of it are made with the load, and wait in memory
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) acc[q][t][i] = b;
+                }
             }
     };
     begin();
@@ -415,7 +439,11 @@ __global__ void __launch_bounds__(64 * RW * CW, RW * CW * PER_CU / 4) k_linear_a
                 for (int i = 0; i < 16; ++i) {
                     float v[NT];
 #pragma unroll
-                    for (int t = 0; t < NT; ++t) v[t] = acc[q][t][i];
+                    for (int t = 0; t < NT; ++t) {
+                        // (Of an element of a vector in place the cast takes another.)
+                        const auto sum = acc[q][t][i];
+                        v[t] = __builtin_bit_cast(float, sum);
+                    }
                     store_adjacent<kF32, NT>(pres, to, (uint32_t) ((q * 32 + i / 4 * 8 + i % 4) * p.co * 4), v);
                 }
             return;
@@ -427,11 +455,17 @@ __global__ void __launch_bounds__(64 * RW * CW, RW * CW * PER_CU / 4) k_linear_a
             (char *) (p.residual != nullptr ? p.residual : p.y) + row0 * pitch, 0, rows * pitch, 0x00020000);
         const uint32_t at =
             ch < p.co ? (uint32_t) ((rw * RB * 32 + 4 * half) * pitch + ch * (int) sizeof(T)) : kOutside;
+        const __amdgpu_buffer_rsrc_t sres = __builtin_amdgcn_make_buffer_rsrc(
+            (void *) ((const float *) p.x_scales + (kInt ? row0 : 0)), 0, kInt ? rows * 4 : 0, 0x00020000);
         const auto finish = [&](auto act_c, auto res_c) {
-            // Four rows at a time, the next four's residuals on their way.
+            // Four rows at a time, the next four's residuals (and scales) on their way.
             constexpr bool kRes = decltype(res_c)::value;
             Adjacent<DT, NT> r[2][4];
+            Adjacent<kF32, 4> row_scale[2];
             const auto fetch = [&](int k) {
+                if constexpr (kInt)
+                    row_scale[k % 2] = load_adjacent<kF32, 4>(sres, (uint32_t) ((rw * RB * 32 + 4 * half) * 4),
+                                                              (uint32_t) ((k / 4 * 32 + k % 4 * 8) * 4));
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
                     if constexpr (kRes)
@@ -446,7 +480,14 @@ __global__ void __launch_bounds__(64 * RW * CW, RW * CW * PER_CU / 4) k_linear_a
                     float v[NT];
 #pragma unroll
                     for (int t = 0; t < NT; ++t) {
-                        v[t] = activate<DT, decltype(act_c)::value>(acc[k / 4][t][4 * (k % 4) + i]);
+                        float z;
+                        if constexpr (kInt) {
+                            z = fmaf((float) acc[k / 4][t][4 * (k % 4) + i] * row_scale[k % 2].h[i], channel_scale.h[t],
+                                     bias.h[t]);
+                        } else {
+                            z = acc[k / 4][t][4 * (k % 4) + i];
+                        }
+                        v[t] = activate<DT, decltype(act_c)::value>(z);
                         if constexpr (kRes) v[t] += Store<DT>::ld(r[k % 2][i].h, t);
                     }
                     store_adjacent<DT, NT>(yres, at, (uint32_t) ((k / 4 * 32 + k % 4 * 8 + i) * pitch), v);
@@ -495,6 +536,7 @@ __global__ void __launch_bounds__(64 * RW * CW, RW * CW * PER_CU / 4) k_linear_a
         }
         if (stop < steps) {
             stop = steps;
+            if constexpr (kInt) load_bias();  // of this tile, for its outputs
             more = unit + stride < end ? 1 : 0;
             if (more) place(unit + stride);
             aim(more);
@@ -506,7 +548,7 @@ __global__ void __launch_bounds__(64 * RW * CW, RW * CW * PER_CU / 4) k_linear_a
         row0 = next_row0;
         col0 = next_col0;
         unit += stride;
-        if (unit < end) load_bias();
+        if (!kInt && unit < end) load_bias();
         leave(row, col);
         if (unit >= end) break;
         s = first_step;
@@ -521,26 +563,38 @@ __global__ void __launch_bounds__(64 * RW * CW, RW * CW * PER_CU / 4) k_linear_a
 // Joins the splits' sums in their order, then bias, activation and residual: N
 // adjacent outputs a thread (N divides co).  One row 1024 -> 4096 fp16: 4.8 us of products
 // and 2.6 here.
-template <int DT, int N> __global__ void __launch_bounds__(256) k_linear_join(LinearAct p) {
+template <bool INT, int DT, int N> __global__ void __launch_bounds__(256) k_linear_join(LinearAct p) {
     using T = typename Store<DT>::T;
+    using Sum = typename std::conditional<INT, int, float>::type;
     const int64_t e = ((int64_t) blockIdx.x * 256 + threadIdx.x) * N, count = p.n * p.co;
     if (e >= count) return;
     const int ch = (int) (e % p.co);
-    float v[N];
+    Sum sum[N];
 #pragma unroll
-    for (int u = 0; u < N; ++u) v[u] = p.bias != nullptr ? p.bias[ch + u] : 0.0f;
+    for (int u = 0; u < N; ++u) sum[u] = !INT && p.bias != nullptr ? (Sum) p.bias[ch + u] : (Sum) 0;
 #pragma unroll 4
     for (int s = 0; s < p.splits; ++s) {
-        const float * q = p.partial + s * count + e;
+        const Sum * q = (const Sum *) p.partial + s * count + e;
         if constexpr (N == 4) {
-            const float4 c = *(const float4 *) q;
-            v[0] += c.x;
-            v[1] += c.y;
-            v[2] += c.z;
-            v[3] += c.w;
+            struct alignas(16) Four {
+                Sum c[4];
+            };
+            const Four f = *(const Four *) q;
+#pragma unroll
+            for (int u = 0; u < N; ++u) sum[u] += f.c[u];
         } else {
 #pragma unroll
-            for (int u = 0; u < N; ++u) v[u] += q[u];
+            for (int u = 0; u < N; ++u) sum[u] += q[u];
+        }
+    }
+    float v[N];
+#pragma unroll
+    for (int u = 0; u < N; ++u) {
+        if constexpr (INT) {
+            v[u] = fmaf((float) sum[u] * ((const float *) p.x_scales)[e / p.co], ((const float *) p.w_scales)[ch + u],
+                        p.bias != nullptr ? p.bias[ch + u] : 0.0f);
+        } else {
+            v[u] = sum[u];
         }
     }
     const T * residual = (const T *) p.residual;
@@ -642,7 +696,7 @@ constexpr Blocks kBlocks[] = {
 constexpr double kOnce = 1.5;
 constexpr int kShapes = sizeof(kBlocks) / sizeof(kBlocks[0]);
 
-inline float step_us(const Blocks & b, int mt) { return mt == kF32 ? b.step32 : (mt == kRows8 ? b.step8 : b.step16); }
+inline float step_us(const Blocks & b, int mt) { return mt == kF32 ? b.step32 : (is_rows8(mt) ? b.step8 : b.step16); }
 
 struct Choice {
     int shape = -1, splits = 1;
@@ -704,9 +758,9 @@ hipError_t launch_shape(LinearAct p, const Blocks & b, hipStream_t s) {
         const int64_t joins = (p.n * p.co + (four ? 1023 : 255)) / (four ? 1024 : 256);
         if (joins > 0x7fffffffLL) return hipErrorInvalidValue;
         if (four) {
-            k_linear_join<DT, 4><<<(unsigned) joins, 256, 0, s>>>(p);
+            k_linear_join<MT == kRowsInt8, DT, 4><<<(unsigned) joins, 256, 0, s>>>(p);
         } else {
-            k_linear_join<DT, 1><<<(unsigned) joins, 256, 0, s>>>(p);
+            k_linear_join<MT == kRowsInt8, DT, 1><<<(unsigned) joins, 256, 0, s>>>(p);
         }
         err = hipGetLastError();
     }
@@ -743,13 +797,15 @@ template <int DT> hipError_t launch_dt(const LinearAct & p, int x_type, const Li
         LinearAct q = p;
         const int64_t e = (int64_t) sizeof(typename Store<DT>::T);
         q.x = (const char *) p.x + row * p.row_bytes;
-        if (p.x_scales != nullptr) q.x_scales = p.x_scales + row * (p.row_bytes / 32);
+        if (p.x_scales != nullptr)
+            q.x_scales = (const char *) p.x_scales + row * (x_type == kRowsInt8 ? (int64_t) sizeof(float) : p.row_bytes / 32);
         if (p.residual != nullptr) q.residual = (const char *) p.residual + row * p.co * e;
         q.y = (char *) p.y + row * p.co * e;
         q.n = part.rows;
         const int splits = p.partial != nullptr ? part.splits : 1;
-        const hipError_t err = x_type == kRows8 ? launch_gemm<kRows8, DT>(q, part.shape, splits, s)
-                                                : launch_gemm<DT, DT>(q, part.shape, splits, s);
+        const hipError_t err = x_type == kRows8      ? launch_gemm<kRows8, DT>(q, part.shape, splits, s)
+                               : x_type == kRowsInt8 ? launch_gemm<kRowsInt8, DT>(q, part.shape, splits, s)
+                                                     : launch_gemm<DT, DT>(q, part.shape, splits, s);
         if (err != hipSuccess) return err;
         row += part.rows;
     }
@@ -764,8 +820,8 @@ template <int DT> hipError_t launch_dt(const LinearAct & p, int x_type, const Li
 LinearActPlan linear_act_plan(int dtype, int x_type, int64_t n, int co, int row_bytes, int w_bytes, int cus,
                               bool may_split) {
     LinearActPlan plan{};
-    if (x_type != kRows8 && row_bytes % 16 != 0) return plan;
-    const int mt = x_type == kRows8 ? kRows8 : dtype;
+    if (!is_rows8(x_type) && row_bytes % 16 != 0) return plan;
+    const int mt = is_rows8(x_type) ? x_type : dtype;
     const auto scratch = [&](const LinearActPart & part) {
         return part.splits > 1 ? (size_t) part.splits * part.rows * co * sizeof(float) : 0;
     };

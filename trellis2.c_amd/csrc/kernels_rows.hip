@@ -1,34 +1,11 @@
-// kernels_rows.hip - row operators of transformer blocks over voxel rows: RMS norm, 8-bit rows, rotary positions.
+// kernels_rows.hip - row operators of transformer blocks over voxel rows: RMS norm, 8-bit rows (floating and integer),
+// rotary positions.
 #include <type_traits>
 
-#include "mfma_common.h"
+#include "rows_common.h"
 
 namespace tsh {
 namespace {
-
-// ---- chunks of 16 bytes -------------------------------------------------------------------------
-
-// Values per 16-byte chunk.
-template <int DT> constexpr int kChunk = DT == kF32 ? 4 : 8;
-
-template <int DT> __device__ __forceinline__ void unpack_chunk_of(const int4 & c, float * v) {
-    if constexpr (DT == kF32) {
-        v[0] = __builtin_bit_cast(float, c.x);
-        v[1] = __builtin_bit_cast(float, c.y);
-        v[2] = __builtin_bit_cast(float, c.z);
-        v[3] = __builtin_bit_cast(float, c.w);
-    } else {
-        unpack_chunk<DT>(c, v);
-    }
-}
-
-template <int DT> __device__ __forceinline__ void store_chunk(typename Store<DT>::T * p, const float * v) {
-    if constexpr (DT == kF32) {
-        *(float4 *) p = float4{v[0], v[1], v[2], v[3]};
-    } else {
-        *(int4 *) p = pack_chunk<DT>(v);
-    }
-}
 
 // ---- 8-bit rows ---------------------------------------------------------------------------------
 
@@ -336,6 +313,257 @@ hipError_t norm_dt(const void * x, const void * residual, const float * gamma, v
     return launch(integral_constant<int, 64>(), integral_constant<int, 8>());
 }
 
+// ---- 8-bit integer rows ---------------------------------------------------------------------------
+
+// A row's scale is its largest magnitude T over 127, and a value v's code 127 v / T to the
+// nearest whole number, halves to the even one.  Of a norm, s_i g_i / rms, the root mean
+// square cancels in the codes: they are those of t_i = s_i g_i, a product that 64 bits
+// hold.  A code is found in fp32 (its error is below 2^-14 of a step), and where that is
+// near a border, in 64 bits: 127 t - k T is exact there for t of up to 46 bits.
+struct IntRows {
+    int8_t * codes;  // [n][cp]
+    float * scales;  // [n]
+    int cp;
+};
+
+struct IntScale {
+    double most;   // T
+    double inv;    // 127 / T, 0 for a row of zeros
+    bool plain;    // T is far from the ends of fp32's range
+};
+__device__ __forceinline__ IntScale int_scale(double most) {
+    return {most, most > 0.0 ? 127.0 / most : 0.0, most > 1e-30 && most < 1e30};
+}
+template <class V> __device__ __forceinline__ int int_code(V t, const IntScale & s) {
+    const float f = s.plain ? (float) t * (float) s.inv : (float) ((double) t * s.inv);
+    const float k = rintf(f);
+    int code = (int) k;
+    if (fabsf(f - k) > 0.4999f) {
+        const double rest = fma(-(double) k, s.most, 127.0 * (double) t), half = 0.5 * s.most;
+        const bool odd = (code & 1) != 0;
+        if (rest > half || (rest == half && odd)) ++code;
+        if (rest < -half || (rest == -half && odd)) --code;
+    }
+    return code;
+}
+// The scale of a row of values t * inv; NaN where there is none that is finite.
+__device__ __forceinline__ float int_row_scale(double most, double inv) {
+    const float s = (float) (most * inv / 127.0);
+    return s < __builtin_inff() ? s : __builtin_nanf("");
+}
+
+__device__ __forceinline__ uint32_t four_codes(const int * k) {
+    return (uint32_t) (k[0] & 255) | (uint32_t) (k[1] & 255) << 8 | (uint32_t) (k[2] & 255) << 16 | (uint32_t) k[3] << 24;
+}
+
+__device__ __forceinline__ double inverse_root(double m) {
+    double y = (double) __builtin_amdgcn_rsqf((float) m);
+    y = fma(0.5 * y, fma(-m * y, y, 1.0), y);
+    return m > 1e-30 && m < 1e38 ? y : 1.0 / sqrt(m);
+}
+
+// The larger of non-negative doubles as bits (a NaN's are larger than any number's), over groups of G lanes.
+template <int G> __device__ __forceinline__ double group_most(double v) {
+    const auto larger = [](double a, double b) {
+        return __builtin_bit_cast(uint64_t, a) > __builtin_bit_cast(uint64_t, b) ? a : b;
+    };
+#pragma unroll
+    for (int d = 1; d < G; d <<= 1) v = larger(v, __shfl_xor(v, d));
+    return v;
+}
+__device__ __forceinline__ double most_of(double a, double t) {
+    const uint64_t b = __builtin_bit_cast(uint64_t, t) & 0x7fffffffffffffffull;
+    return b > __builtin_bit_cast(uint64_t, a) ? __builtin_bit_cast(double, b) : a;
+}
+
+// Rows, or their norms (NORM, as k_norm_vec), to integer rows: LPR lanes hold a row in
+// registers, CPL chunks each.
+template <int DT, int LPR, int CPL, bool NORM>
+__global__ void __launch_bounds__(256) k_rows_int8(const typename Store<DT>::T * x,
+                                                   const typename Store<DT>::T * residual,
+                                                   const float * __restrict__ gamma, typename Store<DT>::T * total,
+                                                   IntRows out, int64_t n, int c, float eps) {
+    using T = typename Store<DT>::T;
+    using V = typename std::conditional<NORM, double, float>::type;
+    constexpr int N = kChunk<DT>, RPB = 256 / LPR;
+    const int l = threadIdx.x % LPR;
+    float g[CPL][N];
+#pragma unroll
+    for (int i = 0; i < CPL; ++i)
+#pragma unroll
+        for (int u = 0; u < N; ++u) {
+            const int at = (i * LPR + l) * N + u;
+            g[i][u] = NORM && gamma != nullptr && at < c ? gamma[at] : 1.0f;
+        }
+    int4 xc[CPL], rc[CPL];
+    const auto fetch = [&](int64_t row) {
+#pragma unroll
+        for (int i = 0; i < CPL; ++i) {
+            const int at = (i * LPR + l) * N;
+            xc[i] = rc[i] = int4{0, 0, 0, 0};
+            if (at < c) {
+                xc[i] = *(const int4 *) (x + row * c + at);
+                if (NORM && residual != nullptr) rc[i] = *(const int4 *) (residual + row * c + at);
+            }
+        }
+    };
+    int64_t row = (int64_t) blockIdx.x * RPB + threadIdx.x / LPR;
+    const int64_t stride = (int64_t) gridDim.x * RPB;
+    if (row < n) fetch(row);
+    for (; row < n; row += stride) {
+        V t[CPL][N];
+        double sum = 0.0, most = 0.0;
+#pragma unroll
+        for (int i = 0; i < CPL; ++i) {
+            float v[N], r[N];
+            unpack_chunk_of<DT>(xc[i], v);
+            if constexpr (NORM) {
+                if (residual != nullptr) unpack_chunk_of<DT>(rc[i], r);
+#pragma unroll
+                for (int u = 0; u < N; ++u) {
+                    double s = (double) v[u];
+                    if (residual != nullptr) {
+                        s += (double) r[u];
+                        v[u] += r[u];
+                    }
+                    sum = fma(s, s, sum);
+                    t[i][u] = s * (double) g[i][u];
+                    most = most_of(most, t[i][u]);
+                }
+                const int at = (i * LPR + l) * N;
+                if (total != nullptr && at < c) store_chunk<DT>(total + row * c + at, v);
+            } else {
+#pragma unroll
+                for (int u = 0; u < N; ++u) {
+                    t[i][u] = v[u];
+                    most = most_of(most, (double) v[u]);
+                }
+            }
+        }
+        if (row + stride < n) fetch(row + stride);
+        most = group_most<LPR>(most);
+        double inv = 1.0;
+        if constexpr (NORM) inv = inverse_root(group_sum<LPR>(sum) / c + (double) eps);
+        const float scale = int_row_scale(most, inv);
+        const IntScale s = int_scale(scale == scale ? most : 0.0);
+#pragma unroll
+        for (int i = 0; i < CPL; ++i) {
+            const int at = (i * LPR + l) * N;
+            if (at >= out.cp) continue;
+            int k[N];
+#pragma unroll
+            for (int u = 0; u < N; ++u) k[u] = s.inv == 0.0 ? 0 : int_code(t[i][u], s);
+            int8_t * p = out.codes + row * out.cp + at;
+            if constexpr (N == 8) {
+                *(uint2 *) p = uint2{four_codes(k), four_codes(k + 4)};
+            } else {
+                *(uint32_t *) p = four_codes(k);
+            }
+        }
+        if (l == 0) out.scales[row] = scale;
+    }
+}
+
+// Any width: one wavefront per row, which it reads twice.
+template <int DT, bool NORM>
+__global__ void __launch_bounds__(256) k_rows_int8_any(const typename Store<DT>::T * x,
+                                                       const typename Store<DT>::T * residual,
+                                                       const float * __restrict__ gamma, typename Store<DT>::T * total,
+                                                       IntRows out, int64_t n, int c, float eps) {
+    const int lane = threadIdx.x & 63;
+    const int64_t row = (int64_t) blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (row >= n) return;
+    const auto at = [&](int i) {
+        const double v = (double) Store<DT>::ld(x, row * c + i);
+        return NORM && residual != nullptr ? v + (double) Store<DT>::ld(residual, row * c + i) : v;
+    };
+    const auto weighted = [&](int i, double s) { return NORM && gamma != nullptr ? s * (double) gamma[i] : s; };
+    double sum = 0.0, most = 0.0;
+    for (int i = lane; i < c; i += 64) {
+        const double s = at(i);
+        sum = fma(s, s, sum);
+        most = most_of(most, weighted(i, s));
+    }
+    most = group_most<64>(most);
+    double inv = 1.0;
+    if constexpr (NORM) inv = inverse_root(group_sum<64>(sum) / c + (double) eps);
+    const float scale = int_row_scale(most, inv);
+    const IntScale q = int_scale(scale == scale ? most : 0.0);
+    for (int i = lane; i < out.cp; i += 64) {
+        int code = 0;
+        if (i < c) {
+            const double s = at(i);
+            if (total != nullptr) {
+                float v = Store<DT>::ld(x, row * c + i);
+                if (residual != nullptr) v += Store<DT>::ld(residual, row * c + i);
+                Store<DT>::st(total, row * c + i, v);
+            }
+            if (q.inv != 0.0) code = int_code(weighted(i, s), q);
+        }
+        out.codes[row * out.cp + i] = (int8_t) code;
+    }
+    if (lane == 0) out.scales[row] = scale;
+}
+
+// The values that integer rows stand for: 16 codes a thread.
+template <int DT>
+__global__ void __launch_bounds__(256) k_expand_int8(const int8_t * __restrict__ codes, const float * __restrict__ scales,
+                                                     typename Store<DT>::T * __restrict__ y, int64_t n, int c, int cp,
+                                                     bool whole) {
+    constexpr int N = kChunk<DT>;
+    const int pieces = (c + 15) / 16;
+    const int64_t i = (int64_t) blockIdx.x * 256 + threadIdx.x;
+    if (i >= n * pieces) return;
+    const int64_t row = n * pieces <= INT32_MAX ? (int64_t) ((uint32_t) i / (uint32_t) pieces) : i / pieces;
+    const int at = (int) (i - row * pieces) * 16;
+    const int4 w = *(const int4 *) (codes + row * cp + at);
+    const float scale = scales[row];
+    const int quad[4] = {w.x, w.y, w.z, w.w};
+    float v[16];
+#pragma unroll
+    for (int k = 0; k < 16; ++k) v[k] = (float) (int8_t) (quad[k / 4] >> (8 * (k % 4))) * scale;
+    typename Store<DT>::T * yr = y + row * c + at;
+    if (whole) {
+#pragma unroll
+        for (int u = 0; u < 16; u += N)
+            if (at + u < c) store_chunk<DT>(yr + u, v + u);
+    } else {
+#pragma unroll
+        for (int u = 0; u < 16; ++u)
+            if (at + u < c) Store<DT>::st(yr, u, v[u]);
+    }
+}
+
+template <int DT, bool NORM>
+hipError_t rows_int8_dt(const void * x, const void * residual, const float * gamma, void * total, const IntRows & out,
+                        int64_t n, int c, float eps, int cus, hipStream_t s) {
+    using T = typename Store<DT>::T;
+    constexpr int N = kChunk<DT>;
+    const int chunks = out.cp / N;
+    if (c % N != 0 || chunks > 64 * 8) {
+        const int64_t g = (n + 3) / 4;
+        if (g > 0x7fffffffLL) return hipErrorInvalidValue;
+        k_rows_int8_any<DT, NORM><<<(unsigned) g, 256, 0, s>>>((const T *) x, (const T *) residual, gamma, (T *) total, out,
+                                                               n, c, eps);
+        return hipGetLastError();
+    }
+    const auto launch = [&](auto lpr, auto cpl) {
+        constexpr int LPR = decltype(lpr)::value, CPL = decltype(cpl)::value;
+        constexpr int RPB = 256 / LPR;
+        const int64_t g = std::min<int64_t>((n + RPB - 1) / RPB, (int64_t) cus * 4);
+        k_rows_int8<DT, LPR, CPL, NORM><<<(unsigned) g, 256, 0, s>>>((const T *) x, (const T *) residual, gamma, (T *) total,
+                                                                     out, n, c, eps);
+        return hipGetLastError();
+    };
+    using std::integral_constant;
+    if (chunks <= 16) return launch(integral_constant<int, 16>(), integral_constant<int, 1>());
+    if (chunks <= 32) return launch(integral_constant<int, 16>(), integral_constant<int, 2>());
+    if (chunks <= 64) return launch(integral_constant<int, 32>(), integral_constant<int, 2>());
+    if (chunks <= 128) return launch(integral_constant<int, 64>(), integral_constant<int, 2>());
+    if (chunks <= 256) return launch(integral_constant<int, 64>(), integral_constant<int, 4>());
+    return launch(integral_constant<int, 64>(), integral_constant<int, 8>());
+}
+
 // ---- rotary positions ---------------------------------------------------------------------------
 
 // Each head's D channels are D / 2 pairs: (2p, 2p + 1), or (p, p + D / 2) with
@@ -542,6 +770,40 @@ hipError_t launch_expand8(int dtype, const uint8_t * codes, const uint8_t * scal
         } else {
             k_expand8<DT, false><<<(unsigned) g, 256, 0, s>>>(codes, scales, (T *) y, n, c, cp);
         }
+        return hipGetLastError();
+    };
+    switch (dtype) {
+        case kF32: return launch(std::integral_constant<int, kF32>());
+        case kF16: return launch(std::integral_constant<int, kF16>());
+        default: return launch(std::integral_constant<int, kBF16>());
+    }
+}
+
+// Integer rows: `norm` of x + residual (gamma, total may be null), or x itself.
+hipError_t launch_rows_int8(int dtype, bool norm, const void * x, const void * residual, const float * gamma, void * total,
+                            int8_t * codes, float * scales, int64_t n, int c, float eps, int cus, hipStream_t s) {
+    const IntRows out{codes, scales, rows8_width(c)};
+    const auto launch = [&](auto dt) {
+        constexpr int DT = decltype(dt)::value;
+        return norm ? rows_int8_dt<DT, true>(x, residual, gamma, total, out, n, c, eps, cus, s)
+                    : rows_int8_dt<DT, false>(x, nullptr, nullptr, nullptr, out, n, c, eps, cus, s);
+    };
+    switch (dtype) {
+        case kF32: return launch(std::integral_constant<int, kF32>());
+        case kF16: return launch(std::integral_constant<int, kF16>());
+        default: return launch(std::integral_constant<int, kBF16>());
+    }
+}
+
+hipError_t launch_expand_int8(int dtype, const int8_t * codes, const float * scales, void * y, int64_t n, int c,
+                              hipStream_t s) {
+    const int64_t g = (n * ((c + 15) / 16) + 255) / 256;
+    if (g > 0x7fffffffLL) return hipErrorInvalidValue;
+    const int cp = rows8_width(c);
+    const auto launch = [&](auto dt) {
+        constexpr int DT = decltype(dt)::value;
+        using T = typename Store<DT>::T;
+        k_expand_int8<DT><<<(unsigned) g, 256, 0, s>>>(codes, scales, (T *) y, n, c, cp, c % kChunk<DT> == 0);
         return hipGetLastError();
     };
     switch (dtype) {

@@ -74,6 +74,12 @@ constexpr int kRows8 = 3;
 __host__ __device__ inline int rows8_width(int c) { return (c + 127) / 128 * 128; }
 inline size_t rows8_scales(int64_t n, int c) { return ((size_t) n * rows8_width(c) + 255) / 256 * 256; }
 inline size_t rows8_bytes(int64_t n, int c) { return rows8_scales(n, c) + (size_t) n * (rows8_width(c) / 32); }
+// 8-bit integer rows: codes -127 .. 127 in the same places, then one fp32 scale per row
+// (NaN for a row that is not finite, whose codes are zeros).
+constexpr int kRowsInt8 = 4;
+constexpr int kIntMostTerms = 131072;  // products of two codes that 32 bits add up
+inline bool is_rows8(int dtype) { return dtype == kRows8 || dtype == kRowsInt8; }
+inline size_t rows_int8_bytes(int64_t n, int c) { return rows8_scales(n, c) + (size_t) n * sizeof(float); }
 
 // A 16-byte chunk of 16-bit storage values (8 of them) to fp32 and back,
 // with round-to-nearest-even on the way back.
@@ -144,7 +150,7 @@ struct trellis_sparse_buffer {
     size_t count;   // elements
     size_t bytes;   // count * element size
     size_t cap;     // bytes actually reserved (pool size class); 0: the caller's own memory
-    int dtype;      // tsh::Dtype of the storage, -1 for raw int32, tsh::kRows8
+    int dtype;      // tsh::Dtype of the storage, -1 for raw int32, tsh::kRows8, tsh::kRowsInt8
     int64_t rows;   // 8-bit rows: their count
     int width;      // 8-bit rows: channels
 };
@@ -363,6 +369,10 @@ hipError_t launch_pack8(int dtype, const void * x, uint8_t * codes, uint8_t * sc
                         hipStream_t s);
 hipError_t launch_expand8(int dtype, const uint8_t * codes, const uint8_t * scales, void * y, int64_t n, int c,
                           hipStream_t s);
+hipError_t launch_rows_int8(int dtype, bool norm, const void * x, const void * residual, const float * gamma, void * total,
+                            int8_t * codes, float * scales, int64_t n, int c, float eps, int cus, hipStream_t s);
+hipError_t launch_expand_int8(int dtype, const int8_t * codes, const float * scales, void * y, int64_t n, int c,
+                              hipStream_t s);
 constexpr int kRotaryMaxDim = 256;
 struct RotaryPlan {
     int64_t n, x_stride, y_stride;
@@ -375,12 +385,12 @@ hipError_t launch_rotary(int dtype, const void * x, const int32_t * coords, cons
                          const RotaryPlan & plan, int cus, hipStream_t s);
 // Linear with activation and residual (kernels_act.hip).  w: rows of w_bytes (a
 // multiple of 128, zeros beyond ci), linear_act_rows(co) of them, in the
-// storage type or, for x_type kRows8, as 8-bit rows.
+// storage type or, for x_type kRows8 and kRowsInt8, as 8-bit rows of the kind.
 struct LinearAct {
     const void * x;
-    const uint8_t * x_scales;
+    const void * x_scales;   // uint8_t [n][row_bytes / 32]; of integer rows float [n]
     const void * w;
-    const uint8_t * w_scales;
+    const void * w_scales;   // the same of w's rows
     const float * bias;      // [co] or null
     const void * residual;   // [n][co] or null; may be y
     void * y;
@@ -437,6 +447,30 @@ struct AttentionShape {
 AttentionShape attention_shape(int dtype, const Attention & p, int cus);
 hipError_t launch_attention(int dtype, const Attention & p, const AttentionShape & shape, void * scratch,
                             hipStream_t s);
+
+// Attention whose scores are changed before the softmax (kernels_scored.hip).
+struct Scores {
+    float cap, cap_scale;    // cap times log2(e), 0: none; what a product of q and k is multiplied with inside the tanh
+    const float * slopes;    // [heads] or null
+    const int32_t * q_xyz;   // [nq][4] and [nk][4], or null: distances are of rows
+    const int32_t * k_xyz;
+    const int32_t * prefix;  // [seqs] or null
+    int causal;
+};
+hipError_t launch_attention_scored(int dtype, const Attention & p, const Scores & scores, hipStream_t s);
+
+// Group norm (kernels_gnorm.hip).  gamma, beta and at may be null; y may be x.
+struct GroupNorm {
+    const void * x;
+    void * y;
+    const int32_t * at;      // [seqs + 1] or null: one sequence of all rows
+    const float * gamma;
+    const float * beta;
+    int64_t n;
+    int seqs, c, groups, act;
+    float eps;
+};
+hipError_t launch_group_norm(int dtype, const GroupNorm & p, hipStream_t s);
 
 // Narrow MFMA linear (bf16/fp16, Co <= 16, Ci a power of two in 32..1024):
 // weights [co][ci] in the storage type.

@@ -109,6 +109,11 @@ class AttentionDesc(Structure):
                 ("y_stride", c_int64)]
 
 
+class ScoresDesc(Structure):
+    _fields_ = [("struct_size", c_uint32), ("causal", c_int32), ("cap", c_float), ("slopes", c_void_p),
+                ("q_coords", c_void_p), ("k_coords", c_void_p), ("prefix", c_void_p)]
+
+
 class BlockDesc(Structure):
     _fields_ = ([("struct_size", c_uint32)] + [(k, c_int32) for k in ("heads", "head_dim", "hidden", "act", "rows8")] +
                 [("pairs", c_int32 * 3), ("split", c_int32), ("eps", c_float), ("qk_eps", c_float), ("base", c_double)] +
@@ -164,6 +169,11 @@ ABI = {
     "trellis_sparse_hip_set_scratch": (c_int, [_p, _p]),
     "trellis_sparse_hip_scratch_bytes": (c_size_t, [_p]),
     "trellis_sparse_hip_alloc_rows8": (c_int, [_p, c_int64, c_int, POINTER(_p)]),
+    "trellis_sparse_hip_alloc_rows_int8": (c_int, [_p, c_int64, c_int, POINTER(_p)]),
+    "trellis_sparse_hip_group_norm": (c_int, [_p, _p, _p, c_int, c_void_p, c_void_p, _p, c_int64, c_int, c_int, c_float,
+                                              c_int]),
+    "trellis_sparse_hip_attention_scored": (c_int, [_p, _p, _p, _p, _p, c_int64, c_int64, _p, _p, c_int,
+                                                    POINTER(AttentionDesc), POINTER(ScoresDesc)]),
     "trellis_sparse_hip_pack_rows8": (c_int, [_p, _p, _p, c_int64, c_int]),
     "trellis_sparse_hip_expand_rows8": (c_int, [_p, _p, _p, c_int64, c_int]),
     "trellis_sparse_hip_rms_norm": (c_int, [_p, _p, _p, c_void_p, _p, _p, c_int64, c_int, c_float]),
@@ -508,6 +518,12 @@ class Backend:
         self._check(LIB.trellis_sparse_hip_alloc_rows8(self.ptr, n, c, ctypes.byref(h)), "alloc_rows8")
         return Buffer(self, h, n * c)
 
+    def alloc_rows_int8(self, n: int, c: int) -> Buffer:
+        """8-bit integer rows, one scale a row; pack_rows8, expand_rows8, rms_norm and linear_act take them as 8-bit rows."""
+        h = c_void_p()
+        self._check(LIB.trellis_sparse_hip_alloc_rows_int8(self.ptr, n, c, ctypes.byref(h)), "alloc_rows_int8")
+        return Buffer(self, h, n * c)
+
     def pack_rows8(self, x: Buffer, rows8: Buffer, n: int, c: int):
         self._check(LIB.trellis_sparse_hip_pack_rows8(self.ptr, x.handle, rows8.handle, n, c), "pack_rows8")
 
@@ -520,6 +536,15 @@ class Backend:
         g = None if gamma is None else self.keep(_f32(gamma))
         self._check(LIB.trellis_sparse_hip_rms_norm(self.ptr, x.handle, residual and residual.handle, _address(g),
                                                     total and total.handle, y.handle, n, c, eps), "rms_norm")
+
+    def group_norm(self, x: Buffer, gamma, beta, y: Buffer, n: int, c: int, groups: int, eps: float, act: str = "none",
+                   offsets: Buffer | None = None):
+        """Group norm over the rows of each sequence (offsets int32 [sequences + 1], or one of all rows), then act."""
+        g = None if gamma is None else self.keep(_f32(gamma))
+        b = None if beta is None else self.keep(_f32(beta))
+        self._check(LIB.trellis_sparse_hip_group_norm(self.ptr, x.handle, offsets and offsets.handle,
+                                                      1 if offsets is None else offsets.count - 1, _address(g), _address(b),
+                                                      y.handle, n, c, groups, eps, ACTS[act]), "group_norm")
 
     def linear_act(self, x: Buffer, weight, bias, y: Buffer, n: int, ci: int, co: int, act: str = "none",
                    residual: Buffer | None = None):
@@ -552,11 +577,30 @@ class Backend:
                                                      kv_offsets and kv_offsets.handle, seqs, ctypes.byref(d)),
                     "attention")
 
+    def attention_scored(self, q: Buffer, k: Buffer | None, v: Buffer | None, y: Buffer, nq: int, nkv: int, heads: int,
+                         kv_heads: int, head_dim: int, scale: float = 0.0, q_offsets: Buffer | None = None,
+                         kv_offsets: Buffer | None = None, q_offset: int = 0, q_stride: int = 0, k_offset: int = 0,
+                         k_stride: int = 0, v_offset: int = 0, v_stride: int = 0, y_offset: int = 0, y_stride: int = 0,
+                         cap: float = 0.0, slopes=None, q_coords: Buffer | None = None, k_coords: Buffer | None = None,
+                         causal: bool = False, prefix: Buffer | None = None):
+        """Attention with scores capped by a tanh, lowered by slopes[head] times a distance (of voxels with q_coords and
+        k_coords int32 [rows][4], else of rows) and masked (causal, but for the first prefix[sequence] keys)."""
+        d = AttentionDesc(ctypes.sizeof(AttentionDesc), heads, kv_heads, head_dim, scale, q_offset, q_stride, k_offset,
+                          k_stride, v_offset, v_stride, y_offset, y_stride)
+        w = None if slopes is None else self.keep(_f32(slopes))
+        s = ScoresDesc(ctypes.sizeof(ScoresDesc), int(causal), cap, _address(w), q_coords and q_coords.handle,
+                       k_coords and k_coords.handle, prefix and prefix.handle)
+        seqs = 1 if q_offsets is None else q_offsets.count - 1
+        self._check(LIB.trellis_sparse_hip_attention_scored(self.ptr, q.handle, k and k.handle, v and v.handle, y.handle, nq,
+                                                            nkv, q_offsets and q_offsets.handle,
+                                                            kv_offsets and kv_offsets.handle, seqs, ctypes.byref(d),
+                                                            ctypes.byref(s)), "attention_scored")
+
     def transformer_block(self, h: Buffer, coords, out: Buffer, n: int, heads: int, head_dim: int, hidden: int, weights: dict,
-                          pairs, act: str = "gelu_tanh", rows8: bool = False, split: bool = False, eps: float = 1e-6,
+                          pairs, act: str = "gelu_tanh", rows8: int = 0, split: bool = False, eps: float = 1e-6,
                           qk_eps: float = 0.0, base: float = 10000.0, offsets: Buffer | None = None):
         """A whole block over voxel rows; weights: the arrays of BlockDesc by name (qkv_w, out_w, mlp0_w and mlp2_w, the
-        others if there)."""
+        others if there); rows8: linears read 8-bit rows (1) or 8-bit integer rows (2)."""
         names = [f[0] for f in BlockDesc._fields_ if f[1] is c_void_p]
         if set(weights) - set(names):
             raise TypeError(f"transformer_block: unknown weights {sorted(set(weights) - set(names))}")
