@@ -2272,9 +2272,16 @@ trellis_status group_norm_impl(trellis_sparse_backend * backend, const trellis_s
     p.groups = groups;
     p.act = act;
     p.eps = eps;
+    const size_t bytes = group_norm_scratch(be->policy.compute_dtype, p, be->cus);
+    if (scratch_clash(be, bytes, {sx, sy, so})) {
+        return fail(be, TRELLIS_STATUS_INVALID_ARGUMENT, "group_norm: rows in the scratch");
+    }
+    DevMem scratch;
+    if (bytes > 0) p.scratch = take_scratch(be, bytes, &scratch);
     stage_begin(be, TRELLIS_SPARSE_HIP_STAGE_ELEMENTWISE);
     const hipError_t err = launch_group_norm(be->policy.compute_dtype, p, be->stream);
     stage_end(be, TRELLIS_SPARSE_HIP_STAGE_ELEMENTWISE);
+    dev_release(be, &scratch);
     return hip_status(be, err, "group_norm");
 }
 

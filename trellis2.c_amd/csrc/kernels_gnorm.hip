@@ -1,6 +1,7 @@
 // kernels_gnorm.hip - group norm over the rows of each sequence, channels last, with the activation that follows.
 #include <type_traits>
 
+#include "act_common.h"
 #include "rows_common.h"
 
 namespace tsh {
@@ -12,14 +13,18 @@ struct GroupStat {
     float mean, mean_low, inverse, pad;
 };
 
-// Sums over a group are of d = x - k and d^2 in 64 bits, k the group's first value in its
-// sequence: as k is one of them, (k - m)^2 is at most as many variances as there are
-// values, and var = mean d^2 - (mean d)^2 loses no more than that many of 2^53.
+// Sums over a group, in 64 bits: of d = x - k and of d^2, k the group's first value in its
+// sequence in fp32 (as k is one of the values, (k - m)^2 is at most as many variances as
+// there are values, and var = mean d^2 - (mean d)^2 loses no more than that many of
+// 2^-53), zero in 16 bits (whose values are at most 2^11 of their own steps).
 struct GroupSum {
     double d, d2;
 };
-__device__ __forceinline__ void add_value(GroupSum & s, float x, float k) {
-    const double d = (double) x - (double) k;
+__device__ __forceinline__ GroupStat * stats_of(const GroupNorm & p) {
+    return (GroupStat *) ((GroupSum *) p.scratch + p.tiles * p.slabs * p.groups);
+}
+template <int DT> __device__ __forceinline__ void add_value(GroupSum & s, float x, float k) {
+    const double d = DT == kF32 ? (double) x - (double) k : (double) x;
     s.d += d;
     s.d2 = fma(d, d, s.d2);
 }
@@ -31,13 +36,8 @@ __device__ __forceinline__ GroupStat stat_of(const GroupSum & s, double count, f
     // (A NaN stays one; a negative variance is a rounding of zero.)
     return {hi, hi - hi == 0.0f ? (float) low : 0.0f, (float) (1.0 / sqrt((var < 0.0 ? 0.0 : var) + (double) eps)), 0.0f};
 }
-
-__device__ __forceinline__ float gn_act(float v, int act) {
-    if (act == TRELLIS_SPARSE_HIP_ACT_SILU) return v / (1.0f + expf(-v));
-    if (act == TRELLIS_SPARSE_HIP_ACT_GELU) return 0.5f * v * erfcf(-0.70710678f * v);
-    if (act == TRELLIS_SPARSE_HIP_ACT_GELU_TANH)
-        return v / (1.0f + expf(-v * (1.5957691216057308f + 0.0713548162726f * v * v)));
-    return v;
+template <int DT> __device__ __forceinline__ float first_value(const typename Store<DT>::T * p, int64_t i) {
+    return DT == kF32 ? Store<DT>::ld(p, i) : 0.0f;
 }
 
 __device__ __forceinline__ int64_t row_of(const int32_t * at, int i, int64_t n) {
@@ -45,7 +45,9 @@ __device__ __forceinline__ int64_t row_of(const int32_t * at, int i, int64_t n) 
     return v < 0 ? 0 : (v > n ? n : v);
 }
 
-// Any sizes: a block per sequence and group, which reads its values twice.
+// ---- a block per sequence and group -----------------------------------------------------------------
+
+// Any sizes, values read twice: where groups are small, and where there is no scratch.
 template <int DT> __global__ void __launch_bounds__(256) k_group_norm(GroupNorm p) {
     using T = typename Store<DT>::T;
     __shared__ GroupSum s_sum[4];
@@ -59,10 +61,10 @@ template <int DT> __global__ void __launch_bounds__(256) k_group_norm(GroupNorm 
     int wide = 1;
     while (wide < size && wide < 256) wide *= 2;
     const int ch0 = threadIdx.x % wide, r0 = threadIdx.x / wide, step = 256 / wide;
-    const float k = Store<DT>::ld(x, 0);
+    const float k = first_value<DT>(x, 0);
     GroupSum s{0.0, 0.0};
     for (int64_t r = r0; r < end - first; r += step)
-        for (int ch = ch0; ch < size; ch += wide) add_value(s, Store<DT>::ld(x, r * p.c + ch), k);
+        for (int ch = ch0; ch < size; ch += wide) add_value<DT>(s, Store<DT>::ld(x, r * p.c + ch), k);
     s.d = group_sum<64>(s.d);
     s.d2 = group_sum<64>(s.d2);
     if (threadIdx.x % 64 == 0) s_sum[threadIdx.x / 64] = s;
@@ -73,27 +75,250 @@ template <int DT> __global__ void __launch_bounds__(256) k_group_norm(GroupNorm 
         s.d2 += s_sum[i].d2;
     }
     const GroupStat st = stat_of(s, (double) (end - first) * size, k, p.eps);
-    for (int ch = ch0; ch < size; ch += wide) {
-        const float scale = st.inverse * (p.gamma != nullptr ? p.gamma[g * size + ch] : 1.0f);
-        const float shift = p.beta != nullptr ? p.beta[g * size + ch] : 0.0f;
-        for (int64_t r = r0; r < end - first; r += step) {
-            const float v = (Store<DT>::ld(x, r * p.c + ch) - st.mean - st.mean_low) * scale + shift;
-            Store<DT>::st(y, r * p.c + ch, gn_act(v, p.act));
+    by_act(p.act, [&](auto act_c) {
+        for (int ch = ch0; ch < size; ch += wide) {
+            const float scale = st.inverse * (p.gamma != nullptr ? p.gamma[g * size + ch] : 1.0f);
+            const float shift = p.beta != nullptr ? p.beta[g * size + ch] : 0.0f;
+            for (int64_t r = r0; r < end - first; r += step) {
+                const float v = (Store<DT>::ld(x, r * p.c + ch) - st.mean - st.mean_low) * scale + shift;
+                Store<DT>::st(y, r * p.c + ch, activate<DT, decltype(act_c)::value>(v));
+            }
+        }
+    });
+}
+
+// ---- tiles of rows ----------------------------------------------------------------------------------
+
+// A tile's rows [first, first + rows) of sequence seq; rows = 0 where there is none.  Tiles are
+// numbered by what holds for any lengths: sequence s, whose rows begin at a, has its tiles
+// from a / tile_rows + s on, and never reaches past the next one's first.
+struct Tile {
+    int64_t first;
+    int rows, seq;
+};
+__device__ __forceinline__ int64_t first_tile(const GroupNorm & p, int s) {
+    return p.at != nullptr ? row_of(p.at, s, p.n) / p.tile_rows + s : 0;
+}
+__device__ Tile find_tile(const GroupNorm & p, int64_t tile) {
+    int seq = 0;
+    int64_t begin = 0, end = p.n;
+    if (p.at != nullptr) {
+        // The last sequence whose tiles begin at or before this one, 64 of them at a time.
+        const int lane = threadIdx.x & 63;
+        int many = p.seqs;
+        while (many > 1) {
+            const int step = (many + 63) / 64, i = lane * step;
+            const unsigned long long before = __ballot(i < many && first_tile(p, seq + i) <= tile);
+            if (before == 0) return {0, 0, 0};
+            const int at = 63 - __clzll(before);
+            seq += at * step;
+            many = min(step, many - at * step);
+        }
+        begin = row_of(p.at, seq, p.n);
+        end = row_of(p.at, seq + 1, p.n);
+    }
+    const int64_t from = begin + (tile - first_tile(p, seq)) * p.tile_rows;
+    if (from < begin || from >= end) return {0, 0, seq};
+    return {from, (int) min((int64_t) p.tile_rows, end - from), seq};
+}
+
+// V adjacent channels of a row: a chunk of 16 bytes, or (rows that are no whole number of
+// them) a single one.
+template <int DT, int V> __device__ __forceinline__ void load_channels(const typename Store<DT>::T * p, float * v) {
+    if constexpr (V == 1) {
+        v[0] = Store<DT>::ld(p, 0);
+    } else {
+        unpack_chunk_of<DT>(*(const int4 *) p, v);
+    }
+}
+
+// Sums of a tile's rows and 256 chunks of V of their channels (`slab`), per group.  A thread
+// has a chunk of every so many rows, and NG sums of neighbouring channels of it: one where a
+// chunk is of one group, one a channel where groups do not divide chunks.  Each block
+// writes its part of every group's sums (zeros for those that it has nothing of).
+template <int DT, int V, int NG> __global__ void __launch_bounds__(256) k_gn_sums(GroupNorm p) {
+    using T = typename Store<DT>::T;
+    constexpr int W = V / NG;
+    __shared__ GroupSum s_sum[256 * NG];
+    const int64_t tile = blockIdx.x / p.slabs;
+    const int slab = blockIdx.x % p.slabs;
+    const Tile at = find_tile(p, tile);
+    if (at.rows <= 0) return;
+    const int size = p.c / p.groups, chunk0 = slab * 256;
+    const int chunks = min(256, p.c / V - chunk0), step = 256 / chunks;
+    const int col = threadIdx.x % chunks, r0 = threadIdx.x / chunks, ch0 = (chunk0 + col) * V;
+    const T * x = (const T *) p.x + at.first * p.c + ch0;
+    GroupSum s[NG];
+    float k[NG];
+    const int64_t begin = p.at != nullptr ? row_of(p.at, at.seq, p.n) : 0;
+#pragma unroll
+    for (int a = 0; a < NG; ++a) {
+        s[a] = {0.0, 0.0};
+        k[a] = first_value<DT>((const T *) p.x, begin * p.c + (ch0 + a * W) / size * size);
+    }
+    if (r0 < step) {
+#pragma unroll 4
+        for (int r = r0; r < at.rows; r += step) {
+            float v[V];
+            load_channels<DT, V>(x + (int64_t) r * p.c, v);
+#pragma unroll
+            for (int u = 0; u < V; ++u) add_value<DT>(s[u / W], v[u], k[u / W]);
+        }
+    }
+#pragma unroll
+    for (int a = 0; a < NG; ++a) s_sum[threadIdx.x * NG + a] = s[a];
+    __syncthreads();
+    // `each` (a power of two, up to a wavefront) threads a group.
+    const int here = (min(p.c, (chunk0 + chunks) * V) - 1) / size + 1 - chunk0 * V / size;  // groups of the slab
+    int each = 1;
+    while (each < 64 && each * 2 * here <= 256) each *= 2;
+    const int unit = V / NG;  // channels of a sum
+    GroupSum * out = (GroupSum *) p.scratch;
+    for (int g0 = 0; g0 < here; g0 += 256 / each) {
+        const int g = chunk0 * V / size + g0 + threadIdx.x / each;
+        // The slab's sums of group g: [from, to) of every row.
+        const int from = max(0, (g * size - chunk0 * V + unit - 1) / unit);
+        const int to = min(chunks * NG, ((g + 1) * size - chunk0 * V) / unit);
+        GroupSum t{0.0, 0.0};
+        if (g0 + (int) threadIdx.x / each < here) {
+            const int wide = to - from;
+            for (int i = threadIdx.x % each; i < wide * step; i += each) {
+                const GroupSum & q = s_sum[i / wide * chunks * NG + from + i % wide];
+                t.d += q.d;
+                t.d2 += q.d2;
+            }
+        }
+        for (int d = 1; d < each; d <<= 1) {
+            t.d += __shfl_xor(t.d, d);
+            t.d2 += __shfl_xor(t.d2, d);
+        }
+        if (g0 + (int) threadIdx.x / each < here && threadIdx.x % each == 0) out[(g * p.tiles + tile) * p.slabs + slab] = t;
+    }
+    if (p.slabs > 1) {
+        const int g1 = chunk0 * V / size;
+        for (int g = threadIdx.x; g < p.groups; g += 256)
+            if (g < g1 || g >= g1 + here) out[(g * p.tiles + tile) * p.slabs + slab] = {0.0, 0.0};
+    }
+}
+
+// The sums of a sequence's tiles to its groups' statistics: a wavefront each.
+template <int DT> __global__ void __launch_bounds__(256) k_gn_stats(GroupNorm p) {
+    using T = typename Store<DT>::T;
+    const int64_t i = (int64_t) blockIdx.x * 4 + (threadIdx.x >> 6);
+    const int lane = threadIdx.x & 63, seq = (int) (i / p.groups), g = (int) (i % p.groups), size = p.c / p.groups;
+    if (seq >= p.seqs) return;
+    const int64_t begin = p.at != nullptr ? row_of(p.at, seq, p.n) : 0;
+    const int64_t end = p.at != nullptr ? row_of(p.at, seq + 1, p.n) : p.n;
+    if (end <= begin) return;
+    const float k = first_value<DT>((const T *) p.x, begin * p.c + g * size);
+    const GroupSum * in = (const GroupSum *) p.scratch + (g * p.tiles + first_tile(p, seq)) * p.slabs;
+    const int64_t many = (end - begin + p.tile_rows - 1) / p.tile_rows * p.slabs;
+    GroupSum s{0.0, 0.0};
+#pragma unroll 4
+    for (int64_t j = lane; j < many; j += 64) {
+        s.d += in[j].d;
+        s.d2 += in[j].d2;
+    }
+    s.d = group_sum<64>(s.d);
+    s.d2 = group_sum<64>(s.d2);
+    if (lane == 0) stats_of(p)[i] = stat_of(s, (double) (end - begin) * size, k, p.eps);
+}
+
+// The tiles, last ones first: they are what the caches still hold of the sums' pass.
+template <int DT, int V, int ACT> __global__ void __launch_bounds__(256) k_gn_apply(GroupNorm p) {
+    using T = typename Store<DT>::T;
+    const unsigned block = gridDim.x - 1 - blockIdx.x;
+    const int slab = block % p.slabs;
+    const Tile at = find_tile(p, block / p.slabs);
+    if (at.rows <= 0) return;
+    const int size = p.c / p.groups, chunk0 = slab * 256;
+    const int chunks = min(256, p.c / V - chunk0), step = 256 / chunks;
+    const int col = threadIdx.x % chunks, r0 = threadIdx.x / chunks, ch0 = (chunk0 + col) * V;
+    if (r0 >= step) return;
+    const T * x = (const T *) p.x + at.first * p.c + ch0;
+    T * y = (T *) p.y + at.first * p.c + ch0;
+    float mean[V], low[V], scale[V], shift[V];
+#pragma unroll
+    for (int u = 0; u < V; ++u) {
+        const GroupStat st = stats_of(p)[(int64_t) at.seq * p.groups + (ch0 + u) / size];
+        mean[u] = st.mean;
+        low[u] = st.mean_low;
+        scale[u] = st.inverse * (p.gamma != nullptr ? p.gamma[ch0 + u] : 1.0f);
+        shift[u] = p.beta != nullptr ? p.beta[ch0 + u] : 0.0f;
+    }
+#pragma unroll 2
+    for (int r = r0; r < at.rows; r += step) {
+        float v[V];
+        load_channels<DT, V>(x + (int64_t) r * p.c, v);
+#pragma unroll
+        for (int u = 0; u < V; ++u) v[u] = activate<DT, ACT>((v[u] - mean[u] - low[u]) * scale[u] + shift[u]);
+        if constexpr (V == 1) {
+            Store<DT>::st(y + (int64_t) r * p.c, 0, v[0]);
+        } else {
+            store_chunk<DT>(y + (int64_t) r * p.c, v);
         }
     }
 }
 
-}  // namespace
-
-hipError_t launch_group_norm(int dtype, const GroupNorm & p, hipStream_t s) {
-    const int64_t grid = (int64_t) p.seqs * p.groups;
-    if (grid > 0x7fffffffLL) return hipErrorInvalidValue;
-    switch (dtype) {
-        case kF32: k_group_norm<kF32><<<(unsigned) grid, 256, 0, s>>>(p); break;
-        case kF16: k_group_norm<kF16><<<(unsigned) grid, 256, 0, s>>>(p); break;
-        default: k_group_norm<kBF16><<<(unsigned) grid, 256, 0, s>>>(p); break;
+template <int DT, int V> hipError_t launch_tiles(const GroupNorm & p, hipStream_t s) {
+    const int64_t grid = p.tiles * p.slabs, stats = ((int64_t) p.seqs * p.groups + 3) / 4;
+    if (grid > 0x7fffffffLL || stats > 0x7fffffffLL) return hipErrorInvalidValue;
+    const int size = p.c / p.groups;
+    if (size % V == 0) {
+        k_gn_sums<DT, V, 1><<<(unsigned) grid, 256, 0, s>>>(p);
+    } else if (size * 2 == V) {
+        k_gn_sums<DT, V, V == 1 ? 1 : 2><<<(unsigned) grid, 256, 0, s>>>(p);
+    } else {
+        k_gn_sums<DT, V, V><<<(unsigned) grid, 256, 0, s>>>(p);
+    }
+    k_gn_stats<DT><<<(unsigned) stats, 256, 0, s>>>(p);
+    switch (p.act) {
+        case TRELLIS_SPARSE_HIP_ACT_SILU:
+            k_gn_apply<DT, V, TRELLIS_SPARSE_HIP_ACT_SILU><<<(unsigned) grid, 256, 0, s>>>(p);
+            break;
+        case TRELLIS_SPARSE_HIP_ACT_GELU:
+            k_gn_apply<DT, V, TRELLIS_SPARSE_HIP_ACT_GELU><<<(unsigned) grid, 256, 0, s>>>(p);
+            break;
+        case TRELLIS_SPARSE_HIP_ACT_GELU_TANH:
+            k_gn_apply<DT, V, TRELLIS_SPARSE_HIP_ACT_GELU_TANH><<<(unsigned) grid, 256, 0, s>>>(p);
+            break;
+        default: k_gn_apply<DT, V, TRELLIS_SPARSE_HIP_ACT_NONE><<<(unsigned) grid, 256, 0, s>>>(p); break;
     }
     return hipGetLastError();
+}
+
+template <int DT> hipError_t launch_dt(const GroupNorm & p, hipStream_t s) {
+    if (p.scratch != nullptr)
+        return p.c % kChunk<DT> == 0 ? launch_tiles<DT, kChunk<DT>>(p, s) : launch_tiles<DT, 1>(p, s);
+    const int64_t grid = (int64_t) p.seqs * p.groups;
+    if (grid > 0x7fffffffLL) return hipErrorInvalidValue;
+    k_group_norm<DT><<<(unsigned) grid, 256, 0, s>>>(p);
+    return hipGetLastError();
+}
+
+}  // namespace
+
+// Tiles of rows where a group has many values: as many as give each CU four blocks, of at least four rows a
+// thread.
+size_t group_norm_scratch(int dtype, GroupNorm & p, int cus) {
+    const int whole = dtype == kF32 ? 4 : 8, chunk = p.c % whole == 0 ? whole : 1;
+    const int chunks = p.c / chunk, wide = chunks < 256 ? chunks : 256;
+    const int64_t size = p.c / p.groups;
+    if (p.n * size < kGroupNormTiled) return 0;
+    p.slabs = (chunks + 255) / 256;
+    const int64_t step = 256 / wide, want = std::max<int64_t>(1, (int64_t) cus * 4 / p.slabs);
+    const int64_t rows = std::max<int64_t>((p.n + want - 1) / want, 4 * step);
+    p.tile_rows = (int) std::min<int64_t>((rows + step - 1) / step * step, 1 << 20);
+    p.tiles = (p.n + p.tile_rows - 1) / p.tile_rows + (p.at != nullptr ? p.seqs : 0);
+    return (size_t) p.tiles * p.slabs * p.groups * sizeof(GroupSum) + (size_t) p.seqs * p.groups * sizeof(GroupStat);
+}
+
+hipError_t launch_group_norm(int dtype, const GroupNorm & p, hipStream_t s) {
+    switch (dtype) {
+        case kF32: return launch_dt<kF32>(p, s);
+        case kF16: return launch_dt<kF16>(p, s);
+        default: return launch_dt<kBF16>(p, s);
+    }
 }
 
 }  // namespace tsh

@@ -469,7 +469,13 @@ struct GroupNorm {
     int64_t n;
     int seqs, c, groups, act;
     float eps;
+    void * scratch;          // of group_norm_scratch's bytes, or null: a block per sequence and group
+    int64_t tiles;           // set by group_norm_scratch, as are:
+    int tile_rows, slabs;    // rows of a tile, and in how many parts its channels are taken
 };
+// Values per group, of all sequences, from which tiles of rows are summed apart.
+constexpr int64_t kGroupNormTiled = 8192;
+size_t group_norm_scratch(int dtype, GroupNorm & p, int cus);
 hipError_t launch_group_norm(int dtype, const GroupNorm & p, hipStream_t s);
 
 // Narrow MFMA linear (bf16/fp16, Co <= 16, Ci a power of two in 32..1024):
