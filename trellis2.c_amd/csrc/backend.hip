@@ -2593,21 +2593,17 @@ trellis_status attention_impl(trellis_sparse_backend * backend, const trellis_sp
     p.kv_heads = d.kv_heads;
     p.dim = d.head_dim;
     p.scale = scale;
-    if (scores != nullptr) {
-        stage_begin(be, TRELLIS_SPARSE_HIP_STAGE_ELEMENTWISE);
-        const hipError_t err = launch_attention_scored(be->policy.compute_dtype, p, sc, be->stream);
-        stage_end(be, TRELLIS_SPARSE_HIP_STAGE_ELEMENTWISE);
-        return hip_status(be, err, "attention_scored");
-    }
     // Without scratch for split keys one block takes all of a query's keys.
     const AttentionShape shape = attention_shape(be->policy.compute_dtype, p, be->cus);
-    if (scratch_clash(be, shape.scratch, {sq, sk, sv, sy, sqo, sko})) {
+    if (scratch_clash(be, shape.scratch, {sq, sk, sv, sy, sqo, sko, sqc, skc, spf})) {
         return fail(be, TRELLIS_STATUS_INVALID_ARGUMENT, "attention: rows in the scratch");
     }
     DevMem scratch;
     void * split_keys = shape.scratch > 0 ? take_scratch(be, shape.scratch, &scratch) : nullptr;
     stage_begin(be, TRELLIS_SPARSE_HIP_STAGE_ELEMENTWISE);
-    const hipError_t err = launch_attention(be->policy.compute_dtype, p, shape, split_keys, be->stream);
+    const int dt = be->policy.compute_dtype;
+    const hipError_t err = scores != nullptr ? launch_attention_scored(dt, p, sc, shape, split_keys, be->stream)
+                                             : launch_attention(dt, p, shape, split_keys, be->stream);
     stage_end(be, TRELLIS_SPARSE_HIP_STAGE_ELEMENTWISE);
     dev_release(be, &scratch);
     return hip_status(be, err, "attention");

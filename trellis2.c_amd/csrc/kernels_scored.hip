@@ -114,13 +114,718 @@ template <int DT> hipError_t launch_any(const Attention & p, const Scores & sc, 
     return hipGetLastError();
 }
 
+// ---- MFMA ---------------------------------------------------------------------------------------
+
+// The coordinates of a tile's 64 keys, counted from an origin: as they are, and as the A
+// operand of the squared distances.
+struct VoxelTile {
+    int4 parts[64][2];
+    int3 at[64];
+    int far;  // some key is more than 1,023 from the origin on an axis
+
+    __device__ __forceinline__ void set(int key, const int3 & xyz, const int3 & origin);
+};
+struct VoxelQuery {
+    s16x8 parts;
+    float square;
+    int3 at;
+    bool far;
+};
+
+__device__ __forceinline__ short bf16_whole(int v) {
+    return (short) (__builtin_bit_cast(uint32_t, (float) v) >> 16);
+}
+// Whether d (a difference that may have wrapped) is beyond what the products hold.
+__device__ __forceinline__ bool beyond(int d) { return (uint32_t) (d + 1023) > 2046u; }
+
+__device__ __forceinline__ void VoxelTile::set(int key, const int3 & xyz, const int3 & origin) {
+    int x = xyz.x - origin.x, y = xyz.y - origin.y, z = xyz.z - origin.z;
+    const bool out = beyond(x) || beyond(y) || beyond(z);
+    at[key] = xyz;
+    if (out) x = y = z = 0;
+    const int sq = x * x + y * y + z * z;
+    const short xh = bf16_whole(x >> 5), xl = bf16_whole(x & 31), yh = bf16_whole(y >> 5), yl = bf16_whole(y & 31);
+    const short zh = bf16_whole(z >> 5), zl = bf16_whole(z & 31);
+    const s16x8 a{xh, xl, xh, xl, yh, yl, yh, yl};
+    const s16x8 b{zh, zl, zh, zl, bf16_whole(sq >> 16), bf16_whole((sq >> 8) & 255), bf16_whole(sq & 255), 0};
+    parts[key][0] = __builtin_bit_cast(int4, a);
+    parts[key][1] = __builtin_bit_cast(int4, b);
+    const unsigned long long any = __ballot(out);
+    if (key == 0) far = any != 0 ? 1 : 0;
+}
+
+// half: which 8 of the 16 terms the lane holds.
+__device__ __forceinline__ VoxelQuery voxel_query(const int3 & xyz, const int3 & origin, int half) {
+    VoxelQuery q;
+    q.at = xyz;
+    int x = xyz.x - origin.x, y = xyz.y - origin.y, z = xyz.z - origin.z;
+    q.far = beyond(x) || beyond(y) || beyond(z);
+    if (q.far) x = y = z = 0;
+    q.square = (float) (x * x + y * y + z * z);
+    const auto high = [](int v, int by) { return bf16_whole((v >> 5) * by); };
+    const auto low = [](int v, int by) { return bf16_whole((v & 31) * by); };
+    const s16x8 a{high(x, -2048), high(x, -64), low(x, -64), low(x, -2), high(y, -2048), high(y, -64), low(y, -64), low(y, -2)};
+    const s16x8 b{high(z, -2048), high(z, -64), low(z, -64), low(z, -2), bf16_whole(65536), bf16_whole(256), bf16_whole(1), 0};
+    q.parts = half == 0 ? a : b;
+    return q;
+}
+
+// 16-bit values: whether one of eight is an infinity or a NaN, and zeros in place of those.
+template <int DT> __device__ __forceinline__ bool any_not_finite(const int4 & c) {
+    constexpr uint32_t E = DT == kBF16 ? 0x7f80u : 0x7c00u;
+    bool some = false;
+#pragma unroll
+    for (uint32_t w : {(uint32_t) c.x, (uint32_t) c.y, (uint32_t) c.z, (uint32_t) c.w})
+        some |= (w & E) == E || ((w >> 16) & E) == E;
+    return some;
+}
+template <int DT> __device__ __forceinline__ s16x8 finite_part(s16x8 v) {
+    constexpr short E = DT == kBF16 ? 0x7f80 : 0x7c00;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = (v[i] & E) == E ? (short) 0 : v[i];
+    return v;
+}
+
+// As k_attention, its scores changed between the products and the softmax.  What that adds
+// runs on the vector unit, which bounds attention already; distances of voxels are the
+// matrix unit's: |p - k|^2 = |p|^2 - 2 p . k + |k|^2 as one product of 16 terms, coordinates
+// in two parts of 5 bits and |k|^2 in three of 8, all whole numbers that bf16 holds.
+// Counted from the block's first query they are exact as long as none is more than
+// 1,023 away on an axis (all sums then stay below 2^24); farther ones are taken one by one.
+template <int DT, int DC, int NW, bool FINE>
+__global__ void __launch_bounds__(64 * NW, 2) k_scored(Attention p, Scores sc, Partial part, int tiles) {
+    using T = typename Store<DT>::T;
+    constexpr int TQ = 32 * NW, TK = 64;
+    constexpr int LP = DC <= 64 ? 64 : 128;      // values per LDS row
+    constexpr int ROW = LP * 2, CH = LP / 8;     // its bytes and chunks
+    constexpr int KS = DC / 16, DT32 = DC / 32;  // K steps of the scores, 32-row tiles of the output
+    constexpr int TILE = TK * ROW;
+    constexpr int RPL = 64 / CH;                 // rows per load of 1 KB
+    constexpr int LOADS = TILE / 1024;
+    constexpr int PER = LOADS / NW;              // of K, and of V, per wavefront
+    static_assert(LOADS % NW == 0, "whole loads");
+    __shared__ __attribute__((aligned(1024))) unsigned char s_tile[4 * TILE];  // K, V of two tiles
+    __shared__ VoxelTile s_voxel[2];
+
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int l32 = lane & 31, half = lane >> 5;
+    const int group = p.heads / p.kv_heads;
+
+    // Neighbouring blocks share a kv head; each XCD takes a contiguous range, in causal calls
+    // from the last queries, which see most, to the first.
+    const int64_t unit = xcd_remap(blockIdx.x, gridDim.x);
+    const int split = (int) (unit % part.splits);
+    const int kv = (int) (unit / part.splits / tiles);
+    const int64_t tile_at = unit / part.splits % tiles;
+    const Place at = find_place<TQ>(p, sc.causal != 0 ? tiles - 1 - tile_at : tile_at, group);
+    if (at.nq <= 0) return;
+    const int seen = (int) keys_seen(at, sc, (at.first + at.nq - 1) / group);
+    const int all = (seen + TK - 1) / TK;
+    const int t0 = (int) ((int64_t) all * split / part.splits), t1 = (int) ((int64_t) all * (split + 1) / part.splits);
+
+    // This lane's query.
+    const int qi = wave * 32 + l32;
+    const int64_t vq = at.first + qi;
+    const int64_t row = at.q0 + vq / group;
+    const int head = kv * group + (int) (vq % group);
+    const bool live = qi < at.nq;
+    s16x8 q[KS];
+    {
+        const T * qr = (const T *) p.q + row * p.q_stride + (int64_t) head * p.dim;
+        const int flip = p.scale < 0.0f ? (int) 0x80008000u : 0;  // the reference follows the largest score
+#pragma unroll
+        for (int k = 0; k < KS; ++k) {
+            const int c = (2 * k + half) * 8;
+            int4 v{0, 0, 0, 0};
+            if (live && c < p.dim) v = *(const int4 *) (qr + c);
+            q[k] = __builtin_bit_cast(s16x8, int4{v.x ^ flip, v.y ^ flip, v.z ^ flip, v.w ^ flip});
+        }
+    }
+    const bool changed = sc.cap > 0.0f || sc.slopes != nullptr;  // scores are then in log2 units
+    const float scale = changed ? 1.0f : fabsf(p.scale);
+    // The query's place among the keys, and the last key that it sees.
+    const int64_t query = vq / group;
+    const int place = (int) (query + at.nk - at.rows);
+    const int limit = (live ? (int) keys_seen(at, sc, query) : seen) - 1;  // (lanes without one mask nothing)
+    const float slope = sc.slopes != nullptr && live ? sc.slopes[head] * 1.44269504f : 0.0f;
+    VoxelQuery voxel;
+    int3 origin{0, 0, 0};
+    if (sc.q_xyz != nullptr) {
+        origin = voxel_of(sc.q_xyz, at.q0 + at.first / group);
+        voxel = voxel_query(live ? voxel_of(sc.q_xyz, row) : origin, origin, half);
+    }
+    // The coordinates of tile t's keys, a key a lane of the first wavefront: fetched, and left in LDS.
+    int3 key_xyz{0, 0, 0};
+    const auto fetch_xyz = [&](int t) {
+        if (sc.k_xyz == nullptr || wave != 0) return;
+        key_xyz = t * TK + lane < at.nk ? voxel_of(sc.k_xyz, at.k0 + t * TK + lane) : origin;
+    };
+    const auto leave_xyz = [&](int j) {
+        if (sc.k_xyz == nullptr || wave != 0) return;
+        s_voxel[j & 1].set(lane, key_xyz, origin);
+    };
+
+    const auto swizzle = [](int r) {
+        if constexpr (LP == 128) return ((r & 3) << 2) | ((r >> 2) & 3);
+        return (((r >> 1) & 1) << 2) | (((r >> 2) & 1) << 1) | ((r >> 3) & 1);
+    };
+    // Loads: row lane / CH of RPL, the chunk that lands at place lane % CH.
+    // Rows of one load and the next differ in bits that swizzle sees, so each
+    // load has its own chunk.
+    const char * kb = (const char *) ((const T *) p.k + at.k0 * p.k_stride + (int64_t) kv * p.dim);
+    const char * vb = (const char *) ((const T *) p.v + at.k0 * p.v_stride + (int64_t) kv * p.dim);
+    const int ks = (int) p.k_stride * 2, vs = (int) p.v_stride * 2;
+    constexpr uint32_t kOutside = 0x80000000u;
+    uint32_t k_off[PER], v_off[PER];
+#pragma unroll
+    for (int j = 0; j < PER; ++j) {
+        const int r = (wave * PER + j) * RPL + lane / CH;
+        const int c = (lane % CH) ^ swizzle(r);
+        const bool in = c * 8 < p.dim;
+        k_off[j] = in ? (uint32_t) (r * ks + c * 16) : kOutside;
+        v_off[j] = in ? (uint32_t) (r * vs + c * 16) : kOutside;
+    }
+    const uint32_t lds0 = (uint32_t) (uintptr_t) (__attribute__((address_space(3))) unsigned char *) s_tile;
+    const auto load = [&](const char * base, int pitch, const uint32_t (&off)[PER], int rows, uint32_t to) {
+        if (rows >= TK) {
+            const __amdgpu_buffer_rsrc_t res =
+                __builtin_amdgcn_make_buffer_rsrc((void *) base, 0, (TK - 1) * pitch + p.dim * 2, 0x00020000);
+#pragma unroll
+            for (int j = 0; j < PER; ++j) dma_b128_m0(res, lds0 + to + (wave * PER + j) * 1024u, off[j], 0);
+        } else {
+            // Rows past the end are zeros.
+            const __amdgpu_buffer_rsrc_t res =
+                __builtin_amdgcn_make_buffer_rsrc((void *) base, 0, (rows - 1) * pitch + p.dim * 2, 0x00020000);
+#pragma unroll
+            for (int j = 0; j < PER; ++j)
+                dma_b128_m0(res, lds0 + to + (wave * PER + j) * 1024u,
+                            (wave * PER + j) * RPL + lane / CH < rows ? off[j] : kOutside, 0);
+        }
+    };
+    // Tile t's keys go to buffer (t - t0) % 2, its values to the same of two more;
+    // the next tile to load of each, and where it is.
+    int tk = t0, tv = t0;
+    const char * k_at = kb + (int64_t) t0 * TK * ks;
+    const char * v_at = vb + (int64_t) t0 * TK * vs;
+    const auto load_k = [&]() {
+        load(k_at, ks, k_off, at.nk - tk * TK, (uint32_t) (((tk - t0) & 1) * TILE));
+        ++tk;
+        k_at += (int64_t) TK * ks;
+    };
+    const auto load_v = [&]() {
+        load(v_at, vs, v_off, at.nk - tv * TK, (uint32_t) (((tv - t0) & 1) * TILE + 2 * TILE));
+        ++tv;
+        v_at += (int64_t) TK * vs;
+    };
+
+    // Reads: K row l32 (+ 32), chunk 2 k + half; V rows 4 half + (lane % 16) / 4
+    // (+ 8, + 16 g), 16-value column block (lane / 16) % 2 of each 32.
+    uint32_t k_read[KS];
+#pragma unroll
+    for (int k = 0; k < KS; ++k) k_read[k] = (uint32_t) (l32 * ROW + (((2 * k + half) ^ swizzle(l32)) * 16));
+    uint32_t v_read[DT32][2];
+#pragma unroll
+    for (int d = 0; d < DT32; ++d)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            const int r = 8 * e + 4 * half + ((lane & 15) >> 2);
+            const int c = 4 * d + 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
+            v_read[d][e] = (uint32_t) (r * ROW + ((c ^ swizzle(r)) * 16) + (lane & 1) * 8);
+        }
+
+    f32x16 out[DT32];
+#pragma unroll
+    for (int d = 0; d < DT32; ++d)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) out[d][i] = 0.0f;
+    float ref = -__builtin_inff(), sum0 = 0.0f, sum1 = 0.0f;
+
+    // The scores' product k (of KS) of keys n (of 2).
+    const auto read_k = [&](const unsigned char * sk, int n, int k) {
+        return *(const s16x8 *) (sk + n * 32 * ROW + k_read[k]);
+    };
+    const auto zero = [](f32x16 & v) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) v[i] = 0.0f;
+    };
+    // Products to scores in log2 units: the cap, then the distance.  `d2` is free for now.
+    const auto change_scores = [&](int t, int j, f32x16 (&cur)[2], f32x16 (&d2)[2]) {
+        if (sc.cap > 0.0f) {
+            // cap tanh(z) = cap - 2 cap / (1 + exp(2 z)).
+            const float twice = 2.88539008f * fabsf(sc.cap_scale), both = -2.0f * sc.cap;
+#pragma unroll
+            for (int n = 0; n < 2; ++n)
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+                    cur[n][i] = fmaf(both, __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(cur[n][i] * twice)), sc.cap);
+        } else {
+            const float by = fabsf(p.scale);
+#pragma unroll
+            for (int n = 0; n < 2; ++n)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) cur[n][i] *= by;
+        }
+        if (sc.slopes == nullptr) return;
+        if (sc.q_xyz == nullptr) {
+            const float from = (float) (place - t * TK - 4 * half);
+#pragma unroll
+            for (int n = 0; n < 2; ++n)
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+                    cur[n][i] = fmaf(-slope, fabsf(from - (float) (n * 32 + 8 * (i / 4) + i % 4)), cur[n][i]);
+            return;
+        }
+        const VoxelTile & keys = s_voxel[j & 1];
+        if (uniform(keys.far) == 0 && !__any(voxel.far)) {
+#pragma unroll
+            for (int n = 0; n < 2; ++n) {
+#pragma unroll
+                for (int i = 0; i < 16; ++i) d2[n][i] = voxel.square;
+                d2[n] = mac32<kBF16>(*(const s16x8 *) &keys.parts[n * 32 + l32][half], voxel.parts, d2[n]);
+            }
+#pragma unroll
+            for (int n = 0; n < 2; ++n)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) cur[n][i] = fmaf(-slope, __builtin_amdgcn_sqrtf(d2[n][i]), cur[n][i]);
+        } else {
+#pragma unroll
+            for (int n = 0; n < 2; ++n)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    const float d = distance_of(voxel.at, keys.at[n * 32 + 8 * (i / 4) + 4 * half + i % 4]);
+                    cur[n][i] = fmaf(-slope, d, cur[n][i]);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+        }
+    };
+
+    // What a query does not see has weight zero, but zero times an infinity or a NaN is a
+    // NaN: where a tile with unseen keys has such values, the products take zeros for
+    // them, and those that are seen are added apart.
+    const auto values_not_finite = [&](const unsigned char * sv) {
+        bool some = false;
+        for (int i = lane * 16; i < TILE; i += 1024) some |= any_not_finite<DT>(*(const int4 *) (sv + i));
+        return (bool) __any(some);
+    };
+    const auto add_not_finite = [&](const unsigned char * sv, int last) {
+#pragma unroll 1
+        for (int r = 0; r < TK; ++r) {
+            if (r - 4 * half > last) break;
+#pragma unroll
+            for (int d = 0; d < DT32; ++d)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int c = d * 32 + i * 8 + half * 4;
+                    const T * v = (const T *) (sv + r * ROW + (((c / 8) ^ swizzle(r)) * 16) + half * 8);
+#pragma unroll
+                    for (int u = 0; u < 4; ++u) {
+                        const float x = Store<DT>::ld(v, u);
+                        if (!(fabsf(x) < __builtin_inff())) out[d][4 * i + u] += x;
+                    }
+                }
+        }
+    };
+
+    // One tile: softmax of `cur`, the scores of tile t, and their products with
+    // its values, and the scores of tile t + 1 into `nxt`.  Products and
+    // exponentials are written down in turns, in four steps of 16 keys:
+    //   step g: weights of group g; the values' products of group g - 1 beside the
+    //   first half of them, a quarter of the next scores beside the second.
+    // Fragments are read half a step before their products.
+    const auto tile = [&](int t, int j, f32x16 (&cur)[2], f32x16 (&nxt)[2]) {
+        if (changed) change_scores(t, j, cur, nxt);
+        const int last = limit - t * TK - 4 * half;  // of this tile's keys, less what the lane's half adds
+        const bool masked = __any(last < TK - 5);
+        if (masked) {
+#pragma unroll
+            for (int n = 0; n < 2; ++n)
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+                    if (n * 32 + 8 * (i / 4) + i % 4 > last) cur[n][i] = -__builtin_inff();
+        }
+        float m = cur[0][0];
+#pragma unroll
+        for (int n = 0; n < 2; ++n)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) m = fmaxf(m, cur[n][i]);
+        m = max_halves(m) * scale;
+        if (__any(m > ref + 8.0f)) {
+            const float next = m > ref + 8.0f ? m : ref;  // each query by itself: what it does not see moves nothing
+            const float keep = next == -__builtin_inff() ? 1.0f : __builtin_amdgcn_exp2f(ref - next);
+            ref = next;
+            sum0 *= keep;
+            sum1 *= keep;
+#pragma unroll
+            for (int d = 0; d < DT32; ++d)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) out[d][i] *= keep;
+        }
+        constexpr float kLift = DT == kF16 ? 7.0f : 0.0f;
+        const float base = ref == -__builtin_inff() ? 0.0f : ref - kLift;
+        // Keys of t + 1 and values of t have landed; every wavefront is done with
+        // the keys of t and the values of t - 1.
+        wait_vmcnt<0>();
+        leave_xyz(j + 1);
+        lds_barrier();
+        if (t + 2 < t1) load_k();
+        if (t + 1 < t1) load_v();
+        fetch_xyz(t + 2);
+        // (Past the last tile these are old keys, and the scores are not used.)
+        const unsigned char * sk = s_tile + ((j & 1) ^ 1) * TILE;
+        const unsigned char * sv = s_tile + (j & 1) * TILE + 2 * TILE;
+        const bool odd = masked && values_not_finite(sv);
+        zero(nxt[0]);
+        zero(nxt[1]);
+        constexpr int QPS = KS / 2;  // products of the next scores per step
+        s16x8 kf[QPS], vf[DT32], w, rest;
+        const auto values = [&](int d) {
+            out[d] = mac32<DT>(vf[d], w, out[d]);
+            if constexpr (FINE) out[d] = mac32<DT>(vf[d], rest, out[d]);
+        };
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            float e[8];
+            const auto weight = [&](int i) {
+                e[i] = __builtin_amdgcn_exp2f(fmaf(cur[g / 2][8 * (g % 2) + i], scale, -base));
+            };
+#pragma unroll
+            for (int i = 0; i < QPS; ++i) kf[i] = read_k(sk, g / 2, g % 2 * QPS + i);
+            __builtin_amdgcn_sched_barrier(0);
+            if (g > 0) {
+#pragma unroll
+                for (int d = 0; d < DT32; ++d) {
+                    values(d);
+#pragma unroll
+                    for (int i = 4 * d / DT32; i < 4 * (d + 1) / DT32; ++i) weight(i);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) weight(i);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+#pragma unroll
+            for (int d = 0; d < DT32; ++d) {
+                union {
+                    s16x4 h[2];
+                    s16x8 v;
+                } a;
+#pragma unroll
+                for (int x = 0; x < 2; ++x)
+                    a.h[x] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                        (__attribute__((address_space(3))) s16x4 *) (sv + g * 16 * ROW + v_read[d][x]));
+                vf[d] = a.v;
+                if (odd) vf[d] = finite_part<DT>(vf[d]);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int i = 0; i < QPS; ++i) {
+                nxt[g / 2] = mac32<DT>(kf[i], q[g % 2 * QPS + i], nxt[g / 2]);
+#pragma unroll
+                for (int x = 4 + 4 * i / QPS; x < 4 + 4 * (i + 1) / QPS; ++x) weight(x);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            union {
+                T h[8];
+                s16x8 v;
+            } r;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                if constexpr (!FINE) r.h[i] = round_to_store<DT>(e[i]);
+                if (i % 2 == 0) {
+                    sum0 += e[i];
+                } else {
+                    sum1 += e[i];
+                }
+            }
+            if constexpr (FINE) {
+                two_parts<DT>(e, w, rest);
+            } else {
+                w = r.v;
+            }
+        }
+#pragma unroll
+        for (int d = 0; d < DT32; ++d) values(d);
+        if (odd) add_not_finite(sv, last);
+    };
+
+    if (t0 < t1) {
+        fetch_xyz(t0);
+        leave_xyz(0);
+        fetch_xyz(t0 + 1);
+        load_k();
+        load_v();
+        if (t0 + 1 < t1) load_k();
+        wait_vmcnt<0>();
+        lds_barrier();
+        f32x16 sa[2], sb[2];
+#pragma unroll
+        for (int n = 0; n < 2; ++n) {
+            zero(sa[n]);
+#pragma unroll
+            for (int k = 0; k < KS; ++k) sa[n] = mac32<DT>(read_k(s_tile, n, k), q[k], sa[n]);
+        }
+        for (int t = t0; t < t1; t += 2) {
+            tile(t, 0, sa, sb);
+            if (t + 1 >= t1) break;
+            tile(t + 1, 1, sb, sa);
+        }
+    }
+
+    leave<DT>(p, part, out, ref, sum_halves(sum0 + sum1), live, t0 < t1, split, row, head, half);
+}
+
+template <int DC, int NW>
+__global__ void __launch_bounds__(64 * NW, 2) k_scored32(Attention p, Scores sc, Partial part, int tiles) {
+    constexpr int TQ = 32 * NW, TK = 32;
+    constexpr int LP = DC <= 32 ? 32 : (DC <= 64 ? 64 : 128);  // values per LDS row
+    constexpr int ROW = LP * 4, CH = LP / 4;
+    constexpr int KS = DC / 8, DT32 = DC / 32;
+    constexpr int TILE = TK * ROW;
+    constexpr int RPL = 64 / CH;
+    constexpr int PER = TILE / 1024 / NW;
+    static_assert(TILE / 1024 % NW == 0, "whole loads");
+    __shared__ __attribute__((aligned(1024))) unsigned char s_tile[4 * TILE];  // K, V of two tiles
+
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int l32 = lane & 31, half = lane >> 5;
+    const int group = p.heads / p.kv_heads;
+    const int64_t unit = xcd_remap(blockIdx.x, gridDim.x);
+    const int split = (int) (unit % part.splits);
+    const int kv = (int) (unit / part.splits / tiles);
+    const int64_t tile_at = unit / part.splits % tiles;
+    const Place at = find_place<TQ>(p, sc.causal != 0 ? tiles - 1 - tile_at : tile_at, group);
+    if (at.nq <= 0) return;
+    const int seen = (int) keys_seen(at, sc, (at.first + at.nq - 1) / group);
+    const int all = (seen + TK - 1) / TK;
+    const int t0 = (int) ((int64_t) all * split / part.splits), t1 = (int) ((int64_t) all * (split + 1) / part.splits);
+
+    const int qi = wave * 32 + l32;
+    const int64_t vq = at.first + qi;
+    const int64_t row = at.q0 + vq / group;
+    const int head = kv * group + (int) (vq % group);
+    const bool live = qi < at.nq;
+    const bool changed = sc.cap > 0.0f || sc.slopes != nullptr;
+    const float sign = p.scale < 0.0f ? -1.0f : 1.0f, scale = changed ? 1.0f : fabsf(p.scale);
+    const int64_t query = vq / group;
+    const int place = (int) (query + at.nk - at.rows);
+    const int limit = (live ? (int) keys_seen(at, sc, query) : seen) - 1;  // (lanes without one mask nothing)
+    const float slope = sc.slopes != nullptr && live ? sc.slopes[head] * 1.44269504f : 0.0f;
+    const int3 here = sc.q_xyz != nullptr && live ? voxel_of(sc.q_xyz, row) : int3{0, 0, 0};
+    float q[KS][4];
+    {
+        const float * qr = (const float *) p.q + row * p.q_stride + (int64_t) head * p.dim;
+#pragma unroll
+        for (int k = 0; k < KS; ++k) {
+            const int c = 8 * k + 4 * half;
+            float4 v{0.f, 0.f, 0.f, 0.f};
+            if (live && c < p.dim) v = *(const float4 *) (qr + c);
+            q[k][0] = v.x * sign;
+            q[k][1] = v.y * sign;
+            q[k][2] = v.z * sign;
+            q[k][3] = v.w * sign;
+        }
+    }
+
+    const auto swizzle = [](int r) {
+        if constexpr (CH == 8) return (r >> 1) & 7;
+        return ((r & 4) << 1) | ((r & 8) >> 1) | (r & 3);
+    };
+    const char * kb = (const char *) ((const float *) p.k + at.k0 * p.k_stride + (int64_t) kv * p.dim);
+    const char * vb = (const char *) ((const float *) p.v + at.k0 * p.v_stride + (int64_t) kv * p.dim);
+    const int ks = (int) p.k_stride * 4, vs = (int) p.v_stride * 4;
+    constexpr uint32_t kOutside = 0x80000000u;
+    const uint32_t lds0 = (uint32_t) (uintptr_t) (__attribute__((address_space(3))) unsigned char *) s_tile;
+    // Rows past the last and channels past dim are zeros.
+    const auto load = [&](int t) {
+        const int rows = min(TK, at.nk - t * TK);
+        const uint32_t to = lds0 + (uint32_t) (((t - t0) & 1) * TILE);
+        const __amdgpu_buffer_rsrc_t kres = __builtin_amdgcn_make_buffer_rsrc(
+            (void *) (kb + (int64_t) t * TK * ks), 0, (rows - 1) * ks + p.dim * 4, 0x00020000);
+        const __amdgpu_buffer_rsrc_t vres = __builtin_amdgcn_make_buffer_rsrc(
+            (void *) (vb + (int64_t) t * TK * vs), 0, (rows - 1) * vs + p.dim * 4, 0x00020000);
+#pragma unroll
+        for (int j = 0; j < PER; ++j) {
+            const int r = (wave * PER + j) * RPL + lane / CH;
+            const int c = (lane % CH) ^ swizzle(r);
+            const bool in = r < rows && c * 4 < p.dim;
+            dma_b128_m0(kres, to + (wave * PER + j) * 1024u, in ? (uint32_t) (r * ks + c * 16) : kOutside, 0);
+            dma_b128_m0(vres, to + 2 * TILE + (wave * PER + j) * 1024u, in ? (uint32_t) (r * vs + c * 16) : kOutside, 0);
+        }
+    };
+
+    f32x16 out[DT32];
+#pragma unroll
+    for (int d = 0; d < DT32; ++d)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) out[d][i] = 0.0f;
+    float ref = -__builtin_inff(), sum0 = 0.0f, sum1 = 0.0f;
+    if (t0 < t1) load(t0);
+    for (int t = t0; t < t1; ++t) {
+        // Tile t has landed; every wavefront is done with tile t - 1.
+        wait_vmcnt<0>();
+        lds_barrier();
+        if (t + 1 < t1) load(t + 1);
+        const unsigned char * sk = s_tile + ((t - t0) & 1) * TILE;
+        const unsigned char * sv = sk + 2 * TILE;
+        f32x16 cur;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) cur[i] = 0.0f;
+#pragma unroll
+        for (int k = 0; k < KS; ++k) {
+            const float4 a = *(const float4 *) (sk + l32 * ROW + (((2 * k + half) ^ swizzle(l32)) * 16));
+            cur = __builtin_amdgcn_mfma_f32_32x32x2f32(a.x, q[k][0], cur, 0, 0, 0);
+            cur = __builtin_amdgcn_mfma_f32_32x32x2f32(a.y, q[k][1], cur, 0, 0, 0);
+            cur = __builtin_amdgcn_mfma_f32_32x32x2f32(a.z, q[k][2], cur, 0, 0, 0);
+            cur = __builtin_amdgcn_mfma_f32_32x32x2f32(a.w, q[k][3], cur, 0, 0, 0);
+        }
+        if (changed) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                const int key = min(t * TK + 8 * (i / 4) + 4 * half + i % 4, at.nk - 1);
+                cur[i] = sc.cap > 0.0f ? sc.cap * tanhf(cur[i] * fabsf(sc.cap_scale)) : cur[i] * fabsf(p.scale);
+                if (sc.slopes != nullptr) {
+                    const float d = sc.q_xyz != nullptr ? distance_of(here, voxel_of(sc.k_xyz, at.k0 + key))
+                                                        : fabsf((float) (place - key));
+                    cur[i] = fmaf(-slope, d, cur[i]);
+                }
+            }
+        }
+        const int last = limit - t * TK - 4 * half;
+        const bool masked = __any(last < TK - 5);
+        if (masked) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+                if (8 * (i / 4) + i % 4 > last) cur[i] = -__builtin_inff();
+        }
+        // As in k_scored: of values that are not finite the products take zeros where some are not seen.
+        bool odd = false;
+        if (masked) {
+            for (int i = lane * 16; i < TILE; i += 1024) {
+                const float4 v = *(const float4 *) (sv + i);
+                const float most = fmaxf(fmaxf(fabsf(v.x), fabsf(v.y)), fmaxf(fabsf(v.z), fabsf(v.w)));
+                odd |= !(most < __builtin_inff()) || v.x != v.x || v.y != v.y || v.z != v.z || v.w != v.w;
+            }
+            odd = __any(odd);
+        }
+        float m = cur[0];
+#pragma unroll
+        for (int i = 1; i < 16; ++i) m = fmaxf(m, cur[i]);
+        m = max_halves(m) * scale;
+        if (__any(m > ref + 8.0f)) {
+            const float next = m > ref + 8.0f ? m : ref;  // each query by itself: what it does not see moves nothing
+            const float keep = next == -__builtin_inff() ? 1.0f : __builtin_amdgcn_exp2f(ref - next);
+            ref = next;
+            sum0 *= keep;
+            sum1 *= keep;
+#pragma unroll
+            for (int d = 0; d < DT32; ++d)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) out[d][i] *= keep;
+        }
+        const float base = ref == -__builtin_inff() ? 0.0f : ref;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            const float e = __builtin_amdgcn_exp2f(fmaf(cur[i], scale, -base));
+            (i % 2 == 0 ? sum0 : sum1) += e;
+            const int r = 8 * (i / 4) + 4 * half + i % 4;
+#pragma unroll
+            for (int d = 0; d < DT32; ++d) {
+                float a = *(const float *) (sv + r * ROW + (((8 * d + l32 / 4) ^ swizzle(r)) * 16) + l32 % 4 * 4);
+                if (odd && !(fabsf(a) < __builtin_inff())) a = 0.0f;
+                out[d] = __builtin_amdgcn_mfma_f32_32x32x2f32(a, e, out[d], 0, 0, 0);
+            }
+        }
+        if (odd) {
+#pragma unroll 1
+            for (int r = 0; r < TK; ++r) {
+                if (r - 4 * half > last) break;
+#pragma unroll
+                for (int d = 0; d < DT32; ++d)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const float * v =
+                            (const float *) (sv + r * ROW + (((d * 8 + i * 2 + half) ^ swizzle(r)) * 16));
+#pragma unroll
+                        for (int u = 0; u < 4; ++u)
+                            if (!(fabsf(v[u]) < __builtin_inff())) out[d][4 * i + u] += v[u];
+                    }
+            }
+        }
+    }
+    leave<kF32>(p, part, out, ref, sum_halves(sum0 + sum1), live, t0 < t1, split, row, head, half);
+}
+
+template <int DT, int DC, int NW>
+hipError_t launch_nw(const Attention & p, const Scores & sc, const Partial & part, int64_t tiles, bool fine, hipStream_t s) {
+    const int64_t grid = tiles * p.kv_heads * part.splits;
+    if (grid > 0x7fffffffLL) return hipErrorInvalidValue;
+    if constexpr (DT == kF32) {
+        k_scored32<DC, NW><<<(unsigned) grid, 64 * NW, 0, s>>>(p, sc, part, (int) tiles);
+    } else {
+        if (fine) {
+            k_scored<DT, DC, NW, true><<<(unsigned) grid, 64 * NW, 0, s>>>(p, sc, part, (int) tiles);
+        } else {
+            k_scored<DT, DC, NW, false><<<(unsigned) grid, 64 * NW, 0, s>>>(p, sc, part, (int) tiles);
+        }
+    }
+    hipError_t err = hipGetLastError();
+    if (err == hipSuccess && part.splits > 1) {
+        int qp = 1;
+        while (qp * 4 < p.dim) qp *= 2;
+        // 77 splits of 64 channels: 12 us with a wavefront a query, 6.5 with four.
+        const bool wide = part.splits >= 32;
+        const int64_t joins = tiles * p.kv_heads * (wide ? 32 * NW : 8 * NW);
+        if (joins > 0x7fffffffLL) return hipErrorInvalidValue;
+        if (wide) {
+            k_join<DT, 32 * NW, 4><<<(unsigned) joins, 256, 0, s>>>(p, part, (int) tiles, qp);
+        } else {
+            k_join<DT, 32 * NW, 1><<<(unsigned) joins, 256, 0, s>>>(p, part, (int) tiles, qp);
+        }
+        err = hipGetLastError();
+    }
+    return err;
+}
+
+template <int DT, int DC>
+hipError_t launch_dc(const Attention & p, const Scores & sc, const Partial & part, const AttentionShape & sh, hipStream_t s) {
+    return sh.waves == 1 ? launch_nw<DT, DC, 1>(p, sc, part, sh.tiles, sh.fine, s)
+                         : launch_nw<DT, DC, 4>(p, sc, part, sh.tiles, sh.fine, s);
+}
+
+template <int DT>
+hipError_t launch_mfma(const Attention & p, const Scores & sc, const Partial & part, const AttentionShape & sh, hipStream_t s) {
+    if (p.dim <= 32) return launch_dc<DT, 32>(p, sc, part, sh, s);
+    if (p.dim <= 64) return launch_dc<DT, 64>(p, sc, part, sh, s);
+    if (p.dim <= 96) return launch_dc<DT, 96>(p, sc, part, sh, s);
+    return launch_dc<DT, 128>(p, sc, part, sh, s);
+}
+
 }  // namespace
 
-hipError_t launch_attention_scored(int dtype, const Attention & p, const Scores & sc, hipStream_t s) {
+// Run as attention of the same sizes is (attention_shape).
+hipError_t launch_attention_scored(int dtype, const Attention & p, const Scores & sc, const AttentionShape & sh,
+                                   void * scratch, hipStream_t s) {
+    if (sh.waves == 0) {
+        switch (dtype) {
+            case kF32: return launch_any<kF32>(p, sc, s);
+            case kF16: return launch_any<kF16>(p, sc, s);
+            default: return launch_any<kBF16>(p, sc, s);
+        }
+    }
+    Partial part{nullptr, nullptr, 1};
+    if (scratch != nullptr && sh.splits > 1) {
+        part.splits = sh.splits;
+        part.out = (float *) scratch;
+        part.stat = (float2 *) (part.out + (size_t) sh.splits * p.nq * p.heads * p.dim);
+    }
+    if (sh.tiles > 0x7fffffffLL) return hipErrorInvalidValue;
     switch (dtype) {
-        case kF32: return launch_any<kF32>(p, sc, s);
-        case kF16: return launch_any<kF16>(p, sc, s);
-        default: return launch_any<kBF16>(p, sc, s);
+        case kF32: return launch_mfma<kF32>(p, sc, part, sh, s);
+        case kF16: return launch_mfma<kF16>(p, sc, part, sh, s);
+        default: return launch_mfma<kBF16>(p, sc, part, sh, s);
     }
 }
 

@@ -457,7 +457,8 @@ struct Scores {
     const int32_t * prefix;  // [seqs] or null
     int causal;
 };
-hipError_t launch_attention_scored(int dtype, const Attention & p, const Scores & scores, hipStream_t s);
+hipError_t launch_attention_scored(int dtype, const Attention & p, const Scores & scores, const AttentionShape & shape,
+                                   void * scratch, hipStream_t s);
 
 // Group norm (kernels_gnorm.hip).  gamma, beta and at may be null; y may be x.
 struct GroupNorm {
