@@ -2475,7 +2475,7 @@ trellis_status check_scores(Backend * be, const trellis_sparse_hip_scores_desc &
         return fail(be, TRELLIS_STATUS_INVALID_ARGUMENT, "attention: bad scores");
     }
     // Twice the tanh's argument and the cap, both in log2 units, are taken with numbers of fp32.
-    if (!std::isfinite(d.cap * 1.4426950f) || (d.cap > 0.0f && !std::isfinite(2.0f * scale / d.cap))) {
+    if (!std::isfinite(d.cap * 2.8853902f) || (d.cap > 0.0f && !std::isfinite(4.0f * scale / d.cap))) {
         return fail(be, TRELLIS_STATUS_INVALID_ARGUMENT, "attention: cap beyond fp32's range");
     }
     if (d.slopes != nullptr) {
@@ -2570,6 +2570,9 @@ trellis_status attention_impl(trellis_sparse_backend * backend, const trellis_sp
         sc.slopes = (const float *) slopes;
         sc.cap = scores->cap * 1.4426950408889634f;
         sc.cap_scale = scores->cap > 0.0f ? (float) (natural / (double) scores->cap) : 0.0f;
+        sc.twice = 2.8853900817779268f * std::fabs(sc.cap_scale);
+        sc.by = scores->cap > 0.0f ? 2.0f * sc.cap : std::fabs(scale);
+        sc.over = (float) (1.4426950408889634 / (double) sc.by);
         sc.q_xyz = (const int32_t *) sqc.at;
         sc.k_xyz = (const int32_t *) skc.at;
         sc.prefix = (const int32_t *) spf.at;

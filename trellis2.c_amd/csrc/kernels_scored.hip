@@ -116,25 +116,25 @@ template <int DT> hipError_t launch_any(const Attention & p, const Scores & sc, 
 
 // ---- MFMA ---------------------------------------------------------------------------------------
 
-// The coordinates of a tile's 64 keys, counted from an origin: as they are, and as the A
-// operand of the squared distances.
+// The coordinates of a tile's 64 keys: as they are, and, counted from an origin, as the A
+// operand of the squared distances, |p - k|^2 = |p|^2 - 2 p . k + |k|^2 as one product of
+// seven terms in fp16: coordinates, and squares in two parts, all whole numbers of 11 bits.
+// The sums are exact as long as no voxel is more than 1,023 from the origin on an axis
+// (|p|^2 + |k|^2 + 2 |p . k| then stays below 2^24).
 struct VoxelTile {
-    int4 parts[64][2];
+    int4 terms[64];
     int3 at[64];
-    int far;  // some key is more than 1,023 from the origin on an axis
+    int far;  // some key is farther
 
     __device__ __forceinline__ void set(int key, const int3 & xyz, const int3 & origin);
 };
 struct VoxelQuery {
-    s16x8 parts;
-    float square;
+    s16x8 terms;
     int3 at;
     bool far;
 };
 
-__device__ __forceinline__ short bf16_whole(int v) {
-    return (short) (__builtin_bit_cast(uint32_t, (float) v) >> 16);
-}
+__device__ __forceinline__ short f16_whole(int v) { return __builtin_bit_cast(short, (_Float16) (float) v); }
 // Whether d (a difference that may have wrapped) is beyond what the products hold.
 __device__ __forceinline__ bool beyond(int d) { return (uint32_t) (d + 1023) > 2046u; }
 
@@ -144,29 +144,24 @@ __device__ __forceinline__ void VoxelTile::set(int key, const int3 & xyz, const 
     at[key] = xyz;
     if (out) x = y = z = 0;
     const int sq = x * x + y * y + z * z;
-    const short xh = bf16_whole(x >> 5), xl = bf16_whole(x & 31), yh = bf16_whole(y >> 5), yl = bf16_whole(y & 31);
-    const short zh = bf16_whole(z >> 5), zl = bf16_whole(z & 31);
-    const s16x8 a{xh, xl, xh, xl, yh, yl, yh, yl};
-    const s16x8 b{zh, zl, zh, zl, bf16_whole(sq >> 16), bf16_whole((sq >> 8) & 255), bf16_whole(sq & 255), 0};
-    parts[key][0] = __builtin_bit_cast(int4, a);
-    parts[key][1] = __builtin_bit_cast(int4, b);
+    const s16x8 a{f16_whole(x), f16_whole(y), f16_whole(z), f16_whole(sq >> 11), f16_whole(sq & 2047), f16_whole(2048),
+                  f16_whole(1), 0};
+    terms[key] = __builtin_bit_cast(int4, a);
     const unsigned long long any = __ballot(out);
     if (key == 0) far = any != 0 ? 1 : 0;
 }
 
-// half: which 8 of the 16 terms the lane holds.
+// The terms are those of the lanes' first half; the other's are zeros.
 __device__ __forceinline__ VoxelQuery voxel_query(const int3 & xyz, const int3 & origin, int half) {
     VoxelQuery q;
     q.at = xyz;
     int x = xyz.x - origin.x, y = xyz.y - origin.y, z = xyz.z - origin.z;
     q.far = beyond(x) || beyond(y) || beyond(z);
     if (q.far) x = y = z = 0;
-    q.square = (float) (x * x + y * y + z * z);
-    const auto high = [](int v, int by) { return bf16_whole((v >> 5) * by); };
-    const auto low = [](int v, int by) { return bf16_whole((v & 31) * by); };
-    const s16x8 a{high(x, -2048), high(x, -64), low(x, -64), low(x, -2), high(y, -2048), high(y, -64), low(y, -64), low(y, -2)};
-    const s16x8 b{high(z, -2048), high(z, -64), low(z, -64), low(z, -2), bf16_whole(65536), bf16_whole(256), bf16_whole(1), 0};
-    q.parts = half == 0 ? a : b;
+    const int sq = x * x + y * y + z * z;
+    const s16x8 b{f16_whole(-2 * x), f16_whole(-2 * y), f16_whole(-2 * z), f16_whole(2048), f16_whole(1),
+                  f16_whole(sq >> 11), f16_whole(sq & 2047), 0};
+    q.terms = half == 0 ? b : s16x8{0, 0, 0, 0, 0, 0, 0, 0};
     return q;
 }
 
@@ -187,11 +182,8 @@ template <int DT> __device__ __forceinline__ s16x8 finite_part(s16x8 v) {
 }
 
 // As k_attention, its scores changed between the products and the softmax.  What that adds
-// runs on the vector unit, which bounds attention already; distances of voxels are the
-// matrix unit's: |p - k|^2 = |p|^2 - 2 p . k + |k|^2 as one product of 16 terms, coordinates
-// in two parts of 5 bits and |k|^2 in three of 8, all whole numbers that bf16 holds.
-// Counted from the block's first query they are exact as long as none is more than
-// 1,023 away on an axis (all sums then stay below 2^24); farther ones are taken one by one.
+// runs on the vector unit, which bounds attention already; squared distances of voxels are the
+// matrix unit's, counted from the block's first query, but where some are too far for that.
 template <int DT, int DC, int NW, bool FINE>
 __global__ void __launch_bounds__(64 * NW, 2) k_scored(Attention p, Scores sc, Partial part, int tiles) {
     using T = typename Store<DT>::T;
@@ -242,13 +234,13 @@ __global__ void __launch_bounds__(64 * NW, 2) k_scored(Attention p, Scores sc, P
             q[k] = __builtin_bit_cast(s16x8, int4{v.x ^ flip, v.y ^ flip, v.z ^ flip, v.w ^ flip});
         }
     }
-    const bool changed = sc.cap > 0.0f || sc.slopes != nullptr;  // scores are then in log2 units
-    const float scale = changed ? 1.0f : fabsf(p.scale);
+    const bool changed = sc.cap > 0.0f || sc.slopes != nullptr;
+    const float scale = sc.by;
     // The query's place among the keys, and the last key that it sees.
     const int64_t query = vq / group;
     const int place = (int) (query + at.nk - at.rows);
     const int limit = (live ? (int) keys_seen(at, sc, query) : seen) - 1;  // (lanes without one mask nothing)
-    const float slope = sc.slopes != nullptr && live ? sc.slopes[head] * 1.44269504f : 0.0f;
+    const float slope = sc.slopes != nullptr && live ? -sc.slopes[head] * sc.over : 0.0f;
     VoxelQuery voxel;
     int3 origin{0, 0, 0};
     if (sc.q_xyz != nullptr) {
@@ -349,22 +341,16 @@ __global__ void __launch_bounds__(64 * NW, 2) k_scored(Attention p, Scores sc, P
 #pragma unroll
         for (int i = 0; i < 16; ++i) v[i] = 0.0f;
     };
-    // Products to scores in log2 units: the cap, then the distance.  `d2` is free for now.
+    // Products to what times `scale` is a score in log2 units: the cap, then the distance.
+    // `d2` is free for now.
     const auto change_scores = [&](int t, int j, f32x16 (&cur)[2], f32x16 (&d2)[2]) {
         if (sc.cap > 0.0f) {
-            // cap tanh(z) = cap - 2 cap / (1 + exp(2 z)).
-            const float twice = 2.88539008f * fabsf(sc.cap_scale), both = -2.0f * sc.cap;
+            // cap tanh(z) is cap less 2 cap / (1 + exp(2 z)), the cap the same for all keys.
 #pragma unroll
             for (int n = 0; n < 2; ++n)
 #pragma unroll
                 for (int i = 0; i < 16; ++i)
-                    cur[n][i] = fmaf(both, __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(cur[n][i] * twice)), sc.cap);
-        } else {
-            const float by = fabsf(p.scale);
-#pragma unroll
-            for (int n = 0; n < 2; ++n)
-#pragma unroll
-                for (int i = 0; i < 16; ++i) cur[n][i] *= by;
+                    cur[n][i] = __builtin_amdgcn_rcpf(-1.0f - __builtin_amdgcn_exp2f(cur[n][i] * sc.twice));
         }
         if (sc.slopes == nullptr) return;
         if (sc.q_xyz == nullptr) {
@@ -373,28 +359,27 @@ __global__ void __launch_bounds__(64 * NW, 2) k_scored(Attention p, Scores sc, P
             for (int n = 0; n < 2; ++n)
 #pragma unroll
                 for (int i = 0; i < 16; ++i)
-                    cur[n][i] = fmaf(-slope, fabsf(from - (float) (n * 32 + 8 * (i / 4) + i % 4)), cur[n][i]);
+                    cur[n][i] = fmaf(slope, fabsf(from - (float) (n * 32 + 8 * (i / 4) + i % 4)), cur[n][i]);
             return;
         }
         const VoxelTile & keys = s_voxel[j & 1];
         if (uniform(keys.far) == 0 && !__any(voxel.far)) {
 #pragma unroll
             for (int n = 0; n < 2; ++n) {
-#pragma unroll
-                for (int i = 0; i < 16; ++i) d2[n][i] = voxel.square;
-                d2[n] = mac32<kBF16>(*(const s16x8 *) &keys.parts[n * 32 + l32][half], voxel.parts, d2[n]);
+                zero(d2[n]);
+                d2[n] = mac32<kF16>(__builtin_bit_cast(s16x8, keys.terms[n * 32 + l32]), voxel.terms, d2[n]);
             }
 #pragma unroll
             for (int n = 0; n < 2; ++n)
 #pragma unroll
-                for (int i = 0; i < 16; ++i) cur[n][i] = fmaf(-slope, __builtin_amdgcn_sqrtf(d2[n][i]), cur[n][i]);
+                for (int i = 0; i < 16; ++i) cur[n][i] = fmaf(slope, __builtin_amdgcn_sqrtf(d2[n][i]), cur[n][i]);
         } else {
 #pragma unroll
             for (int n = 0; n < 2; ++n)
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
                     const float d = distance_of(voxel.at, keys.at[n * 32 + 8 * (i / 4) + 4 * half + i % 4]);
-                    cur[n][i] = fmaf(-slope, d, cur[n][i]);
+                    cur[n][i] = fmaf(slope, d, cur[n][i]);
                     __builtin_amdgcn_sched_barrier(0);
                 }
         }
@@ -608,7 +593,7 @@ __global__ void __launch_bounds__(64 * NW, 2) k_scored32(Attention p, Scores sc,
     const int head = kv * group + (int) (vq % group);
     const bool live = qi < at.nq;
     const bool changed = sc.cap > 0.0f || sc.slopes != nullptr;
-    const float sign = p.scale < 0.0f ? -1.0f : 1.0f, scale = changed ? 1.0f : fabsf(p.scale);
+    const float sign = p.scale < 0.0f ? -1.0f : 1.0f, scale = changed ? 1.0f : sc.by;
     const int64_t query = vq / group;
     const int place = (int) (query + at.nk - at.rows);
     const int limit = (live ? (int) keys_seen(at, sc, query) : seen) - 1;  // (lanes without one mask nothing)
@@ -808,7 +793,8 @@ hipError_t launch_mfma(const Attention & p, const Scores & sc, const Partial & p
 // Run as attention of the same sizes is (attention_shape).
 hipError_t launch_attention_scored(int dtype, const Attention & p, const Scores & sc, const AttentionShape & sh,
                                    void * scratch, hipStream_t s) {
-    if (sh.waves == 0) {
+    // (Slopes over a scale that small could leave fp32.)
+    if (sh.waves == 0 || (sc.slopes != nullptr && sc.by < 0x1p-30f)) {
         switch (dtype) {
             case kF32: return launch_any<kF32>(p, sc, s);
             case kF16: return launch_any<kF16>(p, sc, s);

@@ -451,6 +451,8 @@ hipError_t launch_attention(int dtype, const Attention & p, const AttentionShape
 // Attention whose scores are changed before the softmax (kernels_scored.hip).
 struct Scores {
     float cap, cap_scale;    // cap times log2(e), 0: none; what a product of q and k is multiplied with inside the tanh
+    float twice;             // the exponent's factor in 1 / (1 + 2^(twice q . k)), for q of the scale's sign
+    float by, over;          // of products (capped: of -1 / (1 + ..)) to log2 units, and log2(e) over it
     const float * slopes;    // [heads] or null
     const int32_t * q_xyz;   // [nq][4] and [nk][4], or null: distances are of rows
     const int32_t * k_xyz;
