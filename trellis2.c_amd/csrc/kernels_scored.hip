@@ -1,5 +1,7 @@
 // kernels_scored.hip - attention whose scores are capped by a tanh, lowered by a distance, or masked:
 // out_i = sum_j softmax_j(cap tanh(scale q_i . k_j / cap) - slope d(i, j)) v_j over the keys that i sees.
+#include <type_traits>
+
 #include "attn_common.h"
 
 namespace tsh {
@@ -128,11 +130,6 @@ struct VoxelTile {
 
     __device__ __forceinline__ void set(int key, const int3 & xyz, const int3 & origin);
 };
-struct VoxelQuery {
-    s16x8 terms;
-    int3 at;
-    bool far;
-};
 
 __device__ __forceinline__ short f16_whole(int v) { return __builtin_bit_cast(short, (_Float16) (float) v); }
 // Whether d (a difference that may have wrapped) is beyond what the products hold.
@@ -151,18 +148,16 @@ __device__ __forceinline__ void VoxelTile::set(int key, const int3 & xyz, const 
     if (key == 0) far = any != 0 ? 1 : 0;
 }
 
-// The terms are those of the lanes' first half; the other's are zeros.
-__device__ __forceinline__ VoxelQuery voxel_query(const int3 & xyz, const int3 & origin, int half) {
-    VoxelQuery q;
-    q.at = xyz;
+// A query's terms (those of the lanes' first half; the other's are zeros); whether a lane's are beyond the products.
+__device__ __forceinline__ bool voxel_terms(const int3 & xyz, const int3 & origin, int half, s16x8 & terms) {
     int x = xyz.x - origin.x, y = xyz.y - origin.y, z = xyz.z - origin.z;
-    q.far = beyond(x) || beyond(y) || beyond(z);
-    if (q.far) x = y = z = 0;
+    const bool out = beyond(x) || beyond(y) || beyond(z);
+    if (out) x = y = z = 0;
     const int sq = x * x + y * y + z * z;
     const s16x8 b{f16_whole(-2 * x), f16_whole(-2 * y), f16_whole(-2 * z), f16_whole(2048), f16_whole(1),
                   f16_whole(sq >> 11), f16_whole(sq & 2047), 0};
-    q.terms = half == 0 ? b : s16x8{0, 0, 0, 0, 0, 0, 0, 0};
-    return q;
+    terms = half == 0 ? b : s16x8{0, 0, 0, 0, 0, 0, 0, 0};
+    return (bool) __any(out);
 }
 
 // 16-bit values: whether one of eight is an infinity or a NaN, and zeros in place of those.
@@ -184,8 +179,8 @@ template <int DT> __device__ __forceinline__ s16x8 finite_part(s16x8 v) {
 // As k_attention, its scores changed between the products and the softmax.  What that adds
 // runs on the vector unit, which bounds attention already; squared distances of voxels are the
 // matrix unit's, counted from the block's first query, but where some are too far for that.
-template <int DT, int DC, int NW, bool FINE>
-__global__ void __launch_bounds__(64 * NW, 2) k_scored(Attention p, Scores sc, Partial part, int tiles) {
+template <int DT, int DC, int NW, bool FINE, bool VOXELS>
+__global__ void __launch_bounds__(64 * NW, DC <= 64 ? 3 : 2) k_scored(Attention p, Scores sc, Partial part, int tiles) {
     using T = typename Store<DT>::T;
     constexpr int TQ = 32 * NW, TK = 64;
     constexpr int LP = DC <= 64 ? 64 : 128;      // values per LDS row
@@ -197,7 +192,7 @@ __global__ void __launch_bounds__(64 * NW, 2) k_scored(Attention p, Scores sc, P
     constexpr int PER = LOADS / NW;              // of K, and of V, per wavefront
     static_assert(LOADS % NW == 0, "whole loads");
     __shared__ __attribute__((aligned(1024))) unsigned char s_tile[4 * TILE];  // K, V of two tiles
-    __shared__ VoxelTile s_voxel[2];
+    __shared__ typename std::conditional<VOXELS, VoxelTile, char>::type s_voxel[2];
 
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -241,21 +236,22 @@ __global__ void __launch_bounds__(64 * NW, 2) k_scored(Attention p, Scores sc, P
     const int place = (int) (query + at.nk - at.rows);
     const int limit = (live ? (int) keys_seen(at, sc, query) : seen) - 1;  // (lanes without one mask nothing)
     const float slope = sc.slopes != nullptr && live ? -sc.slopes[head] * sc.over : 0.0f;
-    VoxelQuery voxel;
+    s16x8 voxel;
+    bool far = false;
     int3 origin{0, 0, 0};
-    if (sc.q_xyz != nullptr) {
+    if constexpr (VOXELS) {
         origin = voxel_of(sc.q_xyz, at.q0 + at.first / group);
-        voxel = voxel_query(live ? voxel_of(sc.q_xyz, row) : origin, origin, half);
+        far = voxel_terms(live ? voxel_of(sc.q_xyz, row) : origin, origin, half, voxel);
     }
     // The coordinates of tile t's keys, a key a lane of the first wavefront: fetched, and left in LDS.
     int3 key_xyz{0, 0, 0};
     const auto fetch_xyz = [&](int t) {
-        if (sc.k_xyz == nullptr || wave != 0) return;
+        if (!VOXELS || wave != 0) return;
         key_xyz = t * TK + lane < at.nk ? voxel_of(sc.k_xyz, at.k0 + t * TK + lane) : origin;
     };
     const auto leave_xyz = [&](int j) {
-        if (sc.k_xyz == nullptr || wave != 0) return;
-        s_voxel[j & 1].set(lane, key_xyz, origin);
+        if (!VOXELS || wave != 0) return;
+        if constexpr (VOXELS) s_voxel[j & 1].set(lane, key_xyz, origin);
     };
 
     const auto swizzle = [](int r) {
@@ -341,47 +337,36 @@ __global__ void __launch_bounds__(64 * NW, 2) k_scored(Attention p, Scores sc, P
 #pragma unroll
         for (int i = 0; i < 16; ++i) v[i] = 0.0f;
     };
-    // Products to what times `scale` is a score in log2 units: the cap, then the distance.
-    // `d2` is free for now.
-    const auto change_scores = [&](int t, int j, f32x16 (&cur)[2], f32x16 (&d2)[2]) {
+    // Products with keys n * 32 .. of tile t to what times `scale` is a score in log2 units: the
+    // cap, then the distance.
+    const auto change_scores = [&](int t, int n, f32x16 & cur) {
         if (sc.cap > 0.0f) {
             // cap tanh(z) is cap less 2 cap / (1 + exp(2 z)), the cap the same for all keys.
 #pragma unroll
-            for (int n = 0; n < 2; ++n)
-#pragma unroll
-                for (int i = 0; i < 16; ++i)
-                    cur[n][i] = __builtin_amdgcn_rcpf(-1.0f - __builtin_amdgcn_exp2f(cur[n][i] * sc.twice));
+            for (int i = 0; i < 16; ++i) cur[i] = __builtin_amdgcn_rcpf(-1.0f - __builtin_amdgcn_exp2f(cur[i] * sc.twice));
         }
         if (sc.slopes == nullptr) return;
-        if (sc.q_xyz == nullptr) {
-            const float from = (float) (place - t * TK - 4 * half);
+        if constexpr (VOXELS) {
+            const VoxelTile & keys = (const VoxelTile &) s_voxel[(t - t0) & 1];
+            if (uniform(keys.far) == 0 && !far) {
+                f32x16 d2;
+                zero(d2);
+                d2 = mac32<kF16>(__builtin_bit_cast(s16x8, keys.terms[n * 32 + l32]), voxel, d2);
 #pragma unroll
-            for (int n = 0; n < 2; ++n)
-#pragma unroll
-                for (int i = 0; i < 16; ++i)
-                    cur[n][i] = fmaf(slope, fabsf(from - (float) (n * 32 + 8 * (i / 4) + i % 4)), cur[n][i]);
-            return;
-        }
-        const VoxelTile & keys = s_voxel[j & 1];
-        if (uniform(keys.far) == 0 && !__any(voxel.far)) {
-#pragma unroll
-            for (int n = 0; n < 2; ++n) {
-                zero(d2[n]);
-                d2[n] = mac32<kF16>(__builtin_bit_cast(s16x8, keys.terms[n * 32 + l32]), voxel.terms, d2[n]);
-            }
-#pragma unroll
-            for (int n = 0; n < 2; ++n)
-#pragma unroll
-                for (int i = 0; i < 16; ++i) cur[n][i] = fmaf(slope, __builtin_amdgcn_sqrtf(d2[n][i]), cur[n][i]);
-        } else {
-#pragma unroll
-            for (int n = 0; n < 2; ++n)
+                for (int i = 0; i < 16; ++i) cur[i] = fmaf(slope, __builtin_amdgcn_sqrtf(d2[i]), cur[i]);
+            } else {
+                const int3 here = voxel_of(sc.q_xyz, live ? row : at.q0);
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
-                    const float d = distance_of(voxel.at, keys.at[n * 32 + 8 * (i / 4) + 4 * half + i % 4]);
-                    cur[n][i] = fmaf(slope, d, cur[n][i]);
+                    cur[i] = fmaf(slope, distance_of(here, keys.at[n * 32 + 8 * (i / 4) + 4 * half + i % 4]), cur[i]);
                     __builtin_amdgcn_sched_barrier(0);
                 }
+            }
+        } else {
+            const float from = (float) (place - t * TK - 4 * half);
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+                cur[i] = fmaf(slope, fabsf(from - (float) (n * 32 + 8 * (i / 4) + i % 4)), cur[i]);
         }
     };
 
@@ -412,14 +397,30 @@ __global__ void __launch_bounds__(64 * NW, 2) k_scored(Attention p, Scores sc, P
         }
     };
 
-    // One tile: softmax of `cur`, the scores of tile t, and their products with
-    // its values, and the scores of tile t + 1 into `nxt`.  Products and
-    // exponentials are written down in turns, in four steps of 16 keys:
-    //   step g: weights of group g; the values' products of group g - 1 beside the
-    //   first half of them, a quarter of the next scores beside the second.
-    // Fragments are read half a step before their products.
-    const auto tile = [&](int t, int j, f32x16 (&cur)[2], f32x16 (&nxt)[2]) {
-        if (changed) change_scores(t, j, cur, nxt);
+    // One tile: its scores, their softmax, and the products of weights and values a group of
+    // 16 keys behind the exponentials.
+    const auto tile = [&](int t) {
+        const int j = (t - t0) & 1;
+        // Keys and values of t have landed; every wavefront is done with those of t - 1.
+        wait_vmcnt<0>();
+        leave_xyz(j);
+        lds_barrier();
+        if (t + 1 < t1) {
+            load_k();
+            load_v();
+            fetch_xyz(t + 1);
+        }
+        const unsigned char * sk = s_tile + j * TILE;
+        const unsigned char * sv = s_tile + (j + 2) * TILE;
+        f32x16 cur[2];
+#pragma unroll
+        for (int n = 0; n < 2; ++n) {
+            zero(cur[n]);
+#pragma unroll
+            for (int k = 0; k < KS; ++k) cur[n] = mac32<DT>(read_k(sk, n, k), q[k], cur[n]);
+        }
+#pragma unroll
+        for (int n = 0; n < 2; ++n) change_scores(t, n, cur[n]);
         const int last = limit - t * TK - 4 * half;  // of this tile's keys, less what the lane's half adds
         const bool masked = __any(last < TK - 5);
         if (masked) {
@@ -448,22 +449,8 @@ __global__ void __launch_bounds__(64 * NW, 2) k_scored(Attention p, Scores sc, P
         }
         constexpr float kLift = DT == kF16 ? 7.0f : 0.0f;
         const float base = ref == -__builtin_inff() ? 0.0f : ref - kLift;
-        // Keys of t + 1 and values of t have landed; every wavefront is done with
-        // the keys of t and the values of t - 1.
-        wait_vmcnt<0>();
-        leave_xyz(j + 1);
-        lds_barrier();
-        if (t + 2 < t1) load_k();
-        if (t + 1 < t1) load_v();
-        fetch_xyz(t + 2);
-        // (Past the last tile these are old keys, and the scores are not used.)
-        const unsigned char * sk = s_tile + ((j & 1) ^ 1) * TILE;
-        const unsigned char * sv = s_tile + (j & 1) * TILE + 2 * TILE;
         const bool odd = masked && values_not_finite(sv);
-        zero(nxt[0]);
-        zero(nxt[1]);
-        constexpr int QPS = KS / 2;  // products of the next scores per step
-        s16x8 kf[QPS], vf[DT32], w, rest;
+        s16x8 vf[DT32], w, rest;
         const auto values = [&](int d) {
             out[d] = mac32<DT>(vf[d], w, out[d]);
             if constexpr (FINE) out[d] = mac32<DT>(vf[d], rest, out[d]);
@@ -474,20 +461,17 @@ __global__ void __launch_bounds__(64 * NW, 2) k_scored(Attention p, Scores sc, P
             const auto weight = [&](int i) {
                 e[i] = __builtin_amdgcn_exp2f(fmaf(cur[g / 2][8 * (g % 2) + i], scale, -base));
             };
-#pragma unroll
-            for (int i = 0; i < QPS; ++i) kf[i] = read_k(sk, g / 2, g % 2 * QPS + i);
-            __builtin_amdgcn_sched_barrier(0);
             if (g > 0) {
 #pragma unroll
                 for (int d = 0; d < DT32; ++d) {
                     values(d);
 #pragma unroll
-                    for (int i = 4 * d / DT32; i < 4 * (d + 1) / DT32; ++i) weight(i);
+                    for (int i = 8 * d / DT32; i < 8 * (d + 1) / DT32; ++i) weight(i);
                     __builtin_amdgcn_sched_barrier(0);
                 }
             } else {
 #pragma unroll
-                for (int i = 0; i < 4; ++i) weight(i);
+                for (int i = 0; i < 8; ++i) weight(i);
                 __builtin_amdgcn_sched_barrier(0);
             }
 #pragma unroll
@@ -502,14 +486,6 @@ __global__ void __launch_bounds__(64 * NW, 2) k_scored(Attention p, Scores sc, P
                         (__attribute__((address_space(3))) s16x4 *) (sv + g * 16 * ROW + v_read[d][x]));
                 vf[d] = a.v;
                 if (odd) vf[d] = finite_part<DT>(vf[d]);
-            }
-            __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-            for (int i = 0; i < QPS; ++i) {
-                nxt[g / 2] = mac32<DT>(kf[i], q[g % 2 * QPS + i], nxt[g / 2]);
-#pragma unroll
-                for (int x = 4 + 4 * i / QPS; x < 4 + 4 * (i + 1) / QPS; ++x) weight(x);
-                __builtin_amdgcn_sched_barrier(0);
             }
             union {
                 T h[8];
@@ -537,25 +513,9 @@ __global__ void __launch_bounds__(64 * NW, 2) k_scored(Attention p, Scores sc, P
 
     if (t0 < t1) {
         fetch_xyz(t0);
-        leave_xyz(0);
-        fetch_xyz(t0 + 1);
         load_k();
         load_v();
-        if (t0 + 1 < t1) load_k();
-        wait_vmcnt<0>();
-        lds_barrier();
-        f32x16 sa[2], sb[2];
-#pragma unroll
-        for (int n = 0; n < 2; ++n) {
-            zero(sa[n]);
-#pragma unroll
-            for (int k = 0; k < KS; ++k) sa[n] = mac32<DT>(read_k(s_tile, n, k), q[k], sa[n]);
-        }
-        for (int t = t0; t < t1; t += 2) {
-            tile(t, 0, sa, sb);
-            if (t + 1 >= t1) break;
-            tile(t + 1, 1, sb, sa);
-        }
+        for (int t = t0; t < t1; ++t) tile(t);
     }
 
     leave<DT>(p, part, out, ref, sum_halves(sum0 + sum1), live, t0 < t1, split, row, head, half);
@@ -750,10 +710,15 @@ hipError_t launch_nw(const Attention & p, const Scores & sc, const Partial & par
     if constexpr (DT == kF32) {
         k_scored32<DC, NW><<<(unsigned) grid, 64 * NW, 0, s>>>(p, sc, part, (int) tiles);
     } else {
-        if (fine) {
-            k_scored<DT, DC, NW, true><<<(unsigned) grid, 64 * NW, 0, s>>>(p, sc, part, (int) tiles);
+        const auto launch = [&](auto fine_c, auto voxels_c) {
+            k_scored<DT, DC, NW, decltype(fine_c)::value, decltype(voxels_c)::value>
+                <<<(unsigned) grid, 64 * NW, 0, s>>>(p, sc, part, (int) tiles);
+        };
+        using std::false_type, std::true_type;
+        if (sc.q_xyz != nullptr) {
+            fine ? launch(true_type(), true_type()) : launch(false_type(), true_type());
         } else {
-            k_scored<DT, DC, NW, false><<<(unsigned) grid, 64 * NW, 0, s>>>(p, sc, part, (int) tiles);
+            fine ? launch(true_type(), false_type()) : launch(false_type(), false_type());
         }
     }
     hipError_t err = hipGetLastError();
