@@ -193,6 +193,7 @@ __global__ void __launch_bounds__(64 * NW, DC <= 64 ? 3 : 2) k_scored(Attention 
     static_assert(LOADS % NW == 0, "whole loads");
     __shared__ __attribute__((aligned(1024))) unsigned char s_tile[4 * TILE];  // K, V of two tiles
     __shared__ typename std::conditional<VOXELS, VoxelTile, char>::type s_voxel[2];
+    __shared__ int s_odd[NW];
 
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -229,7 +230,6 @@ __global__ void __launch_bounds__(64 * NW, DC <= 64 ? 3 : 2) k_scored(Attention 
             q[k] = __builtin_bit_cast(s16x8, int4{v.x ^ flip, v.y ^ flip, v.z ^ flip, v.w ^ flip});
         }
     }
-    const bool changed = sc.cap > 0.0f || sc.slopes != nullptr;
     const float scale = sc.by;
     // The query's place among the keys, and the last key that it sees.
     const int64_t query = vq / group;
@@ -339,7 +339,7 @@ __global__ void __launch_bounds__(64 * NW, DC <= 64 ? 3 : 2) k_scored(Attention 
     };
     // Products with keys n * 32 .. of tile t to what times `scale` is a score in log2 units: the
     // cap, then the distance.
-    const auto change_scores = [&](int t, int n, f32x16 & cur) {
+    const auto change_scores = [&](int t, int n, f32x16 & cur, bool near, const int4 & terms) {
         if (sc.cap > 0.0f) {
             // cap tanh(z) is cap less 2 cap / (1 + exp(2 z)), the cap the same for all keys.
 #pragma unroll
@@ -347,14 +347,14 @@ __global__ void __launch_bounds__(64 * NW, DC <= 64 ? 3 : 2) k_scored(Attention 
         }
         if (sc.slopes == nullptr) return;
         if constexpr (VOXELS) {
-            const VoxelTile & keys = (const VoxelTile &) s_voxel[(t - t0) & 1];
-            if (uniform(keys.far) == 0 && !far) {
+            if (near) {
                 f32x16 d2;
                 zero(d2);
-                d2 = mac32<kF16>(__builtin_bit_cast(s16x8, keys.terms[n * 32 + l32]), voxel, d2);
+                d2 = mac32<kF16>(__builtin_bit_cast(s16x8, terms), voxel, d2);
 #pragma unroll
                 for (int i = 0; i < 16; ++i) cur[i] = fmaf(slope, __builtin_amdgcn_sqrtf(d2[i]), cur[i]);
             } else {
+                const VoxelTile & keys = (const VoxelTile &) s_voxel[(t - t0) & 1];
                 const int3 here = voxel_of(sc.q_xyz, live ? row : at.q0);
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
@@ -371,14 +371,22 @@ __global__ void __launch_bounds__(64 * NW, DC <= 64 ? 3 : 2) k_scored(Attention 
     };
 
     // What a query does not see has weight zero, but zero times an infinity or a NaN is a
-    // NaN: where a tile with unseen keys has such values, the products take zeros for
-    // them, and those that are seen are added apart.
-    const auto values_not_finite = [&](const unsigned char * sv) {
+    // NaN: of tiles with keys that some query of the block does not see, such values are
+    // added to the queries that see them here, and are zeros for the products.
+    const int least_seen = (int) keys_seen(at, sc, at.first / group);
+    const auto set_aside = [&](unsigned char * sv, int last) {
+        constexpr int PART = TILE / NW;
+        unsigned char * mine = sv + wave * PART + lane * 16;
         bool some = false;
-        for (int i = lane * 16; i < TILE; i += 1024) some |= any_not_finite<DT>(*(const int4 *) (sv + i));
-        return (bool) __any(some);
-    };
-    const auto add_not_finite = [&](const unsigned char * sv, int last) {
+#pragma unroll
+        for (int i = 0; i < PART; i += 1024) some |= any_not_finite<DT>(*(const int4 *) (mine + i));
+        const bool any = __any(some);
+        if (lane == 0) s_odd[wave] = any;
+        lds_barrier();
+        int odd = 0;
+#pragma unroll
+        for (int w = 0; w < NW; ++w) odd |= s_odd[w];
+        if (uniform(odd) == 0) return;
 #pragma unroll 1
         for (int r = 0; r < TK; ++r) {
             if (r - 4 * half > last) break;
@@ -395,6 +403,13 @@ __global__ void __launch_bounds__(64 * NW, DC <= 64 ? 3 : 2) k_scored(Attention 
                     }
                 }
         }
+        lds_barrier();
+#pragma unroll 1
+        for (int i = 0; i < PART; i += 1024) {
+            int4 * c = (int4 *) (mine + i);
+            *c = __builtin_bit_cast(int4, finite_part<DT>(__builtin_bit_cast(s16x8, *c)));
+        }
+        lds_barrier();
     };
 
     // One tile: its scores, their softmax, and the products of weights and values a group of
@@ -411,7 +426,15 @@ __global__ void __launch_bounds__(64 * NW, DC <= 64 ? 3 : 2) k_scored(Attention 
             fetch_xyz(t + 1);
         }
         const unsigned char * sk = s_tile + j * TILE;
-        const unsigned char * sv = s_tile + (j + 2) * TILE;
+        unsigned char * sv = s_tile + (j + 2) * TILE;
+        bool near = false;
+        int4 terms[2];
+        if constexpr (VOXELS) {
+            const VoxelTile & keys = (const VoxelTile &) s_voxel[j];
+            near = uniform(keys.far) == 0 && !far;
+#pragma unroll
+            for (int n = 0; n < 2; ++n) terms[n] = keys.terms[n * 32 + l32];
+        }
         f32x16 cur[2];
 #pragma unroll
         for (int n = 0; n < 2; ++n) {
@@ -420,7 +443,7 @@ __global__ void __launch_bounds__(64 * NW, DC <= 64 ? 3 : 2) k_scored(Attention 
             for (int k = 0; k < KS; ++k) cur[n] = mac32<DT>(read_k(sk, n, k), q[k], cur[n]);
         }
 #pragma unroll
-        for (int n = 0; n < 2; ++n) change_scores(t, n, cur[n]);
+        for (int n = 0; n < 2; ++n) change_scores(t, n, cur[n], near, terms[n]);
         const int last = limit - t * TK - 4 * half;  // of this tile's keys, less what the lane's half adds
         const bool masked = __any(last < TK - 5);
         if (masked) {
@@ -449,7 +472,7 @@ __global__ void __launch_bounds__(64 * NW, DC <= 64 ? 3 : 2) k_scored(Attention 
         }
         constexpr float kLift = DT == kF16 ? 7.0f : 0.0f;
         const float base = ref == -__builtin_inff() ? 0.0f : ref - kLift;
-        const bool odd = masked && values_not_finite(sv);
+        if (t * TK + TK > least_seen) set_aside(sv, last);
         s16x8 vf[DT32], w, rest;
         const auto values = [&](int d) {
             out[d] = mac32<DT>(vf[d], w, out[d]);
@@ -485,7 +508,6 @@ __global__ void __launch_bounds__(64 * NW, DC <= 64 ? 3 : 2) k_scored(Attention 
                     a.h[x] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
                         (__attribute__((address_space(3))) s16x4 *) (sv + g * 16 * ROW + v_read[d][x]));
                 vf[d] = a.v;
-                if (odd) vf[d] = finite_part<DT>(vf[d]);
             }
             union {
                 T h[8];
@@ -508,7 +530,6 @@ __global__ void __launch_bounds__(64 * NW, DC <= 64 ? 3 : 2) k_scored(Attention 
         }
 #pragma unroll
         for (int d = 0; d < DT32; ++d) values(d);
-        if (odd) add_not_finite(sv, last);
     };
 
     if (t0 < t1) {
