@@ -155,14 +155,15 @@ struct Partial {
     int splits;
 };
 
-// Lane (query, half) leaves channels d * 32 + 8 i + 4 half + 0 .. 3: of its split, or of y.
-template <int DT, int N>
-__device__ __forceinline__ void leave(const Attention & p, const Partial & part, const f32x16 (&out)[N], float ref,
-                                      float sum, bool live, bool some, int split, int64_t row, int head, int half) {
+// Lane (query, half) leaves channels d * 32 + 8 i + 4 half + 0 .. 3: of its split, at place
+// at_q() of part, or of y.
+template <int DT, int N, class At>
+__device__ __forceinline__ void leave_at(const Attention & p, const Partial & part, const f32x16 (&out)[N], float ref,
+                                         float sum, bool live, bool some, At && place, int64_t row, int head, int half) {
     using T = typename Store<DT>::T;
     if (!live) return;
     if (part.splits > 1) {
-        const int64_t at_q = ((int64_t) split * p.nq + row) * p.heads + head;
+        const int64_t at_q = place();
         if (half == 0) part.stat[at_q] = float2{ref, sum};
         if (!some) return;
         float * o = part.out + at_q * p.dim;
@@ -193,25 +194,19 @@ __device__ __forceinline__ void leave(const Attention & p, const Partial & part,
         }
 }
 
-// Joins the splits, a query to WAVES wavefronts (one with few splits, four with
-// many): QP lanes (a power of two) have four channels each, and the 64 WAVES / QP
-// groups of them every so many splits.  Queries are found as k_attention<.., NW>
-// does, TQ blocks' worth for each of its tiles.
-template <int DT, int TQ, int WAVES>
-__global__ void __launch_bounds__(256) k_join(Attention p, Partial part, int tiles, int qp) {
+template <int DT, int N>
+__device__ __forceinline__ void leave(const Attention & p, const Partial & part, const f32x16 (&out)[N], float ref,
+                                      float sum, bool live, bool some, int split, int64_t row, int head, int half) {
+    const auto place = [&] { return ((int64_t) split * p.nq + row) * p.heads + head; };
+    leave_at<DT>(p, part, out, ref, sum, live, some, place, row, head, half);
+}
+
+// The splits of a query, at places q + split * step of part, joined by WAVES wavefronts (see k_join).
+template <int DT, int WAVES>
+__device__ __forceinline__ void join_query(const Attention & p, const Partial & part, int qp, int64_t q, int64_t step,
+                                           int64_t row, int head, float (&s_sum)[4][64][5]) {
     using T = typename Store<DT>::T;
-    constexpr int QUERIES = 4 / WAVES, PER = TQ / QUERIES;
-    __shared__ float s_sum[4][64][5];
-    const int group = p.heads / p.kv_heads, kv = blockIdx.x / PER / tiles;
-    const Place at = find_place<TQ>(p, blockIdx.x / PER % tiles, group);
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-    const int i = blockIdx.x % PER * QUERIES + wave / WAVES;
-    // With one wavefront a query no barrier follows.
-    if (WAVES == 1 ? i >= at.nq : (int) (blockIdx.x % PER) * QUERIES >= at.nq) return;
-    const int64_t vq = at.first + i;
-    const int64_t row = at.q0 + vq / group;
-    const int head = kv * group + (int) (vq % group);
-    const int64_t q = row * p.heads + head, step = p.nq * p.heads;
     float most = -__builtin_inff();
     for (int s = lane; s < part.splits; s += 64) most = fmaxf(most, part.stat[s * step + q].x);
     most = group_reduce<64>(most, [](float a, float b) { return fmaxf(a, b); });
@@ -256,6 +251,25 @@ __global__ void __launch_bounds__(256) k_join(Attention p, Partial part, int til
 #pragma unroll
         for (int j = 0; j < 4; ++j) Store<DT>::st(y, j, v[j] * inv);
     }
+}
+
+// Joins the splits, a query to WAVES wavefronts (one with few splits, four with
+// many): QP lanes (a power of two) have four channels each, and the 64 WAVES / QP
+// groups of them every so many splits.  Queries are found as k_attention<.., NW>
+// does, TQ blocks' worth for each of its tiles.
+template <int DT, int TQ, int WAVES>
+__global__ void __launch_bounds__(256) k_join(Attention p, Partial part, int tiles, int qp) {
+    constexpr int QUERIES = 4 / WAVES, PER = TQ / QUERIES;
+    __shared__ float s_sum[4][64][5];
+    const int group = p.heads / p.kv_heads, kv = blockIdx.x / PER / tiles;
+    const Place at = find_place<TQ>(p, blockIdx.x / PER % tiles, group);
+    const int i = blockIdx.x % PER * QUERIES + (threadIdx.x >> 6) / WAVES;
+    // With one wavefront a query no barrier follows.
+    if (WAVES == 1 ? i >= at.nq : (int) (blockIdx.x % PER) * QUERIES >= at.nq) return;
+    const int64_t vq = at.first + i;
+    const int64_t row = at.q0 + vq / group;
+    const int head = kv * group + (int) (vq % group);
+    join_query<DT, WAVES>(p, part, qp, row * p.heads + head, p.nq * p.heads, row, head, s_sum);
 }
 
 }  // namespace

@@ -2597,15 +2597,17 @@ trellis_status attention_impl(trellis_sparse_backend * backend, const trellis_sp
     p.dim = d.head_dim;
     p.scale = scale;
     // Without scratch for split keys one block takes all of a query's keys.
-    const AttentionShape shape = attention_shape(be->policy.compute_dtype, p, be->cus);
-    if (scratch_clash(be, shape.scratch, {sq, sk, sv, sy, sqo, sko, sqc, skc, spf})) {
+    const int dt = be->policy.compute_dtype;
+    const AttentionShape shape = scores == nullptr ? attention_shape(dt, p, be->cus) : AttentionShape{};
+    const ScoredShape scored = scores != nullptr ? scored_shape(dt, p, sc, be->cus) : ScoredShape{};
+    const size_t bytes = scores != nullptr ? scored.scratch : shape.scratch;
+    if (scratch_clash(be, bytes, {sq, sk, sv, sy, sqo, sko, sqc, skc, spf})) {
         return fail(be, TRELLIS_STATUS_INVALID_ARGUMENT, "attention: rows in the scratch");
     }
     DevMem scratch;
-    void * split_keys = shape.scratch > 0 ? take_scratch(be, shape.scratch, &scratch) : nullptr;
+    void * split_keys = bytes > 0 ? take_scratch(be, bytes, &scratch) : nullptr;
     stage_begin(be, TRELLIS_SPARSE_HIP_STAGE_ELEMENTWISE);
-    const int dt = be->policy.compute_dtype;
-    const hipError_t err = scores != nullptr ? launch_attention_scored(dt, p, sc, shape, split_keys, be->stream)
+    const hipError_t err = scores != nullptr ? launch_attention_scored(dt, p, sc, scored, split_keys, be->stream)
                                              : launch_attention(dt, p, shape, split_keys, be->stream);
     stage_end(be, TRELLIS_SPARSE_HIP_STAGE_ELEMENTWISE);
     dev_release(be, &scratch);

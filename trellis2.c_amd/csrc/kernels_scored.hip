@@ -118,6 +118,47 @@ template <int DT> hipError_t launch_any(const Attention & p, const Scores & sc, 
 
 // ---- MFMA ---------------------------------------------------------------------------------------
 
+// Units of work, a tile of queries with a kv head each, neighbouring units of the same kv
+// head, in causal calls from the last queries, which see most, to the first.  The first
+// `whole` take all of their keys; the rest, which the CUs would not share evenly, are split
+// over blocks of their own, started last.
+struct Split {
+    Partial part;      // of the rest: its splits
+    int whole, rest;
+    __host__ __device__ int64_t blocks() const { return whole + (int64_t) rest * part.splits; }
+    // Where query i of a unit of the rest leaves its split's part.
+    struct Unit {
+        int64_t unit;
+        int split, splits;
+    };
+    __device__ __forceinline__ int64_t place(const Unit & u, int tq, int i) const {
+        return ((int64_t) u.split * rest + (u.unit - whole)) * tq + i;
+    }
+};
+using Unit = Split::Unit;
+// Each XCD takes contiguous ranges of both.
+__device__ __forceinline__ Unit unit_of(const Split & s) {
+    const int64_t b = blockIdx.x;
+    if (b < s.whole) return {xcd_remap(b, s.whole), 0, 1};
+    const int64_t r = xcd_remap(b - s.whole, gridDim.x - s.whole);
+    return {s.whole + r / s.part.splits, (int) (r % s.part.splits), s.part.splits};
+}
+
+// Joins the rest's splits as k_join does.
+template <int DT, int TQ, int WAVES>
+__global__ void __launch_bounds__(256) k_scored_join(Attention p, Split shape, int tiles, int qp, int causal) {
+    constexpr int QUERIES = 4 / WAVES, PER = TQ / QUERIES;
+    __shared__ float s_sum[4][64][5];
+    const int64_t unit = shape.whole + blockIdx.x / PER;
+    const int group = p.heads / p.kv_heads, kv = (int) (unit / tiles);
+    const Place at = find_place<TQ>(p, causal != 0 ? tiles - 1 - unit % tiles : unit % tiles, group);
+    const int i = blockIdx.x % PER * QUERIES + (threadIdx.x >> 6) / WAVES;
+    if (WAVES == 1 ? i >= at.nq : (int) (blockIdx.x % PER) * QUERIES >= at.nq) return;
+    const int64_t vq = at.first + i;
+    join_query<DT, WAVES>(p, shape.part, qp, shape.place({unit, 0, 0}, TQ, i), (int64_t) shape.rest * TQ, at.q0 + vq / group,
+                          kv * group + (int) (vq % group), s_sum);
+}
+
 // The coordinates of a tile's 64 keys: as they are, and, counted from an origin, as the A
 // operand of the squared distances, |p - k|^2 = |p|^2 - 2 p . k + |k|^2 as one product of
 // seven terms in fp16: coordinates, and squares in two parts, all whole numbers of 11 bits.
@@ -180,7 +221,7 @@ template <int DT> __device__ __forceinline__ s16x8 finite_part(s16x8 v) {
 // runs on the vector unit, which bounds attention already; squared distances of voxels are the
 // matrix unit's, counted from the block's first query, but where some are too far for that.
 template <int DT, int DC, int NW, bool FINE, bool VOXELS>
-__global__ void __launch_bounds__(64 * NW, DC <= 64 ? 3 : 2) k_scored(Attention p, Scores sc, Partial part, int tiles) {
+__global__ void __launch_bounds__(64 * NW, DC <= 64 ? (VOXELS ? 3 : 4) : 2) k_scored(Attention p, Scores sc, Split shape, int tiles) {
     using T = typename Store<DT>::T;
     constexpr int TQ = 32 * NW, TK = 64;
     constexpr int LP = DC <= 64 ? 64 : 128;      // values per LDS row
@@ -200,12 +241,10 @@ __global__ void __launch_bounds__(64 * NW, DC <= 64 ? 3 : 2) k_scored(Attention 
     const int l32 = lane & 31, half = lane >> 5;
     const int group = p.heads / p.kv_heads;
 
-    // Neighbouring blocks share a kv head; each XCD takes a contiguous range, in causal calls
-    // from the last queries, which see most, to the first.
-    const int64_t unit = xcd_remap(blockIdx.x, gridDim.x);
-    const int split = (int) (unit % part.splits);
-    const int kv = (int) (unit / part.splits / tiles);
-    const int64_t tile_at = unit / part.splits % tiles;
+    const Unit u = unit_of(shape);
+    const Partial part = u.splits > 1 ? shape.part : Partial{nullptr, nullptr, 1};
+    const int split = u.split, kv = (int) (u.unit / tiles);
+    const int64_t tile_at = u.unit % tiles;
     const Place at = find_place<TQ>(p, sc.causal != 0 ? tiles - 1 - tile_at : tile_at, group);
     if (at.nq <= 0) return;
     const int seen = (int) keys_seen(at, sc, (at.first + at.nq - 1) / group);
@@ -539,11 +578,12 @@ __global__ void __launch_bounds__(64 * NW, DC <= 64 ? 3 : 2) k_scored(Attention 
         for (int t = t0; t < t1; ++t) tile(t);
     }
 
-    leave<DT>(p, part, out, ref, sum_halves(sum0 + sum1), live, t0 < t1, split, row, head, half);
+    const auto left = [&] { return shape.place(u, TQ, qi); };
+    leave_at<DT>(p, part, out, ref, sum_halves(sum0 + sum1), live, t0 < t1, left, row, head, half);
 }
 
 template <int DC, int NW>
-__global__ void __launch_bounds__(64 * NW, 2) k_scored32(Attention p, Scores sc, Partial part, int tiles) {
+__global__ void __launch_bounds__(64 * NW, 2) k_scored32(Attention p, Scores sc, Split shape, int tiles) {
     constexpr int TQ = 32 * NW, TK = 32;
     constexpr int LP = DC <= 32 ? 32 : (DC <= 64 ? 64 : 128);  // values per LDS row
     constexpr int ROW = LP * 4, CH = LP / 4;
@@ -558,10 +598,10 @@ __global__ void __launch_bounds__(64 * NW, 2) k_scored32(Attention p, Scores sc,
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int l32 = lane & 31, half = lane >> 5;
     const int group = p.heads / p.kv_heads;
-    const int64_t unit = xcd_remap(blockIdx.x, gridDim.x);
-    const int split = (int) (unit % part.splits);
-    const int kv = (int) (unit / part.splits / tiles);
-    const int64_t tile_at = unit / part.splits % tiles;
+    const Unit u = unit_of(shape);
+    const Partial part = u.splits > 1 ? shape.part : Partial{nullptr, nullptr, 1};
+    const int split = u.split, kv = (int) (u.unit / tiles);
+    const int64_t tile_at = u.unit % tiles;
     const Place at = find_place<TQ>(p, sc.causal != 0 ? tiles - 1 - tile_at : tile_at, group);
     if (at.nq <= 0) return;
     const int seen = (int) keys_seen(at, sc, (at.first + at.nq - 1) / group);
@@ -721,39 +761,40 @@ __global__ void __launch_bounds__(64 * NW, 2) k_scored32(Attention p, Scores sc,
             }
         }
     }
-    leave<kF32>(p, part, out, ref, sum_halves(sum0 + sum1), live, t0 < t1, split, row, head, half);
+    const auto left = [&] { return shape.place(u, TQ, qi); };
+    leave_at<kF32>(p, part, out, ref, sum_halves(sum0 + sum1), live, t0 < t1, left, row, head, half);
 }
 
 template <int DT, int DC, int NW>
-hipError_t launch_nw(const Attention & p, const Scores & sc, const Partial & part, int64_t tiles, bool fine, hipStream_t s) {
-    const int64_t grid = tiles * p.kv_heads * part.splits;
+hipError_t launch_nw(const Attention & p, const Scores & sc, const Split & split, const ScoredShape & sh, hipStream_t s) {
+    const int64_t grid = split.blocks();
     if (grid > 0x7fffffffLL) return hipErrorInvalidValue;
+    const int tiles = (int) sh.tiles;
     if constexpr (DT == kF32) {
-        k_scored32<DC, NW><<<(unsigned) grid, 64 * NW, 0, s>>>(p, sc, part, (int) tiles);
+        k_scored32<DC, NW><<<(unsigned) grid, 64 * NW, 0, s>>>(p, sc, split, tiles);
     } else {
         const auto launch = [&](auto fine_c, auto voxels_c) {
             k_scored<DT, DC, NW, decltype(fine_c)::value, decltype(voxels_c)::value>
-                <<<(unsigned) grid, 64 * NW, 0, s>>>(p, sc, part, (int) tiles);
+                <<<(unsigned) grid, 64 * NW, 0, s>>>(p, sc, split, tiles);
         };
         using std::false_type, std::true_type;
         if (sc.q_xyz != nullptr) {
-            fine ? launch(true_type(), true_type()) : launch(false_type(), true_type());
+            sh.fine ? launch(true_type(), true_type()) : launch(false_type(), true_type());
         } else {
-            fine ? launch(true_type(), false_type()) : launch(false_type(), false_type());
+            sh.fine ? launch(true_type(), false_type()) : launch(false_type(), false_type());
         }
     }
     hipError_t err = hipGetLastError();
-    if (err == hipSuccess && part.splits > 1) {
+    if (err == hipSuccess && split.part.splits > 1) {
         int qp = 1;
         while (qp * 4 < p.dim) qp *= 2;
-        // 77 splits of 64 channels: 12 us with a wavefront a query, 6.5 with four.
-        const bool wide = part.splits >= 32;
-        const int64_t joins = tiles * p.kv_heads * (wide ? 32 * NW : 8 * NW);
+        const bool wide = split.part.splits >= 32;
+        const int64_t joins = (int64_t) split.rest * (wide ? 32 * NW : 8 * NW);
         if (joins > 0x7fffffffLL) return hipErrorInvalidValue;
         if (wide) {
-            k_join<DT, 32 * NW, 4><<<(unsigned) joins, 256, 0, s>>>(p, part, (int) tiles, qp);
+            k_scored_join<DT, 32 * NW, 4><<<(unsigned) joins, 256, 0, s>>>(p, split, tiles, qp, sc.causal);
         } else {
-            k_join<DT, 32 * NW, 1><<<(unsigned) joins, 256, 0, s>>>(p, part, (int) tiles, qp);
+            k_scored_join<DT, 32 * NW, 1><<<(unsigned) joins, 256, 0, s>>>(p, split, tiles, qp, sc.causal);
         }
         err = hipGetLastError();
     }
@@ -761,43 +802,68 @@ hipError_t launch_nw(const Attention & p, const Scores & sc, const Partial & par
 }
 
 template <int DT, int DC>
-hipError_t launch_dc(const Attention & p, const Scores & sc, const Partial & part, const AttentionShape & sh, hipStream_t s) {
-    return sh.waves == 1 ? launch_nw<DT, DC, 1>(p, sc, part, sh.tiles, sh.fine, s)
-                         : launch_nw<DT, DC, 4>(p, sc, part, sh.tiles, sh.fine, s);
+hipError_t launch_dc(const Attention & p, const Scores & sc, const Split & split, const ScoredShape & sh, hipStream_t s) {
+    return sh.waves == 1 ? launch_nw<DT, DC, 1>(p, sc, split, sh, s) : launch_nw<DT, DC, 4>(p, sc, split, sh, s);
 }
 
 template <int DT>
-hipError_t launch_mfma(const Attention & p, const Scores & sc, const Partial & part, const AttentionShape & sh, hipStream_t s) {
-    if (p.dim <= 32) return launch_dc<DT, 32>(p, sc, part, sh, s);
-    if (p.dim <= 64) return launch_dc<DT, 64>(p, sc, part, sh, s);
-    if (p.dim <= 96) return launch_dc<DT, 96>(p, sc, part, sh, s);
-    return launch_dc<DT, 128>(p, sc, part, sh, s);
+hipError_t launch_mfma(const Attention & p, const Scores & sc, const Split & split, const ScoredShape & sh, hipStream_t s) {
+    if (p.dim <= 32) return launch_dc<DT, 32>(p, sc, split, sh, s);
+    if (p.dim <= 64) return launch_dc<DT, 64>(p, sc, split, sh, s);
+    if (p.dim <= 96) return launch_dc<DT, 96>(p, sc, split, sh, s);
+    return launch_dc<DT, 128>(p, sc, split, sh, s);
 }
 
 }  // namespace
 
-// Run as attention of the same sizes is (attention_shape).
-hipError_t launch_attention_scored(int dtype, const Attention & p, const Scores & sc, const AttentionShape & sh,
-                                   void * scratch, hipStream_t s) {
-    // (Slopes over a scale that small could leave fp32.)
-    if (sh.waves == 0 || (sc.slopes != nullptr && sc.by < 0x1p-30f)) {
+// Few queries: all units split as attention's are.  Many: CUs get equal numbers of whole
+// units, and what is left over is split.  (Causal units are of unequal lengths, and go
+// from the longest to the shortest.)
+ScoredShape scored_shape(int dtype, const Attention & p, const Scores & sc, int cus) {
+    const AttentionShape a = attention_shape(dtype, p, cus);
+    ScoredShape sh{a.waves, a.tiles, a.fine, 0, 0, 1, 0};
+    // (Slopes over a scale that small could leave fp32: the general kernel.)
+    if (sc.slopes != nullptr && sc.by < 0x1p-30f) sh.waves = 0;
+    if (sh.waves == 0) return sh;
+    const int64_t units = sh.tiles * p.kv_heads;
+    if (units > 0x7fffffffLL) return sh;
+    sh.whole = (int) units;
+    const int64_t key_tiles = (p.nk / (p.q_at != nullptr ? p.seqs : 1) + 63) / 64;
+    if (a.splits > 1) {
+        sh.whole = 0;
+        sh.splits = a.splits;
+    } else if (sc.causal == 0 && sh.waves == 4 && units > 2 * cus) {
+        const int splits = (int) std::min<int64_t>(8, key_tiles / 16);
+        if (splits > 1) {
+            sh.whole = (int) (units / cus * cus);
+            sh.splits = splits;
+        }
+    }
+    sh.rest = (int) (units - sh.whole);
+    if (sh.rest == 0) sh.splits = 1;
+    if (sh.splits > 1) sh.scratch = (size_t) sh.splits * sh.rest * 32 * sh.waves * (p.dim + 2) * sizeof(float);
+    return sh;
+}
+
+hipError_t launch_attention_scored(int dtype, const Attention & p, const Scores & sc, const ScoredShape & sh, void * scratch,
+                                   hipStream_t s) {
+    if (sh.waves == 0) {
         switch (dtype) {
             case kF32: return launch_any<kF32>(p, sc, s);
             case kF16: return launch_any<kF16>(p, sc, s);
             default: return launch_any<kBF16>(p, sc, s);
         }
     }
-    Partial part{nullptr, nullptr, 1};
+    if (sh.tiles * p.kv_heads > 0x7fffffffLL) return hipErrorInvalidValue;
+    Split split{Partial{nullptr, nullptr, 1}, sh.whole + sh.rest, 0};
     if (scratch != nullptr && sh.splits > 1) {
-        part.splits = sh.splits;
-        part.out = (float *) scratch;
-        part.stat = (float2 *) (part.out + (size_t) sh.splits * p.nq * p.heads * p.dim);
+        split = Split{Partial{(float *) scratch, nullptr, sh.splits}, sh.whole, sh.rest};
+        split.part.stat = (float2 *) (split.part.out + (size_t) sh.splits * sh.rest * 32 * sh.waves * p.dim);
     }
-    if (sh.tiles > 0x7fffffffLL) return hipErrorInvalidValue;
     switch (dtype) {
-        case kF32: return launch_mfma<kF32>(p, sc, part, sh, s);
-        case kF16: return launch_mfma<kF16>(p, sc, part, sh, s);
-        default: return launch_mfma<kBF16>(p, sc, part, sh, s);
+        case kF32: return launch_mfma<kF32>(p, sc, split, sh, s);
+        case kF16: return launch_mfma<kF16>(p, sc, split, sh, s);
+        default: return launch_mfma<kBF16>(p, sc, split, sh, s);
     }
 }
 

@@ -459,7 +459,18 @@ struct Scores {
     const int32_t * prefix;  // [seqs] or null
     int causal;
 };
-hipError_t launch_attention_scored(int dtype, const Attention & p, const Scores & scores, const AttentionShape & shape,
+// How it is run: wavefronts per block (0: the general kernel), tiles of queries, weights in
+// two parts; units of work (a tile with a kv head) that take all of their keys and those
+// that are split, into how many, and the scratch for these (without it none is).
+struct ScoredShape {
+    int waves;
+    int64_t tiles;
+    bool fine;
+    int whole, rest, splits;
+    size_t scratch;
+};
+ScoredShape scored_shape(int dtype, const Attention & p, const Scores & scores, int cus);
+hipError_t launch_attention_scored(int dtype, const Attention & p, const Scores & scores, const ScoredShape & shape,
                                    void * scratch, hipStream_t s);
 
 // Group norm (kernels_gnorm.hip).  gamma, beta and at may be null; y may be x.
