@@ -318,7 +318,7 @@ hipError_t norm_dt(const void * x, const void * residual, const float * gamma, v
 // A row's scale is its largest magnitude T over 127, and a value v's code 127 v / T to the
 // nearest whole number, halves to the even one.  Of a norm, s_i g_i / rms, the root mean
 // square cancels in the codes: they are those of t_i = s_i g_i, a product that 64 bits
-// hold.  A code is found in fp32 (its error is below 2^-14 of a step), and where that is
+// hold.  A code is found in fp32 (off by less than 2^-15 of a step), and where that is
 // near a border, in 64 bits: 127 t - k T is exact there for t of up to 46 bits.
 struct IntRows {
     int8_t * codes;  // [n][cp]
@@ -327,29 +327,41 @@ struct IntRows {
 };
 
 struct IntScale {
-    double most;   // T
-    double inv;    // 127 / T, 0 for a row of zeros
-    bool plain;    // T is far from the ends of fp32's range
+    double most, by;  // T, and 127 / T (0 for a row of zeros, or without a finite scale: codes are zeros)
+    float by32;
+    bool far;         // T is near the ends of fp32's range: codes from 64 bits
 };
-__device__ __forceinline__ IntScale int_scale(double most) {
-    return {most, most > 0.0 ? 127.0 / most : 0.0, most > 1e-30 && most < 1e30};
-}
-template <class V> __device__ __forceinline__ int int_code(V t, const IntScale & s) {
-    const float f = s.plain ? (float) t * (float) s.inv : (float) ((double) t * s.inv);
-    const float k = rintf(f);
-    int code = (int) k;
-    if (fabsf(f - k) > 0.4999f) {
-        const double rest = fma(-(double) k, s.most, 127.0 * (double) t), half = 0.5 * s.most;
-        const bool odd = (code & 1) != 0;
-        if (rest > half || (rest == half && odd)) ++code;
-        if (rest < -half || (rest == -half && odd)) --code;
-    }
-    return code;
+__device__ __forceinline__ IntScale int_scale(double most, float row_scale) {
+    const double by = most > 0.0 && row_scale == row_scale ? 127.0 / most : 0.0;
+    return {most, by, (float) by, by != 0.0 && !(most > 1e-30 && most < 1e30)};
 }
 // The scale of a row of values t * inv; NaN where there is none that is finite.
 __device__ __forceinline__ float int_row_scale(double most, double inv) {
     const float s = (float) (most * inv / 127.0);
     return s < __builtin_inff() ? s : __builtin_nanf("");
+}
+__device__ __forceinline__ int int_code64(double t, const IntScale & s) {
+    if (s.by == 0.0) return 0;
+    const double k = rint(t * s.by), rest = fma(-k, s.most, 127.0 * t), half = 0.5 * s.most;
+    int code = (int) k;
+    const bool odd = (code & 1) != 0;
+    if (rest > half || (rest == half && odd)) ++code;
+    if (rest < -half || (rest == -half && odd)) --code;
+    return code;
+}
+// N codes, from f (127 t / T in fp32), or where one of these is near a border from t(u) in 64 bits.
+template <int N, class F> __device__ __forceinline__ void int_codes(const float * f, const IntScale & s, F && t, int * code) {
+    float near = 0.0f;
+#pragma unroll
+    for (int u = 0; u < N; ++u) {
+        const float k = rintf(f[u]);
+        code[u] = (int) k;
+        near = fmaxf(near, fabsf(f[u] - k));
+    }
+    if (s.far || near > 0.4999f) {
+#pragma unroll
+        for (int u = 0; u < N; ++u) code[u] = int_code64(t(u), s);
+    }
 }
 
 __device__ __forceinline__ uint32_t four_codes(const int * k) {
@@ -362,39 +374,34 @@ __device__ __forceinline__ double inverse_root(double m) {
     return m > 1e-30 && m < 1e38 ? y : 1.0 / sqrt(m);
 }
 
-// The larger of non-negative doubles as bits (a NaN's are larger than any number's), over groups of G lanes.
 template <int G> __device__ __forceinline__ double group_most(double v) {
-    const auto larger = [](double a, double b) {
-        return __builtin_bit_cast(uint64_t, a) > __builtin_bit_cast(uint64_t, b) ? a : b;
-    };
-#pragma unroll
-    for (int d = 1; d < G; d <<= 1) v = larger(v, __shfl_xor(v, d));
-    return v;
-}
-__device__ __forceinline__ double most_of(double a, double t) {
-    const uint64_t b = __builtin_bit_cast(uint64_t, t) & 0x7fffffffffffffffull;
-    return b > __builtin_bit_cast(uint64_t, a) ? __builtin_bit_cast(double, b) : a;
+    return group_reduce<G>(v, [](double a, double b) { return fmax(a, b); });
 }
 
 // Rows, or their norms (NORM, as k_norm_vec), to integer rows: LPR lanes hold a row in
-// registers, CPL chunks each.
+// registers, CPL chunks each.  Of 16-bit rows x + residual is exact in fp32 but where one is
+// 2^13 times the other, and 8 squares at a time are summed in fp32; of fp32 rows both are of
+// 64 bits.  Bound by memory and nearly as much by the vector unit.
 template <int DT, int LPR, int CPL, bool NORM>
 __global__ void __launch_bounds__(256) k_rows_int8(const typename Store<DT>::T * x,
                                                    const typename Store<DT>::T * residual,
                                                    const float * __restrict__ gamma, typename Store<DT>::T * total,
                                                    IntRows out, int64_t n, int c, float eps) {
     using T = typename Store<DT>::T;
-    using V = typename std::conditional<NORM, double, float>::type;
+    using S = typename std::conditional<NORM && DT == kF32, double, float>::type;
     constexpr int N = kChunk<DT>, RPB = 256 / LPR;
     const int l = threadIdx.x % LPR;
     float g[CPL][N];
+    bool odd = false;  // some gamma is not finite: so is every row
 #pragma unroll
     for (int i = 0; i < CPL; ++i)
 #pragma unroll
         for (int u = 0; u < N; ++u) {
             const int at = (i * LPR + l) * N + u;
             g[i][u] = NORM && gamma != nullptr && at < c ? gamma[at] : 1.0f;
+            odd |= !(fabsf(g[i][u]) < __builtin_inff());
         }
+    if constexpr (NORM) odd = group_reduce<LPR>(odd ? 1.0f : 0.0f, [](float a, float b) { return fmaxf(a, b); }) > 0.0f;
     int4 xc[CPL], rc[CPL];
     const auto fetch = [&](int64_t row) {
 #pragma unroll
@@ -411,48 +418,59 @@ __global__ void __launch_bounds__(256) k_rows_int8(const typename Store<DT>::T *
     const int64_t stride = (int64_t) gridDim.x * RPB;
     if (row < n) fetch(row);
     for (; row < n; row += stride) {
-        V t[CPL][N];
+        S s[CPL][N];
         double sum = 0.0, most = 0.0;
+        uint32_t bits = 0;
 #pragma unroll
         for (int i = 0; i < CPL; ++i) {
-            float v[N], r[N];
+            float v[N];
             unpack_chunk_of<DT>(xc[i], v);
             if constexpr (NORM) {
+                float r[N];
                 if (residual != nullptr) unpack_chunk_of<DT>(rc[i], r);
+                S part = 0;
 #pragma unroll
                 for (int u = 0; u < N; ++u) {
-                    double s = (double) v[u];
+                    s[i][u] = (S) v[u];
                     if (residual != nullptr) {
-                        s += (double) r[u];
+                        s[i][u] += (S) r[u];
                         v[u] += r[u];
                     }
-                    sum = fma(s, s, sum);
-                    t[i][u] = s * (double) g[i][u];
-                    most = most_of(most, t[i][u]);
+                    part += s[i][u] * s[i][u];
+                    most = fmax(most, fabs((double) s[i][u] * (double) g[i][u]));
                 }
+                sum += (double) part;
                 const int at = (i * LPR + l) * N;
                 if (total != nullptr && at < c) store_chunk<DT>(total + row * c + at, v);
             } else {
 #pragma unroll
                 for (int u = 0; u < N; ++u) {
-                    t[i][u] = v[u];
-                    most = most_of(most, (double) v[u]);
+                    s[i][u] = v[u];
+                    bits = max(bits, abs_bits(v[u]));
                 }
             }
         }
         if (row + stride < n) fetch(row + stride);
-        most = group_most<LPR>(most);
         double inv = 1.0;
-        if constexpr (NORM) inv = inverse_root(group_sum<LPR>(sum) / c + (double) eps);
+        if constexpr (NORM) {
+            most = group_most<LPR>(most);
+            sum = group_sum<LPR>(sum);
+            inv = inverse_root(sum / c + (double) eps);
+            if (odd || !(sum < __builtin_inf())) inv = __builtin_nan("");
+        } else {
+            most = (double) __builtin_bit_cast(float, group_max<LPR>(bits));
+        }
         const float scale = int_row_scale(most, inv);
-        const IntScale s = int_scale(scale == scale ? most : 0.0);
+        const IntScale q = int_scale(most, scale);
 #pragma unroll
         for (int i = 0; i < CPL; ++i) {
             const int at = (i * LPR + l) * N;
             if (at >= out.cp) continue;
-            int k[N];
+            float f[N];
 #pragma unroll
-            for (int u = 0; u < N; ++u) k[u] = s.inv == 0.0 ? 0 : int_code(t[i][u], s);
+            for (int u = 0; u < N; ++u) f[u] = q.by32 == 0.0f ? 0.0f : (float) s[i][u] * g[i][u] * q.by32;
+            int k[N];
+            int_codes<N>(f, q, [&](int u) { return (double) s[i][u] * (double) g[i][u]; }, k);
             int8_t * p = out.codes + row * out.cp + at;
             if constexpr (N == 8) {
                 *(uint2 *) p = uint2{four_codes(k), four_codes(k + 4)};
@@ -478,17 +496,19 @@ __global__ void __launch_bounds__(256) k_rows_int8_any(const typename Store<DT>:
         return NORM && residual != nullptr ? v + (double) Store<DT>::ld(residual, row * c + i) : v;
     };
     const auto weighted = [&](int i, double s) { return NORM && gamma != nullptr ? s * (double) gamma[i] : s; };
-    double sum = 0.0, most = 0.0;
+    double sum = 0.0, most = 0.0, all = 0.0;
     for (int i = lane; i < c; i += 64) {
-        const double s = at(i);
+        const double s = at(i), t = weighted(i, s);
         sum = fma(s, s, sum);
-        most = most_of(most, weighted(i, s));
+        most = fmax(most, fabs(t));
+        all = fma(t, 0.0, all);  // a NaN where one is not finite
     }
     most = group_most<64>(most);
     double inv = 1.0;
     if constexpr (NORM) inv = inverse_root(group_sum<64>(sum) / c + (double) eps);
+    if (group_sum<64>(all) != 0.0) inv = __builtin_nan("");
     const float scale = int_row_scale(most, inv);
-    const IntScale q = int_scale(scale == scale ? most : 0.0);
+    const IntScale q = int_scale(most, scale);
     for (int i = lane; i < out.cp; i += 64) {
         int code = 0;
         if (i < c) {
@@ -498,7 +518,7 @@ __global__ void __launch_bounds__(256) k_rows_int8_any(const typename Store<DT>:
                 if (residual != nullptr) v += Store<DT>::ld(residual, row * c + i);
                 Store<DT>::st(total, row * c + i, v);
             }
-            if (q.inv != 0.0) code = int_code(weighted(i, s), q);
+            code = int_code64(weighted(i, s), q);
         }
         out.codes[row * out.cp + i] = (int8_t) code;
     }

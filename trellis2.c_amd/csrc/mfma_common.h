@@ -150,7 +150,7 @@ template <int G> __device__ __forceinline__ float group_sum(float v) {
     return group_reduce<G>(v, [](float a, float b) { return a + b; });
 }
 // In 64 bits: the halves of a value go the same ways.
-template <int G> __device__ __forceinline__ double group_sum(double v) {
+template <int G, class Op> __device__ __forceinline__ double group_reduce(double v, Op op) {
     const auto halves = [](double d) { return __builtin_bit_cast(int2, d); };
     const auto dpp = [&](auto ctrl) {
         constexpr int C = decltype(ctrl)::value;
@@ -158,21 +158,24 @@ template <int G> __device__ __forceinline__ double group_sum(double v) {
         return __builtin_bit_cast(double, int2{__builtin_amdgcn_mov_dpp(h.x, C, 0xf, 0xf, false),
                                                __builtin_amdgcn_mov_dpp(h.y, C, 0xf, 0xf, false)});
     };
-    if constexpr (G > 1) v += dpp(std::integral_constant<int, 0xB1>());
-    if constexpr (G > 2) v += dpp(std::integral_constant<int, 0x4E>());
-    if constexpr (G > 4) v += dpp(std::integral_constant<int, 0x141>());
-    if constexpr (G > 8) v += dpp(std::integral_constant<int, 0x140>());
+    if constexpr (G > 1) v = op(v, dpp(std::integral_constant<int, 0xB1>()));
+    if constexpr (G > 2) v = op(v, dpp(std::integral_constant<int, 0x4E>()));
+    if constexpr (G > 4) v = op(v, dpp(std::integral_constant<int, 0x141>()));
+    if constexpr (G > 8) v = op(v, dpp(std::integral_constant<int, 0x140>()));
     const auto join = [&](auto both) {
         const int2 h = halves(v);
         float ax, bx, ay, by;
         both(__builtin_bit_cast(float, h.x), ax, bx);
         both(__builtin_bit_cast(float, h.y), ay, by);
-        v = __builtin_bit_cast(double, int2{__builtin_bit_cast(int, ax), __builtin_bit_cast(int, ay)}) +
-            __builtin_bit_cast(double, int2{__builtin_bit_cast(int, bx), __builtin_bit_cast(int, by)});
+        v = op(__builtin_bit_cast(double, int2{__builtin_bit_cast(int, ax), __builtin_bit_cast(int, ay)}),
+               __builtin_bit_cast(double, int2{__builtin_bit_cast(int, bx), __builtin_bit_cast(int, by)}));
     };
     if constexpr (G > 16) join([](float f, float & a, float & b) { both_rows(f, a, b); });
     if constexpr (G > 32) join([](float f, float & a, float & b) { both_halves(f, a, b); });
     return v;
+}
+template <int G> __device__ __forceinline__ double group_sum(double v) {
+    return group_reduce<G>(v, [](double a, double b) { return a + b; });
 }
 // The largest of non-negative values as bits (a NaN's are larger than any number's).
 template <int G> __device__ __forceinline__ uint32_t group_max(uint32_t v) {
