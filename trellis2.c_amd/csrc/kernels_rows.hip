@@ -318,51 +318,33 @@ hipError_t norm_dt(const void * x, const void * residual, const float * gamma, v
 // A row's scale is its largest magnitude T over 127, and a value v's code 127 v / T to the
 // nearest whole number, halves to the even one.  Of a norm, s_i g_i / rms, the root mean
 // square cancels in the codes: they are those of t_i = s_i g_i, a product that 64 bits
-// hold.  A code is found in fp32 (off by less than 2^-15 of a step), and where that is
-// near a border, in 64 bits: 127 t - k T is exact there for t of up to 46 bits.
+// hold.  A code is found in fp32, and where that is near a border, in 64 bits: 127 t - k T is
+// exact there for t of up to 46 bits.
 struct IntRows {
     int8_t * codes;  // [n][cp]
     float * scales;  // [n]
     int cp;
 };
 
-struct IntScale {
-    double most, by;  // T, and 127 / T (0 for a row of zeros, or without a finite scale: codes are zeros)
-    float by32;
-    bool far;         // T is near the ends of fp32's range: codes from 64 bits
-};
-__device__ __forceinline__ IntScale int_scale(double most, float row_scale) {
-    const double by = most > 0.0 && row_scale == row_scale ? 127.0 / most : 0.0;
-    return {most, by, (float) by, by != 0.0 && !(most > 1e-30 && most < 1e30)};
-}
-// The scale of a row of values t * inv; NaN where there is none that is finite.
-__device__ __forceinline__ float int_row_scale(double most, double inv) {
-    const float s = (float) (most * inv / 127.0);
-    return s < __builtin_inff() ? s : __builtin_nanf("");
-}
-__device__ __forceinline__ int int_code64(double t, const IntScale & s) {
-    if (s.by == 0.0) return 0;
-    const double k = rint(t * s.by), rest = fma(-k, s.most, 127.0 * t), half = 0.5 * s.most;
+__device__ __forceinline__ int int_code64(double t, double most) {
+    const double k = rint(127.0 * t / most), rest = fma(-k, most, 127.0 * t), half = 0.5 * most;
     int code = (int) k;
     const bool odd = (code & 1) != 0;
     if (rest > half || (rest == half && odd)) ++code;
     if (rest < -half || (rest == -half && odd)) --code;
     return code;
 }
-// N codes, from f (127 t / T in fp32), or where one of these is near a border from t(u) in 64 bits.
-template <int N, class F> __device__ __forceinline__ void int_codes(const float * f, const IntScale & s, F && t, int * code) {
-    float near = 0.0f;
-#pragma unroll
-    for (int u = 0; u < N; ++u) {
-        const float k = rintf(f[u]);
-        code[u] = (int) k;
-        near = fmaxf(near, fabsf(f[u] - k));
-    }
-    if (s.far || near > 0.4999f) {
-#pragma unroll
-        for (int u = 0; u < N; ++u) code[u] = int_code64(t(u), s);
-    }
+// Of 16-bit values 127 t and k T have no more than 18 bits.
+__device__ __forceinline__ int int_code16(float t, float most, float by) {
+    const float k = rintf(t * by), rest = 2.0f * fmaf(-k, most, 127.0f * t);
+    int code = (int) k;
+    const bool odd = (code & 1) != 0;
+    if (rest > most || (rest == most && odd)) ++code;
+    if (rest < -most || (rest == -most && odd)) --code;
+    return code;
 }
+// NaN for a scale that is not finite.
+__device__ __forceinline__ float finite_or_nan(float s) { return s < __builtin_inff() ? s : __builtin_nanf(""); }
 
 __device__ __forceinline__ uint32_t four_codes(const int * k) {
     return (uint32_t) (k[0] & 255) | (uint32_t) (k[1] & 255) << 8 | (uint32_t) (k[2] & 255) << 16 | (uint32_t) k[3] << 24;
@@ -374,23 +356,23 @@ __device__ __forceinline__ double inverse_root(double m) {
     return m > 1e-30 && m < 1e38 ? y : 1.0 / sqrt(m);
 }
 
-template <int G> __device__ __forceinline__ double group_most(double v) {
-    return group_reduce<G>(v, [](double a, double b) { return fmax(a, b); });
-}
-
 // Rows, or their norms (NORM, as k_norm_vec), to integer rows: LPR lanes hold a row in
 // registers, CPL chunks each.  Of 16-bit rows x + residual is exact in fp32 but where one is
-// 2^13 times the other, and 8 squares at a time are summed in fp32; of fp32 rows both are of
-// 64 bits.  Bound by memory and nearly as much by the vector unit.
+// 2^13 times the other, and the largest t is found in fp32, in 64 bits only for a code beside
+// a border (one in 10,000, a tenth of a wavefront's rows); statistics of fp32 rows are of 64
+// bits.  Bound by memory: 18,216 x 4096 fp16 47 us, 4.8 TB/s; norms nearly as much by the
+// vector unit: 79,523 x 512 bf16 @NORM@.
 template <int DT, int LPR, int CPL, bool NORM>
 __global__ void __launch_bounds__(256) k_rows_int8(const typename Store<DT>::T * x,
                                                    const typename Store<DT>::T * residual,
                                                    const float * __restrict__ gamma, typename Store<DT>::T * total,
                                                    IntRows out, int64_t n, int c, float eps) {
     using T = typename Store<DT>::T;
-    using S = typename std::conditional<NORM && DT == kF32, double, float>::type;
+    constexpr bool FINE = DT == kF32;
+    using S = typename std::conditional<NORM && FINE, double, float>::type;
     constexpr int N = kChunk<DT>, RPB = 256 / LPR;
     const int l = threadIdx.x % LPR;
+    const double per_c = 1.0 / c;
     float g[CPL][N];
     bool odd = false;  // some gamma is not finite: so is every row
 #pragma unroll
@@ -401,7 +383,8 @@ __global__ void __launch_bounds__(256) k_rows_int8(const typename Store<DT>::T *
             g[i][u] = NORM && gamma != nullptr && at < c ? gamma[at] : 1.0f;
             odd |= !(fabsf(g[i][u]) < __builtin_inff());
         }
-    if constexpr (NORM) odd = group_reduce<LPR>(odd ? 1.0f : 0.0f, [](float a, float b) { return fmaxf(a, b); }) > 0.0f;
+    const auto larger = [](float a, float b) { return fmaxf(a, b); };
+    if constexpr (NORM) odd = group_reduce<LPR>(odd ? 1.0f : 0.0f, larger) > 0.0f;
     int4 xc[CPL], rc[CPL];
     const auto fetch = [&](int64_t row) {
 #pragma unroll
@@ -414,12 +397,18 @@ __global__ void __launch_bounds__(256) k_rows_int8(const typename Store<DT>::T *
             }
         }
     };
+    // In 64 bits, where few need it: gammas kept in 64 bits would take too many registers.
+    const auto product = [](S a, float b) {
+        asm volatile("" : "+v"(b));
+        return (double) a * (double) b;
+    };
     int64_t row = (int64_t) blockIdx.x * RPB + threadIdx.x / LPR;
     const int64_t stride = (int64_t) gridDim.x * RPB;
     if (row < n) fetch(row);
     for (; row < n; row += stride) {
         S s[CPL][N];
-        double sum = 0.0, most = 0.0;
+        NormSum<FINE> sum = 0;
+        float top = 0.0f;
         uint32_t bits = 0;
 #pragma unroll
         for (int i = 0; i < CPL; ++i) {
@@ -428,7 +417,7 @@ __global__ void __launch_bounds__(256) k_rows_int8(const typename Store<DT>::T *
             if constexpr (NORM) {
                 float r[N];
                 if (residual != nullptr) unpack_chunk_of<DT>(rc[i], r);
-                S part = 0;
+                NormSum<FINE> part = 0;
 #pragma unroll
                 for (int u = 0; u < N; ++u) {
                     s[i][u] = (S) v[u];
@@ -437,9 +426,9 @@ __global__ void __launch_bounds__(256) k_rows_int8(const typename Store<DT>::T *
                         v[u] += r[u];
                     }
                     part += s[i][u] * s[i][u];
-                    most = fmax(most, fabs((double) s[i][u] * (double) g[i][u]));
+                    if constexpr (!FINE) top = fmaxf(top, fabsf(s[i][u] * g[i][u]));
                 }
-                sum += (double) part;
+                sum += part;
                 const int at = (i * LPR + l) * N;
                 if (total != nullptr && at < c) store_chunk<DT>(total + row * c + at, v);
             } else {
@@ -451,32 +440,79 @@ __global__ void __launch_bounds__(256) k_rows_int8(const typename Store<DT>::T *
             }
         }
         if (row + stride < n) fetch(row + stride);
-        double inv = 1.0;
-        if constexpr (NORM) {
-            most = group_most<LPR>(most);
+        // The largest |t| in 64 bits (all lanes take part).
+        const auto exact_most = [&]() {
+            double most = 0.0;
+#pragma unroll
+            for (int i = 0; i < CPL; ++i)
+#pragma unroll
+                for (int u = 0; u < N; ++u) most = fmax(most, fabs(product(s[i][u], g[i][u])));
+            return group_reduce<LPR>(most, [](double a, double b) { return fmax(a, b); });
+        };
+        float scale;
+        double most = 0.0;
+        if constexpr (NORM && FINE) {
+            most = exact_most();
+            top = (float) most;
             sum = group_sum<LPR>(sum);
-            inv = inverse_root(sum / c + (double) eps);
-            if (odd || !(sum < __builtin_inf())) inv = __builtin_nan("");
+            scale = (float) (most * inverse_root(fma(sum, per_c, (double) eps)) * (1.0 / 127.0));
+            if (odd || !(sum < __builtin_inf())) scale = __builtin_nanf("");
+        } else if constexpr (NORM) {
+            top = group_reduce<LPR>(top, larger);
+            sum = group_sum<LPR>(sum);
+            scale = top * (1.0f / sqrtf(fmaf(sum, (float) per_c, eps))) * (1.0f / 127.0f);
+            if (odd || !(sum < __builtin_inff())) scale = __builtin_nanf("");
         } else {
-            most = (double) __builtin_bit_cast(float, group_max<LPR>(bits));
+            top = __builtin_bit_cast(float, group_max<LPR>(bits));
+            scale = (float) ((double) top * (1.0 / 127.0));
         }
-        const float scale = int_row_scale(most, inv);
-        const IntScale q = int_scale(most, scale);
+        scale = finite_or_nan(scale);
+        const bool zero = !(top > 0.0f) || scale != scale;  // codes are zeros
+        const bool far = !zero && !(top > 1e-30f && top < 1e30f);  // near the ends of fp32's range: codes from 64 bits
+        const float by = zero ? 0.0f : 127.0f * __builtin_amdgcn_rcpf(top);
+        // 127 t / T, off by no more than 127 times 6 roundings, 4.6e-5.
+        const auto about = [&](S a, float b) { return (float) a * b * by; };
+        constexpr float kNear = 0.49995f;
+        float near = 0.0f;
 #pragma unroll
         for (int i = 0; i < CPL; ++i) {
+            int code[N];
+            if constexpr (!NORM) near = 0.0f;
+#pragma unroll
+            for (int u = 0; u < N; ++u) {
+                const float f = about(s[i][u], g[i][u]), k = rintf(f);
+                code[u] = (int) k;
+                near = fmaxf(near, fabsf(f - k));
+            }
+            if constexpr (!NORM) {
+                if (far || near > kNear) {
+#pragma unroll
+                    for (int u = 0; u < N; ++u)
+                        code[u] = FINE || far ? int_code64((double) s[i][u], (double) top) : int_code16(s[i][u], top, by);
+                }
+            }
             const int at = (i * LPR + l) * N;
             if (at >= out.cp) continue;
-            float f[N];
-#pragma unroll
-            for (int u = 0; u < N; ++u) f[u] = q.by32 == 0.0f ? 0.0f : (float) s[i][u] * g[i][u] * q.by32;
-            int k[N];
-            int_codes<N>(f, q, [&](int u) { return (double) s[i][u] * (double) g[i][u]; }, k);
             int8_t * p = out.codes + row * out.cp + at;
             if constexpr (N == 8) {
-                *(uint2 *) p = uint2{four_codes(k), four_codes(k + 4)};
+                *(uint2 *) p = zero ? uint2{0, 0} : uint2{four_codes(code), four_codes(code + 4)};
             } else {
-                *(uint32_t *) p = four_codes(k);
+                *(uint32_t *) p = zero ? 0u : four_codes(code);
             }
+        }
+        if (NORM && __any(far || (!zero && near > kNear))) {
+            if constexpr (!FINE) most = exact_most();
+#pragma unroll
+            for (int i = 0; i < CPL; ++i)
+#pragma unroll
+                for (int u = 0; u < N; ++u) {
+                    const int at = (i * LPR + l) * N + u;
+                    S a = s[i][u];
+                    asm volatile("" : "+v"(a));  // else what is above stays in registers for here
+                    const float f = about(a, g[i][u]);
+                    if (!zero && at < c && (far || fabsf(f - rintf(f)) > kNear))
+                        out.codes[row * out.cp + at] = (int8_t) int_code64(product(a, g[i][u]), most);
+                }
         }
         if (l == 0) out.scales[row] = scale;
     }
@@ -503,12 +539,12 @@ __global__ void __launch_bounds__(256) k_rows_int8_any(const typename Store<DT>:
         most = fmax(most, fabs(t));
         all = fma(t, 0.0, all);  // a NaN where one is not finite
     }
-    most = group_most<64>(most);
+    most = group_reduce<64>(most, [](double a, double b) { return fmax(a, b); });
     double inv = 1.0;
     if constexpr (NORM) inv = inverse_root(group_sum<64>(sum) / c + (double) eps);
     if (group_sum<64>(all) != 0.0) inv = __builtin_nan("");
-    const float scale = int_row_scale(most, inv);
-    const IntScale q = int_scale(most, scale);
+    const float scale = finite_or_nan((float) (most * inv * (1.0 / 127.0)));
+    const bool zero = !(most > 0.0) || scale != scale;
     for (int i = lane; i < out.cp; i += 64) {
         int code = 0;
         if (i < c) {
@@ -518,7 +554,7 @@ __global__ void __launch_bounds__(256) k_rows_int8_any(const typename Store<DT>:
                 if (residual != nullptr) v += Store<DT>::ld(residual, row * c + i);
                 Store<DT>::st(total, row * c + i, v);
             }
-            code = int_code64(weighted(i, s), q);
+            if (!zero) code = int_code64(weighted(i, s), most);
         }
         out.codes[row * out.cp + i] = (int8_t) code;
     }
