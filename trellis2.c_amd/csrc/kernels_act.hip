@@ -599,6 +599,59 @@ template <int DT> __global__ void __launch_bounds__(256) k_linear_act_any(Linear
     });
 }
 
+// Up to ROWS (4) integer rows, whose products would fill an eighth of a matrix tile at most and
+// whose time is that of the weights' way: a wavefront has 4 output channels, a lane 16 of
+// every 1,024 K values, and the sums, whole numbers, are those of the tiles to the last bit.
+// One row 1024 -> 4096 3.4 us (its 4 MB take 0.8 at the rate of a large copy), in tiles with split sums 7.7.
+template <int DT, int ROWS> __global__ void __launch_bounds__(256) k_linear_few(LinearAct p) {
+    using T = typename Store<DT>::T;
+    constexpr int CH = 4;
+    const int lane = threadIdx.x & 63;
+    const int ch0 = (blockIdx.x * 4 + (threadIdx.x >> 6)) * CH;
+    if (ch0 >= p.co) return;
+    const char * x = (const char *) p.x;
+    const char * w = (const char *) p.w + (int64_t) ch0 * p.w_bytes;  // (there are rows up to whole 256)
+    int sum[ROWS][CH] = {};
+#pragma unroll 2
+    for (int k = lane * 16; k < p.w_bytes; k += 1024) {
+        int4 a[ROWS], b[CH];
+#pragma unroll
+        for (int c = 0; c < CH; ++c) b[c] = *(const int4 *) (w + (int64_t) c * p.w_bytes + k);
+#pragma unroll
+        for (int r = 0; r < ROWS; ++r) a[r] = *(const int4 *) (x + min((int64_t) r, p.n - 1) * p.row_bytes + k);
+#pragma unroll
+        for (int r = 0; r < ROWS; ++r)
+#pragma unroll
+            for (int c = 0; c < CH; ++c) {
+                sum[r][c] = __builtin_amdgcn_sdot4(a[r].x, b[c].x, sum[r][c], false);
+                sum[r][c] = __builtin_amdgcn_sdot4(a[r].y, b[c].y, sum[r][c], false);
+                sum[r][c] = __builtin_amdgcn_sdot4(a[r].z, b[c].z, sum[r][c], false);
+                sum[r][c] = __builtin_amdgcn_sdot4(a[r].w, b[c].w, sum[r][c], false);
+            }
+    }
+    // Lane r * CH + c leaves output c of row r.
+    int mine = 0;
+#pragma unroll
+    for (int r = 0; r < ROWS; ++r)
+#pragma unroll
+        for (int c = 0; c < CH; ++c) {
+            const float all = group_reduce<64>(__builtin_bit_cast(float, sum[r][c]), [](float u, float v) {
+                return __builtin_bit_cast(float, __builtin_bit_cast(int, u) + __builtin_bit_cast(int, v));
+            });
+            if (lane == r * CH + c) mine = __builtin_bit_cast(int, all);
+        }
+    const int row = lane / CH, ch = ch0 + lane % CH;
+    if (row >= ROWS || row >= p.n || ch >= p.co) return;
+    const float z = fmaf((float) mine * ((const float *) p.x_scales)[row], ((const float *) p.w_scales)[ch],
+                         p.bias != nullptr ? p.bias[ch] : 0.0f);
+    const int64_t e = (int64_t) row * p.co + ch;
+    by_act(p.act, [&](auto act_c) {
+        float v = activate<DT, decltype(act_c)::value>(z);
+        if (p.residual != nullptr) v += Store<DT>::ld((const T *) p.residual, e);
+        Store<DT>::st((T *) p.y, e, v);
+    });
+}
+
 // ---- which blocks, and how many splits --------------------------------------------------------------
 
 // Block shapes: rows, channels, adjacent channels per lane (which divide co),
@@ -606,22 +659,26 @@ template <int DT> __global__ void __launch_bounds__(256) k_linear_act_any(Linear
 // all CUs busy, in us (measured on whole rounds of blocks, 1,024 channels, K of 4
 // and of 32 steps, four rounds of 16 or 8 bits and two of fp32; the first loads and
 // the last outputs of all, kOnce, are not in it).
+// (Integers: no scales on the way, but in the outputs.)
 struct Blocks {
     int rows, channels, adjacent, per_cu;
-    float step16, step8, step32, rest, rest32;
+    float step16, step8, step_int, step32, rest, rest_int, rest32;
 };
 constexpr Blocks kBlocks[] = {
-    {256, 256, 4, 1, 1.78f, 2.10f, 7.1f, 4.2f, 13.7f},
-    {192, 256, 2, 1, 1.52f, 1.75f, 5.4f, 2.7f, 12.0f},
-    {128, 128, 2, 2, 1.27f, 1.58f, 3.85f, 1.1f, 7.3f},
-    {64, 128, 2, 3, 1.20f, 1.57f, 3.1f, 0.9f, 5.5f},
-    {128, 128, 1, 2, 1.31f, 1.70f, 3.9f, 1.8f, 7.5f},
-    {64, 64, 1, 4, 0.88f, 1.24f, 2.3f, 1.6f, 4.7f},
+    {256, 256, 4, 1, 1.78f, 2.10f, 2.14f, 7.1f, 4.2f, 5.2f, 13.7f},
+    {192, 256, 2, 1, 1.52f, 1.75f, 1.75f, 5.4f, 2.7f, 3.6f, 12.0f},
+    {128, 128, 2, 2, 1.27f, 1.58f, 1.15f, 3.85f, 1.1f, 3.4f, 7.3f},
+    {64, 128, 2, 3, 1.20f, 1.57f, 1.19f, 3.1f, 0.9f, 2.2f, 5.5f},
+    {128, 128, 1, 2, 1.31f, 1.70f, 1.25f, 3.9f, 1.8f, 3.7f, 7.5f},
+    {64, 64, 1, 4, 0.88f, 1.24f, 0.83f, 2.3f, 1.6f, 2.9f, 4.7f},
 };
 constexpr double kOnce = 1.5;
 constexpr int kShapes = sizeof(kBlocks) / sizeof(kBlocks[0]);
 
-inline float step_us(const Blocks & b, int mt) { return mt == kF32 ? b.step32 : (is_rows8(mt) ? b.step8 : b.step16); }
+inline float step_us(const Blocks & b, int mt) {
+    return mt == kF32 ? b.step32 : (mt == kRows8 ? b.step8 : (mt == kRowsInt8 ? b.step_int : b.step16));
+}
+inline float rest_us(const Blocks & b, int mt) { return mt == kF32 ? b.rest32 : (mt == kRowsInt8 ? b.rest_int : b.rest); }
 
 struct Choice {
     int shape = -1, splits = 1;
@@ -643,7 +700,7 @@ Choice choose(int mt, int64_t n, int co, int w_bytes, int cus, bool may_split) {
         const Blocks & b = kBlocks[i];
         if (co % b.adjacent != 0) continue;
         const double blocks = (double) ((n + b.rows - 1) / b.rows) * ((co + b.channels - 1) / b.channels);
-        const double step = step_us(b, mt), rest = mt == kF32 ? b.rest32 : b.rest;
+        const double step = step_us(b, mt), rest = rest_us(b, mt);
         for (int s = 1; s <= (may_split ? 16 : 1); s *= 2) {
             if (s > 1 && (s > steps / 2 || i == 0)) break;  // (the largest blocks do not split)
             const double rounds = blocks * s / ((double) cus * b.per_cu), whole = std::floor(rounds);
@@ -714,8 +771,20 @@ template <int DT> hipError_t launch_any(LinearAct p, hipStream_t s) {
     return hipGetLastError();
 }
 
+template <int DT> hipError_t launch_few(const LinearAct & p, hipStream_t s) {
+    const unsigned grid = (unsigned) ((p.co + 15) / 16);
+    if (p.n == 1) {
+        k_linear_few<DT, 1><<<grid, 256, 0, s>>>(p);
+    } else if (p.n == 2) {
+        k_linear_few<DT, 2><<<grid, 256, 0, s>>>(p);
+    } else {
+        k_linear_few<DT, 4><<<grid, 256, 0, s>>>(p);
+    }
+    return hipGetLastError();
+}
+
 template <int DT> hipError_t launch_dt(const LinearAct & p, int x_type, const LinearActPlan & plan, hipStream_t s) {
-    if (plan.parts == 0) return launch_any<DT>(p, s);
+    if (plan.parts == 0) return x_type == kRowsInt8 ? launch_few<DT>(p, s) : launch_any<DT>(p, s);
     int64_t row = 0;
     for (int i = 0; i < plan.parts; ++i) {
         const auto & part = plan.part[i];
@@ -745,7 +814,7 @@ template <int DT> hipError_t launch_dt(const LinearAct & p, int x_type, const Li
 LinearActPlan linear_act_plan(int dtype, int x_type, int64_t n, int co, int row_bytes, int w_bytes, int cus,
                               bool may_split) {
     LinearActPlan plan{};
-    if (!is_rows8(x_type) && row_bytes % 16 != 0) return plan;
+    if (x_type == kRowsInt8 ? n <= kFewRows : (x_type != kRows8 && row_bytes % 16 != 0)) return plan;
     const int mt = is_rows8(x_type) ? x_type : dtype;
     const auto scratch = [&](const LinearActPart & part) {
         return part.splits > 1 ? (size_t) part.splits * part.rows * co * sizeof(float) : 0;
@@ -763,7 +832,7 @@ LinearActPlan linear_act_plan(int dtype, int x_type, int64_t n, int co, int row_
         const int64_t rows = rounds * cus / col_tiles * b.rows;
         if (rounds < 1 || rows <= 0 || rows >= n) continue;
         const Choice rest = choose(mt, n - rows, co, w_bytes, cus, may_split);
-        const double block = w_bytes / 128 * step_us(b, mt) + (mt == kF32 ? b.rest32 : b.rest);
+        const double block = w_bytes / 128 * step_us(b, mt) + rest_us(b, mt);
         const float us = (float) (kOnce + rounds * block) + rest.us + 3.0f;
         if (us >= least) continue;
         least = us;

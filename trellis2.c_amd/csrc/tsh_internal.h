@@ -405,7 +405,7 @@ struct LinearAct {
 };
 // How a linear is run: parts of its rows one after the other, each with a block
 // shape and its K in splits (for which the scratch memory is; without it they are
-// not split).  No parts: the general kernel.
+// not split).  No parts: the general kernel, or the one for few integer rows.
 struct LinearActPart {
     int64_t rows;
     int shape, splits;
@@ -417,6 +417,7 @@ struct LinearActPlan {
 };
 LinearActPlan linear_act_plan(int dtype, int x_type, int64_t n, int co, int row_bytes, int w_bytes, int cus,
                               bool may_split);
+constexpr int kFewRows = 4;
 inline int linear_act_rows(int co) { return (co + 255) / 256 * 256; }
 // Widest row: a block's 256 rows stay below 2 GiB.
 constexpr int kLinearActMaxBytes = 1 << 22;
