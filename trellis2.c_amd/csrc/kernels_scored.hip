@@ -582,6 +582,20 @@ __global__ void __launch_bounds__(64 * NW, DC <= 64 ? (VOXELS ? 3 : 4) : 2) k_sc
     leave_at<DT>(p, part, out, ref, sum_halves(sum0 + sum1), live, t0 < t1, left, row, head, half);
 }
 
+// tanh to 3 roundings of its value: its series below 0.35 (the next term is 2^-26 of it),
+// else 1 - t over 1 + t, t = exp(-2 |u|).
+__device__ __forceinline__ float tanh32(float u) {
+    const float a = fabsf(u), q = u * u;
+    const float t = __builtin_amdgcn_exp2f(-2.88539008f * a);
+    const float far = copysignf((1.0f - t) * __builtin_amdgcn_rcpf(1.0f + t), u);
+    float s = fmaf(q, -8.86323553e-3f, 2.18694885e-2f);
+    s = fmaf(q, s, -5.39682540e-2f);
+    s = fmaf(q, s, 1.33333333e-1f);
+    s = fmaf(q, s, -3.33333333e-1f);
+    return a < 0.35f ? fmaf(u * q, s, u) : far;
+}
+
+// fp32, as k_attention32: its products leave the vector unit time for exact changes.
 template <int DC, int NW>
 __global__ void __launch_bounds__(64 * NW, 2) k_scored32(Attention p, Scores sc, Split shape, int tiles) {
     constexpr int TQ = 32 * NW, TK = 32;
@@ -593,6 +607,8 @@ __global__ void __launch_bounds__(64 * NW, 2) k_scored32(Attention p, Scores sc,
     constexpr int PER = TILE / 1024 / NW;
     static_assert(TILE / 1024 % NW == 0, "whole loads");
     __shared__ __attribute__((aligned(1024))) unsigned char s_tile[4 * TILE];  // K, V of two tiles
+    __shared__ int4 s_xyz[2][TK];  // the coordinates of their keys
+    __shared__ int s_odd[NW];
 
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -613,12 +629,11 @@ __global__ void __launch_bounds__(64 * NW, 2) k_scored32(Attention p, Scores sc,
     const int64_t row = at.q0 + vq / group;
     const int head = kv * group + (int) (vq % group);
     const bool live = qi < at.nq;
-    const bool changed = sc.cap > 0.0f || sc.slopes != nullptr;
-    const float sign = p.scale < 0.0f ? -1.0f : 1.0f, scale = changed ? 1.0f : sc.by;
+    const float sign = p.scale < 0.0f ? -1.0f : 1.0f, scale = sc.cap > 0.0f ? sc.cap : sc.by;
     const int64_t query = vq / group;
     const int place = (int) (query + at.nk - at.rows);
     const int limit = (live ? (int) keys_seen(at, sc, query) : seen) - 1;  // (lanes without one mask nothing)
-    const float slope = sc.slopes != nullptr && live ? sc.slopes[head] * 1.44269504f : 0.0f;
+    const float slope = sc.slopes != nullptr && live ? -sc.slopes[head] * (sc.cap > 0.0f ? 2.0f : 1.0f) * sc.over : 0.0f;
     const int3 here = sc.q_xyz != nullptr && live ? voxel_of(sc.q_xyz, row) : int3{0, 0, 0};
     float q[KS][4];
     {
@@ -662,20 +677,75 @@ __global__ void __launch_bounds__(64 * NW, 2) k_scored32(Attention p, Scores sc,
         }
     };
 
+    int4 key_xyz{0, 0, 0, 0};
+    const auto fetch_xyz = [&](int t) {
+        if (sc.k_xyz != nullptr && wave == 0 && lane < TK && t * TK + lane < at.nk)
+            key_xyz = *(const int4 *) (sc.k_xyz + (at.k0 + t * TK + lane) * 4);
+    };
+
     f32x16 out[DT32];
 #pragma unroll
     for (int d = 0; d < DT32; ++d)
 #pragma unroll
         for (int i = 0; i < 16; ++i) out[d][i] = 0.0f;
+    // As k_scored's.
+    const int least_seen = (int) keys_seen(at, sc, at.first / group);
+    const auto set_aside = [&](unsigned char * sv, int last) {
+        constexpr int PART = TILE / NW;
+        unsigned char * mine = sv + wave * PART + lane * 16;
+        const auto odd_value = [](float v) { return !(fabsf(v) < __builtin_inff()); };
+        bool some = false;
+#pragma unroll 1
+        for (int i = 0; i < PART; i += 1024) {
+            const float4 v = *(const float4 *) (mine + i);
+            some |= odd_value(v.x) || odd_value(v.y) || odd_value(v.z) || odd_value(v.w);
+        }
+        const bool any = __any(some);
+        if (lane == 0) s_odd[wave] = any;
+        lds_barrier();
+        int odd = 0;
+#pragma unroll
+        for (int w = 0; w < NW; ++w) odd |= s_odd[w];
+        if (uniform(odd) == 0) return;
+#pragma unroll 1
+        for (int r = 0; r < TK; ++r) {
+            if (r - 4 * half > last) break;
+#pragma unroll
+            for (int d = 0; d < DT32; ++d)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float * v = (const float *) (sv + r * ROW + (((d * 8 + i * 2 + half) ^ swizzle(r)) * 16));
+#pragma unroll
+                    for (int u = 0; u < 4; ++u)
+                        if (odd_value(v[u])) out[d][4 * i + u] += v[u];
+                }
+        }
+        lds_barrier();
+#pragma unroll 1
+        for (int i = 0; i < PART; i += 1024) {
+            float4 * c = (float4 *) (mine + i);
+            const float4 v = *c;
+            *c = float4{odd_value(v.x) ? 0.0f : v.x, odd_value(v.y) ? 0.0f : v.y, odd_value(v.z) ? 0.0f : v.z,
+                        odd_value(v.w) ? 0.0f : v.w};
+        }
+        lds_barrier();
+    };
     float ref = -__builtin_inff(), sum0 = 0.0f, sum1 = 0.0f;
-    if (t0 < t1) load(t0);
+    if (t0 < t1) {
+        load(t0);
+        fetch_xyz(t0);
+    }
     for (int t = t0; t < t1; ++t) {
         // Tile t has landed; every wavefront is done with tile t - 1.
         wait_vmcnt<0>();
+        if (sc.k_xyz != nullptr && wave == 0 && lane < TK) s_xyz[(t - t0) & 1][lane] = key_xyz;
         lds_barrier();
-        if (t + 1 < t1) load(t + 1);
+        if (t + 1 < t1) {
+            load(t + 1);
+            fetch_xyz(t + 1);
+        }
         const unsigned char * sk = s_tile + ((t - t0) & 1) * TILE;
-        const unsigned char * sv = sk + 2 * TILE;
+        unsigned char * sv = s_tile + ((t - t0) & 1) * TILE + 2 * TILE;
         f32x16 cur;
 #pragma unroll
         for (int i = 0; i < 16; ++i) cur[i] = 0.0f;
@@ -687,34 +757,28 @@ __global__ void __launch_bounds__(64 * NW, 2) k_scored32(Attention p, Scores sc,
             cur = __builtin_amdgcn_mfma_f32_32x32x2f32(a.z, q[k][2], cur, 0, 0, 0);
             cur = __builtin_amdgcn_mfma_f32_32x32x2f32(a.w, q[k][3], cur, 0, 0, 0);
         }
-        if (changed) {
+        if (sc.cap > 0.0f) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) cur[i] = tanh32(cur[i] * fabsf(sc.cap_scale));
+        }
+        if (sc.slopes != nullptr && sc.q_xyz == nullptr) {
+            const float from = (float) (place - t * TK - 4 * half);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) cur[i] = fmaf(slope, fabsf(from - (float) (8 * (i / 4) + i % 4)), cur[i]);
+        }
+        if (sc.q_xyz != nullptr) {
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
-                const int key = min(t * TK + 8 * (i / 4) + 4 * half + i % 4, at.nk - 1);
-                cur[i] = sc.cap > 0.0f ? sc.cap * tanhf(cur[i] * fabsf(sc.cap_scale)) : cur[i] * fabsf(p.scale);
-                if (sc.slopes != nullptr) {
-                    const float d = sc.q_xyz != nullptr ? distance_of(here, voxel_of(sc.k_xyz, at.k0 + key))
-                                                        : fabsf((float) (place - key));
-                    cur[i] = fmaf(-slope, d, cur[i]);
-                }
+                const int4 key = s_xyz[(t - t0) & 1][8 * (i / 4) + 4 * half + i % 4];
+                const float x = (float) (here.x - key.y), y = (float) (here.y - key.z), z = (float) (here.z - key.w);
+                cur[i] = fmaf(slope, __builtin_amdgcn_sqrtf(fmaf(x, x, fmaf(y, y, z * z))), cur[i]);
             }
         }
         const int last = limit - t * TK - 4 * half;
-        const bool masked = __any(last < TK - 5);
-        if (masked) {
+        if (__any(last < TK - 5)) {
 #pragma unroll
             for (int i = 0; i < 16; ++i)
                 if (8 * (i / 4) + i % 4 > last) cur[i] = -__builtin_inff();
-        }
-        // As in k_scored: of values that are not finite the products take zeros where some are not seen.
-        bool odd = false;
-        if (masked) {
-            for (int i = lane * 16; i < TILE; i += 1024) {
-                const float4 v = *(const float4 *) (sv + i);
-                const float most = fmaxf(fmaxf(fabsf(v.x), fabsf(v.y)), fmaxf(fabsf(v.z), fabsf(v.w)));
-                odd |= !(most < __builtin_inff()) || v.x != v.x || v.y != v.y || v.z != v.z || v.w != v.w;
-            }
-            odd = __any(odd);
         }
         float m = cur[0];
 #pragma unroll
@@ -732,6 +796,7 @@ __global__ void __launch_bounds__(64 * NW, 2) k_scored32(Attention p, Scores sc,
                 for (int i = 0; i < 16; ++i) out[d][i] *= keep;
         }
         const float base = ref == -__builtin_inff() ? 0.0f : ref;
+        if (t * TK + TK > least_seen) set_aside(sv, last);
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
             const float e = __builtin_amdgcn_exp2f(fmaf(cur[i], scale, -base));
@@ -739,25 +804,8 @@ __global__ void __launch_bounds__(64 * NW, 2) k_scored32(Attention p, Scores sc,
             const int r = 8 * (i / 4) + 4 * half + i % 4;
 #pragma unroll
             for (int d = 0; d < DT32; ++d) {
-                float a = *(const float *) (sv + r * ROW + (((8 * d + l32 / 4) ^ swizzle(r)) * 16) + l32 % 4 * 4);
-                if (odd && !(fabsf(a) < __builtin_inff())) a = 0.0f;
+                const float a = *(const float *) (sv + r * ROW + (((8 * d + l32 / 4) ^ swizzle(r)) * 16) + l32 % 4 * 4);
                 out[d] = __builtin_amdgcn_mfma_f32_32x32x2f32(a, e, out[d], 0, 0, 0);
-            }
-        }
-        if (odd) {
-#pragma unroll 1
-            for (int r = 0; r < TK; ++r) {
-                if (r - 4 * half > last) break;
-#pragma unroll
-                for (int d = 0; d < DT32; ++d)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const float * v =
-                            (const float *) (sv + r * ROW + (((d * 8 + i * 2 + half) ^ swizzle(r)) * 16));
-#pragma unroll
-                        for (int u = 0; u < 4; ++u)
-                            if (!(fabsf(v[u]) < __builtin_inff())) out[d][4 * i + u] += v[u];
-                    }
             }
         }
     }
