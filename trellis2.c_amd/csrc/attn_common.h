@@ -204,7 +204,7 @@ __device__ __forceinline__ void leave(const Attention & p, const Partial & part,
 // The splits of a query, at places q + split * step of part, joined by WAVES wavefronts (see k_join).
 template <int DT, int WAVES>
 __device__ __forceinline__ void join_query(const Attention & p, const Partial & part, int qp, int64_t q, int64_t step,
-                                           int64_t row, int head, float (&s_sum)[4][64][5]) {
+                                           int64_t row, int head, float (&s_sum)[WAVES > 4 ? WAVES : 4][64][5]) {
     using T = typename Store<DT>::T;
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
     float most = -__builtin_inff();
