@@ -108,6 +108,42 @@ def test_norm(backends, dtype, c):
             ref.check(be.download(total).reshape(n, c), s, ref.E * np.abs(s) + ref.stored(s, dtype), "total")
 
 
+@pytest.mark.parametrize("c", [64, 512, 1000, 300])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_norm_at_the_ends_of_the_range(backends, dtype, c):
+    """Values whose squares, or whose products with gamma, leave fp32; rows of zeros, of infinities and of NaN beside them,
+    gammas of every size; a gamma that is not finite makes every row NaN."""
+    be, rng = backends[dtype], np.random.default_rng(c)
+    big, small = {sh.F32: (1e37, 1e-37), sh.F16: (6e4, 1e-7), sh.BF16: (1e37, 1e-37)}[dtype]
+    size = np.array([1.0, big, big / 1e3, small, small * 10, 0.0, 1.0, 1.0, 1.0])
+    n = len(size)
+    x = sh.storage_round((np.clip(rng.standard_normal((n, c)), -3, 3) * size[:, None]).astype(np.float32), dtype)
+    x[6, 3], x[7, c - 1] = np.inf, np.nan
+    for eps, gamma in ((1e-5, None), (1e-5, np.exp(8 * rng.standard_normal(c)).astype(np.float32)),
+                       (1e-30, np.full(c, 1e6, np.float32))):
+        rows = be.alloc_rows_int8(n, c)
+        be.rms_norm(be.upload(x), gamma, rows, n, c, eps)
+        s = x.astype(np.float64)
+        fine = np.isfinite(s).all(1)
+        with np.errstate(invalid="ignore"):
+            norm = 1 / np.sqrt((s * s).mean(1, keepdims=True) + float(np.float32(eps)))
+            codes, scales = more.int8_rows(s * (1 if gamma is None else gamma.astype(np.float64)))
+            exp = codes * scales * norm
+        got = expanded(be, rows, n, c)
+        assert np.isnan(got[~fine]).all()
+        # What the type cannot hold is an infinity; scales below fp32's normal numbers have fewer digits.
+        exp, got = exp[fine], got[fine]
+        held = np.abs(exp) < {sh.F32: 3e38, sh.F16: 65000.0, sh.BF16: 3e38}[dtype]
+        tol = 4 * ref.E * np.abs(exp) + ref.stored(exp, dtype) + 128 * 2.0 ** -149
+        ref.check(np.where(held, got, 0), np.where(held, exp, 0), tol, f"ends {c} {eps}")
+    for bad in (np.nan, np.inf):
+        g = np.ones(c, np.float32)
+        g[c // 2] = bad
+        rows = be.alloc_rows_int8(n, c)
+        be.rms_norm(be.upload(np.ones((n, c), np.float32)), g, rows, n, c, 1e-5)
+        assert np.isnan(expanded(be, rows, n, c)).all()
+
+
 def run_linear(be, dtype, n, ci, co, act, bias, residual, seed=0, norm=False):
     rng = np.random.default_rng(seed + n + 3 * ci + 5 * co)
     x = sh.storage_round((rng.standard_normal((n, ci)) * np.exp(rng.standard_normal((n, 1)))).astype(np.float32), dtype)

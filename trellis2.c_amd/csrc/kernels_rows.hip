@@ -367,7 +367,6 @@ __global__ void __launch_bounds__(256) k_rows_int8(const typename Store<DT>::T *
                                                    const typename Store<DT>::T * residual,
                                                    const float * __restrict__ gamma, typename Store<DT>::T * total,
                                                    IntRows out, int64_t n, int c, float eps) {
-    using T = typename Store<DT>::T;
     constexpr bool FINE = DT == kF32;
     using S = typename std::conditional<NORM && FINE, double, float>::type;
     constexpr int N = kChunk<DT>, RPB = 256 / LPR;
@@ -461,7 +460,18 @@ __global__ void __launch_bounds__(256) k_rows_int8(const typename Store<DT>::T *
             top = group_reduce<LPR>(top, larger);
             sum = group_sum<LPR>(sum);
             scale = top * (1.0f / sqrtf(fmaf(sum, (float) per_c, eps))) * (1.0f / 127.0f);
-            if (odd || !(sum < __builtin_inff())) scale = __builtin_nanf("");
+            // Squares or products at the ends of fp32's range: both again in 64 bits.
+            if (__any(!(sum < 1e30f && top < 1e30f) || (sum < 1e-30f && top > 0.0f))) {
+                double squares = 0.0;
+#pragma unroll
+                for (int i = 0; i < CPL; ++i)
+#pragma unroll
+                    for (int u = 0; u < N; ++u) squares += product(s[i][u], s[i][u]);
+                squares = group_sum<LPR>(squares);
+                scale = (float) (exact_most() * inverse_root(fma(squares, per_c, (double) eps)) * (1.0 / 127.0));
+                if (!(squares < __builtin_inf())) scale = __builtin_nanf("");
+            }
+            if (odd) scale = __builtin_nanf("");
         } else {
             top = __builtin_bit_cast(float, group_max<LPR>(bits));
             scale = (float) ((double) top * (1.0 / 127.0));
