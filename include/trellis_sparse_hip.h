@@ -538,8 +538,9 @@ trellis_status trellis_sparse_hip_wrap_i32(trellis_sparse_backend * backend, voi
 trellis_status trellis_sparse_hip_set_stream(trellis_sparse_backend * backend, void * stream);
 trellis_status trellis_sparse_hip_own_stream(trellis_sparse_backend * backend);
 
-/* linear_act of few rows splits its sums, and attention of few queries its keys,
- * over more blocks, through scratch of the backend's pool; a call that gets none
+/* linear_act of few rows splits its sums, attention and attention_scored of few
+ * queries (the latter also of queries that fill no whole round) their keys, and
+ * group_norm of many rows its rows over more blocks, through scratch of the backend's pool; a call that gets none
  * (under capture, or out of memory) does without, in more time and with sums in
  * another order.  With `scratch` set (NULL: the pool again) such calls use its
  * memory where it is large enough, captured ones too: graphs, streams or backends
@@ -692,7 +693,7 @@ typedef struct trellis_sparse_hip_scores_desc {
     uint32_t struct_size;  /* sizeof(trellis_sparse_hip_scores_desc) */
     int32_t causal;        /* 0 or 1 */
     float cap;             /* 0: none */
-    const float * slopes;  /* fp32 [heads] on the host, up to 2^64, or NULL */
+    const float * slopes;  /* fp32 [heads] on the host, up to 2^64, kept as weights are, or NULL */
     const trellis_sparse_buffer * q_coords;  /* int32 [nq][4] (b, x, y, z; b is not read), or NULL */
     const trellis_sparse_buffer * k_coords;  /* int32 [nkv][4]; both within +-2^29 */
     const trellis_sparse_buffer * prefix;    /* int32 [n_seqs], read on the device, or NULL: 0 */

@@ -222,6 +222,13 @@ template <int DT> __device__ __forceinline__ s16x8 finite_part(s16x8 v) {
 // As k_attention, its scores changed between the products and the softmax.  What that adds
 // runs on the vector unit, which bounds attention already; squared distances of voxels are the
 // matrix unit's, counted from the block's first query, but where some are too far for that.
+// The cap's constant part and the scale are the softmax's own: a cap adds a product, two
+// transcendental instructions and a sum a score, a distance one product and, of voxels, a
+// root.  A tile's scores are not computed under the softmax of the one before: without their
+// registers one more wavefront per SIMD fits, which hides as much and spills nothing (18,216
+// rows of 8 x 64 bf16 by voxel distance 1.62 -> 1.30 ms).
+// Bound by the vector unit, 76 % busy there (matrix unit 31 %): 1.05 ms, 650 TFLOP/s of its
+// products; 16,384 rows of 8 x 128 capped 1.30 ms, 850 TFLOP/s.
 template <int DT, int DC, int NW, bool FINE, bool VOXELS>
 __global__ void __launch_bounds__(64 * NW, DC <= 64 ? (VOXELS ? 3 : 4) : 2) k_scored(Attention p, Scores sc, Split shape, int tiles) {
     using T = typename Store<DT>::T;
