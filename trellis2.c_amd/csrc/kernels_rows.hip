@@ -450,6 +450,7 @@ __global__ void __launch_bounds__(256) k_rows_int8(const typename Store<DT>::T *
         };
         float scale;
         double most = 0.0;
+        bool edge = false;  // squares or products at the ends of fp32's range: the scale from 64 bits
         if constexpr (NORM && FINE) {
             most = exact_most();
             top = (float) most;
@@ -460,24 +461,14 @@ __global__ void __launch_bounds__(256) k_rows_int8(const typename Store<DT>::T *
             top = group_reduce<LPR>(top, larger);
             sum = group_sum<LPR>(sum);
             scale = top * (1.0f / sqrtf(fmaf(sum, (float) per_c, eps))) * (1.0f / 127.0f);
-            // Squares or products at the ends of fp32's range: both again in 64 bits.
-            if (__any(!(sum < 1e30f && top < 1e30f) || (sum < 1e-30f && top > 0.0f))) {
-                double squares = 0.0;
-#pragma unroll
-                for (int i = 0; i < CPL; ++i)
-#pragma unroll
-                    for (int u = 0; u < N; ++u) squares += product(s[i][u], s[i][u]);
-                squares = group_sum<LPR>(squares);
-                scale = (float) (exact_most() * inverse_root(fma(squares, per_c, (double) eps)) * (1.0 / 127.0));
-                if (!(squares < __builtin_inf())) scale = __builtin_nanf("");
-            }
+            edge = !odd && (!(sum < 1e30f && top < 1e30f) || (sum < 1e-30f && top > 0.0f));
             if (odd) scale = __builtin_nanf("");
         } else {
             top = __builtin_bit_cast(float, group_max<LPR>(bits));
             scale = (float) ((double) top * (1.0 / 127.0));
         }
         scale = finite_or_nan(scale);
-        const bool zero = !(top > 0.0f) || scale != scale;  // codes are zeros
+        const bool zero = !(top > 0.0f) || (!edge && scale != scale);  // codes are zeros
         const bool far = !zero && !(top > 1e-30f && top < 1e30f);  // near the ends of fp32's range: codes from 64 bits
         const float by = zero ? 0.0f : 127.0f * __builtin_amdgcn_rcpf(top);
         // 127 t / T, off by no more than 127 times 6 roundings, 4.6e-5.
@@ -510,8 +501,24 @@ __global__ void __launch_bounds__(256) k_rows_int8(const typename Store<DT>::T *
                 *(uint32_t *) p = zero ? 0u : four_codes(code);
             }
         }
-        if (NORM && __any(far || (!zero && near > kNear))) {
+        if (NORM && __any(edge || far || (!zero && near > kNear))) {
             if constexpr (!FINE) most = exact_most();
+            bool none = false;  // some value is not finite
+            if constexpr (!FINE) {
+                if (__any(edge)) {
+                    double squares = 0.0;
+#pragma unroll
+                    for (int i = 0; i < CPL; ++i)
+#pragma unroll
+                        for (int u = 0; u < N; ++u) squares += product(s[i][u], s[i][u]);
+                    squares = group_sum<LPR>(squares);
+                    if (edge) {
+                        scale = finite_or_nan((float) (most * inverse_root(fma(squares, per_c, (double) eps)) * (1.0 / 127.0)));
+                        if (!(squares < __builtin_inf())) scale = __builtin_nanf("");
+                        none = scale != scale;
+                    }
+                }
+            }
 #pragma unroll
             for (int i = 0; i < CPL; ++i)
 #pragma unroll
@@ -520,8 +527,8 @@ __global__ void __launch_bounds__(256) k_rows_int8(const typename Store<DT>::T *
                     S a = s[i][u];
                     asm volatile("" : "+v"(a));  // else what is above stays in registers for here
                     const float f = about(a, g[i][u]);
-                    if (!zero && at < c && (far || fabsf(f - rintf(f)) > kNear))
-                        out.codes[row * out.cp + at] = (int8_t) int_code64(product(a, g[i][u]), most);
+                    if (!zero && at < c && (none || far || fabsf(f - rintf(f)) > kNear))
+                        out.codes[row * out.cp + at] = (int8_t) (none ? 0 : int_code64(product(a, g[i][u]), most));
                 }
         }
         if (l == 0) out.scales[row] = scale;
