@@ -144,6 +144,27 @@ def test_norm_at_the_ends_of_the_range(backends, dtype, c):
         assert np.isnan(expanded(be, rows, n, c)).all()
 
 
+@pytest.mark.parametrize("c", [64, 512, 1024])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_norm_of_a_row_does_not_see_its_neighbours(backends, dtype, c):
+    """Ordinary rows among rows at the ends of the range, infinite, NaN and zero: each as if normed alone, to the last bit."""
+    be, rng = backends[dtype], np.random.default_rng(c + 1)
+    big, small = {sh.F32: (1e37, 1e-37), sh.F16: (6e4, 1e-7), sh.BF16: (1e37, 1e-37)}[dtype]
+    size = rng.permutation(np.repeat(np.array([1.0, 1.0, 1.0, big, small, 0.0, 1.0, 1.0]), 5))
+    n = len(size)
+    x = np.clip(rng.standard_normal((n, c)), -0.9, 0.9) * size[:, None]
+    ones = np.flatnonzero(size == 1.0)
+    x[ones[3], 5], x[ones[9], c - 1] = np.inf, np.nan
+    x = sh.storage_round(x.astype(np.float32), dtype)
+    gamma = np.exp(rng.standard_normal(c)).astype(np.float32)
+    rows, one = be.alloc_rows_int8(n, c), be.alloc_rows_int8(1, c)
+    be.rms_norm(be.upload(x), gamma, rows, n, c, 1e-5)
+    got = expanded(be, rows, n, c)
+    for i in range(n):
+        be.rms_norm(be.upload(x[i:i + 1]), gamma, one, 1, c, 1e-5)
+        assert np.array_equal(got[i:i + 1], expanded(be, one, 1, c), equal_nan=True), (i, size[i])
+
+
 def run_linear(be, dtype, n, ci, co, act, bias, residual, seed=0, norm=False):
     rng = np.random.default_rng(seed + n + 3 * ci + 5 * co)
     x = sh.storage_round((rng.standard_normal((n, ci)) * np.exp(rng.standard_normal((n, 1)))).astype(np.float32), dtype)
