@@ -692,7 +692,7 @@ trellis_status trellis_sparse_hip_attention(trellis_sparse_backend * backend, co
 typedef struct trellis_sparse_hip_scores_desc {
     uint32_t struct_size;  /* sizeof(trellis_sparse_hip_scores_desc) */
     int32_t causal;        /* 0 or 1 */
-    float cap;             /* 0: none */
+    float cap;             /* 0: none; in 16 bits scores under caps up to 512 are off by up to 2^-22 of the cap */
     const float * slopes;  /* fp32 [heads] on the host, up to 2^64, kept as weights are, or NULL */
     const trellis_sparse_buffer * q_coords;  /* int32 [nq][4] (b, x, y, z; b is not read), or NULL */
     const trellis_sparse_buffer * k_coords;  /* int32 [nkv][4]; both within +-2^29 */

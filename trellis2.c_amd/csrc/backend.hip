@@ -2570,8 +2570,10 @@ trellis_status attention_impl(trellis_sparse_backend * backend, const trellis_sp
         sc.slopes = (const float *) slopes;
         sc.cap = scores->cap * 1.4426950408889634f;
         sc.cap_scale = scores->cap > 0.0f ? (float) (natural / (double) scores->cap) : 0.0f;
+        const bool quick = scores->cap > 0.0f && scores->cap <= kQuickCap && be->policy.compute_dtype != kF32;
+        if (scores->cap > 0.0f && !quick) sc.top = (float) std::min(3e38, (double) scores->cap / std::fabs(natural));
         sc.twice = 2.8853900817779268f * std::fabs(sc.cap_scale);
-        sc.by = scores->cap > 0.0f ? 2.0f * sc.cap : std::fabs(scale);
+        sc.by = quick ? 2.0f * sc.cap : std::fabs(scale);
         sc.over = (float) (1.4426950408889634 / (double) sc.by);
         sc.q_xyz = (const int32_t *) sqc.at;
         sc.k_xyz = (const int32_t *) skc.at;

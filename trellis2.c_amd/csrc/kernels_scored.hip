@@ -40,7 +40,9 @@ template <int DT> __global__ void __launch_bounds__(256) k_scored_any(Attention 
     if (sc.q_xyz != nullptr && row < at.nq) here = voxel_of(sc.q_xyz, at.q0 + at.first + row);
     const auto score = [&](float dot, int j) {
         float s = dot * p.scale;
-        if (sc.cap > 0.0f) s = sc.cap * tanhf(dot * sc.cap_scale);
+        // (Below that tanh(u) is u, which may have lost digits where the cap is very large.)
+        const float u = dot * sc.cap_scale;
+        if (sc.cap > 0.0f && !(fabsf(u) < 0x1p-13f)) s = sc.cap * tanhf(u);
         if (sc.slopes != nullptr && j < at.nk) {
             const float d = sc.q_xyz != nullptr ? distance_of(here, voxel_of(sc.k_xyz, at.k0 + j)) : fabsf((float) (place - j));
             s -= slope * d;
@@ -203,6 +205,20 @@ __device__ __forceinline__ bool voxel_terms(const int3 & xyz, const int3 & origi
     return (bool) __any(out);
 }
 
+// top tanh(u) for a product z, u = |z by| and top = 1 / by, to 16 roundings of its own value: z times the series of
+// tanh(u) / u below 0.35 (the next term is 2^-26 of it), where u's own digits matter little, else 1 - t over 1 + t,
+// t = exp(-2 u).
+__device__ __forceinline__ float capped(float z, float by, float top) {
+    const float u = fabsf(z * by), q = u * u;
+    const float t = __builtin_amdgcn_exp2f(-2.88539008f * u);
+    const float far = copysignf((1.0f - t) * __builtin_amdgcn_rcpf(1.0f + t) * top, z);
+    float s = fmaf(q, -8.86323553e-3f, 2.18694885e-2f);
+    s = fmaf(q, s, -5.39682540e-2f);
+    s = fmaf(q, s, 1.33333333e-1f);
+    s = fmaf(q, s, -3.33333333e-1f);
+    return u < 0.35f ? fmaf(z * q, s, z) : far;
+}
+
 // 16-bit values: whether one of eight is an infinity or a NaN, and zeros in place of those.
 template <int DT> __device__ __forceinline__ bool any_not_finite(const int4 & c) {
     constexpr uint32_t E = DT == kBF16 ? 0x7f80u : 0x7c00u;
@@ -229,7 +245,7 @@ template <int DT> __device__ __forceinline__ s16x8 finite_part(s16x8 v) {
 // rows of 8 x 64 bf16 by voxel distance 1.62 -> 1.30 ms).
 // Bound by the vector unit, 76 % busy there (matrix unit 31 %): 1.05 ms, 650 TFLOP/s of its
 // products; 16,384 rows of 8 x 128 capped 1.30 ms, 850 TFLOP/s.
-template <int DT, int DC, int NW, bool FINE, bool VOXELS>
+template <int DT, int DC, int NW, bool FINE, bool VOXELS, bool TANH>
 __global__ void __launch_bounds__(64 * NW, DC <= 64 ? (VOXELS ? 3 : 4) : 2) k_scored(Attention p, Scores sc, Split shape, int tiles) {
     using T = typename Store<DT>::T;
     constexpr int TQ = 32 * NW, TK = 64;
@@ -388,8 +404,12 @@ __global__ void __launch_bounds__(64 * NW, DC <= 64 ? (VOXELS ? 3 : 4) : 2) k_sc
     // Products with keys n * 32 .. of tile t to what times `scale` is a score in log2 units: the
     // cap, then the distance.
     const auto change_scores = [&](int t, int n, f32x16 & cur, bool near, const int4 & terms) {
-        if (sc.cap > 0.0f) {
-            // cap tanh(z) is cap less 2 cap / (1 + exp(2 z)), the cap the same for all keys.
+        if constexpr (TANH) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) cur[i] = capped(cur[i], sc.cap_scale, sc.top);
+        } else if (sc.cap > 0.0f) {
+            // cap tanh(z) is cap less 2 cap / (1 + exp(2 z)), the cap the same for all keys: off by
+            // some 2^-22.5 of the cap, whatever the score.
 #pragma unroll
             for (int i = 0; i < 16; ++i) cur[i] = __builtin_amdgcn_rcpf(-1.0f - __builtin_amdgcn_exp2f(cur[i] * sc.twice));
         }
@@ -591,19 +611,6 @@ __global__ void __launch_bounds__(64 * NW, DC <= 64 ? (VOXELS ? 3 : 4) : 2) k_sc
     leave_at<DT>(p, part, out, ref, sum_halves(sum0 + sum1), live, t0 < t1, left, row, head, half);
 }
 
-// tanh to 3 roundings of its value: its series below 0.35 (the next term is 2^-26 of it),
-// else 1 - t over 1 + t, t = exp(-2 |u|).
-__device__ __forceinline__ float tanh32(float u) {
-    const float a = fabsf(u), q = u * u;
-    const float t = __builtin_amdgcn_exp2f(-2.88539008f * a);
-    const float far = copysignf((1.0f - t) * __builtin_amdgcn_rcpf(1.0f + t), u);
-    float s = fmaf(q, -8.86323553e-3f, 2.18694885e-2f);
-    s = fmaf(q, s, -5.39682540e-2f);
-    s = fmaf(q, s, 1.33333333e-1f);
-    s = fmaf(q, s, -3.33333333e-1f);
-    return a < 0.35f ? fmaf(u * q, s, u) : far;
-}
-
 // fp32, as k_attention32: its products leave the vector unit time for exact changes.
 template <int DC, int NW>
 __global__ void __launch_bounds__(64 * NW, 2) k_scored32(Attention p, Scores sc, Split shape, int tiles) {
@@ -638,11 +645,11 @@ __global__ void __launch_bounds__(64 * NW, 2) k_scored32(Attention p, Scores sc,
     const int64_t row = at.q0 + vq / group;
     const int head = kv * group + (int) (vq % group);
     const bool live = qi < at.nq;
-    const float sign = p.scale < 0.0f ? -1.0f : 1.0f, scale = sc.cap > 0.0f ? sc.cap : sc.by;
+    const float sign = p.scale < 0.0f ? -1.0f : 1.0f, scale = sc.by;
     const int64_t query = vq / group;
     const int place = (int) (query + at.nk - at.rows);
     const int limit = (live ? (int) keys_seen(at, sc, query) : seen) - 1;  // (lanes without one mask nothing)
-    const float slope = sc.slopes != nullptr && live ? -sc.slopes[head] * (sc.cap > 0.0f ? 2.0f : 1.0f) * sc.over : 0.0f;
+    const float slope = sc.slopes != nullptr && live ? -sc.slopes[head] * sc.over : 0.0f;
     const int3 here = sc.q_xyz != nullptr && live ? voxel_of(sc.q_xyz, row) : int3{0, 0, 0};
     float q[KS][4];
     {
@@ -766,9 +773,9 @@ __global__ void __launch_bounds__(64 * NW, 2) k_scored32(Attention p, Scores sc,
             cur = __builtin_amdgcn_mfma_f32_32x32x2f32(a.z, q[k][2], cur, 0, 0, 0);
             cur = __builtin_amdgcn_mfma_f32_32x32x2f32(a.w, q[k][3], cur, 0, 0, 0);
         }
-        if (sc.cap > 0.0f) {
+        if (sc.top > 0.0f) {
 #pragma unroll
-            for (int i = 0; i < 16; ++i) cur[i] = tanh32(cur[i] * fabsf(sc.cap_scale));
+            for (int i = 0; i < 16; ++i) cur[i] = capped(cur[i], sc.cap_scale, sc.top);
         }
         if (sc.slopes != nullptr && sc.q_xyz == nullptr) {
             const float from = (float) (place - t * TK - 4 * half);
@@ -830,16 +837,17 @@ hipError_t launch_nw(const Attention & p, const Scores & sc, const Split & split
     if constexpr (DT == kF32) {
         k_scored32<DC, NW><<<(unsigned) grid, 64 * NW, 0, s>>>(p, sc, split, tiles);
     } else {
-        const auto launch = [&](auto fine_c, auto voxels_c) {
-            k_scored<DT, DC, NW, decltype(fine_c)::value, decltype(voxels_c)::value>
+        const auto launch = [&](auto fine_c, auto voxels_c, auto tanh_c) {
+            k_scored<DT, DC, NW, decltype(fine_c)::value, decltype(voxels_c)::value, decltype(tanh_c)::value>
                 <<<(unsigned) grid, 64 * NW, 0, s>>>(p, sc, split, tiles);
         };
         using std::false_type, std::true_type;
-        if (sc.q_xyz != nullptr) {
-            sh.fine ? launch(true_type(), true_type()) : launch(false_type(), true_type());
-        } else {
-            sh.fine ? launch(true_type(), false_type()) : launch(false_type(), false_type());
-        }
+        // (Large caps are rare: one instance, for any number of queries.)
+        const auto kind = [&](auto voxels_c) {
+            if (sc.top > 0.0f) return launch(true_type(), voxels_c, true_type());
+            sh.fine ? launch(true_type(), voxels_c, false_type()) : launch(false_type(), voxels_c, false_type());
+        };
+        sc.q_xyz != nullptr ? kind(true_type()) : kind(false_type());
     }
     hipError_t err = hipGetLastError();
     if (err == hipSuccess && split.part.splits > 1) {

@@ -452,14 +452,19 @@ hipError_t launch_attention(int dtype, const Attention & p, const AttentionShape
 // Attention whose scores are changed before the softmax (kernels_scored.hip).
 struct Scores {
     float cap, cap_scale;    // cap times log2(e), 0: none; what a product of q and k is multiplied with inside the tanh
-    float twice;             // the exponent's factor in 1 / (1 + 2^(twice q . k)), for q of the scale's sign
-    float by, over;          // of products (capped: of -1 / (1 + ..)) to log2 units, and log2(e) over it
+    float top;               // the cap over |the products' scale| where the tanh is relative to the score, or 0:
+    float twice;             // else the exponent's factor in 1 / (1 + 2^(twice q . k)), for q of the scale's sign
+    float by, over;          // of products (of -1 / (1 + ..) there) to log2 units, and log2(e) over it
     const float * slopes;    // [heads] or null
     const int32_t * q_xyz;   // [nq][4] and [nk][4], or null: distances are of rows
     const int32_t * k_xyz;
     const int32_t * prefix;  // [seqs] or null
     int causal;
 };
+// Largest cap of 16-bit rows that is taken from a constant: scores are then off by up to 2^-22.5 of
+// it, which at 512 is 2^-13.5, a quarter or less of half a step of fp16 (2^-11); under larger
+// ones a tanh of the score's own precision (16,384 rows of 8 x 128 fp16 1.34 -> 2.40 ms).
+constexpr float kQuickCap = 512.0f;
 // How it is run: wavefronts per block (0: the general kernel), tiles of queries, weights in
 // two parts; units of work (a tile with a kv head) that take all of their keys and those
 // that are split, into how many, and the scratch for these (without it none is).
