@@ -574,7 +574,7 @@ trellis_status trellis_sparse_hip_alloc_rows_int8(trellis_sparse_backend * backe
                                                   trellis_sparse_buffer ** out);
 /* rows8 = x, rounded to nearest even; y = the values of rows8 (exact in
  * bf16 and fp32 but for 2^128, the code nearest fp32's largest; of integer rows the
- * product with the scale, rounded). */
+ * product with the scale, rounded, which of fp32's largest is 2^128 too). */
 trellis_status trellis_sparse_hip_pack_rows8(trellis_sparse_backend * backend, const trellis_sparse_buffer * x,
                                              trellis_sparse_buffer * rows8, int64_t n, int c);
 trellis_status trellis_sparse_hip_expand_rows8(trellis_sparse_backend * backend, const trellis_sparse_buffer * rows8,

@@ -67,6 +67,19 @@ struct Frag {
 // Sums of integer rows are whole numbers of 32 bits, exact for up to 131,072 products.
 template <int MT> using Sums = typename std::conditional<MT == kRowsInt8, i32x16, f32x16>::type;
 
+// A sum of integers in the units of its row and channel, and the bias.  A sum is up to 2^31, and with
+// a row's scale beyond 2^96 (which rows of fp16 have not) their product could leave fp32 where the
+// output does not: such a row's scale goes down by 2^32 and the channel's (`raised`) up, both
+// exactly.  A select an output: 79,523 x 512 -> 2048 bf16 222 -> 226 us with its norm; as a branch 234.
+__device__ __forceinline__ float raised(float channel) {
+    const float up = channel * 0x1p32f;
+    return up == __builtin_inff() ? 3.40282347e38f : up;  // (a sum of zero times it is zero)
+}
+template <int DT> __device__ __forceinline__ float in_units(int sum, float row, float channel, float up, float bias) {
+    const bool large = DT != kF16 && row > 0x1p96f;
+    return fmaf((float) sum * (large ? row * 0x1p-32f : row), large ? up : channel, bias);
+}
+
 // SEL: which of a scale register's bytes counts (0 or 2).
 template <int MT, int SEL>
 __device__ __forceinline__ Sums<MT> mac(const Frag & a, const Frag & b, Sums<MT> c, int sa, int sb) {
@@ -407,8 +420,8 @@ __global__ void __launch_bounds__(64 * RW * CW, RW * CW * PER_CU / 4) k_linear_a
                     for (int t = 0; t < NT; ++t) {
                         float z;
                         if constexpr (kInt) {
-                            z = fmaf((float) acc[k / 4][t][4 * (k % 4) + i] * row_scale[k % 2].h[i], channel_scale.h[t],
-                                     bias.h[t]);
+                            z = in_units<DT>(acc[k / 4][t][4 * (k % 4) + i], row_scale[k % 2].h[i], channel_scale.h[t],
+                                         raised(channel_scale.h[t]), bias.h[t]);
                         } else {
                             z = acc[k / 4][t][4 * (k % 4) + i];
                         }
@@ -516,8 +529,9 @@ template <bool INT, int DT, int N> __global__ void __launch_bounds__(256) k_line
 #pragma unroll
     for (int u = 0; u < N; ++u) {
         if constexpr (INT) {
-            v[u] = fmaf((float) sum[u] * ((const float *) p.x_scales)[e / p.co], ((const float *) p.w_scales)[ch + u],
-                        p.bias != nullptr ? p.bias[ch + u] : 0.0f);
+            const float channel = ((const float *) p.w_scales)[ch + u];
+            v[u] = in_units<DT>(sum[u], ((const float *) p.x_scales)[e / p.co], channel, raised(channel),
+                            p.bias != nullptr ? p.bias[ch + u] : 0.0f);
         } else {
             v[u] = sum[u];
         }
@@ -642,8 +656,9 @@ template <int DT, int ROWS> __global__ void __launch_bounds__(256) k_linear_few(
         }
     const int row = lane / CH, ch = ch0 + lane % CH;
     if (row >= ROWS || row >= p.n || ch >= p.co) return;
-    const float z = fmaf((float) mine * ((const float *) p.x_scales)[row], ((const float *) p.w_scales)[ch],
-                         p.bias != nullptr ? p.bias[ch] : 0.0f);
+    const float channel = ((const float *) p.w_scales)[ch];
+    const float z = in_units<DT>(mine, ((const float *) p.x_scales)[row], channel, raised(channel),
+                             p.bias != nullptr ? p.bias[ch] : 0.0f);
     const int64_t e = (int64_t) row * p.co + ch;
     by_act(p.act, [&](auto act_c) {
         float v = activate<DT, decltype(act_c)::value>(z);
