@@ -723,7 +723,7 @@ typedef struct trellis_sparse_hip_block_desc {
     int32_t head_dim;      /* a multiple of 8, up to 192 */
     int32_t hidden;
     int32_t act;           /* trellis_sparse_hip_act */
-    int32_t rows8;         /* 0, 1 or 2 */
+    int32_t rows8;         /* 0, 1 or 2; 2: c and hidden up to 131,072 */
     int32_t pairs[3];      /* as in trellis_sparse_hip_rotary_desc */
     int32_t split;
     float eps;             /* of norm1 and norm2, > 0 */

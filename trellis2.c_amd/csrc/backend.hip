@@ -2643,8 +2643,10 @@ trellis_status transformer_block_impl(trellis_sparse_backend * backend, const tr
     const int64_t wide = (int64_t) d.heads * d.head_dim;
     if (n <= 0 || n > INT32_MAX || d.heads <= 0 || d.heads > 32768 || d.head_dim <= 0 || d.hidden <= 0 ||
         wide > (1 << 18) || d.hidden > (1 << 20) || d.qkv_w == nullptr || d.out_w == nullptr || d.mlp0_w == nullptr ||
-        d.mlp2_w == nullptr || d.rows8 < 0 || d.rows8 > 2 || !float_buffer_ok(be, h, (size_t) (n * wide)) ||
-        !float_buffer_ok(be, out, (size_t) (n * wide)) || spans_clash(packed(out, n, wide), packed(h, n, wide), true)) {
+        d.mlp2_w == nullptr || d.rows8 < 0 || d.rows8 > 2 || d.act < TRELLIS_SPARSE_HIP_ACT_NONE ||
+        d.act > TRELLIS_SPARSE_HIP_ACT_GELU_TANH || (d.rows8 == 2 && (wide > kIntMostTerms || d.hidden > kIntMostTerms)) ||
+        !float_buffer_ok(be, h, (size_t) (n * wide)) || !float_buffer_ok(be, out, (size_t) (n * wide)) ||
+        spans_clash(packed(out, n, wide), packed(h, n, wide), true)) {
         return fail(be, TRELLIS_STATUS_INVALID_ARGUMENT, "transformer_block: bad argument");
     }
     const int c = (int) wide;
