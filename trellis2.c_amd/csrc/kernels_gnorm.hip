@@ -8,10 +8,16 @@ namespace tsh {
 namespace {
 
 // A group's mean m and the inverse of its root variance; the mean in two parts, so that
-// x - m keeps its digits where the mean is far larger than the deviations.
+// x - m keeps its digits where the mean is far larger than the deviations.  Of groups beyond 2^64
+// values and mean are taken 2^32 (`unit`) smaller and the inverse larger, exactly: x - m
+// can be twice fp32's largest, and the inverse of that is subnormal.
 struct GroupStat {
-    float mean, mean_low, inverse, pad;
+    float mean, mean_low, inverse, unit;
 };
+// x - m in those units.  (fp16 has no such groups.)
+template <int DT> __device__ __forceinline__ float centred(float x, const GroupStat & st) {
+    return (DT == kF16 ? x - st.mean : fmaf(x, st.unit, -st.mean)) - st.mean_low;
+}
 
 // Sums over a group, in 64 bits: of d = x - k and of d^2, k the group's first value in its
 // sequence in fp32 (as k is one of the values, (k - m)^2 is at most as many variances as
@@ -30,11 +36,12 @@ template <int DT> __device__ __forceinline__ void add_value(GroupSum & s, float 
 }
 __device__ __forceinline__ GroupStat stat_of(const GroupSum & s, double count, float k, float eps) {
     const double off = s.d / count, var = s.d2 / count - off * off;
-    const double mean = (double) k + off;
+    // (A NaN stays one; a negative variance is a rounding of zero.)
+    const double root = sqrt((var < 0.0 ? 0.0 : var) + (double) eps), most = 0x1p64;
+    const double unit = root > most || fabs((double) k + off) > most ? 0x1p-32 : 1.0, mean = ((double) k + off) * unit;
     const float hi = (float) mean;
     const double low = mean - (double) hi;
-    // (A NaN stays one; a negative variance is a rounding of zero.)
-    return {hi, hi - hi == 0.0f ? (float) low : 0.0f, (float) (1.0 / sqrt((var < 0.0 ? 0.0 : var) + (double) eps)), 0.0f};
+    return {hi, hi - hi == 0.0f ? (float) low : 0.0f, (float) (1.0 / (root * unit)), (float) unit};
 }
 template <int DT> __device__ __forceinline__ float first_value(const typename Store<DT>::T * p, int64_t i) {
     return DT == kF32 ? Store<DT>::ld(p, i) : 0.0f;
@@ -80,7 +87,7 @@ template <int DT> __global__ void __launch_bounds__(256) k_group_norm(GroupNorm 
             const float scale = st.inverse * (p.gamma != nullptr ? p.gamma[g * size + ch] : 1.0f);
             const float shift = p.beta != nullptr ? p.beta[g * size + ch] : 0.0f;
             for (int64_t r = r0; r < end - first; r += step) {
-                const float v = (Store<DT>::ld(x, r * p.c + ch) - st.mean - st.mean_low) * scale + shift;
+                const float v = centred<DT>(Store<DT>::ld(x, r * p.c + ch), st) * scale + shift;
                 Store<DT>::st(y, r * p.c + ch, activate<DT, decltype(act_c)::value>(v));
             }
         }
@@ -264,13 +271,12 @@ template <int DT, int V, int ACT> __global__ void __launch_bounds__(256) k_gn_ap
     if (r0 >= step) return;
     const T * x = (const T *) p.x + at.first * p.c + ch0;
     T * y = (T *) p.y + at.first * p.c + ch0;
-    float mean[V], low[V], scale[V], shift[V];
+    GroupStat st[V];
+    float scale[V], shift[V];
 #pragma unroll
     for (int u = 0; u < V; ++u) {
-        const GroupStat st = stats_of(p)[(int64_t) at.seq * p.groups + (ch0 + u) / size];
-        mean[u] = st.mean;
-        low[u] = st.mean_low;
-        scale[u] = st.inverse * (p.gamma != nullptr ? p.gamma[ch0 + u] : 1.0f);
+        st[u] = stats_of(p)[(int64_t) at.seq * p.groups + (ch0 + u) / size];
+        scale[u] = st[u].inverse * (p.gamma != nullptr ? p.gamma[ch0 + u] : 1.0f);
         shift[u] = p.beta != nullptr ? p.beta[ch0 + u] : 0.0f;
     }
     // Four rows at a time, the next four on their way.
@@ -293,7 +299,7 @@ template <int DT, int V, int ACT> __global__ void __launch_bounds__(256) k_gn_ap
             float v[V];
             unpack_channels<DT, V>(here[i], v);
 #pragma unroll
-            for (int u = 0; u < V; ++u) v[u] = activate<DT, ACT>((v[u] - mean[u] - low[u]) * scale[u] + shift[u]);
+            for (int u = 0; u < V; ++u) v[u] = activate<DT, ACT>(centred<DT>(v[u], st[u]) * scale[u] + shift[u]);
             if constexpr (V == 1) {
                 Store<DT>::st(y + (int64_t) (r + i * step) * p.c, 0, v[0]);
             } else {
