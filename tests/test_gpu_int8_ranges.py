@@ -81,3 +81,24 @@ def test_large_rows_in_many_tiles(backends, dtype):
         d = lambda a: a.astype(np.float64)  # noqa: E731
         exp, tol = more.int8_linear(*more.int8_rows(d(x)), d(w), None, act, d(r), dtype == sh.F32)
         ref.check(linear(be, x, w, None, act, r), exp, tol + ref.stored(exp, dtype), f"{n} {ci} {co} {act}")
+
+
+@pytest.mark.parametrize("c", [64, 300, 512, 1000, 1024])
+@pytest.mark.parametrize("dtype", [sh.F32, sh.F16, sh.BF16])
+def test_norms_with_tiny_gammas(backends, dtype, c):
+    """Products of values and gammas below fp32's range, whose norms are not; gammas of zero, and rows of zeros among others."""
+    be, rng, n = backends[dtype], np.random.default_rng(c), 33
+    size = rng.choice({sh.F32: [1e-30, 1e-14, 1e-3, 1.0, 0.0], sh.F16: [2e-6, 1e-3, 1.0, 0.0],
+                       sh.BF16: [1e-30, 1e-14, 1e-3, 1.0, 0.0]}[dtype], (n, 1))
+    x = sh.storage_round((np.clip(rng.standard_normal((n, c)), -3, 3) * size).astype(np.float32), dtype)
+    for eps, g in ((1e-30, 1e-32), (1e-38, 1e-30), (1e-5, 1e-37), (1e-12, 1e-36), (1e-5, 0.0)):
+        gamma = (g * np.exp(rng.standard_normal(c))).astype(np.float32)
+        rows, y = be.alloc_rows_int8(n, c), be.alloc(n * c)
+        be.rms_norm(be.upload(x), gamma, rows, n, c, eps)
+        be.expand_rows8(rows, y, n, c)
+        s = x.astype(np.float64)
+        codes, scales = more.int8_rows(s * gamma.astype(np.float64))
+        exp = codes * scales / np.sqrt((s * s).mean(1, keepdims=True) + float(np.float32(eps)))
+        # (A scale below fp32's normal numbers is off by up to half of 2^-149, a value by 127 times that.)
+        ref.check(be.download(y).reshape(n, c), exp, 4 * ref.E * np.abs(exp) + ref.stored(exp, dtype) + 128 * 2.0 ** -149,
+                  f"{c} {eps} {g}")

@@ -450,27 +450,29 @@ __global__ void __launch_bounds__(256) k_rows_int8(const typename Store<DT>::T *
         };
         float scale;
         double most = 0.0;
-        bool edge = false;  // squares or products at the ends of fp32's range: the scale from 64 bits
+        bool zero, far = false;  // codes are zeros; sums or products near the ends of fp32's range, or none: from 64 bits
         if constexpr (NORM && FINE) {
             most = exact_most();
             top = (float) most;
             sum = group_sum<LPR>(sum);
-            scale = (float) (most * inverse_root(fma(sum, per_c, (double) eps)) * (1.0 / 127.0));
+            scale = finite_or_nan((float) (most * inverse_root(fma(sum, per_c, (double) eps)) * (1.0 / 127.0)));
             if (odd || !(sum < __builtin_inf())) scale = __builtin_nanf("");
+            zero = !(most > 0.0) || scale != scale;
+            far = !zero && !(top > 1e-30f && top < 1e30f);
         } else if constexpr (NORM) {
             top = group_reduce<LPR>(top, larger);
             sum = group_sum<LPR>(sum);
             scale = top * (1.0f / sqrtf(fmaf(sum, (float) per_c, eps))) * (1.0f / 127.0f);
-            edge = !odd && (!(sum < 1e30f && top < 1e30f) || (sum < 1e-30f && top > 0.0f));
-            if (odd) scale = __builtin_nanf("");
+            far = !odd && !(sum > 1e-30f && sum < 1e30f && top > 1e-30f && top < 1e30f);
+            scale = odd ? __builtin_nanf("") : finite_or_nan(scale);
+            zero = odd || far;
         } else {
             top = __builtin_bit_cast(float, group_max<LPR>(bits));
-            scale = (float) ((double) top * (1.0 / 127.0));
+            scale = finite_or_nan((float) ((double) top * (1.0 / 127.0)));
+            zero = !(top > 0.0f) || scale != scale;
+            far = !zero && !(top > 1e-30f && top < 1e30f);
         }
-        scale = finite_or_nan(scale);
-        const bool zero = !(top > 0.0f) || (!edge && scale != scale);  // codes are zeros
-        const bool far = !zero && !(top > 1e-30f && top < 1e30f);  // near the ends of fp32's range: codes from 64 bits
-        const float by = zero ? 0.0f : 127.0f * __builtin_amdgcn_rcpf(top);
+        const float by = zero || far ? 0.0f : 127.0f * __builtin_amdgcn_rcpf(top);
         // 127 t / T, off by no more than 127 times 6 roundings, 4.6e-5.
         const auto about = [&](S a, float b) { return (float) a * b * by; };
         constexpr float kNear = 0.49995f;
@@ -501,35 +503,36 @@ __global__ void __launch_bounds__(256) k_rows_int8(const typename Store<DT>::T *
                 *(uint32_t *) p = zero ? 0u : four_codes(code);
             }
         }
-        if (NORM && __any(edge || far || (!zero && near > kNear))) {
-            if constexpr (!FINE) most = exact_most();
-            bool none = false;  // some value is not finite
+        if (NORM && __any(far || (!zero && near > kNear))) {
             if constexpr (!FINE) {
-                if (__any(edge)) {
+                most = exact_most();
+                if (__any(far && (most > 0.0 || !(sum < __builtin_inff())))) {
                     double squares = 0.0;
 #pragma unroll
                     for (int i = 0; i < CPL; ++i)
 #pragma unroll
                         for (int u = 0; u < N; ++u) squares += product(s[i][u], s[i][u]);
                     squares = group_sum<LPR>(squares);
-                    if (edge) {
+                    if (far) {
                         scale = finite_or_nan((float) (most * inverse_root(fma(squares, per_c, (double) eps)) * (1.0 / 127.0)));
                         if (!(squares < __builtin_inf())) scale = __builtin_nanf("");
-                        none = scale != scale;
                     }
                 }
             }
+            const bool all = far && most > 0.0 && scale == scale;  // (else zeros, which they are)
+            if (__any(all || (!zero && near > kNear))) {
 #pragma unroll
-            for (int i = 0; i < CPL; ++i)
+                for (int i = 0; i < CPL; ++i)
 #pragma unroll
-                for (int u = 0; u < N; ++u) {
-                    const int at = (i * LPR + l) * N + u;
-                    S a = s[i][u];
-                    asm volatile("" : "+v"(a));  // else what is above stays in registers for here
-                    const float f = about(a, g[i][u]);
-                    if (!zero && at < c && (none || far || fabsf(f - rintf(f)) > kNear))
-                        out.codes[row * out.cp + at] = (int8_t) (none ? 0 : int_code64(product(a, g[i][u]), most));
-                }
+                    for (int u = 0; u < N; ++u) {
+                        const int at = (i * LPR + l) * N + u;
+                        S a = s[i][u];
+                        asm volatile("" : "+v"(a));  // else what is above stays in registers for here
+                        const float f = about(a, g[i][u]);
+                        if (at < c && (all || (!zero && fabsf(f - rintf(f)) > kNear)))
+                            out.codes[row * out.cp + at] = (int8_t) int_code64(product(a, g[i][u]), most);
+                    }
+            }
         }
         if (l == 0) out.scales[row] = scale;
     }
