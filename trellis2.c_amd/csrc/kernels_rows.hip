@@ -473,9 +473,10 @@ __global__ void __launch_bounds__(256) k_rows_int8(const typename Store<DT>::T *
             far = !zero && !(top > 1e-30f && top < 1e30f);
         }
         const float by = zero || far ? 0.0f : 127.0f * __builtin_amdgcn_rcpf(top);
-        // 127 t / T, off by no more than 127 times 6 roundings, 4.6e-5.
+        // 127 t / T, off by no more than 127 times 6 roundings, 4.6e-5: of T, its inverse (two), 127
+        // times that, t, and t times that; a sum x + residual in 64 bits has one more, 5.3e-5.
         const auto about = [&](S a, float b) { return (float) a * b * by; };
-        constexpr float kNear = 0.49995f;
+        constexpr float kNear = NORM && FINE ? 0.4999f : 0.49995f;
         float near = 0.0f;
 #pragma unroll
         for (int i = 0; i < CPL; ++i) {
