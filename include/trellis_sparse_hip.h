@@ -581,7 +581,8 @@ trellis_status trellis_sparse_hip_expand_rows8(trellis_sparse_backend * backend,
                                                trellis_sparse_buffer * y, int64_t n, int c);
 
 /* s = x + residual; total = s; y = s / sqrt(mean(s^2) + eps) * gamma, the mean
- * over a row's c channels and s unrounded in y.  residual, gamma (fp32 [c]) and
+ * over a row's c channels and s in y as fp32 holds it (of fp32 rows in 8-bit integer rows as
+ * 64 bits do), unrounded to the compute_dtype.  residual, gamma (fp32 [c]) and
  * total may be NULL; y is rows of the compute_dtype or 8-bit rows (n, c).  y and
  * total may each be x or residual.  eps > 0. */
 trellis_status trellis_sparse_hip_rms_norm(trellis_sparse_backend * backend, const trellis_sparse_buffer * x,

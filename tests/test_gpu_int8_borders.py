@@ -64,3 +64,26 @@ def test_rows_as_they_are(dtype, c):
         assert np.array_equal(codes_of(be, rows, n, c, top / 127), codes)
     finally:
         be.destroy()
+
+
+@pytest.mark.parametrize("dtype", [sh.F16, sh.BF16])
+def test_sums_are_the_same_at_every_width(dtype):
+    """x + residual of 16-bit rows where fp32 has no such number: a width that is a whole number of chunks and one that is not
+    (a zero more) give the same codes, those of the sum in fp32."""
+    be, rng, n, c = sh.Backend(0, dtype), np.random.default_rng(1), 50, 1000
+    try:
+        x = (rng.integers(-63, 63, (n, c)) + 0.5).astype(np.float32)
+        x[:, 0] = 127
+        r = (2.0 ** -20 * rng.choice([-1, 1], (n, c))).astype(np.float32)
+        r[:, 0] = 0
+        codes = np.rint(x + r)  # (where |x| is 16 or more the sum is x, half way between two codes)
+        assert (np.rint(x.astype(np.float64) + r) != codes).mean() > 0.2
+        for wide in (0, 1):
+            m = c + wide
+            xs, rs = (np.concatenate([a, np.zeros((n, wide), np.float32)], 1) for a in (x, r))
+            rows = be.alloc_rows_int8(n, m)
+            be.rms_norm(be.upload(xs), None, rows, n, m, 1e-5, residual=be.upload(rs))
+            got = codes_of(be, rows, n, m, 1 / np.sqrt((xs.astype(np.float64) ** 2).mean(1, keepdims=True) + 1e-5))
+            np.testing.assert_array_equal(got[:, :c], codes)
+    finally:
+        be.destroy()

@@ -357,8 +357,8 @@ __device__ __forceinline__ double inverse_root(double m) {
 }
 
 // Rows, or their norms (NORM, as k_norm_vec), to integer rows: LPR lanes hold a row in
-// registers, CPL chunks each.  Of 16-bit rows x + residual is exact in fp32 but where one is
-// 2^13 times the other, and the largest t is found in fp32, in 64 bits only for a code beside
+// registers, CPL chunks each.  Of 16-bit rows x + residual is taken in fp32, which holds it but
+// where one is 2^13 times the other, and the largest t is found in fp32, in 64 bits only for a code beside
 // a border (one in 10,000, a tenth of a wavefront's rows); statistics of fp32 rows are of 64
 // bits.  Bound by memory: 18,216 x 4096 fp16 47 us, 4.8 TB/s; norms nearly as much by the
 // vector unit: 79,523 x 512 bf16 41 us, 3.0 TB/s.
@@ -548,9 +548,10 @@ __global__ void __launch_bounds__(256) k_rows_int8_any(const typename Store<DT>:
     const int lane = threadIdx.x & 63;
     const int64_t row = (int64_t) blockIdx.x * 4 + (threadIdx.x >> 6);
     if (row >= n) return;
-    const auto at = [&](int i) {
-        const double v = (double) Store<DT>::ld(x, row * c + i);
-        return NORM && residual != nullptr ? v + (double) Store<DT>::ld(residual, row * c + i) : v;
+    const auto at = [&](int i) {  // (sums of 16-bit rows as k_rows_int8's)
+        using S = typename std::conditional<DT == kF32, double, float>::type;
+        const S v = (S) Store<DT>::ld(x, row * c + i);
+        return (double) (NORM && residual != nullptr ? v + (S) Store<DT>::ld(residual, row * c + i) : v);
     };
     const auto weighted = [&](int i, double s) { return NORM && gamma != nullptr ? s * (double) gamma[i] : s; };
     double sum = 0.0, most = 0.0, all = 0.0;
