@@ -257,8 +257,8 @@ template <int DT> __device__ __forceinline__ void store_past_caches(typename Sto
 }
 
 // The tiles, last ones first: they are what the caches still hold of the sums' pass.
-// Bound by memory: 79,523 x 512 bf16 17 us of sums (4.8 TB/s), 4 of statistics, 29 here; all
-// three kernels 50, of which reading and writing once would take 32 at a large copy's 5.1 TB/s.
+// Bound by memory: 79,523 x 512 bf16 16 us of sums (5.0 TB/s), 5 of statistics, 30 here on average (15, 4
+// and 29 at best); the call 49, of which reading and writing once would take 31 at a large copy's 5.3 TB/s.
 template <int DT, int V, int ACT> __global__ void __launch_bounds__(256) k_gn_apply(GroupNorm p) {
     using T = typename Store<DT>::T;
     const unsigned block = gridDim.x - 1 - blockIdx.x;

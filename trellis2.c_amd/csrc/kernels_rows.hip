@@ -360,8 +360,8 @@ __device__ __forceinline__ double inverse_root(double m) {
 // registers, CPL chunks each.  Of 16-bit rows x + residual is taken in fp32, which holds it but
 // where one is 2^13 times the other, and the largest t is found in fp32, in 64 bits only for a code beside
 // a border (one in 10,000, a tenth of a wavefront's rows); statistics of fp32 rows are of 64
-// bits.  Bound by memory: 18,216 x 4096 fp16 47 us, 4.8 TB/s; norms nearly as much by the
-// vector unit: 79,523 x 512 bf16 41 us, 3.0 TB/s.
+// bits.  Bound by memory: 18,216 x 4096 fp16 46 us on average (42 at best), 4.9 TB/s; norms nearly as much by the
+// vector unit: 79,523 x 512 bf16 41 us (37), 3.0 TB/s.
 template <int DT, int LPR, int CPL, bool NORM>
 __global__ void __launch_bounds__(256) k_rows_int8(const typename Store<DT>::T * x,
                                                    const typename Store<DT>::T * residual,

@@ -121,7 +121,7 @@ template <int DT> hipError_t launch_any(const Attention & p, const Scores & sc, 
 // ---- MFMA ---------------------------------------------------------------------------------------
 
 // Units of work, a tile of queries with a kv head each, neighbouring units of the same kv
-// head, in causal calls from the last queries, which see most, to the first.  The first
+// head, in causal calls within a head from the last queries, which see most, to the first.  The first
 // `whole` take all of their keys; the rest, which the CUs would not share evenly, are split
 // over blocks of their own, started last.
 struct Split {
@@ -243,8 +243,14 @@ template <int DT> __device__ __forceinline__ s16x8 finite_part(s16x8 v) {
 // root.  A tile's scores are not computed under the softmax of the one before: without their
 // registers one more wavefront per SIMD fits, which hides as much and spills nothing (18,216
 // rows of 8 x 64 bf16 by voxel distance 1.62 -> 1.30 ms).
-// Bound by the vector unit, 76 % busy there (matrix unit 31 %): 1.05 ms, 650 TFLOP/s of its
-// products; 16,384 rows of 8 x 128 capped 1.30 ms, 850 TFLOP/s.
+// Bound by the vector unit, 76 % busy there (matrix unit 31 %): now 1.07 ms, 637 TFLOP/s of its
+// products; 16,384 rows of 8 x 128 fp16 capped 1.36 ms, 808 TFLOP/s.
+//
+// Weights meet the values in the storage type, rounded to nearest (their sum is of fp32 ones): an error
+// of the size of the output's own rounding (fp16 2.9e-4 of the output's root mean square where that
+// rounding alone leaves 2.1e-4).  FINE: in two parts, which few blocks hide in their
+// latencies; for many they cost 23 % (18,216 rows of 8 x 64 bf16 by voxel distance) to 41 %
+// (9,001 causal rows of 8 x 128 fp16).
 template <int DT, int DC, int NW, bool FINE, bool VOXELS, bool TANH>
 __global__ void __launch_bounds__(64 * NW, DC <= 64 ? (VOXELS ? 3 : 4) : 2) k_scored(Attention p, Scores sc, Split shape, int tiles) {
     using T = typename Store<DT>::T;
@@ -884,8 +890,8 @@ hipError_t launch_mfma(const Attention & p, const Scores & sc, const Split & spl
 }  // namespace
 
 // Few queries: all units split as attention's are.  Many: CUs get equal numbers of whole
-// units, and what is left over is split.  (Causal units are of unequal lengths, and go
-// from the longest to the shortest.)
+// units, and what is left over is split.  (Causal units are of unequal lengths; they are not
+// split, and go from the longest to the shortest of each kv head.)
 ScoredShape scored_shape(int dtype, const Attention & p, const Scores & sc, int cus) {
     const AttentionShape a = attention_shape(dtype, p, cus);
     ScoredShape sh{a.waves, a.tiles, a.fine, 0, 0, 1, 0};
